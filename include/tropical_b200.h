@@ -65,6 +65,12 @@ extern "C" {
                                   returned in fp32, bias/scale applied in fp32.
                                   Forward only (tp_maxplus_fwd[_strided]). */
 
+#define TP_GATE_DECAY 0    /* h = gate * h + x                                     */
+#define TP_GATE_SIGMOID 1  /* h = f * h + (1 - f) * x, f = sigmoid(gate)           */
+
+#define TP_NORM_LAYER 0  /* (v - mean) / sqrt(var + eps)                         */
+#define TP_NORM_RMS 1    /* v / sqrt(mean(v^2) + eps)                            */
+
 #define TP_BWD_STE 1     /* d/ds of sum(softmax(s/tau)*s): TropicalLinear train mode */
 #define TP_BWD_LSE 2     /* softmax(s/tau): gradient of tau*logsumexp(s/tau) (Maslov) */
 
@@ -298,6 +304,131 @@ TP_API int tp_layernorm_bwd(int64_t rows, int64_t D, const float* x, const float
                             const float* gamma, float eps, float* dx, float* dgamma,
                             float* dbeta, void* workspace, int64_t workspace_bytes,
                             void* stream);
+
+/* ======================================================================== *
+ *  The residual stream between two blocks (language models)
+ *
+ *    p = branch_norm ? N(branch) * branch_weight + branch_bias : branch
+ *    t = gate ? sigmoid(gate) * p : p
+ *    y = x + scale * t              scale: none, one number, or [D]
+ *    n = N(y) * weight + bias       the next block's input
+ *
+ *  in one pass: the TSRN block's `x = x + branch(ln(x))`
+ *  (research/tsrn_dml.py:1096-1106) with TropicalSSM's gate and mix (:975-980)
+ *  and the next LayerNorm.  N is LayerNorm or RMS over the D channels (norm:
+ *  TP_NORM_*), 1 <= D <= 8192.
+ *
+ *  dtype (TP_DTYPE_F32 or TP_DTYPE_BF16) is that of x, branch, gate ([rows, D]
+ *  at row strides ldx, ldb, ldg), y, n and the gradients dy, dn, dx, dbranch,
+ *  dgate (contiguous); params_dtype that of scale and the weights and biases
+ *  (contiguous; each may be NULL: no scale, ones, zeros).  Arithmetic is fp32,
+ *  rounded once per output (n from the unrounded y).  n NULL: no second norm.
+ *  stats [rows, 4] fp32, 16-byte aligned (NULL: not kept): mean and 1 /
+ *  deviation of branch and y, for the backward.
+ *
+ *  Backward: from dy and dn (either may be NULL: zeros; n NULL in the forward
+ *  means dn NULL here) writes dx, dbranch, dgate (with a gate) and those of the
+ *  fp32 parameter gradients that are not NULL: dscale [1] or [D], the others
+ *  [D].  workspace: tp_residual_norm_bwd_workspace_bytes(rows, D) (-1: bad D)
+ *  for column sums per block, added in a fixed order (deterministic).  Outputs
+ *  may not overlap inputs.  No C counterpart in the reference.
+ * ======================================================================== */
+TP_API int tp_residual_norm_fwd(int dtype, int params_dtype, int norm, int64_t rows, int64_t D,
+                                const void* x, int64_t ldx, const void* branch, int64_t ldb,
+                                const void* gate, int64_t ldg, const void* scale,
+                                int scale_per_channel, int branch_norm,
+                                const void* branch_weight, const void* branch_bias,
+                                const void* weight, const void* bias, float eps, void* y,
+                                void* n, float* stats, void* stream);
+TP_API int64_t tp_residual_norm_bwd_workspace_bytes(int64_t rows, int64_t D);
+TP_API int tp_residual_norm_bwd(int dtype, int params_dtype, int norm, int64_t rows, int64_t D,
+                                const void* x, int64_t ldx, const void* branch, int64_t ldb,
+                                const void* gate, int64_t ldg, const void* scale,
+                                int scale_per_channel, int branch_norm,
+                                const void* branch_weight, const void* branch_bias,
+                                const void* weight, const void* bias, float eps,
+                                const float* stats, const void* dy, const void* dn, void* dx,
+                                void* dbranch, void* dgate, float* dscale,
+                                float* dbranch_weight, float* dbranch_bias, float* dweight,
+                                float* dbias, void* workspace, int64_t workspace_bytes,
+                                void* stream);
+
+/* ======================================================================== *
+ *  Gated linear recurrence: the (plus, times) counterpart of tp_scan_fwd with
+ *  a gate for every element
+ *
+ *    TP_GATE_DECAY    h_t = gate_t * h_{t-1} + x_t
+ *    TP_GATE_SIGMOID  h_t = f h_{t-1} + (1 - f) x_t,  f = sigmoid(gate_t)
+ *
+ *  gate, x: [B, T, C], channels contiguous, at batch and step strides (0: a
+ *  broadcast operand); h [B, T, C] contiguous; all dtype (TP_DTYPE_F32 or
+ *  TP_DTYPE_BF16).  States are fp32: h0 [B, C] (NULL: zeros), h_last [B, C]
+ *  (NULL: not wanted).  lengths [B] (NULL: T): row b ends after lengths[b]
+ *  steps (clamped to 0 .. T); its h is zero behind the end and its h_last the
+ *  state at the end; gate and x behind the end are not read.  states
+ *  (tp_gated_scan_states_floats floats; NULL: not kept): one state per 64
+ *  steps, for the backward.  Products of gates are formed over runs of up to
+ *  1024 steps: meant for gates of magnitude at most 1, whose products cannot
+ *  overflow.  A non-finite state or input makes the later states of its
+ *  channel non-finite.
+ *
+ *  Backward: from dh [B, T, C] (NULL: zeros) and dh_last [B, C] (NULL: zeros)
+ *  writes dgate and dx ([B, T, C] contiguous, zero behind a row's end) and dh0
+ *  (NULL: not wanted).  dh behind a row's end is not read.
+ *
+ *  Step: one step of B rows for serving; gate, x at row strides ldg, ldx, the
+ *  fp32 state [B, C] at row stride lds (>= C) updated in place, h [B, C]
+ *  contiguous.  No C counterpart in the reference.
+ * ======================================================================== */
+TP_API int64_t tp_gated_scan_states_floats(int64_t B, int64_t T, int64_t C);
+TP_API int tp_gated_scan_fwd(int dtype, int form, int64_t B, int64_t T, int64_t C,
+                             const void* gate, int64_t gate_sb, int64_t gate_st, const void* x,
+                             int64_t x_sb, int64_t x_st, const float* h0,
+                             const int32_t* lengths, void* h, float* h_last, float* states,
+                             void* stream);
+TP_API int tp_gated_scan_bwd(int dtype, int form, int64_t B, int64_t T, int64_t C,
+                             const void* gate, int64_t gate_sb, int64_t gate_st, const void* x,
+                             int64_t x_sb, int64_t x_st, const int32_t* lengths,
+                             const float* states, const void* dh, const float* dh_last,
+                             void* dgate, void* dx, float* dh0, void* stream);
+TP_API int tp_gated_scan_step(int dtype, int form, int64_t B, int64_t C, const void* gate,
+                              int64_t ldg, const void* x, int64_t ldx, float* state,
+                              int64_t lds, void* h, void* stream);
+
+/* ======================================================================== *
+ *  Token embedding with scaling and position rows, and its gradient
+ *
+ *    out[i] = weight[ids[i]] * scale (+ pos_weight[p_i])     i < N
+ *
+ *  weight [V, D] and pos_weight [L, D] (NULL: none) at row strides ldw, ldp,
+ *  out [N, D] contiguous, all dtype (TP_DTYPE_F32 or TP_DTYPE_BF16); ids and
+ *  positions [N] of index_bits (32 or 64).  positions NULL: p_i = i % T (T <= L).
+ *  fp32: product and sum rounded one by one, as tropformer_dropin.py:616-720
+ *  rounds them; bf16: rounded once.  An id or position outside its table is not
+ *  read: its row of out is NaN and TP_DEVERR_INDEX is recorded
+ *  (tp_device_error).
+ *
+ *  tp_embedding_bwd: dweight[v] = scale * sum of dout[i] over ids[i] = v, every
+ *  row of [V, D] written; ids outside the table and padding_idx (negative:
+ *  none) add nothing.  Sums in fp32 over the tokens sorted by id: the same bits
+ *  on every call.  workspace: tp_embedding_bwd_workspace_bytes(N, V, D) bytes
+ *  (-1: bad sizes), 16-byte aligned.  N and V below 2^31.  The gradient of a
+ *  position table at given positions is the same call (scale 1).
+ *
+ *  tp_embedding_pos_bwd: dpos[t] = sum of dout[b * T + t] over b for t < T, zeros
+ *  in the other rows of [L, D] (positions NULL).
+ * ======================================================================== */
+TP_API int tp_embedding_fwd(int dtype, int index_bits, int64_t N, int64_t T, int64_t D,
+                            const void* ids, const void* weight, int64_t V, int64_t ldw,
+                            float scale, const void* pos_weight, int64_t L, int64_t ldp,
+                            const void* positions, void* out, void* stream);
+TP_API int64_t tp_embedding_bwd_workspace_bytes(int64_t N, int64_t V, int64_t D);
+TP_API int tp_embedding_bwd(int dtype, int index_bits, int64_t N, int64_t D, const void* ids,
+                            const void* dout, int64_t V, float scale, int64_t padding_idx,
+                            void* dweight, void* workspace, int64_t workspace_bytes,
+                            void* stream);
+TP_API int tp_embedding_pos_bwd(int dtype, int64_t N, int64_t T, int64_t D, const void* dout,
+                                int64_t L, void* dpos, void* stream);
 
 /* Backward of tp_tsrn_attention_prologue (training): from the gradients of Q,
  * K, V ([B, H, T, dh] contiguous) and the projections qkv, the gradient of qkv
@@ -699,6 +830,7 @@ TP_API int tp_last_error(void);
  * context stays usable.  The word keeps the FIRST code recorded. */
 #define TP_DEVERR_BARRIER_TIMEOUT 1   /* an mbarrier wait ran out of budget  */
 #define TP_DEVERR_FLAG_TIMEOUT 2      /* a flag wait ran out of budget       */
+#define TP_DEVERR_INDEX 3             /* an id or position outside its table */
 
 /* Device-side error word of the current device: 0 when no kernel reported a
  * problem, else a TP_DEVERR_* code.  Synchronises with the device (it reads

@@ -147,6 +147,48 @@ SIGNATURES: dict[str, tuple] = {
          _c_f, _c_p, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_p],
     ),
     "tp_tsrn_attention_workspace_bytes": (_c_i64, [_c_i64, _c_i64, _c_i64, _c_i64, _c_i64]),
+    "tp_residual_norm_fwd": (
+        _c_int,
+        [_c_int, _c_int, _c_int, _c_i64, _c_i64, _c_p, _c_i64, _c_p, _c_i64, _c_p, _c_i64, _c_p,
+         _c_int, _c_int, _c_p, _c_p, _c_p, _c_p, _c_f, _c_p, _c_p, _c_p, _c_p],
+    ),
+    "tp_residual_norm_bwd_workspace_bytes": (_c_i64, [_c_i64, _c_i64]),
+    "tp_residual_norm_bwd": (
+        _c_int,
+        [_c_int, _c_int, _c_int, _c_i64, _c_i64, _c_p, _c_i64, _c_p, _c_i64, _c_p, _c_i64, _c_p,
+         _c_int, _c_int, _c_p, _c_p, _c_p, _c_p, _c_f, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p,
+         _c_p, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_p],
+    ),
+    "tp_gated_scan_states_floats": (_c_i64, [_c_i64, _c_i64, _c_i64]),
+    "tp_gated_scan_fwd": (
+        _c_int,
+        [_c_int, _c_int, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64,
+         _c_p, _c_p, _c_p, _c_p, _c_p, _c_p],
+    ),
+    "tp_gated_scan_bwd": (
+        _c_int,
+        [_c_int, _c_int, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64,
+         _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p],
+    ),
+    "tp_gated_scan_step": (
+        _c_int,
+        [_c_int, _c_int, _c_i64, _c_i64, _c_p, _c_i64, _c_p, _c_i64, _c_p, _c_i64, _c_p, _c_p],
+    ),
+    "tp_embedding_fwd": (
+        _c_int,
+        [_c_int, _c_int, _c_i64, _c_i64, _c_i64, _c_p, _c_p, _c_i64, _c_i64, _c_f, _c_p, _c_i64,
+         _c_i64, _c_p, _c_p, _c_p],
+    ),
+    "tp_embedding_bwd_workspace_bytes": (_c_i64, [_c_i64, _c_i64, _c_i64]),
+    "tp_embedding_bwd": (
+        _c_int,
+        [_c_int, _c_int, _c_i64, _c_i64, _c_p, _c_p, _c_i64, _c_f, _c_i64, _c_p, _c_p, _c_i64,
+         _c_p],
+    ),
+    "tp_embedding_pos_bwd": (
+        _c_int,
+        [_c_int, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_p, _c_p],
+    ),
     "tp_tsrn_attention_fwd": (
         _c_int,
         [_c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_int, _c_int,
@@ -208,6 +250,11 @@ TP_BWD_STE = 1
 TP_BWD_LSE = 2
 TP_DEVERR_BARRIER_TIMEOUT = 1
 TP_DEVERR_FLAG_TIMEOUT = 2
+TP_DEVERR_INDEX = 3
+TP_GATE_DECAY = 0
+TP_GATE_SIGMOID = 1
+TP_NORM_LAYER = 0
+TP_NORM_RMS = 1
 TP_ATT_PATH_AUTO = 0
 TP_ATT_PATH_CUDA_CORES = 1
 TP_ATT_PATH_TENSOR_CORES = 2

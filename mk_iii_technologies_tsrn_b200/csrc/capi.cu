@@ -6,6 +6,7 @@
 // cuda/maxplus_gemm.cu:297-341 (launchers) and cuda/maxplus_binding.py:42-97
 // (the ctypes calls that fed them).
 #include <atomic>
+#include <initializer_list>
 #include <mutex>
 
 #include "maxplus_internal.cuh"
@@ -138,6 +139,82 @@ static int validate_strided(const StridedMaxPlus& p) {
   TP_RETURN_IF(!(p.tau > 0.0f), TP_ERR_INVALID_ARG);
   return TP_OK;
 }
+
+namespace {
+
+// the arguments that the residual-norm forward and backward share
+int residual_norm_args(tp::ResNormArgs& a, int dtype, int params_dtype, int norm, int64_t rows,
+                       int64_t D, const void* x, int64_t ldx, const void* branch, int64_t ldb,
+                       const void* gate, int64_t ldg, const void* scale, int scale_per_channel,
+                       int branch_norm, const void* branch_weight, const void* branch_bias,
+                       const void* weight, const void* bias, float eps) {
+  TP_RETURN_IF(rows < 0 || D <= 0 || ldx < 0 || ldb < 0, TP_ERR_INVALID_ARG);
+  TP_RETURN_IF(norm != TP_NORM_LAYER && norm != TP_NORM_RMS, TP_ERR_INVALID_ARG);
+  TP_RETURN_IF((dtype != TP_DTYPE_F32 && dtype != TP_DTYPE_BF16) ||
+                   (params_dtype != TP_DTYPE_F32 && params_dtype != TP_DTYPE_BF16) ||
+                   !tp::residual_norm_supported(D),
+               TP_ERR_UNSUPPORTED);
+  TP_RETURN_IF(!(eps >= 0.0f) || (gate != nullptr && ldg < 0), TP_ERR_INVALID_ARG);
+  TP_RETURN_IF(!branch_norm && (branch_weight != nullptr || branch_bias != nullptr),
+               TP_ERR_INVALID_ARG);
+  if (rows > 0) {
+    TP_CHECK_PTR(x);
+    TP_CHECK_PTR(branch);
+    TP_CHECK_OPT_PTR(gate);
+  }
+  for (const void* p : {scale, branch_weight, branch_bias, weight, bias}) TP_CHECK_OPT_PTR(p);
+  a.dtype = dtype;
+  a.params_bf16 = params_dtype == TP_DTYPE_BF16;
+  a.rms = norm == TP_NORM_RMS;
+  a.branch_norm = branch_norm != 0;
+  a.scale_mode = scale == nullptr ? 0 : (scale_per_channel ? 2 : 1);
+  a.rows = rows;
+  a.D = D;
+  a.x = x;
+  a.ldx = ldx;
+  a.branch = branch;
+  a.ldb = ldb;
+  a.gate = gate;
+  a.ldg = gate ? ldg : 0;
+  a.scale = scale;
+  a.w = weight;
+  a.b = bias;
+  a.bw = branch_weight;
+  a.bb = branch_bias;
+  a.eps = eps;
+  return TP_OK;
+}
+
+int gated_scan_args(tp::GatedScanArgs& a, int dtype, int form, int64_t B, int64_t T, int64_t C,
+                    const void* gate, int64_t gate_sb, int64_t gate_st, const void* x,
+                    int64_t x_sb, int64_t x_st, const int32_t* lengths) {
+  TP_RETURN_IF(B < 0 || T < 0 || C < 0 || gate_sb < 0 || gate_st < 0 || x_sb < 0 || x_st < 0,
+               TP_ERR_INVALID_ARG);
+  TP_RETURN_IF(dtype != TP_DTYPE_F32 && dtype != TP_DTYPE_BF16, TP_ERR_UNSUPPORTED);
+  TP_RETURN_IF(form != TP_GATE_DECAY && form != TP_GATE_SIGMOID, TP_ERR_INVALID_ARG);
+  if (B > 0 && C > 0) {
+    TP_CHECK_OPT_PTR(lengths);
+    if (T > 0) {
+      TP_CHECK_PTR(gate);
+      TP_CHECK_PTR(x);
+    }
+  }
+  a.dtype = dtype;
+  a.form = form;
+  a.B = B;
+  a.T = T;
+  a.C = C;
+  a.gate = gate;
+  a.gate_sb = gate_sb;
+  a.gate_st = gate_st;
+  a.x = x;
+  a.x_sb = x_sb;
+  a.x_st = x_st;
+  a.lengths = lengths;
+  return TP_OK;
+}
+
+}  // namespace
 
 extern "C" {
 
@@ -596,6 +673,224 @@ int tp_layernorm_bwd(int64_t rows, int64_t D, const float* x, const float* dy,
   }
   return tp::launch_layernorm_bwd(rows, D, x, dy, gamma, eps, dx, dgamma, dbeta,
                                   (float*)workspace, as_stream(stream));
+}
+
+int tp_residual_norm_fwd(int dtype, int params_dtype, int norm, int64_t rows, int64_t D,
+                         const void* x, int64_t ldx, const void* branch, int64_t ldb,
+                         const void* gate, int64_t ldg, const void* scale,
+                         int scale_per_channel, int branch_norm, const void* branch_weight,
+                         const void* branch_bias, const void* weight, const void* bias,
+                         float eps, void* y, void* n, float* stats, void* stream) {
+  tp::ResNormArgs a{};
+  const int st = residual_norm_args(a, dtype, params_dtype, norm, rows, D, x, ldx, branch, ldb,
+                                    gate, ldg, scale, scale_per_channel, branch_norm,
+                                    branch_weight, branch_bias, weight, bias, eps);
+  if (st != TP_OK || rows == 0) return st;
+  TP_CHECK_PTR(y);
+  TP_CHECK_OPT_PTR(n);
+  TP_CHECK_OPT_PTR(stats);
+  TP_RETURN_IF(stats != nullptr && !aligned16(stats), TP_ERR_MISALIGNED);
+  a.y = y;
+  a.n = n;
+  a.stats = stats;
+  return tp::launch_residual_norm_fwd(a, as_stream(stream));
+}
+
+int64_t tp_residual_norm_bwd_workspace_bytes(int64_t rows, int64_t D) {
+  if (rows < 0 || !tp::residual_norm_supported(D)) return -1;
+  return (int64_t)tp::residual_norm_bwd_blocks(rows, D) * (5 * D + 1) * (int64_t)sizeof(float);
+}
+
+int tp_residual_norm_bwd(int dtype, int params_dtype, int norm, int64_t rows, int64_t D,
+                         const void* x, int64_t ldx, const void* branch, int64_t ldb,
+                         const void* gate, int64_t ldg, const void* scale,
+                         int scale_per_channel, int branch_norm, const void* branch_weight,
+                         const void* branch_bias, const void* weight, const void* bias,
+                         float eps, const float* stats, const void* dy, const void* dn,
+                         void* dx, void* dbranch, void* dgate, float* dscale,
+                         float* dbranch_weight, float* dbranch_bias, float* dweight,
+                         float* dbias, void* workspace, int64_t workspace_bytes, void* stream) {
+  tp::ResNormBwdArgs g{};
+  const int st = residual_norm_args(g.f, dtype, params_dtype, norm, rows, D, x, ldx, branch,
+                                    ldb, gate, ldg, scale, scale_per_channel, branch_norm,
+                                    branch_weight, branch_bias, weight, bias, eps);
+  if (st != TP_OK) return st;
+  // a gradient of something that is not there
+  TP_RETURN_IF((gate == nullptr && dgate != nullptr) || (scale == nullptr && dscale != nullptr) ||
+                   (!branch_norm && (dbranch_weight != nullptr || dbranch_bias != nullptr)),
+               TP_ERR_INVALID_ARG);
+  TP_RETURN_IF(workspace == nullptr ||
+                   workspace_bytes < tp_residual_norm_bwd_workspace_bytes(rows, D),
+               TP_ERR_WORKSPACE);
+  TP_CHECK_PTR(workspace);
+  for (const void* p : {dy, dn, (const void*)dscale, (const void*)dbranch_weight,
+                        (const void*)dbranch_bias, (const void*)dweight, (const void*)dbias})
+    TP_CHECK_OPT_PTR(p);
+  if (rows > 0) {
+    TP_CHECK_PTR(stats);
+    TP_RETURN_IF(!aligned16(stats), TP_ERR_MISALIGNED);
+    TP_CHECK_PTR(dx);
+    TP_CHECK_PTR(dbranch);
+    if (gate != nullptr) TP_CHECK_PTR(dgate);
+  }
+  g.f.stats = const_cast<float*>(stats);
+  g.dy = dy;
+  g.dn = dn;
+  g.dx = dx;
+  g.dbranch = dbranch;
+  g.dgate = dgate;
+  g.dscale = dscale;
+  g.dbw = dbranch_weight;
+  g.dbb = dbranch_bias;
+  g.dw = dweight;
+  g.db = dbias;
+  g.part = (float*)workspace;
+  return tp::launch_residual_norm_bwd(g, as_stream(stream));
+}
+
+int64_t tp_gated_scan_states_floats(int64_t B, int64_t T, int64_t C) {
+  if (B < 0 || T < 0 || C < 0) return -1;
+  return B * tp::ceil_div(T, (int64_t)tp::GATED_SCAN_CHUNK) * C;
+}
+
+int tp_gated_scan_fwd(int dtype, int form, int64_t B, int64_t T, int64_t C, const void* gate,
+                      int64_t gate_sb, int64_t gate_st, const void* x, int64_t x_sb,
+                      int64_t x_st, const float* h0, const int32_t* lengths, void* h,
+                      float* h_last, float* states, void* stream) {
+  tp::GatedScanArgs a{};
+  const int st = gated_scan_args(a, dtype, form, B, T, C, gate, gate_sb, gate_st, x, x_sb, x_st,
+                                 lengths);
+  if (st != TP_OK || B == 0 || C == 0) return st;
+  TP_CHECK_OPT_PTR(h0);
+  TP_CHECK_OPT_PTR(h_last);
+  TP_CHECK_OPT_PTR(states);
+  if (T > 0) TP_CHECK_PTR(h);
+  a.h0 = h0;
+  a.h = h;
+  a.h_last = h_last;
+  a.states = states;
+  return tp::launch_gated_scan_fwd(a, as_stream(stream));
+}
+
+int tp_gated_scan_bwd(int dtype, int form, int64_t B, int64_t T, int64_t C, const void* gate,
+                      int64_t gate_sb, int64_t gate_st, const void* x, int64_t x_sb,
+                      int64_t x_st, const int32_t* lengths, const float* states,
+                      const void* dh, const float* dh_last, void* dgate, void* dx, float* dh0,
+                      void* stream) {
+  tp::GatedScanBwdArgs g{};
+  const int st = gated_scan_args(g.f, dtype, form, B, T, C, gate, gate_sb, gate_st, x, x_sb,
+                                 x_st, lengths);
+  if (st != TP_OK || B == 0 || C == 0) return st;
+  TP_CHECK_OPT_PTR(dh);
+  TP_CHECK_OPT_PTR(dh_last);
+  TP_CHECK_OPT_PTR(dh0);
+  if (T > 0) {
+    TP_CHECK_PTR(states);
+    TP_CHECK_PTR(dgate);
+    TP_CHECK_PTR(dx);
+  }
+  g.f.states = const_cast<float*>(states);
+  g.dh = dh;
+  g.dh_last = dh_last;
+  g.dgate = dgate;
+  g.dx = dx;
+  g.dh0 = dh0;
+  return tp::launch_gated_scan_bwd(g, as_stream(stream));
+}
+
+int tp_gated_scan_step(int dtype, int form, int64_t B, int64_t C, const void* gate, int64_t ldg,
+                       const void* x, int64_t ldx, float* state, int64_t lds, void* h,
+                       void* stream) {
+  TP_RETURN_IF(B < 0 || C < 0, TP_ERR_INVALID_ARG);
+  TP_RETURN_IF(dtype != TP_DTYPE_F32 && dtype != TP_DTYPE_BF16, TP_ERR_UNSUPPORTED);
+  TP_RETURN_IF(form != TP_GATE_DECAY && form != TP_GATE_SIGMOID, TP_ERR_INVALID_ARG);
+  if (B == 0 || C == 0) return TP_OK;
+  // rows of the state may not overlap: two rows would update one place
+  TP_RETURN_IF(ldg < 0 || ldx < 0 || (B > 1 && lds < C), TP_ERR_INVALID_ARG);
+  TP_CHECK_PTR(gate);
+  TP_CHECK_PTR(x);
+  TP_CHECK_PTR(state);
+  TP_CHECK_PTR(h);
+  return tp::launch_gated_scan_step(dtype, form, B, C, gate, ldg, x, ldx, state, lds, h,
+                                    as_stream(stream));
+}
+
+int tp_embedding_fwd(int dtype, int index_bits, int64_t N, int64_t T, int64_t D,
+                     const void* ids, const void* weight, int64_t V, int64_t ldw, float scale,
+                     const void* pos_weight, int64_t L, int64_t ldp, const void* positions,
+                     void* out, void* stream) {
+  TP_RETURN_IF(N < 0 || D < 0 || V < 0 || ldw < 0, TP_ERR_INVALID_ARG);
+  TP_RETURN_IF(dtype != TP_DTYPE_F32 && dtype != TP_DTYPE_BF16, TP_ERR_UNSUPPORTED);
+  TP_RETURN_IF(index_bits != 32 && index_bits != 64, TP_ERR_INVALID_ARG);
+  if (N == 0 || D == 0) return TP_OK;
+  TP_RETURN_IF(pos_weight == nullptr && positions != nullptr, TP_ERR_INVALID_ARG);
+  if (pos_weight != nullptr) {
+    TP_RETURN_IF(L < 0 || ldp < 0, TP_ERR_INVALID_ARG);
+    TP_RETURN_IF(positions == nullptr && (T < 1 || T > L), TP_ERR_INVALID_ARG);
+    TP_CHECK_PTR(pos_weight);
+    TP_CHECK_OPT_PTR(positions);
+  }
+  TP_CHECK_PTR(ids);
+  // an empty table (V == 0) has no address: every row of the output is NaN
+  if (V > 0) TP_CHECK_PTR(weight);
+  TP_CHECK_PTR(out);
+  tp::EmbeddingArgs a{};
+  a.dtype = dtype;
+  a.ids64 = index_bits == 64;
+  a.N = N;
+  a.D = D;
+  a.ids = ids;
+  a.weight = weight;
+  a.V = V;
+  a.ldw = ldw;
+  a.scale = scale;
+  a.pos_weight = pos_weight;
+  a.L = L;
+  a.ldp = ldp;
+  a.positions = positions;
+  a.T = T;
+  a.out = out;
+  return tp::launch_embedding_fwd(a, as_stream(stream));
+}
+
+int64_t tp_embedding_bwd_workspace_bytes(int64_t N, int64_t V, int64_t D) {
+  if (N < 0 || V < 0 || D < 0 || N > INT32_MAX || V >= INT32_MAX) return -1;
+  return tp::embedding_bwd_workspace_bytes(N, V, D);
+}
+
+int tp_embedding_bwd(int dtype, int index_bits, int64_t N, int64_t D, const void* ids,
+                     const void* dout, int64_t V, float scale, int64_t padding_idx,
+                     void* dweight, void* workspace, int64_t workspace_bytes, void* stream) {
+  TP_RETURN_IF(N < 0 || D < 0 || V < 0, TP_ERR_INVALID_ARG);
+  TP_RETURN_IF(dtype != TP_DTYPE_F32 && dtype != TP_DTYPE_BF16, TP_ERR_UNSUPPORTED);
+  TP_RETURN_IF(index_bits != 32 && index_bits != 64, TP_ERR_INVALID_ARG);
+  TP_RETURN_IF(N > INT32_MAX || V >= INT32_MAX, TP_ERR_TOO_LARGE);
+  if (V == 0 || D == 0) return TP_OK;
+  TP_CHECK_PTR(dweight);
+  if (N > 0) {
+    TP_CHECK_PTR(ids);
+    TP_CHECK_PTR(dout);
+  }
+  TP_RETURN_IF(workspace == nullptr ||
+                   workspace_bytes < tp_embedding_bwd_workspace_bytes(N, V, D),
+               TP_ERR_WORKSPACE);
+  TP_CHECK_PTR(workspace);
+  TP_RETURN_IF(!aligned16(workspace), TP_ERR_MISALIGNED);
+  return tp::launch_embedding_bwd(dtype, index_bits == 64, N, D, ids, dout, V, scale,
+                                  padding_idx, dweight, workspace, as_stream(stream));
+}
+
+int tp_embedding_pos_bwd(int dtype, int64_t N, int64_t T, int64_t D, const void* dout,
+                         int64_t L, void* dpos, void* stream) {
+  TP_RETURN_IF(N < 0 || T < 0 || D < 0 || L < 0, TP_ERR_INVALID_ARG);
+  TP_RETURN_IF(dtype != TP_DTYPE_F32 && dtype != TP_DTYPE_BF16, TP_ERR_UNSUPPORTED);
+  TP_RETURN_IF(N > 0 && (T < 1 || N % T != 0 || T > L), TP_ERR_INVALID_ARG);
+  TP_RETURN_IF(L > INT32_MAX || D > (int64_t)65535 * 32, TP_ERR_TOO_LARGE);
+  if (L == 0 || D == 0) return TP_OK;
+  TP_CHECK_PTR(dpos);
+  if (N > 0) TP_CHECK_PTR(dout);
+  return tp::launch_embedding_pos_bwd(dtype, N, N > 0 ? T : 0, D, dout, L, dpos,
+                                      as_stream(stream));
 }
 
 int tp_tsrn_attention_fwd(int64_t B, int64_t H, int64_t T, int64_t Tkv, int64_t Tc, int64_t dh,

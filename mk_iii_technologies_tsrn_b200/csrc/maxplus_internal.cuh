@@ -282,4 +282,96 @@ struct MaslovArgs {
 };
 int launch_maslov(const MaslovArgs& a, bool backward, cudaStream_t stream);
 
+// residual_norm.cu: branch norm, gate, residual scale and sum, next norm.
+// x, branch, gate: rows of D channels at the given strides; y, n and the
+// gradients: [rows, D] contiguous.
+struct ResNormArgs {
+  int dtype;             // TP_DTYPE_F32 or TP_DTYPE_BF16: x, branch, gate, y, n
+  int params_bf16;       // storage of w, b, scale, bw, bb (else fp32)
+  int rms;               // 0 LayerNorm, 1 RMS
+  int branch_norm;
+  int scale_mode;        // 0 none, 1 one number, 2 one of each channel
+  int64_t rows, D;
+  const void* x;
+  int64_t ldx;
+  const void* branch;
+  int64_t ldb;
+  const void* gate;      // optional
+  int64_t ldg;
+  const void* scale;
+  const void *w, *b, *bw, *bb;   // each optional
+  float eps;
+  void* y;
+  void* n;               // NULL: no norm of y
+  float* stats;          // [rows][4]: mean, 1 / deviation of branch and of y
+  int group;             // threads per row, set by the launcher
+};
+struct ResNormBwdArgs {
+  ResNormArgs f;
+  const void* dy;        // optional
+  const void* dn;        // optional
+  void *dx, *dbranch, *dgate;
+  float *dw, *db, *dscale, *dbw, *dbb;   // each optional
+  float* part;           // [blocks][sums * D + 1]
+  int sums, slot_w, slot_b, slot_s, slot_bw, slot_bb;   // set by the launcher
+};
+bool residual_norm_supported(int64_t D);
+int residual_norm_bwd_blocks(int64_t rows, int64_t D);
+int launch_residual_norm_fwd(const ResNormArgs& a, cudaStream_t stream);
+int launch_residual_norm_bwd(const ResNormBwdArgs& a, cudaStream_t stream);
+
+// gated_scan.cu: h_t = a_t h_{t-1} + u_t over [B, T, C], channels contiguous
+constexpr int GATED_SCAN_CHUNK = 64;   // steps between the saved states
+struct GatedScanArgs {
+  int dtype;             // TP_DTYPE_F32 or TP_DTYPE_BF16: gate, x, h and their gradients
+  int form;              // TP_GATE_DECAY, TP_GATE_SIGMOID
+  int64_t B, T, C;
+  const void* gate;
+  int64_t gate_sb, gate_st;
+  const void* x;
+  int64_t x_sb, x_st;
+  const float* h0;       // [B, C] or NULL (zeros)
+  const int32_t* lengths;   // [B] or NULL (T)
+  void* h;               // [B, T, C]
+  float* h_last;         // [B, C] or NULL
+  float* states;         // [B, ceil(T / 64), C]: the state before each chunk, or NULL
+};
+struct GatedScanBwdArgs {
+  GatedScanArgs f;       // h, h_last unused; states from the forward
+  const void* dh;        // [B, T, C] or NULL
+  const float* dh_last;  // [B, C] or NULL
+  void *dgate, *dx;      // [B, T, C]
+  float* dh0;            // [B, C] or NULL
+};
+int launch_gated_scan_fwd(const GatedScanArgs& a, cudaStream_t stream);
+int launch_gated_scan_bwd(const GatedScanBwdArgs& a, cudaStream_t stream);
+int launch_gated_scan_step(int dtype, int form, int64_t B, int64_t C, const void* gate,
+                           int64_t ldg, const void* x, int64_t ldx, float* state, int64_t lds,
+                           void* h, cudaStream_t stream);
+
+// embedding.cu: scaled token embedding with position rows, and its gradient
+struct EmbeddingArgs {
+  int dtype;             // TP_DTYPE_F32 or TP_DTYPE_BF16: weight, pos_weight, out
+  int ids64;             // ids and positions are int64 (else int32)
+  int64_t N, D;
+  const void* ids;       // [N]
+  const void* weight;    // [V, D], rows at stride ldw
+  int64_t V, ldw;
+  float scale;
+  const void* pos_weight;   // [L, D] at stride ldp, or NULL
+  int64_t L, ldp;
+  const void* positions;    // [N], or NULL: token i is at position i % T
+  int64_t T;
+  void* out;             // [N, D]
+};
+int launch_embedding_fwd(const EmbeddingArgs& a, cudaStream_t stream);
+int64_t embedding_bwd_workspace_bytes(int64_t N, int64_t V, int64_t D);
+// gradient of a table of V rows from dout [N, D] and the row index of each token
+int launch_embedding_bwd(int dtype, int ids64, int64_t N, int64_t D, const void* ids,
+                         const void* dout, int64_t V, float scale, int64_t padding_idx,
+                         void* dweight, void* workspace, cudaStream_t stream);
+// gradient of the first T rows of a position table of L rows (the others are zeros)
+int launch_embedding_pos_bwd(int dtype, int64_t N, int64_t T, int64_t D, const void* dout,
+                             int64_t L, void* dpos, cudaStream_t stream);
+
 }  // namespace tp

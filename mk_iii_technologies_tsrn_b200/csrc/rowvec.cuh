@@ -1,0 +1,170 @@
+// rowvec.cuh -- vectors of consecutive channels of a row, in fp32 or bf16
+// storage, unpacked to fp32 registers: shared by the embedding and the
+// residual-norm kernels (embedding.cu, residual_norm.cu).
+#pragma once
+
+#include "common.cuh"
+
+namespace tp {
+
+struct bf16_t {   // storage only
+  uint16_t v;
+};
+
+__device__ __forceinline__ uint16_t f32_to_bf16_bits(float f) {
+  return __bfloat16_as_ushort(__float2bfloat16_rn(f));
+}
+// two rounded values in one word (first value in the low half); the cast of a
+// pair is one instruction on sm_100a
+__device__ __forceinline__ uint32_t f32x2_to_bf16x2_bits(float lo, float hi) {
+  const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&p);
+}
+
+// VEC consecutive elements of type T as one load or store
+template <typename T, int VEC>
+struct RowVec;
+
+template <>
+struct RowVec<float, 4> {
+  float4 r;
+  __device__ __forceinline__ void zero() { r = make_float4(0.f, 0.f, 0.f, 0.f); }
+  __device__ __forceinline__ void load(const float* p) {
+    r = __ldg(reinterpret_cast<const float4*>(p));
+  }
+  __device__ __forceinline__ void load_stream(const float* p) {
+    r = __ldcs(reinterpret_cast<const float4*>(p));
+  }
+  __device__ __forceinline__ void get(float* f) const {
+    f[0] = r.x; f[1] = r.y; f[2] = r.z; f[3] = r.w;
+  }
+  __device__ __forceinline__ void set(const float* f) { r = make_float4(f[0], f[1], f[2], f[3]); }
+  __device__ __forceinline__ void store(float* p) const { *reinterpret_cast<float4*>(p) = r; }
+  __device__ __forceinline__ void store_stream(float* p) const {
+    __stcs(reinterpret_cast<float4*>(p), r);
+  }
+};
+
+template <>
+struct RowVec<float, 1> {
+  float r;
+  __device__ __forceinline__ void zero() { r = 0.f; }
+  __device__ __forceinline__ void load(const float* p) { r = __ldg(p); }
+  __device__ __forceinline__ void load_stream(const float* p) { r = __ldcs(p); }
+  __device__ __forceinline__ void get(float* f) const { f[0] = r; }
+  __device__ __forceinline__ void set(const float* f) { r = f[0]; }
+  __device__ __forceinline__ void store(float* p) const { *p = r; }
+  __device__ __forceinline__ void store_stream(float* p) const { __stcs(p, r); }
+};
+
+template <>
+struct RowVec<bf16_t, 8> {
+  uint4 r;
+  __device__ __forceinline__ void zero() { r = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ void load(const bf16_t* p) {
+    r = __ldg(reinterpret_cast<const uint4*>(p));
+  }
+  __device__ __forceinline__ void load_stream(const bf16_t* p) {
+    r = __ldcs(reinterpret_cast<const uint4*>(p));
+  }
+  __device__ __forceinline__ void get(float* f) const {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[2 * i] = __uint_as_float(w[i] << 16);
+      f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+  __device__ __forceinline__ void set(const float* f) {
+    r.x = f32x2_to_bf16x2_bits(f[0], f[1]);
+    r.y = f32x2_to_bf16x2_bits(f[2], f[3]);
+    r.z = f32x2_to_bf16x2_bits(f[4], f[5]);
+    r.w = f32x2_to_bf16x2_bits(f[6], f[7]);
+  }
+  __device__ __forceinline__ void store(bf16_t* p) const { *reinterpret_cast<uint4*>(p) = r; }
+  __device__ __forceinline__ void store_stream(bf16_t* p) const {
+    __stcs(reinterpret_cast<uint4*>(p), r);
+  }
+};
+
+template <>
+struct RowVec<bf16_t, 4> {
+  uint2 r;
+  __device__ __forceinline__ void zero() { r = make_uint2(0, 0); }
+  __device__ __forceinline__ void load(const bf16_t* p) {
+    r = __ldg(reinterpret_cast<const uint2*>(p));
+  }
+  __device__ __forceinline__ void load_stream(const bf16_t* p) {
+    r = __ldcs(reinterpret_cast<const uint2*>(p));
+  }
+  __device__ __forceinline__ void get(float* f) const {
+    const uint32_t w[2] = {r.x, r.y};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      f[2 * i] = __uint_as_float(w[i] << 16);
+      f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+  __device__ __forceinline__ void set(const float* f) {
+    r.x = f32x2_to_bf16x2_bits(f[0], f[1]);
+    r.y = f32x2_to_bf16x2_bits(f[2], f[3]);
+  }
+  __device__ __forceinline__ void store(bf16_t* p) const { *reinterpret_cast<uint2*>(p) = r; }
+  __device__ __forceinline__ void store_stream(bf16_t* p) const {
+    __stcs(reinterpret_cast<uint2*>(p), r);
+  }
+};
+
+template <>
+struct RowVec<bf16_t, 2> {
+  uint32_t r;
+  __device__ __forceinline__ void zero() { r = 0; }
+  __device__ __forceinline__ void load(const bf16_t* p) {
+    r = __ldg(reinterpret_cast<const unsigned int*>(p));
+  }
+  __device__ __forceinline__ void load_stream(const bf16_t* p) {
+    r = __ldcs(reinterpret_cast<const unsigned int*>(p));
+  }
+  __device__ __forceinline__ void get(float* f) const {
+    f[0] = __uint_as_float(r << 16);
+    f[1] = __uint_as_float(r & 0xffff0000u);
+  }
+  __device__ __forceinline__ void set(const float* f) { r = f32x2_to_bf16x2_bits(f[0], f[1]); }
+  __device__ __forceinline__ void store(bf16_t* p) const { *reinterpret_cast<uint32_t*>(p) = r; }
+  __device__ __forceinline__ void store_stream(bf16_t* p) const {
+    __stcs(reinterpret_cast<unsigned int*>(p), r);
+  }
+};
+
+template <>
+struct RowVec<bf16_t, 1> {
+  uint16_t r;
+  __device__ __forceinline__ void zero() { r = 0; }
+  __device__ __forceinline__ void load(const bf16_t* p) {
+    r = __ldg(reinterpret_cast<const unsigned short*>(p));
+  }
+  __device__ __forceinline__ void load_stream(const bf16_t* p) {
+    r = __ldcs(reinterpret_cast<const unsigned short*>(p));
+  }
+  __device__ __forceinline__ void get(float* f) const { f[0] = tp_bf16_to_f32(r); }
+  __device__ __forceinline__ void set(const float* f) { r = f32_to_bf16_bits(f[0]); }
+  __device__ __forceinline__ void store(bf16_t* p) const {
+    *reinterpret_cast<uint16_t*>(p) = r;
+  }
+  __device__ __forceinline__ void store_stream(bf16_t* p) const {
+    __stcs(reinterpret_cast<unsigned short*>(p), r);
+  }
+};
+
+// sigmoid(v) and 1 - sigmoid(v), both to fp32 accuracy: from e = exp(-|v|) the
+// larger one is 1 / (1 + e) and the smaller e / (1 + e), with no cancellation
+// and no overflow (NaN stays NaN).
+__device__ __forceinline__ void sigmoid_pair(float v, float& s, float& rest) {
+  const float e = expf(-fabsf(v));
+  const float big = __fdividef(1.0f, 1.0f + e);
+  const float small = e * big;
+  s = v >= 0.0f ? big : small;
+  rest = v >= 0.0f ? small : big;
+}
+
+}  // namespace tp

@@ -66,9 +66,20 @@ class DeviceWaitTimeout(RuntimeError):
         self.code = code
 
 
+class DeviceIndexError(IndexError):
+    """A token id or position given to :func:`embedding` was outside its table;
+    its row of the output is NaN and it added to no gradient."""
+
+    def __init__(self, device):
+        super().__init__(f"an id or position given to ops.embedding on {device} is outside its "
+                         "table; its rows of the output are NaN")
+        self.code = _lib.TP_DEVERR_INDEX
+
+
 def check_device_error(device=None, reset: bool = True) -> None:
     """Raise :class:`DeviceWaitTimeout` if a kernel on ``device`` (default: the
-    current CUDA device) recorded a timed-out wait since the last reset.
+    current CUDA device) recorded a timed-out wait since the last reset, or
+    :class:`DeviceIndexError` if one met an id outside its table.
 
     Synchronises with the device.  The library's kernels never hang: a wait that
     cannot complete ends after the budget (:func:`set_wait_budget`) and leaves a
@@ -81,6 +92,8 @@ def check_device_error(device=None, reset: bool = True) -> None:
         code = lib.tp_device_error(1 if reset else 0)
     if code < 0:
         raise _lib.TropicalLibraryError("tp_device_error", -code, f"CUDA error {-code}")
+    if code == _lib.TP_DEVERR_INDEX:
+        raise DeviceIndexError(dev)
     if code:
         raise DeviceWaitTimeout(code, dev)
 
@@ -1241,6 +1254,476 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[t
             and (weight is None or weight.dtype == torch.float32)):
         return LayerNormFunction.apply(x, weight, bias, float(eps))
     return torch.nn.functional.layer_norm(x, (x.shape[-1],), weight, bias, eps)
+
+
+# --------------------------------------------------------------------------- residual stream
+NORMS = {"layer": _lib.TP_NORM_LAYER, "rms": _lib.TP_NORM_RMS}
+RESIDUAL_NORM_MAX_CHANNELS = 8192
+
+
+def _channels(t: torch.Tensor) -> torch.Tensor:
+    # the last dimension contiguous; the others at any strides
+    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+
+
+def _rows_of(t: torch.Tensor, D: int) -> torch.Tensor:
+    return _channels(t.reshape(-1, D))
+
+
+def _floating(t: torch.Tensor, what: str) -> int:
+    if t.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"{what} must be float32 or bfloat16, got {t.dtype}")
+    return TP_DTYPE_F32 if t.dtype == torch.float32 else TP_DTYPE_BF16
+
+
+def _residual_norm_args(x, branch, weight, bias, norm, gate, scale, branch_norm, branch_weight,
+                        branch_bias, normalize):
+    dev = _require_cuda(x, branch, weight, bias, gate, scale, branch_weight, branch_bias)
+    dtype = _floating(x, "residual_norm inputs")
+    D = x.shape[-1] if x.dim() else 0
+    if not 1 <= D <= RESIDUAL_NORM_MAX_CHANNELS:
+        raise ValueError(f"residual_norm takes 1 to {RESIDUAL_NORM_MAX_CHANNELS} channels, got {D}")
+    for t, what in ((branch, "branch"), (gate, "gate")):
+        if t is not None and (t.shape != x.shape or t.dtype != x.dtype):
+            raise ValueError(f"{what} must have the shape and dtype of x: {tuple(x.shape)} "
+                             f"{x.dtype}, got {tuple(t.shape)} {t.dtype}")
+    if norm not in NORMS:
+        raise ValueError(f"norm must be one of {tuple(NORMS)}, got {norm!r}")
+    if not branch_norm and (branch_weight is not None or branch_bias is not None):
+        raise ValueError("branch_weight and branch_bias need branch_norm=True")
+    if not normalize and (weight is not None or bias is not None):
+        raise ValueError("weight and bias need normalize=True")
+    pd = None
+    for t, what in ((weight, "weight"), (bias, "bias"), (branch_weight, "branch_weight"),
+                    (branch_bias, "branch_bias"), (scale, "scale")):
+        if t is None:
+            continue
+        if t.shape != (D,) and not (what == "scale" and t.numel() == 1):
+            raise ValueError(f"{what} must be [{D}]{' or one number' if what == 'scale' else ''}, "
+                             f"got {tuple(t.shape)}")
+        if t.dtype not in (torch.float32, x.dtype) or t.dtype != (pd or t.dtype):
+            raise TypeError("residual_norm parameters must share a dtype: float32 or that of x")
+        pd = t.dtype
+    return dev, dtype, TP_DTYPE_BF16 if pd == torch.bfloat16 else TP_DTYPE_F32, D
+
+
+def _param(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    return None if t is None else t.contiguous()
+
+
+def residual_norm_fwd(x, branch, weight=None, bias=None, eps: float = 1e-5, *, norm: str = "layer",
+                      gate=None, scale=None, branch_norm: bool = False, branch_weight=None,
+                      branch_bias=None, normalize: bool = True, need_stats: bool = False):
+    """Forward of :func:`residual_norm` without autograd: (y, n | None, stats | None), stats
+    [rows, 4] fp32 for :func:`residual_norm_bwd`."""
+    dev, dtype, pdtype, D = _residual_norm_args(x, branch, weight, bias, norm, gate, scale,
+                                                branch_norm, branch_weight, branch_bias, normalize)
+    x2, b2 = _rows_of(x, D), _rows_of(branch, D)
+    g2 = _rows_of(gate, D) if gate is not None else None
+    rows = x2.shape[0]
+    w, b, bw, bb, sc = (_param(t) for t in (weight, bias, branch_weight, branch_bias, scale))
+    y = torch.empty(x.shape, device=dev, dtype=x.dtype)
+    n = torch.empty_like(y) if normalize else None
+    stats = torch.empty((rows, 4), device=dev, dtype=torch.float32) if need_stats else None
+    with torch.cuda.device(dev):
+        st = _lib.load().tp_residual_norm_fwd(
+            dtype, pdtype, NORMS[norm], rows, D, _ptr(x2), x2.stride(0), _ptr(b2), b2.stride(0),
+            _ptr(g2), g2.stride(0) if g2 is not None else 0, _ptr(sc),
+            int(sc is not None and sc.numel() > 1), int(branch_norm), _ptr(bw), _ptr(bb), _ptr(w),
+            _ptr(b), float(eps), _ptr(y), _ptr(n), _ptr(stats), _stream(dev))
+    _lib.check(st, "tp_residual_norm_fwd")
+    return y, n, stats
+
+
+def residual_norm_bwd(stats, dy, dn, x, branch, weight=None, bias=None, eps: float = 1e-5, *,
+                      norm: str = "layer", gate=None, scale=None, branch_norm: bool = False,
+                      branch_weight=None, branch_bias=None, normalize: bool = True):
+    """Backward of :func:`residual_norm` from the gradients of y and n (either may be None):
+    a dict with the gradients of x, branch, gate (in their dtype) and of scale, weight, bias,
+    branch_weight, branch_bias (float32); None for what is not there.  Parameter gradients are
+    summed in a fixed order (the same bits on every call)."""
+    dev, dtype, pdtype, D = _residual_norm_args(x, branch, weight, bias, norm, gate, scale,
+                                                branch_norm, branch_weight, branch_bias, normalize)
+    for t, what in ((dy, "dy"), (dn, "dn")):
+        if t is not None and (t.shape != x.shape or t.dtype != x.dtype or t.device != dev):
+            raise ValueError(f"{what} must have the shape, dtype and device of x")
+    if dn is not None and not normalize:
+        raise ValueError("dn needs normalize=True")
+    x2, b2 = _rows_of(x, D), _rows_of(branch, D)
+    g2 = _rows_of(gate, D) if gate is not None else None
+    rows = x2.shape[0]
+    if stats is None or stats.shape != (rows, 4) or stats.dtype != torch.float32:
+        raise ValueError("stats must be the forward's [rows, 4] float32 tensor")
+    w, b, bw, bb, sc = (_param(t) for t in (weight, bias, branch_weight, branch_bias, scale))
+    dy, dn = (t.contiguous() if t is not None else None for t in (dy, dn))
+    empty = lambda t: torch.empty(x.shape, device=dev, dtype=x.dtype) if t is not None else None  # noqa: E731
+    sums = lambda t: torch.empty(t.shape, device=dev, dtype=torch.float32) if t is not None else None  # noqa: E731
+    g = {"x": empty(x), "branch": empty(branch), "gate": empty(gate), "scale": sums(scale),
+         "weight": sums(weight), "bias": sums(bias), "branch_weight": sums(branch_weight),
+         "branch_bias": sums(branch_bias)}
+    lib = _lib.load()
+    with torch.cuda.device(dev):
+        ws = torch.empty(lib.tp_residual_norm_bwd_workspace_bytes(rows, D) // 4, device=dev,
+                         dtype=torch.float32)
+        st = lib.tp_residual_norm_bwd(
+            dtype, pdtype, NORMS[norm], rows, D, _ptr(x2), x2.stride(0), _ptr(b2), b2.stride(0),
+            _ptr(g2), g2.stride(0) if g2 is not None else 0, _ptr(sc),
+            int(sc is not None and sc.numel() > 1), int(branch_norm), _ptr(bw), _ptr(bb), _ptr(w),
+            _ptr(b), float(eps), _ptr(stats), _ptr(dy), _ptr(dn), _ptr(g["x"]), _ptr(g["branch"]),
+            _ptr(g["gate"]), _ptr(g["scale"]), _ptr(g["branch_weight"]), _ptr(g["branch_bias"]),
+            _ptr(g["weight"]), _ptr(g["bias"]), _ptr(ws), ws.numel() * 4, _stream(dev))
+    _lib.check(st, "tp_residual_norm_bwd")
+    return g
+
+
+class ResidualNormFunction(torch.autograd.Function):
+    """(y, n) of :func:`residual_norm`; the backward recomputes y from x and takes the row
+    statistics from the forward."""
+
+    @staticmethod
+    def forward(ctx, x, branch, gate, scale, weight, bias, branch_weight, branch_bias, eps, norm,
+                branch_norm, normalize):
+        ctx.set_materialize_grads(False)
+        kw = dict(norm=norm, gate=gate, scale=scale, branch_norm=branch_norm,
+                  branch_weight=branch_weight, branch_bias=branch_bias, normalize=normalize)
+        y, n, stats = residual_norm_fwd(x, branch, weight, bias, eps, need_stats=True, **kw)
+        ctx.save_for_backward(x, branch, gate, scale, weight, bias, branch_weight, branch_bias,
+                              stats)
+        ctx.how = (eps, norm, branch_norm, normalize)
+        return y, n
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dn):
+        if dy is None and dn is None:
+            return (None,) * 12
+        x, branch, gate, scale, weight, bias, bw, bb, stats = ctx.saved_tensors
+        eps, norm, branch_norm, normalize = ctx.how
+        g = residual_norm_bwd(stats, dy, dn, x, branch, weight, bias, eps, norm=norm, gate=gate,
+                              scale=scale, branch_norm=branch_norm, branch_weight=bw,
+                              branch_bias=bb, normalize=normalize)
+        out = []
+        for i, (k, t) in enumerate((("x", x), ("branch", branch), ("gate", gate),
+                                    ("scale", scale), ("weight", weight), ("bias", bias),
+                                    ("branch_weight", bw), ("branch_bias", bb))):
+            out.append(g[k].to(t.dtype) if t is not None and ctx.needs_input_grad[i] else None)
+        return (*out, None, None, None, None)
+
+
+def residual_norm(x: torch.Tensor, branch: torch.Tensor, weight: Optional[torch.Tensor] = None,
+                  bias: Optional[torch.Tensor] = None, eps: float = 1e-5, *, norm: str = "layer",
+                  gate: Optional[torch.Tensor] = None, scale: Optional[torch.Tensor] = None,
+                  branch_norm: bool = False, branch_weight: Optional[torch.Tensor] = None,
+                  branch_bias: Optional[torch.Tensor] = None, normalize: bool = True):
+    """The residual stream between two blocks, one pass each way::
+
+        p = N(branch) * branch_weight + branch_bias    if branch_norm, else branch
+        y = x + scale * sigmoid(gate) * p              (without gate: x + scale * p)
+        n = N(y) * weight + bias                       the next block's input
+
+    Returns (y, n); n is None with ``normalize=False``.  ``norm``: "layer" (LayerNorm) or
+    "rms".  ``x``, ``branch``, ``gate``: [..., D] of one shape, float32 or bfloat16, D at most
+    8192, rows at any stride.  ``scale``: None, one learnt number, or [D]; it and the weights and
+    biases are float32 or of x's dtype.  Differentiable in all tensors.  It is the TSRN block's
+    ``x + branch(ln(x))`` (research/tsrn_dml.py:1096-1106) with TropicalSSM's gate and mix
+    (:975-980) and the next LayerNorm."""
+    ts = (x, branch, gate, scale, weight, bias, branch_weight, branch_bias)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+        return ResidualNormFunction.apply(*ts, float(eps), norm, bool(branch_norm),
+                                          bool(normalize))
+    y, n, _ = residual_norm_fwd(x, branch, weight, bias, eps, norm=norm, gate=gate, scale=scale,
+                                branch_norm=branch_norm, branch_weight=branch_weight,
+                                branch_bias=branch_bias, normalize=normalize)
+    return y, n
+
+
+# --------------------------------------------------------------------------- gated scan
+GATE_FORMS = {"decay": _lib.TP_GATE_DECAY, "sigmoid": _lib.TP_GATE_SIGMOID}
+
+
+def _gate_form(form: str) -> int:
+    if form not in GATE_FORMS:
+        raise ValueError(f"form must be one of {tuple(GATE_FORMS)}, got {form!r}")
+    return GATE_FORMS[form]
+
+
+def _gated_scan_inputs(gate, x, h0, lengths):
+    dev = _require_cuda(gate, x, h0, lengths)
+    dtype = _floating(x, "gated_scan inputs")
+    if x.dim() != 3 or gate.shape != x.shape or gate.dtype != x.dtype:
+        raise ValueError("gate and x must be [B, T, C] of one shape and dtype, got "
+                         f"{tuple(gate.shape)} {gate.dtype} and {tuple(x.shape)} {x.dtype}")
+    B, T, C = x.shape
+    if h0 is not None and _f32(h0).shape != (B, C):
+        raise ValueError(f"h0 must be [{B}, {C}], got {tuple(h0.shape)}")
+    if lengths is not None:
+        if lengths.shape != (B,) or lengths.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"lengths must be [{B}] of int32 or int64, got "
+                             f"{tuple(lengths.shape)} {lengths.dtype}")
+        if lengths.dtype == torch.int64:
+            lengths = lengths.clamp(0, T).to(torch.int32)
+        lengths = lengths.contiguous()
+    return (dev, dtype, B, T, C, _channels(gate), _channels(x),
+            h0.contiguous() if h0 is not None else None, lengths)
+
+
+def gated_scan_fwd(gate, x, h0=None, *, form: str = "decay", lengths=None,
+                   need_states: bool = False, need_last: bool = True):
+    """Forward of :func:`gated_scan` without autograd: (h, h_last | None, states | None), states
+    [B, ceil(T / 64), C] fp32 for :func:`gated_scan_bwd`."""
+    code = _gate_form(form)
+    dev, dtype, B, T, C, gate, x, h0, lengths = _gated_scan_inputs(gate, x, h0, lengths)
+    h = torch.empty((B, T, C), device=dev, dtype=x.dtype)
+    last = torch.empty((B, C), device=dev, dtype=torch.float32) if need_last else None
+    states = (torch.empty((B, -(-T // 64), C), device=dev, dtype=torch.float32)
+              if need_states else None)
+    with torch.cuda.device(dev):
+        st = _lib.load().tp_gated_scan_fwd(
+            dtype, code, B, T, C, _ptr(gate), gate.stride(0), gate.stride(1), _ptr(x),
+            x.stride(0), x.stride(1), _ptr(h0), _ptr(lengths), _ptr(h), _ptr(last), _ptr(states),
+            _stream(dev))
+    _lib.check(st, "tp_gated_scan_fwd")
+    return h, last, states
+
+
+def gated_scan_bwd(states, dh, dh_last, gate, x, *, form: str = "decay", lengths=None,
+                   need_dh0: bool = True):
+    """Backward of :func:`gated_scan` from the gradients of h and h_last (either may be None) and
+    the forward's states: (dgate, dx, dh0 | None)."""
+    code = _gate_form(form)
+    dev, dtype, B, T, C, gate, x, _, lengths = _gated_scan_inputs(gate, x, None, lengths)
+    if states is None or states.shape != (B, -(-T // 64), C) or states.dtype != torch.float32:
+        raise ValueError("states must be the forward's [B, ceil(T / 64), C] float32 tensor")
+    if dh is not None and (dh.shape != x.shape or dh.dtype != x.dtype or dh.device != dev):
+        raise ValueError("dh must have the shape, dtype and device of x")
+    if dh_last is not None and (_f32(dh_last).shape != (B, C) or dh_last.device != dev):
+        raise ValueError(f"dh_last must be [{B}, {C}] on the inputs' device")
+    dh, dh_last = (t.contiguous() if t is not None else None for t in (dh, dh_last))
+    dgate = torch.empty((B, T, C), device=dev, dtype=x.dtype)
+    dx = torch.empty_like(dgate)
+    dh0 = torch.empty((B, C), device=dev, dtype=torch.float32) if need_dh0 else None
+    with torch.cuda.device(dev):
+        st = _lib.load().tp_gated_scan_bwd(
+            dtype, code, B, T, C, _ptr(gate), gate.stride(0), gate.stride(1), _ptr(x),
+            x.stride(0), x.stride(1), _ptr(lengths), _ptr(states), _ptr(dh), _ptr(dh_last),
+            _ptr(dgate), _ptr(dx), _ptr(dh0), _stream(dev))
+    _lib.check(st, "tp_gated_scan_bwd")
+    return dgate, dx, dh0
+
+
+class GatedScanFunction(torch.autograd.Function):
+    """(h, h_last) of :func:`gated_scan`; keeps gate, x and one fp32 state per 64 steps."""
+
+    @staticmethod
+    def forward(ctx, gate, x, h0, form: str, lengths):
+        ctx.set_materialize_grads(False)
+        h, last, states = gated_scan_fwd(gate, x, h0, form=form, lengths=lengths,
+                                         need_states=True)
+        ctx.save_for_backward(gate, x, lengths, states)
+        ctx.form = form
+        return h, last
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dh, dh_last):
+        if dh is None and dh_last is None:
+            return (None,) * 5
+        gate, x, lengths, states = ctx.saved_tensors
+        dgate, dx, dh0 = gated_scan_bwd(states, dh, dh_last, gate, x, form=ctx.form,
+                                        lengths=lengths, need_dh0=ctx.needs_input_grad[2])
+        return (dgate if ctx.needs_input_grad[0] else None,
+                dx if ctx.needs_input_grad[1] else None, dh0, None, None)
+
+
+def gated_scan(gate: torch.Tensor, x: torch.Tensor, h0: Optional[torch.Tensor] = None, *,
+               form: str = "decay", lengths: Optional[torch.Tensor] = None,
+               return_state: bool = False):
+    """Gated linear recurrence over time, differentiable: the (plus, times) counterpart of
+    :func:`tropical_scan` with a gate for every element::
+
+        form "decay":    h_t = gate_t * h_{t-1} + x_t
+        form "sigmoid":  f = sigmoid(gate_t);  h_t = f * h_{t-1} + (1 - f) * x_t
+
+    ``gate``, ``x``: [B, T, C] float32 or bfloat16, batch and step strides free (0 too: an
+    expanded gate).  ``h0``: [B, C] float32, the state before the first step (None: zeros).
+    ``lengths`` [B]: row b ends after lengths[b] steps; h is zero behind the end and nothing
+    there is read.  Returns h [B, T, C] in x's dtype, with ``return_state`` also the float32
+    state [B, C] at each row's end (for :func:`gated_scan_step`, or to go on with the next
+    segment).  States are float32 throughout.  Meant for gates of magnitude at most 1."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (gate, x, h0)):
+        h, last = GatedScanFunction.apply(gate, x, h0, form, lengths)
+    else:
+        h, last, _ = gated_scan_fwd(gate, x, h0, form=form, lengths=lengths,
+                                    need_last=return_state)
+    return (h, last) if return_state else h
+
+
+def gated_scan_step(gate: torch.Tensor, x: torch.Tensor, state: torch.Tensor, *,
+                    form: str = "decay") -> torch.Tensor:
+    """One step of :func:`gated_scan` for serving: ``state`` [B, C] float32 (rows at any stride
+    of at least C) is updated in place and the new h [B, C] returned in x's dtype.  ``gate``,
+    ``x``: [B, C].  Not differentiable."""
+    code = _gate_form(form)
+    dev = _require_cuda(gate, x, state)
+    dtype = _floating(x, "gated_scan_step inputs")
+    if x.dim() != 2 or gate.shape != x.shape or gate.dtype != x.dtype:
+        raise ValueError("gate and x must be [B, C] of one shape and dtype, got "
+                         f"{tuple(gate.shape)} {gate.dtype} and {tuple(x.shape)} {x.dtype}")
+    B, C = x.shape
+    if _f32(state).shape != (B, C) or (C > 1 and state.stride(1) != 1) or (
+            B > 1 and state.stride(0) < C):
+        raise ValueError(f"state must be [{B}, {C}] with contiguous, separate rows, got "
+                         f"{tuple(state.shape)} at strides {state.stride()}")
+    if torch.is_grad_enabled() and (gate.requires_grad or x.requires_grad or state.requires_grad):
+        raise RuntimeError("gated_scan_step is not differentiable; use gated_scan, or call it "
+                           "under torch.no_grad()")
+    gate, x = _channels(gate), _channels(x)
+    h = torch.empty((B, C), device=dev, dtype=x.dtype)
+    with torch.cuda.device(dev):
+        st = _lib.load().tp_gated_scan_step(dtype, code, B, C, _ptr(gate), gate.stride(0), _ptr(x),
+                                            x.stride(0), _ptr(state), state.stride(0), _ptr(h),
+                                            _stream(dev))
+    _lib.check(st, "tp_gated_scan_step")
+    torch.autograd.graph.increment_version(state)
+    return h
+
+
+# --------------------------------------------------------------------------- embedding
+def _index_bits(t: torch.Tensor, what: str) -> int:
+    if t.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"{what} must be int32 or int64, got {t.dtype}")
+    return 32 if t.dtype == torch.int32 else 64
+
+
+def _table(t: torch.Tensor, what: str) -> torch.Tensor:
+    if t.dim() != 2:
+        raise ValueError(f"{what} must be [rows, channels], got {tuple(t.shape)}")
+    return _channels(t)
+
+
+def embedding_fwd(ids, weight, scale: float = 1.0, *, pos_weight=None, positions=None):
+    """Forward of :func:`embedding` without autograd."""
+    dev = _require_cuda(ids, weight, pos_weight, positions)
+    dtype, bits = _floating(weight, "embedding tables"), _index_bits(ids, "ids")
+    w = _table(weight, "weight")
+    V, D = w.shape
+    if positions is not None and pos_weight is None:
+        raise ValueError("positions need pos_weight")
+    p, T = None, ids.shape[-1] if ids.dim() else 1
+    if pos_weight is not None:
+        p = _table(pos_weight, "pos_weight")
+        if p.shape[1] != D or p.dtype != w.dtype:
+            raise ValueError("pos_weight must have weight's channels and dtype, got "
+                             f"{tuple(p.shape)} {p.dtype}")
+        if positions is None:
+            if T > p.shape[0]:
+                raise ValueError(f"{T} positions do not fit a table of {p.shape[0]}")
+        else:
+            _index_bits(positions, "positions")
+            positions = positions.expand(ids.shape).to(ids.dtype).contiguous()
+    flat = ids.contiguous()
+    out = torch.empty((*ids.shape, D), device=dev, dtype=w.dtype)
+    with torch.cuda.device(dev):
+        st = _lib.load().tp_embedding_fwd(
+            dtype, bits, flat.numel(), T, D, _ptr(flat), _ptr(w), V, w.stride(0), float(scale),
+            _ptr(p), p.shape[0] if p is not None else 0, p.stride(0) if p is not None else 0,
+            _ptr(positions), _ptr(out), _stream(dev))
+    _lib.check(st, "tp_embedding_fwd")
+    return out
+
+
+def embedding_bwd(ids, dout, rows: int, scale: float = 1.0, *,
+                  padding_idx: Optional[int] = None) -> torch.Tensor:
+    """Gradient [rows, D] of an embedding table from ``dout`` [*ids.shape, D]: row v is
+    ``scale`` times the float32 sum of the rows of dout whose id is v, in the order of the tokens
+    (the same bits on every call); absent rows and ``padding_idx`` are zero."""
+    dev = _require_cuda(ids, dout)
+    dtype, bits = _floating(dout, "dout"), _index_bits(ids, "ids")
+    if dout.shape[:-1] != ids.shape:
+        raise ValueError(f"dout must be [*ids.shape, D], got {tuple(dout.shape)} for ids "
+                         f"{tuple(ids.shape)}")
+    D, N = dout.shape[-1], ids.numel()
+    ids, dout = ids.contiguous(), dout.contiguous()
+    dw = torch.empty((rows, D), device=dev, dtype=dout.dtype)
+    lib = _lib.load()
+    with torch.cuda.device(dev):
+        need = lib.tp_embedding_bwd_workspace_bytes(N, rows, D)
+        if need < 0:
+            raise ValueError(f"embedding_bwd takes fewer than 2^31 tokens and rows, got {N} and "
+                             f"{rows}")
+        ws = torch.empty(max(need, 16), device=dev, dtype=torch.uint8)
+        st = lib.tp_embedding_bwd(dtype, bits, N, D, _ptr(ids), _ptr(dout), rows, float(scale),
+                                  -1 if padding_idx is None else int(padding_idx), _ptr(dw),
+                                  _ptr(ws), ws.numel(), _stream(dev))
+    _lib.check(st, "tp_embedding_bwd")
+    return dw
+
+
+def embedding_pos_bwd(dout: torch.Tensor, rows: int) -> torch.Tensor:
+    """Gradient [rows, D] of a position table whose row t was added to ``dout[..., t, :]``."""
+    dev = _require_cuda(dout)
+    dtype = _floating(dout, "dout")
+    D = dout.shape[-1]
+    T = dout.shape[-2] if dout.dim() > 1 else 1
+    dout = dout.contiguous()
+    dp = torch.empty((rows, D), device=dev, dtype=dout.dtype)
+    N = dout.numel() // D if D else 0
+    with torch.cuda.device(dev):
+        st = _lib.load().tp_embedding_pos_bwd(dtype, N, T, D, _ptr(dout), rows, _ptr(dp),
+                                              _stream(dev))
+    _lib.check(st, "tp_embedding_pos_bwd")
+    return dp
+
+
+class EmbeddingFunction(torch.autograd.Function):
+    """:func:`embedding`; the gradients of the tables are dense."""
+
+    @staticmethod
+    def forward(ctx, ids, weight, pos_weight, positions, scale: float, padding_idx):
+        ctx.save_for_backward(ids, positions)
+        ctx.rows = (weight.shape[0], pos_weight.shape[0] if pos_weight is not None else 0)
+        ctx.scale, ctx.padding_idx = scale, padding_idx
+        return embedding_fwd(ids, weight, scale, pos_weight=pos_weight, positions=positions)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        ids, positions = ctx.saved_tensors
+        dw = dp = None
+        dout = dout.contiguous()
+        if ctx.needs_input_grad[1]:
+            dw = embedding_bwd(ids, dout, ctx.rows[0], ctx.scale, padding_idx=ctx.padding_idx)
+        if ctx.needs_input_grad[2]:
+            dp = (embedding_pos_bwd(dout, ctx.rows[1]) if positions is None
+                  else embedding_bwd(positions.expand(ids.shape), dout, ctx.rows[1]))
+        return None, dw, dp, None, None, None
+
+
+def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, *,
+              pos_weight: Optional[torch.Tensor] = None,
+              positions: Optional[torch.Tensor] = None,
+              padding_idx: Optional[int] = None) -> torch.Tensor:
+    """``weight[ids] * scale (+ pos_weight[positions])``, the token embedding of
+    ``TropicalEncoderModel`` / ``TropicalDecoderModel`` (tropformer_dropin.py:616-720), in one
+    kernel; differentiable in both tables.
+
+    ``ids``: int32 or int64 of any shape; ``weight`` [V, D] float32 or bfloat16; ``pos_weight``
+    [L, D] of the same dtype.  ``positions`` (None: the index along the last dimension of ids;
+    else integers that expand to ids' shape, as in a decoding step).  ``padding_idx``: a row that
+    gets no gradient, as in ``F.embedding``.  float32 rounds the product and the sum one by one,
+    as the unfused expression; bfloat16 rounds once.  An id or position outside its table gives a
+    row of NaN and no gradient, and :func:`check_device_error` raises
+    :class:`DeviceIndexError`."""
+    if padding_idx is not None:
+        V = weight.shape[0]
+        if not -V <= padding_idx < V:
+            raise ValueError(f"padding_idx {padding_idx} is outside a table of {V} rows")
+        padding_idx %= V
+    if torch.is_grad_enabled() and (weight.requires_grad or (
+            pos_weight is not None and pos_weight.requires_grad)):
+        return EmbeddingFunction.apply(ids, weight, pos_weight, positions, float(scale),
+                                       padding_idx)
+    return embedding_fwd(ids, weight, scale, pos_weight=pos_weight, positions=positions)
 
 
 def tsrn_attention_host(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor,
