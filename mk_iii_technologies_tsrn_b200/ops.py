@@ -1261,23 +1261,66 @@ NORMS = {"layer": _lib.TP_NORM_LAYER, "rms": _lib.TP_NORM_RMS}
 RESIDUAL_NORM_MAX_CHANNELS = 8192
 
 
+def _launch(name: str, dev: torch.device, *args) -> None:
+    # an entry point on the device's current stream.  These operators are also called for single
+    # tokens, where the host's time is the call's: the device is switched only if it is another,
+    # and addresses and the stream go through as plain integers
+    fn = getattr(_lib.load(), name)
+    if torch._C._cuda_getDevice() == dev.index:
+        st = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            st = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    if st:
+        _lib.check(st, name)
+
+
+def _on(dev: torch.device):
+    # the device as the current one (for a size that depends on it)
+    return (contextlib.nullcontext() if torch._C._cuda_getDevice() == dev.index
+            else torch.cuda.device(dev))
+
+
+def _at(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
 def _channels(t: torch.Tensor) -> torch.Tensor:
     # the last dimension contiguous; the others at any strides
     return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
 
 
-def _rows_of(t: torch.Tensor, D: int) -> torch.Tensor:
-    return _channels(t.reshape(-1, D))
+def _rows_of(t: Optional[torch.Tensor], D: int):
+    # t as rows of D channels, and their stride
+    if t is None:
+        return None, 0
+    if t.is_contiguous():
+        return t, D
+    t = _channels(t.reshape(-1, D))
+    return t, t.stride(0)
+
+
+def _contiguous(t: Optional[torch.Tensor]):
+    return t if t is None or t.is_contiguous() else t.contiguous()
+
+
+def _empty_as(t: torch.Tensor) -> torch.Tensor:
+    # contiguous, of t's shape, dtype and device
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(
+        t.shape, device=t.device, dtype=t.dtype)
 
 
 def _floating(t: torch.Tensor, what: str) -> int:
-    if t.dtype not in (torch.float32, torch.bfloat16):
-        raise TypeError(f"{what} must be float32 or bfloat16, got {t.dtype}")
-    return TP_DTYPE_F32 if t.dtype == torch.float32 else TP_DTYPE_BF16
+    if t.dtype == torch.float32:
+        return TP_DTYPE_F32
+    if t.dtype == torch.bfloat16:
+        return TP_DTYPE_BF16
+    raise TypeError(f"{what} must be float32 or bfloat16, got {t.dtype}")
 
 
 def _residual_norm_args(x, branch, weight, bias, norm, gate, scale, branch_norm, branch_weight,
                         branch_bias, normalize):
+    """Checks; (device, dtype code, parameters' dtype code, D)."""
     dev = _require_cuda(x, branch, weight, bias, gate, scale, branch_weight, branch_bias)
     dtype = _floating(x, "residual_norm inputs")
     D = x.shape[-1] if x.dim() else 0
@@ -1307,8 +1350,46 @@ def _residual_norm_args(x, branch, weight, bias, norm, gate, scale, branch_norm,
     return dev, dtype, TP_DTYPE_BF16 if pd == torch.bfloat16 else TP_DTYPE_F32, D
 
 
-def _param(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    return None if t is None else t.contiguous()
+def _residual_norm_run(dev, dtype, pdtype, D, x, branch, weight, bias, eps, norm, gate, scale,
+                       branch_norm, branch_weight, branch_bias, normalize, need_stats):
+    (x2, ldx), (b2, ldb), (g2, ldg) = _rows_of(x, D), _rows_of(branch, D), _rows_of(gate, D)
+    w, b, bw, bb, sc = (_contiguous(t) for t in (weight, bias, branch_weight, branch_bias, scale))
+    rows = x.numel() // D
+    y = _empty_as(x)
+    n = torch.empty_like(y) if normalize else None
+    stats = torch.empty((rows, 4), device=dev, dtype=torch.float32) if need_stats else None
+    _launch("tp_residual_norm_fwd", dev, dtype, pdtype, NORMS[norm], rows, D, x2.data_ptr(), ldx,
+            b2.data_ptr(), ldb, _at(g2), ldg, _at(sc), sc is not None and sc.numel() > 1,
+            branch_norm, _at(bw), _at(bb), _at(w), _at(b), eps, y.data_ptr(), _at(n), _at(stats))
+    return y, n, stats
+
+
+def _residual_norm_back(dev, dtype, pdtype, D, stats, dy, dn, x, branch, weight, bias, eps, norm,
+                        gate, scale, branch_norm, branch_weight, branch_bias, wanted):
+    """(dx, dbranch, dgate, [dscale, dweight, dbias, dbranch_weight, dbranch_bias]); the parameter
+    gradients that are ``wanted`` are float32 views of one buffer."""
+    (x2, ldx), (b2, ldb), (g2, ldg) = _rows_of(x, D), _rows_of(branch, D), _rows_of(gate, D)
+    w, b, bw, bb, sc = (_contiguous(t) for t in (weight, bias, branch_weight, branch_bias, scale))
+    dy, dn = _contiguous(dy), _contiguous(dn)
+    rows = x.numel() // D
+    dx, dbranch = _empty_as(x), _empty_as(branch)
+    dgate = _empty_as(gate) if gate is not None else None
+    params = [None] * 5
+    sizes = [t.numel() if want else 0 for t, want in zip((scale, weight, bias, branch_weight,
+                                                          branch_bias), wanted)]
+    if any(wanted):
+        views = torch.empty(sum(sizes), device=dev, dtype=torch.float32).split_with_sizes(sizes)
+        params = [v if want else None for v, want in zip(views, wanted)]
+    with _on(dev):
+        need = _lib.load().tp_residual_norm_bwd_workspace_bytes(rows, D)
+    ws = torch.empty(need, device=dev, dtype=torch.uint8)
+    dsc, dw, db, dbw, dbb = params
+    _launch("tp_residual_norm_bwd", dev, dtype, pdtype, NORMS[norm], rows, D, x2.data_ptr(), ldx,
+            b2.data_ptr(), ldb, _at(g2), ldg, _at(sc), sc is not None and sc.numel() > 1,
+            branch_norm, _at(bw), _at(bb), _at(w), _at(b), eps, stats.data_ptr(), _at(dy), _at(dn),
+            dx.data_ptr(), dbranch.data_ptr(), _at(dgate), _at(dsc), _at(dbw), _at(dbb), _at(dw),
+            _at(db), ws.data_ptr(), need)
+    return dx, dbranch, dgate, params
 
 
 def residual_norm_fwd(x, branch, weight=None, bias=None, eps: float = 1e-5, *, norm: str = "layer",
@@ -1316,23 +1397,10 @@ def residual_norm_fwd(x, branch, weight=None, bias=None, eps: float = 1e-5, *, n
                       branch_bias=None, normalize: bool = True, need_stats: bool = False):
     """Forward of :func:`residual_norm` without autograd: (y, n | None, stats | None), stats
     [rows, 4] fp32 for :func:`residual_norm_bwd`."""
-    dev, dtype, pdtype, D = _residual_norm_args(x, branch, weight, bias, norm, gate, scale,
-                                                branch_norm, branch_weight, branch_bias, normalize)
-    x2, b2 = _rows_of(x, D), _rows_of(branch, D)
-    g2 = _rows_of(gate, D) if gate is not None else None
-    rows = x2.shape[0]
-    w, b, bw, bb, sc = (_param(t) for t in (weight, bias, branch_weight, branch_bias, scale))
-    y = torch.empty(x.shape, device=dev, dtype=x.dtype)
-    n = torch.empty_like(y) if normalize else None
-    stats = torch.empty((rows, 4), device=dev, dtype=torch.float32) if need_stats else None
-    with torch.cuda.device(dev):
-        st = _lib.load().tp_residual_norm_fwd(
-            dtype, pdtype, NORMS[norm], rows, D, _ptr(x2), x2.stride(0), _ptr(b2), b2.stride(0),
-            _ptr(g2), g2.stride(0) if g2 is not None else 0, _ptr(sc),
-            int(sc is not None and sc.numel() > 1), int(branch_norm), _ptr(bw), _ptr(bb), _ptr(w),
-            _ptr(b), float(eps), _ptr(y), _ptr(n), _ptr(stats), _stream(dev))
-    _lib.check(st, "tp_residual_norm_fwd")
-    return y, n, stats
+    head = _residual_norm_args(x, branch, weight, bias, norm, gate, scale, branch_norm,
+                               branch_weight, branch_bias, normalize)
+    return _residual_norm_run(*head, x, branch, weight, bias, eps, norm, gate, scale, branch_norm,
+                              branch_weight, branch_bias, normalize, need_stats)
 
 
 def residual_norm_bwd(stats, dy, dn, x, branch, weight=None, bias=None, eps: float = 1e-5, *,
@@ -1342,38 +1410,23 @@ def residual_norm_bwd(stats, dy, dn, x, branch, weight=None, bias=None, eps: flo
     a dict with the gradients of x, branch, gate (in their dtype) and of scale, weight, bias,
     branch_weight, branch_bias (float32); None for what is not there.  Parameter gradients are
     summed in a fixed order (the same bits on every call)."""
-    dev, dtype, pdtype, D = _residual_norm_args(x, branch, weight, bias, norm, gate, scale,
-                                                branch_norm, branch_weight, branch_bias, normalize)
+    head = _residual_norm_args(x, branch, weight, bias, norm, gate, scale, branch_norm,
+                               branch_weight, branch_bias, normalize)
     for t, what in ((dy, "dy"), (dn, "dn")):
-        if t is not None and (t.shape != x.shape or t.dtype != x.dtype or t.device != dev):
+        if t is not None and (t.shape != x.shape or t.dtype != x.dtype or t.device != head[0]):
             raise ValueError(f"{what} must have the shape, dtype and device of x")
     if dn is not None and not normalize:
         raise ValueError("dn needs normalize=True")
-    x2, b2 = _rows_of(x, D), _rows_of(branch, D)
-    g2 = _rows_of(gate, D) if gate is not None else None
-    rows = x2.shape[0]
-    if stats is None or stats.shape != (rows, 4) or stats.dtype != torch.float32:
+    if (stats is None or stats.shape != (x.numel() // head[3], 4) or stats.device != head[0]
+            or stats.dtype != torch.float32 or not stats.is_contiguous()):
         raise ValueError("stats must be the forward's [rows, 4] float32 tensor")
-    w, b, bw, bb, sc = (_param(t) for t in (weight, bias, branch_weight, branch_bias, scale))
-    dy, dn = (t.contiguous() if t is not None else None for t in (dy, dn))
-    empty = lambda t: torch.empty(x.shape, device=dev, dtype=x.dtype) if t is not None else None  # noqa: E731
-    sums = lambda t: torch.empty(t.shape, device=dev, dtype=torch.float32) if t is not None else None  # noqa: E731
-    g = {"x": empty(x), "branch": empty(branch), "gate": empty(gate), "scale": sums(scale),
-         "weight": sums(weight), "bias": sums(bias), "branch_weight": sums(branch_weight),
-         "branch_bias": sums(branch_bias)}
-    lib = _lib.load()
-    with torch.cuda.device(dev):
-        ws = torch.empty(lib.tp_residual_norm_bwd_workspace_bytes(rows, D) // 4, device=dev,
-                         dtype=torch.float32)
-        st = lib.tp_residual_norm_bwd(
-            dtype, pdtype, NORMS[norm], rows, D, _ptr(x2), x2.stride(0), _ptr(b2), b2.stride(0),
-            _ptr(g2), g2.stride(0) if g2 is not None else 0, _ptr(sc),
-            int(sc is not None and sc.numel() > 1), int(branch_norm), _ptr(bw), _ptr(bb), _ptr(w),
-            _ptr(b), float(eps), _ptr(stats), _ptr(dy), _ptr(dn), _ptr(g["x"]), _ptr(g["branch"]),
-            _ptr(g["gate"]), _ptr(g["scale"]), _ptr(g["branch_weight"]), _ptr(g["branch_bias"]),
-            _ptr(g["weight"]), _ptr(g["bias"]), _ptr(ws), ws.numel() * 4, _stream(dev))
-    _lib.check(st, "tp_residual_norm_bwd")
-    return g
+    given = (scale, weight, bias, branch_weight, branch_bias)
+    dx, dbranch, dgate, ps = _residual_norm_back(
+        *head, stats, dy, dn, x, branch, weight, bias, eps, norm, gate, scale, branch_norm,
+        branch_weight, branch_bias, [t is not None for t in given])
+    ps = [g.view(t.shape) if t is not None else None for g, t in zip(ps, given)]
+    return dict(zip(("x", "branch", "gate", "scale", "weight", "bias", "branch_weight",
+                     "branch_bias"), (dx, dbranch, dgate, *ps)))
 
 
 class ResidualNormFunction(torch.autograd.Function):
@@ -1384,12 +1437,13 @@ class ResidualNormFunction(torch.autograd.Function):
     def forward(ctx, x, branch, gate, scale, weight, bias, branch_weight, branch_bias, eps, norm,
                 branch_norm, normalize):
         ctx.set_materialize_grads(False)
-        kw = dict(norm=norm, gate=gate, scale=scale, branch_norm=branch_norm,
-                  branch_weight=branch_weight, branch_bias=branch_bias, normalize=normalize)
-        y, n, stats = residual_norm_fwd(x, branch, weight, bias, eps, need_stats=True, **kw)
+        head = _residual_norm_args(x, branch, weight, bias, norm, gate, scale, branch_norm,
+                                   branch_weight, branch_bias, normalize)
+        y, n, stats = _residual_norm_run(*head, x, branch, weight, bias, eps, norm, gate, scale,
+                                         branch_norm, branch_weight, branch_bias, normalize, True)
         ctx.save_for_backward(x, branch, gate, scale, weight, bias, branch_weight, branch_bias,
                               stats)
-        ctx.how = (eps, norm, branch_norm, normalize)
+        ctx.how = (head, eps, norm, branch_norm)
         return y, n
 
     @staticmethod
@@ -1398,16 +1452,19 @@ class ResidualNormFunction(torch.autograd.Function):
         if dy is None and dn is None:
             return (None,) * 12
         x, branch, gate, scale, weight, bias, bw, bb, stats = ctx.saved_tensors
-        eps, norm, branch_norm, normalize = ctx.how
-        g = residual_norm_bwd(stats, dy, dn, x, branch, weight, bias, eps, norm=norm, gate=gate,
-                              scale=scale, branch_norm=branch_norm, branch_weight=bw,
-                              branch_bias=bb, normalize=normalize)
-        out = []
-        for i, (k, t) in enumerate((("x", x), ("branch", branch), ("gate", gate),
-                                    ("scale", scale), ("weight", weight), ("bias", bias),
-                                    ("branch_weight", bw), ("branch_bias", bb))):
-            out.append(g[k].to(t.dtype) if t is not None and ctx.needs_input_grad[i] else None)
-        return (*out, None, None, None, None)
+        head, eps, norm, branch_norm = ctx.how
+        need = ctx.needs_input_grad
+        dx, dbranch, dgate, ps = _residual_norm_back(
+            *head, stats, dy, dn, x, branch, weight, bias, eps, norm, gate, scale, branch_norm,
+            bw, bb, need[3:8])
+        for i, t in enumerate((scale, weight, bias, bw, bb)):
+            if ps[i] is not None:
+                if t.dtype != torch.float32:
+                    ps[i] = ps[i].to(t.dtype)
+                if t.dim() != 1:
+                    ps[i] = ps[i].view(t.shape)
+        return (dx if need[0] else None, dbranch if need[1] else None, dgate if need[2] else None,
+                *ps, None, None, None, None)
 
 
 def residual_norm(x: torch.Tensor, branch: torch.Tensor, weight: Optional[torch.Tensor] = None,
@@ -1448,6 +1505,7 @@ def _gate_form(form: str) -> int:
 
 
 def _gated_scan_inputs(gate, x, h0, lengths):
+    """Checks; (device, dtype code, lengths as int32 | None)."""
     dev = _require_cuda(gate, x, h0, lengths)
     dtype = _floating(x, "gated_scan inputs")
     if x.dim() != 3 or gate.shape != x.shape or gate.dtype != x.dtype:
@@ -1463,8 +1521,31 @@ def _gated_scan_inputs(gate, x, h0, lengths):
         if lengths.dtype == torch.int64:
             lengths = lengths.clamp(0, T).to(torch.int32)
         lengths = lengths.contiguous()
-    return (dev, dtype, B, T, C, _channels(gate), _channels(x),
-            h0.contiguous() if h0 is not None else None, lengths)
+    return dev, dtype, lengths
+
+
+def _gated_scan_run(dev, dtype, lengths, code, gate, x, h0, need_states, need_last):
+    B, T, C = x.shape
+    gate, x, h0 = _channels(gate), _channels(x), _contiguous(h0)
+    h = _empty_as(x)
+    last = torch.empty((B, C), device=dev, dtype=torch.float32) if need_last else None
+    states = (torch.empty((B, -(-T // 64), C), device=dev, dtype=torch.float32)
+              if need_states else None)
+    _launch("tp_gated_scan_fwd", dev, dtype, code, B, T, C, gate.data_ptr(), gate.stride(0),
+            gate.stride(1), x.data_ptr(), x.stride(0), x.stride(1), _at(h0), _at(lengths),
+            h.data_ptr(), _at(last), _at(states))
+    return h, last, states
+
+
+def _gated_scan_back(dev, dtype, lengths, code, states, dh, dh_last, gate, x, need_dh0):
+    B, T, C = x.shape
+    gate, x, dh, dh_last = _channels(gate), _channels(x), _contiguous(dh), _contiguous(dh_last)
+    dgate, dx = _empty_as(x), _empty_as(x)
+    dh0 = torch.empty((B, C), device=dev, dtype=torch.float32) if need_dh0 else None
+    _launch("tp_gated_scan_bwd", dev, dtype, code, B, T, C, gate.data_ptr(), gate.stride(0),
+            gate.stride(1), x.data_ptr(), x.stride(0), x.stride(1), _at(lengths), _at(states),
+            _at(dh), _at(dh_last), dgate.data_ptr(), dx.data_ptr(), _at(dh0))
+    return dgate, dx, dh0
 
 
 def gated_scan_fwd(gate, x, h0=None, *, form: str = "decay", lengths=None,
@@ -1472,18 +1553,8 @@ def gated_scan_fwd(gate, x, h0=None, *, form: str = "decay", lengths=None,
     """Forward of :func:`gated_scan` without autograd: (h, h_last | None, states | None), states
     [B, ceil(T / 64), C] fp32 for :func:`gated_scan_bwd`."""
     code = _gate_form(form)
-    dev, dtype, B, T, C, gate, x, h0, lengths = _gated_scan_inputs(gate, x, h0, lengths)
-    h = torch.empty((B, T, C), device=dev, dtype=x.dtype)
-    last = torch.empty((B, C), device=dev, dtype=torch.float32) if need_last else None
-    states = (torch.empty((B, -(-T // 64), C), device=dev, dtype=torch.float32)
-              if need_states else None)
-    with torch.cuda.device(dev):
-        st = _lib.load().tp_gated_scan_fwd(
-            dtype, code, B, T, C, _ptr(gate), gate.stride(0), gate.stride(1), _ptr(x),
-            x.stride(0), x.stride(1), _ptr(h0), _ptr(lengths), _ptr(h), _ptr(last), _ptr(states),
-            _stream(dev))
-    _lib.check(st, "tp_gated_scan_fwd")
-    return h, last, states
+    head = _gated_scan_inputs(gate, x, h0, lengths)
+    return _gated_scan_run(*head, code, gate, x, h0, need_states, need_last)
 
 
 def gated_scan_bwd(states, dh, dh_last, gate, x, *, form: str = "decay", lengths=None,
@@ -1491,24 +1562,16 @@ def gated_scan_bwd(states, dh, dh_last, gate, x, *, form: str = "decay", lengths
     """Backward of :func:`gated_scan` from the gradients of h and h_last (either may be None) and
     the forward's states: (dgate, dx, dh0 | None)."""
     code = _gate_form(form)
-    dev, dtype, B, T, C, gate, x, _, lengths = _gated_scan_inputs(gate, x, None, lengths)
-    if states is None or states.shape != (B, -(-T // 64), C) or states.dtype != torch.float32:
+    head = _gated_scan_inputs(gate, x, None, lengths)
+    B, T, C = x.shape
+    if (states is None or states.shape != (B, -(-T // 64), C) or states.dtype != torch.float32
+            or states.device != head[0] or not states.is_contiguous()):
         raise ValueError("states must be the forward's [B, ceil(T / 64), C] float32 tensor")
-    if dh is not None and (dh.shape != x.shape or dh.dtype != x.dtype or dh.device != dev):
+    if dh is not None and (dh.shape != x.shape or dh.dtype != x.dtype or dh.device != head[0]):
         raise ValueError("dh must have the shape, dtype and device of x")
-    if dh_last is not None and (_f32(dh_last).shape != (B, C) or dh_last.device != dev):
+    if dh_last is not None and (_f32(dh_last).shape != (B, C) or dh_last.device != head[0]):
         raise ValueError(f"dh_last must be [{B}, {C}] on the inputs' device")
-    dh, dh_last = (t.contiguous() if t is not None else None for t in (dh, dh_last))
-    dgate = torch.empty((B, T, C), device=dev, dtype=x.dtype)
-    dx = torch.empty_like(dgate)
-    dh0 = torch.empty((B, C), device=dev, dtype=torch.float32) if need_dh0 else None
-    with torch.cuda.device(dev):
-        st = _lib.load().tp_gated_scan_bwd(
-            dtype, code, B, T, C, _ptr(gate), gate.stride(0), gate.stride(1), _ptr(x),
-            x.stride(0), x.stride(1), _ptr(lengths), _ptr(states), _ptr(dh), _ptr(dh_last),
-            _ptr(dgate), _ptr(dx), _ptr(dh0), _stream(dev))
-    _lib.check(st, "tp_gated_scan_bwd")
-    return dgate, dx, dh0
+    return _gated_scan_back(*head, code, states, dh, dh_last, gate, x, need_dh0)
 
 
 class GatedScanFunction(torch.autograd.Function):
@@ -1517,10 +1580,11 @@ class GatedScanFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, gate, x, h0, form: str, lengths):
         ctx.set_materialize_grads(False)
-        h, last, states = gated_scan_fwd(gate, x, h0, form=form, lengths=lengths,
-                                         need_states=True)
+        code = _gate_form(form)
+        dev, dtype, lengths = _gated_scan_inputs(gate, x, h0, lengths)
+        h, last, states = _gated_scan_run(dev, dtype, lengths, code, gate, x, h0, True, True)
         ctx.save_for_backward(gate, x, lengths, states)
-        ctx.form = form
+        ctx.how = (dev, dtype, code)
         return h, last
 
     @staticmethod
@@ -1529,10 +1593,11 @@ class GatedScanFunction(torch.autograd.Function):
         if dh is None and dh_last is None:
             return (None,) * 5
         gate, x, lengths, states = ctx.saved_tensors
-        dgate, dx, dh0 = gated_scan_bwd(states, dh, dh_last, gate, x, form=ctx.form,
-                                        lengths=lengths, need_dh0=ctx.needs_input_grad[2])
-        return (dgate if ctx.needs_input_grad[0] else None,
-                dx if ctx.needs_input_grad[1] else None, dh0, None, None)
+        dev, dtype, code = ctx.how
+        need = ctx.needs_input_grad
+        dgate, dx, dh0 = _gated_scan_back(dev, dtype, lengths, code, states, dh, dh_last, gate, x,
+                                          need[2])
+        return dgate if need[0] else None, dx if need[1] else None, dh0, None, None
 
 
 def gated_scan(gate: torch.Tensor, x: torch.Tensor, h0: Optional[torch.Tensor] = None, *,
@@ -1578,12 +1643,9 @@ def gated_scan_step(gate: torch.Tensor, x: torch.Tensor, state: torch.Tensor, *,
         raise RuntimeError("gated_scan_step is not differentiable; use gated_scan, or call it "
                            "under torch.no_grad()")
     gate, x = _channels(gate), _channels(x)
-    h = torch.empty((B, C), device=dev, dtype=x.dtype)
-    with torch.cuda.device(dev):
-        st = _lib.load().tp_gated_scan_step(dtype, code, B, C, _ptr(gate), gate.stride(0), _ptr(x),
-                                            x.stride(0), _ptr(state), state.stride(0), _ptr(h),
-                                            _stream(dev))
-    _lib.check(st, "tp_gated_scan_step")
+    h = _empty_as(x)
+    _launch("tp_gated_scan_step", dev, dtype, code, B, C, gate.data_ptr(), gate.stride(0),
+            x.data_ptr(), x.stride(0), state.data_ptr(), state.stride(0), h.data_ptr())
     torch.autograd.graph.increment_version(state)
     return h
 
@@ -1620,15 +1682,14 @@ def embedding_fwd(ids, weight, scale: float = 1.0, *, pos_weight=None, positions
                 raise ValueError(f"{T} positions do not fit a table of {p.shape[0]}")
         else:
             _index_bits(positions, "positions")
-            positions = positions.expand(ids.shape).to(ids.dtype).contiguous()
-    flat = ids.contiguous()
+            if positions.shape != ids.shape:
+                positions = positions.expand(ids.shape)
+            positions = _contiguous(positions.to(ids.dtype))
+    flat = _contiguous(ids)
     out = torch.empty((*ids.shape, D), device=dev, dtype=w.dtype)
-    with torch.cuda.device(dev):
-        st = _lib.load().tp_embedding_fwd(
-            dtype, bits, flat.numel(), T, D, _ptr(flat), _ptr(w), V, w.stride(0), float(scale),
-            _ptr(p), p.shape[0] if p is not None else 0, p.stride(0) if p is not None else 0,
-            _ptr(positions), _ptr(out), _stream(dev))
-    _lib.check(st, "tp_embedding_fwd")
+    _launch("tp_embedding_fwd", dev, dtype, bits, flat.numel(), T, D, flat.data_ptr(),
+            w.data_ptr(), V, w.stride(0), float(scale), _at(p), p.shape[0] if p is not None else 0,
+            p.stride(0) if p is not None else 0, _at(positions), out.data_ptr())
     return out
 
 
@@ -1643,19 +1704,16 @@ def embedding_bwd(ids, dout, rows: int, scale: float = 1.0, *,
         raise ValueError(f"dout must be [*ids.shape, D], got {tuple(dout.shape)} for ids "
                          f"{tuple(ids.shape)}")
     D, N = dout.shape[-1], ids.numel()
-    ids, dout = ids.contiguous(), dout.contiguous()
+    ids, dout = _contiguous(ids), _contiguous(dout)
     dw = torch.empty((rows, D), device=dev, dtype=dout.dtype)
-    lib = _lib.load()
-    with torch.cuda.device(dev):
-        need = lib.tp_embedding_bwd_workspace_bytes(N, rows, D)
-        if need < 0:
-            raise ValueError(f"embedding_bwd takes fewer than 2^31 tokens and rows, got {N} and "
-                             f"{rows}")
-        ws = torch.empty(max(need, 16), device=dev, dtype=torch.uint8)
-        st = lib.tp_embedding_bwd(dtype, bits, N, D, _ptr(ids), _ptr(dout), rows, float(scale),
-                                  -1 if padding_idx is None else int(padding_idx), _ptr(dw),
-                                  _ptr(ws), ws.numel(), _stream(dev))
-    _lib.check(st, "tp_embedding_bwd")
+    with _on(dev):
+        need = _lib.load().tp_embedding_bwd_workspace_bytes(N, rows, D)
+    if need < 0:
+        raise ValueError(f"embedding_bwd takes fewer than 2^31 tokens and rows, got {N} and {rows}")
+    ws = torch.empty(max(need, 16), device=dev, dtype=torch.uint8)
+    _launch("tp_embedding_bwd", dev, dtype, bits, N, D, ids.data_ptr(), dout.data_ptr(), rows,
+            float(scale), -1 if padding_idx is None else padding_idx, dw.data_ptr(), ws.data_ptr(),
+            ws.numel())
     return dw
 
 
@@ -1665,13 +1723,10 @@ def embedding_pos_bwd(dout: torch.Tensor, rows: int) -> torch.Tensor:
     dtype = _floating(dout, "dout")
     D = dout.shape[-1]
     T = dout.shape[-2] if dout.dim() > 1 else 1
-    dout = dout.contiguous()
+    dout = _contiguous(dout)
     dp = torch.empty((rows, D), device=dev, dtype=dout.dtype)
     N = dout.numel() // D if D else 0
-    with torch.cuda.device(dev):
-        st = _lib.load().tp_embedding_pos_bwd(dtype, N, T, D, _ptr(dout), rows, _ptr(dp),
-                                              _stream(dev))
-    _lib.check(st, "tp_embedding_pos_bwd")
+    _launch("tp_embedding_pos_bwd", dev, dtype, N, T, D, dout.data_ptr(), rows, dp.data_ptr())
     return dp
 
 
