@@ -9,21 +9,26 @@
 //
 // Steps compose: a run of steps maps h -> A h + H with A the product of its
 // gates and H its result from a zero state.  One warp owns 32 lanes of channels
-// (two bf16 channels per lane, so a row is 128 bytes either way) and L
-// consecutive steps, all in registers; the W warps of a block own consecutive
-// runs, and the S blocks of a thread-block cluster consecutive groups of those.
-// An iteration loads S * W * L steps, forms every warp's (A, H), exchanges them
-// through shared memory (between the cluster's blocks through distributed
-// shared memory, one cluster barrier), applies the runs in order to the carried
-// state, and runs each warp's steps again from its own starting state.  So the
-// inputs are read once, the order of every operation is fixed (the same bits
-// on each call), and few channels still spread over many SMs.
+// (two per lane where the layout allows: 128 or 256 bytes a row, and packed
+// fp32 pairs in the arithmetic) and L consecutive steps; the W warps of a block
+// own consecutive runs, and the S blocks of a thread-block cluster consecutive
+// groups of those.  An iteration of S * W * L steps forms every warp's (A, H),
+// exchanges them through shared memory (between the cluster's blocks through
+// distributed shared memory, one cluster barrier), applies the runs in order to
+// the carried state, and runs each warp's steps again from its own starting
+// state.  So the inputs are read once, the order of every operation is fixed
+// (the same bits on each call), and few channels still spread over many SMs.
+// The inputs of the next iterations are on their way meanwhile: each thread
+// copies its own elements asynchronously into shared memory, one or two
+// iterations ahead, and reads only those, so the copies need no barrier.
 //
 // The backward walks the iterations from the end with the mirrored recurrence
 //   g_t = dh_t + c_{t+1},  c_t = a_t g_t   (c_t: gradient of h_{t-1})
 // and forms da_t = g_t h_{t-1} from states it recomputes in fp32: the forward
 // keeps one state per 64 steps.  It reads gate, x and dh once and writes dgate
 // and dx: like the forward it is bound by memory.
+#include <initializer_list>
+
 #include "maxplus_internal.cuh"
 #include "rowvec.cuh"
 
@@ -31,7 +36,13 @@ namespace tp {
 
 namespace {
 
-constexpr int GS_MAX_CLUSTER = 8;
+#ifndef GS_MINB
+#define GS_MINB 2
+#endif
+#ifndef GS_WANT
+#define GS_WANT 1.0
+#endif
+constexpr int GS_MAX_CLUSTER = 16;
 
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -39,369 +50,551 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   return r;
 }
 
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile(
-      "barrier.cluster.arrive.release.aligned;\n\t"
-      "barrier.cluster.wait.acquire.aligned;" ::
-          : "memory");
+__device__ __forceinline__ void cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// store a pair into the same shared-memory place of the cluster's block `rank`
-__device__ __forceinline__ void store_remote(float2* local, uint32_t rank, float2 v) {
-  uint32_t dst;
+// One or two channels of a lane.
+template <int CPL>
+struct Lane;
+template <>
+struct Lane<1> {
+  float v;
+  __device__ __forceinline__ static Lane all(float f) { return {f}; }
+  __device__ __forceinline__ float at(int) const { return v; }
+  __device__ __forceinline__ void put(int, float f) { v = f; }
+};
+template <>
+struct Lane<2> {
+  float2 v;
+  __device__ __forceinline__ static Lane all(float f) { return {make_float2(f, f)}; }
+  __device__ __forceinline__ float at(int k) const { return k ? v.y : v.x; }
+  __device__ __forceinline__ void put(int k, float f) { (k ? v.y : v.x) = f; }
+};
+// (rounded one by one: the compiler may not join a product and a sum into one
+// rounding for one channel per lane and not for two)
+__device__ __forceinline__ Lane<1> fma_(Lane<1> a, Lane<1> b, Lane<1> c) {
+  return {fmaf(a.v, b.v, c.v)};
+}
+__device__ __forceinline__ Lane<2> fma_(Lane<2> a, Lane<2> b, Lane<2> c) {
+  return {tp_fma2(a.v, b.v, c.v)};
+}
+__device__ __forceinline__ Lane<1> mul_(Lane<1> a, Lane<1> b) { return {__fmul_rn(a.v, b.v)}; }
+__device__ __forceinline__ Lane<2> mul_(Lane<2> a, Lane<2> b) { return {tp_mul2(a.v, b.v)}; }
+__device__ __forceinline__ Lane<1> add_(Lane<1> a, Lane<1> b) { return {__fadd_rn(a.v, b.v)}; }
+__device__ __forceinline__ Lane<2> add_(Lane<2> a, Lane<2> b) { return {tp_add2(a.v, b.v)}; }
+
+// The run (A, H) of a block, sent into the same shared-memory place of the
+// cluster's block `rank`; the bytes count on that block's barrier, so the
+// receiver needs no fence, and the sender does not wait for its global stores
+// as a cluster barrier's release would.
+template <int CPL>
+struct __align__(8 * CPL) Run {
+  Lane<CPL> a, h;
+};
+__device__ __forceinline__ uint32_t at_rank(const void* p, uint32_t rank) {
+  uint32_t r;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
-               : "=r"(dst)
-               : "r"(tp_smem_addr(local)), "r"(rank));
-  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(dst), "f"(v.x), "f"(v.y)
-               : "memory");
+               : "=r"(r)
+               : "r"(tp_smem_addr(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void send_run(Run<1>* to, uint64_t* bar, uint32_t rank, Run<1> r) {
+  asm volatile(
+      "st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::
+          "r"(at_rank(to, rank)), "f"(r.a.v), "f"(r.h.v), "r"(at_rank(bar, rank))
+      : "memory");
+}
+__device__ __forceinline__ void send_run(Run<2>* to, uint64_t* bar, uint32_t rank, Run<2> r) {
+  asm volatile(
+      "st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 "
+      "[%0], {%1, %2, %3, %4}, [%5];" ::"r"(at_rank(to, rank)),
+      "f"(r.a.v.x), "f"(r.a.v.y), "f"(r.h.v.x), "f"(r.h.v.y), "r"(at_rank(bar, rank))
+      : "memory");
 }
 
-// A h + H; a zero state stays H where the product of many gates overflowed
-__device__ __forceinline__ float apply_run(float A, float H, float h) {
-  return h == 0.0f ? H : fmaf(A, h, H);
+// CPL channels in storage, as one word of shared memory or a register
+template <typename T, int CPL>
+__device__ __forceinline__ Lane<CPL> unpack(const RowVec<T, CPL>& r) {
+  float f[CPL];
+  r.get(f);
+  Lane<CPL> l;
+#pragma unroll
+  for (int k = 0; k < CPL; ++k) l.put(k, f[k]);
+  return l;
+}
+template <typename T, int CPL>
+__device__ __forceinline__ void store_lane(T* p, Lane<CPL> l) {
+  float f[CPL];
+#pragma unroll
+  for (int k = 0; k < CPL; ++k) f[k] = l.at(k);
+  RowVec<T, CPL> r;
+  r.set(f);
+  r.store_stream(p);
 }
 
-// gate and input as the recurrence's a and u (and 1 - a in the sigmoid form)
-template <int FORM>
-__device__ __forceinline__ void gate_of(float z, float x, float& a, float& rest, float& u) {
+// Copies of a warp's n <= L rows of 32 CPL channels into shared memory
+// [L][32] of V.  WIDE: 16 bytes per lane, several rows per instruction (all rows
+// 16-byte aligned); else every lane its own channels, asynchronously where they
+// make at least four bytes.  The caller synchronises the warp around them.
+template <typename T, int CPL, int L, bool WIDE>
+struct Rows {
+  static constexpr int PER = 32 * CPL * (int)sizeof(T) / 16;   // 16-byte pieces of a row
+  // the element of the row at which this lane's copies begin
+  __device__ __forceinline__ static int first_channel(int lane) {
+    return WIDE ? (lane % PER) * (16 / (int)sizeof(T)) : lane * CPL;
+  }
+  // p: this lane's element of the first row
+  __device__ __forceinline__ static void copy(RowVec<T, CPL>* s, const T* p, int64_t stride,
+                                              int n, int lane) {
+    if constexpr (WIDE) {
+      constexpr int ROWS = 32 / PER;      // rows per instruction
+      char* d = reinterpret_cast<char*>(s) + lane * 16;
+      const int r = lane / PER;
+      p += r * stride;
+#pragma unroll
+      for (int i = 0; i < L; i += ROWS) {
+        if (i + r < n)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(tp_smem_addr(d + i * PER * 16)),
+                       "l"(p)
+                       : "memory");
+        p += ROWS * stride;
+      }
+    } else {
+      s += lane;
+#pragma unroll
+      for (int i = 0; i < L; ++i) {
+        if (i < n) {
+          if constexpr (sizeof(T) * CPL == 8)
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(tp_smem_addr(s + i * 32)),
+                         "l"(p)
+                         : "memory");
+          else if constexpr (sizeof(T) * CPL == 4)
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(tp_smem_addr(s + i * 32)),
+                         "l"(p)
+                         : "memory");
+          else
+            s[i * 32].load_stream(p);
+        }
+        p += stride;
+      }
+    }
+  }
+};
+
+// A product of gates kept finite: gates above 1 may overflow it, and a zero
+// state must stay zero.  (A NaN gate is NaN in the run's result as well.)
+template <int CPL>
+__device__ __forceinline__ Lane<CPL> finite(Lane<CPL> a) {
+#pragma unroll
+  for (int k = 0; k < CPL; ++k)
+    a.put(k, fminf(fmaxf(a.at(k), -3.402823466e38f), 3.402823466e38f));
+  return a;
+}
+
+// Gate as the recurrence's a, and 1 - a in the sigmoid form.  bf16 storage: the
+// gate comes from 2^x with the argument rounded once, relative error about
+// (8 + 1.5 |z|) 2^-24, far below the 2^-9 of the stored result; fp32: to fp32
+// accuracy.
+template <typename T, int FORM>
+__device__ __forceinline__ void gate_of(float z, float& a, float& rest) {
   if constexpr (FORM == TP_GATE_SIGMOID) {
-    sigmoid_pair(z, a, rest);
-    u = rest * x;
+    if constexpr (sizeof(T) == 2) fast_sigmoid_pair(z, a, rest);
+    else sigmoid_pair(z, a, rest);
   } else {
     a = z;
     rest = 1.0f;
-    u = x;
+  }
+}
+template <typename T, int FORM, int CPL>
+__device__ __forceinline__ void gates_of(Lane<CPL> z, Lane<CPL>& a, Lane<CPL>& rest) {
+#pragma unroll
+  for (int k = 0; k < CPL; ++k) {
+    float p, q;
+    gate_of<T, FORM>(z.at(k), p, q);
+    a.put(k, p);
+    rest.put(k, q);
   }
 }
 
-struct Where {
+template <typename T, int CPL>
+struct Place {
   int64_t b, c;       // batch row, this lane's first channel
   bool in;            // the lane has channels
   int64_t len;        // live steps of the row
   int rank;           // block of the cluster
+  __device__ __forceinline__ Place(const GatedScanArgs& a, int S, int64_t tiles) {
+    const int64_t id = blockIdx.x / S;
+    rank = S > 1 ? (int)cluster_rank() : 0;
+    b = id / tiles;
+    c = (id - b * tiles) * (32 * CPL) + (threadIdx.x & 31) * CPL;
+    in = c < a.C;
+    len = a.T;
+    if (a.lengths) {
+      const int64_t n = a.lengths[b];
+      len = n < 0 ? 0 : (n < a.T ? n : a.T);
+    }
+  }
+  __device__ __forceinline__ Lane<CPL> load(const float* p, int64_t row, int64_t C) const {
+    Lane<CPL> l = Lane<CPL>::all(0.0f);
+    if (p != nullptr && in) {
+#pragma unroll
+      for (int k = 0; k < CPL; ++k) l.put(k, p[row * C + c + k]);
+    }
+    return l;
+  }
+  __device__ __forceinline__ void store(float* p, int64_t row, int64_t C, Lane<CPL> l) const {
+    if (p != nullptr && in) {
+#pragma unroll
+      for (int k = 0; k < CPL; ++k) p[row * C + c + k] = l.at(k);
+    }
+  }
 };
 
-template <int CPL>
-__device__ __forceinline__ Where place(const GatedScanArgs& a, int S, int64_t tiles) {
-  Where w;
-  const int64_t id = blockIdx.x / S;
-  w.rank = S > 1 ? (int)cluster_rank() : 0;
-  w.b = id / tiles;
-  w.c = (id - w.b * tiles) * (32 * CPL) + (threadIdx.x & 31) * CPL;
-  w.in = w.c < a.C;
-  w.len = a.T;
-  if (a.lengths) {
-    const int64_t n = a.lengths[w.b];
-    w.len = n < 0 ? 0 : (n < a.T ? n : a.T);
-  }
-  return w;
+// steps of [t0, t0 + L) below `end`
+template <int L>
+__device__ __forceinline__ int steps_below(int64_t end, int64_t t0) {
+  const int64_t n = end - t0;
+  return n <= 0 ? 0 : (n < L ? (int)n : L);
 }
 
-template <typename T, int CPL, int FORM, int L, int W>
-__global__ void __launch_bounds__(32 * W) gated_scan_fwd_kernel(const GatedScanArgs a,
-                                                                const int S,
-                                                                const int64_t tiles) {
+template <typename T, int CPL, int FORM, int L, int W, int STAGES, bool WIDE>
+__global__ void __launch_bounds__(32 * W, GS_MINB)
+    gated_scan_fwd_kernel(const GatedScanArgs a, const int S, const int64_t tiles, int* err) {
   using V = RowVec<T, CPL>;
-  __shared__ float2 s_run[2][W][32 * CPL];
-  __shared__ float2 s_blk[2][GS_MAX_CLUSTER][32 * CPL];
+  using N = Lane<CPL>;
+  extern __shared__ __align__(16) unsigned char s_raw[];   // [STAGES][2][W][L][32] of V
+  __shared__ N s_a[2][W][32], s_h[2][W][32];               // runs of the warps
+  V* const raw = reinterpret_cast<V*>(s_raw);
+  // runs of the cluster's blocks: [2][S][32], filled by the blocks themselves
+  Run<CPL>* const s_blk = reinterpret_cast<Run<CPL>*>(raw + STAGES * 2 * L * 32 * W);
+  __shared__ uint64_t s_bar[2];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const Where w = place<CPL>(a, S, tiles);
-  const T* gp = (const T*)a.gate + w.b * a.gate_sb + w.c;
-  const T* xp = (const T*)a.x + w.b * a.x_sb + w.c;
-  T* hp = (T*)a.h + (w.b * a.T) * a.C + w.c;
+  const Place<T, CPL> w(a, S, tiles);
+  T* const hp = (T*)a.h + (w.b * a.T) * a.C + w.c;
   const int64_t chunks = ceil_div(a.T, (int64_t)GATED_SCAN_CHUNK);
   const int64_t step = (int64_t)S * W * L;
   const int64_t iters = ceil_div(a.T, step);
-  float carry[CPL];
-#pragma unroll
-  for (int k = 0; k < CPL; ++k) carry[k] = (a.h0 && w.in) ? a.h0[w.b * a.C + w.c + k] : 0.0f;
+  const int64_t mine0 = ((int64_t)w.rank * W + warp) * L;
+  N carry = w.load(a.h0, w.b, a.C);
 
-  V vg[L], vx[L];
-  auto fetch = [&](int64_t t0) {
-#pragma unroll
-    for (int i = 0; i < L; ++i) {
-      if (w.in && t0 + i < w.len) {
-        vg[i].load_stream(gp + (t0 + i) * a.gate_st);
-        vx[i].load_stream(xp + (t0 + i) * a.x_st);
-      }
+  using R = Rows<T, CPL, L, WIDE>;
+  const int64_t c0 = w.c - lane * CPL + R::first_channel(lane);   // this lane copies from here
+  const T* const gf = (const T*)a.gate + w.b * a.gate_sb + c0;
+  const T* const xf = (const T*)a.x + w.b * a.x_sb + c0;
+  const bool copies = c0 < a.C;
+  auto fetch = [&](int64_t it) {
+    if (it < iters && copies) {
+      const int64_t t0 = it * step + mine0;
+      const int n = steps_below<L>(w.len, t0);
+      V* s = raw + ((it % STAGES) * (2 * W) + warp) * (L * 32);
+      R::copy(s, gf + t0 * a.gate_st, a.gate_st, n, lane);
+      R::copy(s + W * L * 32, xf + t0 * a.x_st, a.x_st, n, lane);
     }
+    tp_cp_async_commit();
   };
-  if (S > 1) cluster_sync();   // every block of the cluster runs before the first remote store
-  fetch(((int64_t)w.rank * W + warp) * L);
+#pragma unroll
+  for (int k = 0; k < STAGES - 1; ++k) fetch(k);
+  if (S > 1) {     // every block of the cluster has its barriers before the first run is sent
+    if (threadIdx.x == 0) {
+      tp_mbar_init(&s_bar[0], 1);
+      tp_mbar_init(&s_bar[1], 1);
+      tp_fence_mbar_init();
+    }
+    cluster_arrive();
+    cluster_wait();
+  }
+  bool ok = true;
   for (int64_t it = 0; it < iters; ++it) {
+    __syncwarp();          // the warp has read the stage that is filled now
+    fetch(it + STAGES - 1);
     const int par = (int)(it & 1);
-    const int64_t t0 = it * step + ((int64_t)w.rank * W + warp) * L;
-    float A[L][CPL], U[L][CPL];
-    float pa[CPL], ph[CPL];
+    const int64_t t0 = it * step + mine0;
+    const int n = steps_below<L>(w.len, t0);
+    tp_cp_async_wait<STAGES - 1>();
+    __syncwarp();          // and every lane's copies of this stage are there
+    const V* s = raw + ((it % STAGES) * (2 * W) + warp) * (L * 32) + lane;
+    N A[L], U[L];
+    N pa = N::all(1.0f), ph = N::all(0.0f);
 #pragma unroll
-    for (int k = 0; k < CPL; ++k) {
-      pa[k] = 1.0f;
-      ph[k] = 0.0f;
+    for (int i = 0; i < L; ++i) {
+      N rest;
+      gates_of<T, FORM>(unpack<T, CPL>(s[i * 32]), A[i], rest);
+      U[i] = unpack<T, CPL>(s[(W * L + i) * 32]);
+      if constexpr (FORM == TP_GATE_SIGMOID) U[i] = mul_(rest, U[i]);
+    }
+    if (n < L) {          // past the end the state stays
+#pragma unroll
+      for (int i = 0; i < L; ++i)
+        if (i >= n) {
+          A[i] = N::all(1.0f);
+          U[i] = N::all(0.0f);
+        }
     }
 #pragma unroll
     for (int i = 0; i < L; ++i) {
-      float z[CPL], x[CPL], rest;
-      vg[i].get(z);
-      vx[i].get(x);
-      const bool live = w.in && t0 + i < w.len;
-#pragma unroll
-      for (int k = 0; k < CPL; ++k) {
-        gate_of<FORM>(z[k], x[k], A[i][k], rest, U[i][k]);
-        if (!live) {            // past the end the state stays
-          A[i][k] = 1.0f;
-          U[i][k] = 0.0f;
-        }
-        ph[k] = fmaf(A[i][k], ph[k], U[i][k]);
-        pa[k] *= A[i][k];
-      }
+      ph = fma_(A[i], ph, U[i]);
+      pa = mul_(pa, A[i]);
     }
-    if (it + 1 < iters) fetch(t0 + step);
-#pragma unroll
-    for (int k = 0; k < CPL; ++k) s_run[par][warp][lane * CPL + k] = make_float2(pa[k], ph[k]);
+    s_a[par][warp][lane] = finite(pa);
+    s_h[par][warp][lane] = ph;
     __syncthreads();
-    float mine[CPL];
+    N mine;
     if (S == 1) {
+      N h = carry;
+      mine = h;
 #pragma unroll
-      for (int k = 0; k < CPL; ++k) {
-        float h = carry[k];
-#pragma unroll
-        for (int q = 0; q < W; ++q) {
-          if (q == warp) mine[k] = h;
-          const float2 r = s_run[par][q][lane * CPL + k];
-          h = apply_run(r.x, r.y, h);
-        }
-        carry[k] = h;
+      for (int q = 0; q < W; ++q) {
+        if (q == warp) mine = h;
+        h = fma_(s_a[par][q][lane], h, s_h[par][q][lane]);
       }
+      carry = h;
     } else {
-      if (warp == 0) {
+      // the runs before this warp's, composed; the last warp has the block's
+      N qa = N::all(1.0f), qh = N::all(0.0f);
 #pragma unroll
-        for (int k = 0; k < CPL; ++k) {
-          float2 r = s_run[par][0][lane * CPL + k];
-#pragma unroll
-          for (int q = 1; q < W; ++q) {
-            const float2 n = s_run[par][q][lane * CPL + k];
-            r.y = apply_run(n.x, n.y, r.y);
-            r.x *= n.x;
+      for (int q = 0; q < W; ++q) {
+        if (q < warp || warp == W - 1) {
+          const N na = s_a[par][q][lane];
+          if (q == warp) {
+            mine = qh;     // (last warp: keep the composition up to itself)
+            pa = qa;
           }
-          for (int q = 0; q < S; ++q) store_remote(&s_blk[par][w.rank][lane * CPL + k], q, r);
+          qh = fma_(na, qh, s_h[par][q][lane]);
+          qa = mul_(qa, na);
         }
       }
-      cluster_sync();
-#pragma unroll
-      for (int k = 0; k < CPL; ++k) {
-        float h = carry[k], start = 0.0f;
-        for (int q = 0; q < S; ++q) {
-          if (q == w.rank) start = h;
-          const float2 r = s_blk[par][q][lane * CPL + k];
-          h = apply_run(r.x, r.y, h);
-        }
-        carry[k] = h;
-        for (int q = 0; q < warp; ++q) {
-          const float2 r = s_run[par][q][lane * CPL + k];
-          start = apply_run(r.x, r.y, start);
-        }
-        mine[k] = start;
+      if (warp == W - 1) {
+        const Run<CPL> r = {finite(qa), qh};
+        for (int q = 0; q < S; ++q)
+          send_run(s_blk + (par * S + w.rank) * 32 + lane, &s_bar[par], q, r);
+        if (lane == 0) tp_mbar_arrive_expect_tx(&s_bar[par], S * 32 * (int)sizeof(Run<CPL>));
+        qa = pa;
+        qh = mine;
       }
+      // (a wait that runs out is recorded; the blocks stay in step and finish)
+      ok = ok && tp_mbar_wait(&s_bar[par], (unsigned)(it >> 1) & 1u, err);
+      N h = carry, start = carry;
+      for (int q = 0; q < S; ++q) {
+        if (q == w.rank) start = h;
+        const Run<CPL> r = s_blk[(par * S + q) * 32 + lane];
+        h = fma_(r.a, h, r.h);
+      }
+      carry = h;
+      mine = fma_(finite(qa), start, qh);
     }
-    if (a.states && w.in && t0 < a.T && (t0 % GATED_SCAN_CHUNK) == 0) {
-#pragma unroll
-      for (int k = 0; k < CPL; ++k)
-        a.states[(w.b * chunks + t0 / GATED_SCAN_CHUNK) * a.C + w.c + k] = mine[k];
-    }
-#pragma unroll
-    for (int i = 0; i < L; ++i) {
-      float o[CPL];
-#pragma unroll
-      for (int k = 0; k < CPL; ++k) {
-        mine[k] = fmaf(A[i][k], mine[k], U[i][k]);
-        o[k] = t0 + i < w.len ? mine[k] : 0.0f;
-      }
-      if (w.in && t0 + i < a.T) {
-        V v;
-        v.set(o);
-        v.store_stream(hp + (t0 + i) * a.C);
-      }
-    }
-  }
-  if (a.h_last && w.rank == 0 && warp == 0 && w.in) {
-#pragma unroll
-    for (int k = 0; k < CPL; ++k) a.h_last[w.b * a.C + w.c + k] = carry[k];
-  }
-}
-
-template <typename T, int CPL, int FORM, int L, int W>
-__global__ void __launch_bounds__(32 * W) gated_scan_bwd_kernel(const GatedScanBwdArgs g,
-                                                                const int S,
-                                                                const int64_t tiles) {
-  static_assert(GATED_SCAN_CHUNK % L == 0 && (W * L) % GATED_SCAN_CHUNK == 0, "");
-  using V = RowVec<T, CPL>;
-  const GatedScanArgs& a = g.f;
-  __shared__ float2 s_run[2][W][32 * CPL];   // product of the gates, H forwards
-  __shared__ float s_rev[2][W][32 * CPL];    // result of the run backwards
-  __shared__ float2 s_blk[2][GS_MAX_CLUSTER][32 * CPL];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const Where w = place<CPL>(a, S, tiles);
-  const T* gp = (const T*)a.gate + w.b * a.gate_sb + w.c;
-  const T* xp = (const T*)a.x + w.b * a.x_sb + w.c;
-  const T* dp = g.dh ? (const T*)g.dh + (w.b * a.T) * a.C + w.c : nullptr;
-  T* dgp = (T*)g.dgate + (w.b * a.T) * a.C + w.c;
-  T* dxp = (T*)g.dx + (w.b * a.T) * a.C + w.c;
-  const int64_t chunks = ceil_div(a.T, (int64_t)GATED_SCAN_CHUNK);
-  const int64_t step = (int64_t)S * W * L;
-  const int64_t iters = ceil_div(a.T, step);
-  float carry[CPL];
-#pragma unroll
-  for (int k = 0; k < CPL; ++k)
-    carry[k] = (g.dh_last && w.in) ? g.dh_last[w.b * a.C + w.c + k] : 0.0f;
-
-  V vg[L], vx[L], vd[L];
-  float first[CPL];
-  auto fetch = [&](int64_t t0) {
-#pragma unroll
-    for (int i = 0; i < L; ++i) {
-      if (w.in && t0 + i < w.len) {
-        vg[i].load_stream(gp + (t0 + i) * a.gate_st);
-        vx[i].load_stream(xp + (t0 + i) * a.x_st);
-        if (dp) vd[i].load_stream(dp + (t0 + i) * a.C);
-        else vd[i].zero();
-      }
-    }
-  };
-  if (S > 1) cluster_sync();   // every block of the cluster runs before the first remote store
-  for (int64_t it = iters - 1; it >= 0; --it) {
-    const int par = (int)(it & 1);
-    const int64_t tb = it * step + (int64_t)w.rank * W * L;   // the block's first step
-    const int64_t t0 = tb + warp * L;
-    fetch(t0);
-    // the state before this warp's 64-step chunk, and the chunk's first warp
-    const int64_t chunk = t0 / GATED_SCAN_CHUNK;
-    const int lead = warp - (int)((t0 % GATED_SCAN_CHUNK) / L);
-#pragma unroll
-    for (int k = 0; k < CPL; ++k)
-      first[k] = (w.in && t0 < w.len) ? a.states[(w.b * chunks + chunk) * a.C + w.c + k] : 0.0f;
-    float A[L][CPL], R[L][CPL], U[L][CPL], D[L][CPL];
-    float pa[CPL], ph[CPL], pr[CPL];
-#pragma unroll
-    for (int k = 0; k < CPL; ++k) {
-      pa[k] = 1.0f;
-      ph[k] = pr[k] = 0.0f;
-    }
-#pragma unroll
-    for (int i = 0; i < L; ++i) {
-      float z[CPL], x[CPL];
-      vg[i].get(z);
-      vx[i].get(x);
-      vd[i].get(D[i]);
-      const bool live = w.in && t0 + i < w.len;
-#pragma unroll
-      for (int k = 0; k < CPL; ++k) {
-        gate_of<FORM>(z[k], x[k], A[i][k], R[i][k], U[i][k]);
-        if (!live) {
-          A[i][k] = 1.0f;
-          U[i][k] = 0.0f;
-          D[i][k] = 0.0f;
-        }
-        ph[k] = fmaf(A[i][k], ph[k], U[i][k]);
-        pa[k] *= A[i][k];
-      }
-    }
-#pragma unroll
-    for (int i = L - 1; i >= 0; --i)
-#pragma unroll
-      for (int k = 0; k < CPL; ++k) pr[k] = A[i][k] * (D[i][k] + pr[k]);
-#pragma unroll
-    for (int k = 0; k < CPL; ++k) {
-      s_run[par][warp][lane * CPL + k] = make_float2(pa[k], ph[k]);
-      s_rev[par][warp][lane * CPL + k] = pr[k];
-    }
-    __syncthreads();
-    float mine[CPL];
-    if (S == 1) {
-#pragma unroll
-      for (int k = 0; k < CPL; ++k) {
-        float c = carry[k];
-#pragma unroll
-        for (int q = W - 1; q >= 0; --q) {
-          if (q == warp) mine[k] = c;
-          c = apply_run(s_run[par][q][lane * CPL + k].x, s_rev[par][q][lane * CPL + k], c);
-        }
-        carry[k] = c;
-      }
-    } else {
-      if (warp == 0) {
-#pragma unroll
-        for (int k = 0; k < CPL; ++k) {
-          float2 r = make_float2(s_run[par][W - 1][lane * CPL + k].x,
-                                 s_rev[par][W - 1][lane * CPL + k]);
-#pragma unroll
-          for (int q = W - 2; q >= 0; --q) {
-            const float n = s_run[par][q][lane * CPL + k].x;
-            r.y = apply_run(n, s_rev[par][q][lane * CPL + k], r.y);
-            r.x *= n;
-          }
-          for (int q = 0; q < S; ++q) store_remote(&s_blk[par][w.rank][lane * CPL + k], q, r);
-        }
-      }
-      cluster_sync();
-#pragma unroll
-      for (int k = 0; k < CPL; ++k) {
-        float c = carry[k], start = 0.0f;
-        for (int q = S - 1; q >= 0; --q) {
-          if (q == w.rank) start = c;
-          const float2 r = s_blk[par][q][lane * CPL + k];
-          c = apply_run(r.x, r.y, c);
-        }
-        carry[k] = c;
-        for (int q = W - 1; q > warp; --q)
-          start = apply_run(s_run[par][q][lane * CPL + k].x, s_rev[par][q][lane * CPL + k],
-                            start);
-        mine[k] = start;
-      }
-    }
-    float before[L][CPL];      // h_{t-1}
-#pragma unroll
-    for (int k = 0; k < CPL; ++k) {
-      float h = first[k];
-      for (int q = lead; q < warp; ++q) {
-        const float2 r = s_run[par][q][lane * CPL + k];
-        h = apply_run(r.x, r.y, h);
-      }
+    if (a.states && t0 < a.T && (t0 % GATED_SCAN_CHUNK) == 0)
+      w.store(a.states, w.b * chunks + t0 / GATED_SCAN_CHUNK, a.C, mine);
+    T* o = hp + t0 * a.C;
+    const int m = steps_below<L>(a.T, t0);
+    if (n == L) {
 #pragma unroll
       for (int i = 0; i < L; ++i) {
-        before[i][k] = h;
-        h = fmaf(A[i][k], h, U[i][k]);
+        mine = fma_(A[i], mine, U[i]);
+        if (w.in) store_lane<T, CPL>(o, mine);
+        o += a.C;
       }
-    }
+    } else {
 #pragma unroll
-    for (int i = L - 1; i >= 0; --i) {
-      float oz[CPL], ox[CPL];
-      const bool live = t0 + i < w.len;
-#pragma unroll
-      for (int k = 0; k < CPL; ++k) {
-        const float gr = D[i][k] + mine[k];
-        mine[k] = A[i][k] * gr;
-        if constexpr (FORM == TP_GATE_SIGMOID) {
-          // d(f h + (1 - f) x)/dz = f (1 - f) (h - x) = f ((1 - f) h - u)
-          oz[k] = gr * (A[i][k] * fmaf(R[i][k], before[i][k], -U[i][k]));
-          ox[k] = gr * R[i][k];
-        } else {
-          oz[k] = gr * before[i][k];
-          ox[k] = gr;
-        }
-        if (!live) oz[k] = ox[k] = 0.0f;
-      }
-      if (w.in && t0 + i < a.T) {
-        V v;
-        v.set(oz);
-        v.store_stream(dgp + (t0 + i) * a.C);
-        v.set(ox);
-        v.store_stream(dxp + (t0 + i) * a.C);
+      for (int i = 0; i < L; ++i) {
+        mine = fma_(A[i], mine, U[i]);
+        if (w.in && i < m) store_lane<T, CPL>(o, i < n ? mine : N::all(0.0f));
+        o += a.C;
       }
     }
   }
-  if (g.dh0 && w.rank == 0 && warp == 0 && w.in) {
+  if (w.rank == 0 && warp == 0) w.store(a.h_last, w.b, a.C, carry);
+  if (S > 1) {     // no block leaves while another may still send to it
+    cluster_arrive();
+    cluster_wait();
+  }
+}
+
+template <typename T, int CPL, int FORM, int L, int W, int STAGES, bool WIDE>
+__global__ void __launch_bounds__(32 * W, GS_MINB)
+    gated_scan_bwd_kernel(const GatedScanBwdArgs g, const int S, const int64_t tiles, int* err) {
+  static_assert(GATED_SCAN_CHUNK % L == 0 && (W * L) % GATED_SCAN_CHUNK == 0, "");
+  using V = RowVec<T, CPL>;
+  using N = Lane<CPL>;
+  const GatedScanArgs& a = g.f;
+  extern __shared__ __align__(16) unsigned char s_raw[];   // [STAGES][3][W][L][32] of V
+  __shared__ N s_a[2][W][32], s_h[2][W][32], s_c[2][W][32];   // runs, forwards and backwards
+  V* const raw = reinterpret_cast<V*>(s_raw);
+  Run<CPL>* const s_blk = reinterpret_cast<Run<CPL>*>(raw + STAGES * 3 * L * 32 * W);
+  __shared__ uint64_t s_bar[2];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const Place<T, CPL> w(a, S, tiles);
+  T* const dgp = (T*)g.dgate + (w.b * a.T) * a.C + w.c;
+  T* const dxp = (T*)g.dx + (w.b * a.T) * a.C + w.c;
+  const int64_t chunks = ceil_div(a.T, (int64_t)GATED_SCAN_CHUNK);
+  const int64_t step = (int64_t)S * W * L;
+  const int64_t iters = ceil_div(a.T, step);
+  const int64_t mine0 = ((int64_t)w.rank * W + warp) * L;
+  // the first warp of this warp's 64-step chunk, whose starting state is kept
+  constexpr int WPC = GATED_SCAN_CHUNK / L;
+  const int lead = warp - warp % WPC;
+  N carry = w.load(g.dh_last, w.b, a.C);
+
+  using R = Rows<T, CPL, L, WIDE>;
+  const int64_t c0 = w.c - lane * CPL + R::first_channel(lane);
+  const T* const gf = (const T*)a.gate + w.b * a.gate_sb + c0;
+  const T* const xf = (const T*)a.x + w.b * a.x_sb + c0;
+  const T* const df = (const T*)g.dh + w.b * a.T * a.C + c0;
+  const bool copies = c0 < a.C, has_dh = g.dh != nullptr;
+  auto fetch = [&](int64_t it) {       // it counts from the end
+    if (it < iters && copies) {
+      const int64_t t0 = (iters - 1 - it) * step + mine0;
+      const int n = steps_below<L>(w.len, t0);
+      V* s = raw + ((it % STAGES) * (3 * W) + warp) * (L * 32);
+      R::copy(s, gf + t0 * a.gate_st, a.gate_st, n, lane);
+      R::copy(s + W * L * 32, xf + t0 * a.x_st, a.x_st, n, lane);
+      if (has_dh) R::copy(s + 2 * W * L * 32, df + t0 * a.C, a.C, n, lane);
+    }
+    tp_cp_async_commit();
+  };
+  auto first_state = [&](int64_t it) {
+    const int64_t t0 = (iters - 1 - it) * step + mine0;
+    if (it >= iters || t0 >= w.len) return N::all(0.0f);
+    return w.load(a.states, w.b * chunks + t0 / GATED_SCAN_CHUNK, a.C);
+  };
 #pragma unroll
-    for (int k = 0; k < CPL; ++k) g.dh0[w.b * a.C + w.c + k] = carry[k];
+  for (int k = 0; k < STAGES - 1; ++k) fetch(k);
+  N next = first_state(0);
+  if (S > 1) {     // every block of the cluster has its barriers before the first run is sent
+    if (threadIdx.x == 0) {
+      tp_mbar_init(&s_bar[0], 1);
+      tp_mbar_init(&s_bar[1], 1);
+      tp_fence_mbar_init();
+    }
+    cluster_arrive();
+    cluster_wait();
+  }
+  bool ok = true;
+  for (int64_t it = 0; it < iters; ++it) {
+    __syncwarp();
+    fetch(it + STAGES - 1);
+    const N first = next;
+    next = first_state(it + 1);
+    const int par = (int)(it & 1);
+    const int64_t t0 = (iters - 1 - it) * step + mine0;
+    const int n = steps_below<L>(w.len, t0);
+    tp_cp_async_wait<STAGES - 1>();
+    __syncwarp();
+    const V* s = raw + ((it % STAGES) * (3 * W) + warp) * (L * 32) + lane;
+    N A[L], O[L], U[L];      // gate, its complement, input
+    N pa = N::all(1.0f), ph = N::all(0.0f);
+    auto dh_at = [&](int i) {
+      return (has_dh && i < n) ? unpack<T, CPL>(s[(2 * W * L + i) * 32]) : N::all(0.0f);
+    };
+#pragma unroll
+    for (int i = 0; i < L; ++i) {
+      gates_of<T, FORM>(unpack<T, CPL>(s[i * 32]), A[i], O[i]);
+      U[i] = unpack<T, CPL>(s[(W * L + i) * 32]);
+      if constexpr (FORM == TP_GATE_SIGMOID) U[i] = mul_(O[i], U[i]);
+    }
+    if (n < L) {
+#pragma unroll
+      for (int i = 0; i < L; ++i)
+        if (i >= n) {
+          A[i] = N::all(1.0f);
+          U[i] = N::all(0.0f);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < L; ++i) {
+      ph = fma_(A[i], ph, U[i]);
+      pa = mul_(pa, A[i]);
+    }
+    N gr = dh_at(L - 1);      // g of the run alone
+#pragma unroll
+    for (int i = L - 2; i >= 0; --i) gr = fma_(A[i + 1], gr, dh_at(i));
+    s_a[par][warp][lane] = finite(pa);
+    s_h[par][warp][lane] = ph;
+    s_c[par][warp][lane] = mul_(A[0], gr);
+    __syncthreads();
+    N mine;
+    if (S == 1) {
+      N c = carry;
+      mine = c;
+#pragma unroll
+      for (int q = W - 1; q >= 0; --q) {
+        if (q == warp) mine = c;
+        c = fma_(s_a[par][q][lane], c, s_c[par][q][lane]);
+      }
+      carry = c;
+    } else {
+      // the runs after this warp's, composed; the first warp has the block's
+      N qa = N::all(1.0f), qc = N::all(0.0f);
+#pragma unroll
+      for (int q = W - 1; q >= 0; --q) {
+        if (q > warp || warp == 0) {
+          const N na = s_a[par][q][lane];
+          if (q == warp) {
+            mine = qc;
+            pa = qa;
+          }
+          qc = fma_(na, qc, s_c[par][q][lane]);
+          qa = mul_(qa, na);
+        }
+      }
+      if (warp == 0) {
+        const Run<CPL> r = {finite(qa), qc};
+        for (int q = 0; q < S; ++q)
+          send_run(s_blk + (par * S + w.rank) * 32 + lane, &s_bar[par], q, r);
+        if (lane == 0) tp_mbar_arrive_expect_tx(&s_bar[par], S * 32 * (int)sizeof(Run<CPL>));
+        qa = pa;
+        qc = mine;
+      }
+      ok = ok && tp_mbar_wait(&s_bar[par], (unsigned)(it >> 1) & 1u, err);
+      N c = carry, start = carry;
+      for (int q = S - 1; q >= 0; --q) {
+        if (q == w.rank) start = c;
+        const Run<CPL> r = s_blk[(par * S + q) * 32 + lane];
+        c = fma_(r.a, c, r.h);
+      }
+      carry = c;
+      mine = fma_(finite(qa), start, qc);
+    }
+    N before[L];      // h_{t-1}
+    {
+      N h = first;
+      for (int q = lead; q < warp; ++q) h = fma_(s_a[par][q][lane], h, s_h[par][q][lane]);
+#pragma unroll
+      for (int i = 0; i < L; ++i) {
+        before[i] = h;
+        h = fma_(A[i], h, U[i]);
+      }
+    }
+    T* oz = dgp + (t0 + L - 1) * a.C;
+    T* ox = dxp + (t0 + L - 1) * a.C;
+    const int m = steps_below<L>(a.T, t0);
+#pragma unroll
+    for (int i = L - 1; i >= 0; --i) {
+      gr = i == L - 1 ? add_(dh_at(i), mine) : fma_(A[i + 1 < L ? i + 1 : i], gr, dh_at(i));
+      N z, x;
+      if constexpr (FORM == TP_GATE_SIGMOID) {
+        // d(f h + (1 - f) x)/dz = f (1 - f) (h - x) = f ((1 - f) h - u)
+        z = mul_(mul_(A[i], gr), fma_(O[i], before[i], mul_(N::all(-1.0f), U[i])));
+        x = mul_(gr, O[i]);
+      } else {
+        z = mul_(gr, before[i]);
+        x = gr;
+      }
+      if (w.in && i < m) {
+        store_lane<T, CPL>(oz, i < n ? z : N::all(0.0f));
+        store_lane<T, CPL>(ox, i < n ? x : N::all(0.0f));
+      }
+      oz -= a.C;
+      ox -= a.C;
+    }
+  }
+  if (w.rank == 0 && warp == 0) w.store(g.dh0, w.b, a.C, carry);
+  if (S > 1) {     // no block leaves while another may still send to it
+    cluster_arrive();
+    cluster_wait();
   }
 }
 
@@ -422,7 +615,8 @@ __global__ void __launch_bounds__(256)
     vx.load(x + b * ldx + c);
     vz.get(&z);
     vx.get(&xv);
-    gate_of<FORM>(z, xv, a, rest, u);
+    gate_of<T, FORM>(z, a, rest);
+    u = FORM == TP_GATE_SIGMOID ? rest * xv : xv;
     const float hn = fmaf(a, state[b * lds + c], u);
     state[b * lds + c] = hn;
     vh.set(&hn);
@@ -430,21 +624,31 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// Blocks of a cluster: enough for two blocks per SM, no more than the steps fill.
-int cluster_size(int64_t blocks, int64_t T, int64_t steps_per_block) {
-  const int64_t want = 2 * (int64_t)num_sms();
+// Blocks of a cluster: enough for two blocks per SM, no more than the steps
+// fill.  It goes by the sizes alone, as L does by the type, so that the order of
+// operations, and with it the bits, do not depend on strides and alignment.
+int cluster_size(int64_t B, int64_t T, int64_t C, int64_t steps_per_block) {
+  const int64_t want = (int64_t)(GS_WANT * num_sms()), blocks = B * ceil_div(C, (int64_t)64);
   int S = 1;
   while (S < GS_MAX_CLUSTER && blocks * S < want && T > S * steps_per_block) S *= 2;
   return S;
 }
 
 template <typename K, typename A>
-int launch_clustered(K kernel, const A& args, int threads, int64_t B, int64_t tiles, int S,
-                     cudaStream_t stream) {
+int launch_clustered(K kernel, const A& args, int threads, size_t smem, size_t runs_bytes,
+                     int64_t B, int64_t tiles, int S, cudaStream_t stream) {
   if (B * tiles > INT32_MAX / GS_MAX_CLUSTER) return TP_ERR_TOO_LARGE;
+  if (S > 1) smem += (size_t)2 * S * runs_bytes;
+  cudaError_t e = cudaFuncSetAttribute((const void*)kernel,
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e == cudaSuccess && S > 8)
+    e = cudaFuncSetAttribute((const void*)kernel,
+                             cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e != cudaSuccess) return cuda_status(e);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(B * tiles * S));
   cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -453,33 +657,61 @@ int launch_clustered(K kernel, const A& args, int threads, int64_t B, int64_t ti
   at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = S > 1 ? 1 : 0;
-  return cuda_status(cudaLaunchKernelEx(&cfg, kernel, args, S, tiles));
+  int* err = device_error_ptr();
+  return cuda_status(cudaLaunchKernelEx(&cfg, kernel, args, S, tiles, err));
 }
 
-// two bf16 channels per lane: even channels at even strides, 4-byte aligned
-bool pairs_ok(const GatedScanArgs& a) {
-  auto al = [](const void* p) { return (((uintptr_t)p) & 3) == 0; };
-  return a.dtype == TP_DTYPE_BF16 && a.C % 2 == 0 && a.gate_sb % 2 == 0 && a.gate_st % 2 == 0 &&
-         a.x_sb % 2 == 0 && a.x_st % 2 == 0 && al(a.gate) && al(a.x) &&
-         (a.h == nullptr || al(a.h));
+// Whether rows, strides and bases are multiples of `bytes`.
+bool rows_at(const GatedScanArgs& a, std::initializer_list<const void*> more, int bytes) {
+  const uintptr_t m = bytes - 1;
+  for (const void* p : {a.gate, a.x})
+    if (((uintptr_t)p) & m) return false;
+  for (const void* p : more)
+    if (((uintptr_t)p) & m) return false;
+  const int64_t n = bytes / (a.dtype == TP_DTYPE_F32 ? 4 : 2);
+  return a.C % n == 0 && a.gate_sb % n == 0 && a.gate_st % n == 0 && a.x_sb % n == 0 &&
+         a.x_st % n == 0;
 }
 
-template <typename T, int CPL, int FORM>
+template <typename T, int CPL, int FORM, bool WIDE>
 int fwd(const GatedScanArgs& a, cudaStream_t stream) {
-  constexpr int L = 16, W = 8;
+#ifdef GS_FL
+  constexpr int L = GS_FL, W = GS_FW, STAGES = GS_FS;
+#else
+  constexpr int L = sizeof(T) == 4 ? 8 : 16, W = 8, STAGES = 3;
+#endif
   const int64_t tiles = ceil_div(a.C, (int64_t)(32 * CPL));
-  const int S = cluster_size(a.B * tiles, a.T, L * W);
-  return launch_clustered(gated_scan_fwd_kernel<T, CPL, FORM, L, W>, a, 32 * W, a.B, tiles, S,
-                          stream);
+  const int S = cluster_size(a.B, a.T, a.C, L * W);
+  return launch_clustered(gated_scan_fwd_kernel<T, CPL, FORM, L, W, STAGES, WIDE>, a, 32 * W,
+                          (size_t)STAGES * 2 * L * 32 * W * CPL * sizeof(T),
+                          32 * sizeof(Run<CPL>), a.B, tiles, S, stream);
 }
 
-template <typename T, int CPL, int FORM>
+template <typename T, int CPL, int FORM, bool WIDE>
 int bwd(const GatedScanBwdArgs& g, cudaStream_t stream) {
-  constexpr int L = 8, W = 8;
+#ifdef GS_BL
+  constexpr int L = GS_BL, W = GS_BW, STAGES = GS_BS;
+#else
+  constexpr int L = 8, W = 8, STAGES = sizeof(T) * CPL == 8 ? 2 : 3;
+#endif
   const int64_t tiles = ceil_div(g.f.C, (int64_t)(32 * CPL));
-  const int S = cluster_size(g.f.B * tiles, g.f.T, L * W);
-  return launch_clustered(gated_scan_bwd_kernel<T, CPL, FORM, L, W>, g, 32 * W, g.f.B, tiles, S,
-                          stream);
+  const int S = cluster_size(g.f.B, g.f.T, g.f.C, L * W);
+  return launch_clustered(gated_scan_bwd_kernel<T, CPL, FORM, L, W, STAGES, WIDE>, g, 32 * W,
+                          (size_t)STAGES * 3 * L * 32 * W * CPL * sizeof(T),
+                          32 * sizeof(Run<CPL>), g.f.B, tiles, S, stream);
+}
+
+// Two channels per lane and 16-byte copies where rows are 16-byte aligned, else
+// one channel per lane.
+template <typename T, int FORM>
+int fwd_any(const GatedScanArgs& a, cudaStream_t stream) {
+  if (rows_at(a, {a.h}, 16)) return fwd<T, 2, FORM, true>(a, stream);
+  return fwd<T, 1, FORM, false>(a, stream);
+}
+template <typename T, int FORM>
+int bwd_any(const GatedScanBwdArgs& g, cudaStream_t stream) {
+  if (rows_at(g.f, {g.dh, g.dgate, g.dx}, 16)) return bwd<T, 2, FORM, true>(g, stream);
+  return bwd<T, 1, FORM, false>(g, stream);
 }
 
 }  // namespace
@@ -487,26 +719,19 @@ int bwd(const GatedScanBwdArgs& g, cudaStream_t stream) {
 int launch_gated_scan_fwd(const GatedScanArgs& a, cudaStream_t stream) {
   const bool sig = a.form == TP_GATE_SIGMOID;
   if (a.dtype == TP_DTYPE_F32)
-    return sig ? fwd<float, 1, TP_GATE_SIGMOID>(a, stream)
-               : fwd<float, 1, TP_GATE_DECAY>(a, stream);
-  if (pairs_ok(a))
-    return sig ? fwd<bf16_t, 2, TP_GATE_SIGMOID>(a, stream)
-               : fwd<bf16_t, 2, TP_GATE_DECAY>(a, stream);
-  return sig ? fwd<bf16_t, 1, TP_GATE_SIGMOID>(a, stream)
-             : fwd<bf16_t, 1, TP_GATE_DECAY>(a, stream);
+    return sig ? fwd_any<float, TP_GATE_SIGMOID>(a, stream)
+               : fwd_any<float, TP_GATE_DECAY>(a, stream);
+  return sig ? fwd_any<bf16_t, TP_GATE_SIGMOID>(a, stream)
+             : fwd_any<bf16_t, TP_GATE_DECAY>(a, stream);
 }
 
 int launch_gated_scan_bwd(const GatedScanBwdArgs& g, cudaStream_t stream) {
   const bool sig = g.f.form == TP_GATE_SIGMOID;
   if (g.f.dtype == TP_DTYPE_F32)
-    return sig ? bwd<float, 1, TP_GATE_SIGMOID>(g, stream)
-               : bwd<float, 1, TP_GATE_DECAY>(g, stream);
-  auto al = [](const void* p) { return (((uintptr_t)p) & 3) == 0; };
-  if (pairs_ok(g.f) && al(g.dh) && al(g.dgate) && al(g.dx))
-    return sig ? bwd<bf16_t, 2, TP_GATE_SIGMOID>(g, stream)
-               : bwd<bf16_t, 2, TP_GATE_DECAY>(g, stream);
-  return sig ? bwd<bf16_t, 1, TP_GATE_SIGMOID>(g, stream)
-             : bwd<bf16_t, 1, TP_GATE_DECAY>(g, stream);
+    return sig ? bwd_any<float, TP_GATE_SIGMOID>(g, stream)
+               : bwd_any<float, TP_GATE_DECAY>(g, stream);
+  return sig ? bwd_any<bf16_t, TP_GATE_SIGMOID>(g, stream)
+             : bwd_any<bf16_t, TP_GATE_DECAY>(g, stream);
 }
 
 int launch_gated_scan_step(int dtype, int form, int64_t B, int64_t C, const void* gate,

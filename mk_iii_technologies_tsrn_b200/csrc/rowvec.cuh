@@ -46,6 +46,24 @@ struct RowVec<float, 4> {
 };
 
 template <>
+struct RowVec<float, 2> {
+  float2 r;
+  __device__ __forceinline__ void zero() { r = make_float2(0.f, 0.f); }
+  __device__ __forceinline__ void load(const float* p) {
+    r = __ldg(reinterpret_cast<const float2*>(p));
+  }
+  __device__ __forceinline__ void load_stream(const float* p) {
+    r = __ldcs(reinterpret_cast<const float2*>(p));
+  }
+  __device__ __forceinline__ void get(float* f) const { f[0] = r.x; f[1] = r.y; }
+  __device__ __forceinline__ void set(const float* f) { r = make_float2(f[0], f[1]); }
+  __device__ __forceinline__ void store(float* p) const { *reinterpret_cast<float2*>(p) = r; }
+  __device__ __forceinline__ void store_stream(float* p) const {
+    __stcs(reinterpret_cast<float2*>(p), r);
+  }
+};
+
+template <>
 struct RowVec<float, 1> {
   float r;
   __device__ __forceinline__ void zero() { r = 0.f; }
@@ -165,6 +183,20 @@ __device__ __forceinline__ void sigmoid_pair(float v, float& s, float& rest) {
   const float small = e * big;
   s = v >= 0.0f ? big : small;
   rest = v >= 0.0f ? small : big;
+}
+
+// The same for results that are rounded to bf16: e = exp(-v) as one power of
+// two.  Relative error about (8 + 1.5 |v|) 2^-24 (argument rounded once, 2^x to
+// 2^-22, 1 + e, reciprocal and product).  The exponent is held at 126, so that
+// sigmoid(-inf) is 2^-126 and its complement exactly 1.
+__device__ __forceinline__ void fast_sigmoid_pair(float v, float& s, float& rest) {
+  float t = v * -1.442695041f;
+  asm("min.NaN.f32 %0, %0, 0f42FC0000;" : "+f"(t));   // 126
+  const float e = tp_ex2(t);
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+  s = r;
+  rest = e * r;
 }
 
 }  // namespace tp
