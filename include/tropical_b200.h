@@ -367,10 +367,13 @@ TP_API int tp_residual_norm_bwd(int dtype, int params_dtype, int norm, int64_t r
  *  steps (clamped to 0 .. T); its h is zero behind the end and its h_last the
  *  state at the end; gate and x behind the end are not read.  states
  *  (tp_gated_scan_states_floats floats; NULL: not kept): one state per 64
- *  steps, for the backward.  Products of gates are formed over runs of up to
- *  1024 steps: meant for gates of magnitude at most 1, whose products cannot
+ *  steps, for the backward.  workspace (both directions):
+ *  tp_gated_scan_workspace_bytes(B, T, C) bytes, 0 unless few rows and channels
+ *  have to be cut in time to fill the GPU.  Products of gates are formed over
+ *  runs of steps: meant for gates of magnitude at most 1, whose products cannot
  *  overflow.  A non-finite state or input makes the later states of its
- *  channel non-finite.
+ *  channel non-finite.  The same sizes and values give the same bits, whatever
+ *  the strides.
  *
  *  Backward: from dh [B, T, C] (NULL: zeros) and dh_last [B, C] (NULL: zeros)
  *  writes dgate and dx ([B, T, C] contiguous, zero behind a row's end) and dh0
@@ -380,17 +383,19 @@ TP_API int tp_residual_norm_bwd(int dtype, int params_dtype, int norm, int64_t r
  *  fp32 state [B, C] at row stride lds (>= C) updated in place, h [B, C]
  *  contiguous.  No C counterpart in the reference.
  * ======================================================================== */
+TP_API int64_t tp_gated_scan_workspace_bytes(int64_t B, int64_t T, int64_t C);
 TP_API int64_t tp_gated_scan_states_floats(int64_t B, int64_t T, int64_t C);
 TP_API int tp_gated_scan_fwd(int dtype, int form, int64_t B, int64_t T, int64_t C,
                              const void* gate, int64_t gate_sb, int64_t gate_st, const void* x,
                              int64_t x_sb, int64_t x_st, const float* h0,
                              const int32_t* lengths, void* h, float* h_last, float* states,
-                             void* stream);
+                             void* workspace, int64_t workspace_bytes, void* stream);
 TP_API int tp_gated_scan_bwd(int dtype, int form, int64_t B, int64_t T, int64_t C,
                              const void* gate, int64_t gate_sb, int64_t gate_st, const void* x,
                              int64_t x_sb, int64_t x_st, const int32_t* lengths,
                              const float* states, const void* dh, const float* dh_last,
-                             void* dgate, void* dx, float* dh0, void* stream);
+                             void* dgate, void* dx, float* dh0, void* workspace,
+                             int64_t workspace_bytes, void* stream);
 TP_API int tp_gated_scan_step(int dtype, int form, int64_t B, int64_t C, const void* gate,
                               int64_t ldg, const void* x, int64_t ldx, float* state,
                               int64_t lds, void* h, void* stream);

@@ -159,16 +159,17 @@ SIGNATURES: dict[str, tuple] = {
          _c_int, _c_int, _c_p, _c_p, _c_p, _c_p, _c_f, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p,
          _c_p, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_p],
     ),
+    "tp_gated_scan_workspace_bytes": (_c_i64, [_c_i64, _c_i64, _c_i64]),
     "tp_gated_scan_states_floats": (_c_i64, [_c_i64, _c_i64, _c_i64]),
     "tp_gated_scan_fwd": (
         _c_int,
         [_c_int, _c_int, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64,
-         _c_p, _c_p, _c_p, _c_p, _c_p, _c_p],
+         _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_p],
     ),
     "tp_gated_scan_bwd": (
         _c_int,
         [_c_int, _c_int, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64,
-         _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p],
+         _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_p],
     ),
     "tp_gated_scan_step": (
         _c_int,

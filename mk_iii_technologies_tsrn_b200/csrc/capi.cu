@@ -214,6 +214,22 @@ int gated_scan_args(tp::GatedScanArgs& a, int dtype, int form, int64_t B, int64_
   return TP_OK;
 }
 
+int gated_scan_workspace(tp::GatedScanArgs& a, bool backward, void* workspace,
+                         int64_t workspace_bytes) {
+  const tp::GatedScanCut cut = tp::gated_scan_cut(a.B, a.T, a.C, backward);
+  a.segs = cut.segs;
+  a.seg_len = cut.seg_len;
+  a.runs = (float*)workspace;
+  if (cut.segs > 1) {
+    TP_RETURN_IF(workspace == nullptr ||
+                     workspace_bytes < tp_gated_scan_workspace_bytes(a.B, a.T, a.C),
+                 TP_ERR_WORKSPACE);
+    TP_CHECK_PTR(workspace);
+    TP_RETURN_IF(((uintptr_t)workspace & 3) != 0, TP_ERR_MISALIGNED);
+  }
+  return TP_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -748,6 +764,12 @@ int tp_residual_norm_bwd(int dtype, int params_dtype, int norm, int64_t rows, in
   return tp::launch_residual_norm_bwd(g, as_stream(stream));
 }
 
+int64_t tp_gated_scan_workspace_bytes(int64_t B, int64_t T, int64_t C) {
+  if (B < 0 || T < 0 || C < 0) return -1;
+  const int segs = tp::gated_scan_cut(B, T, C, true).segs;   // the forward's, or 1 there
+  return segs > 1 ? B * segs * 2 * C * (int64_t)sizeof(float) : 0;
+}
+
 int64_t tp_gated_scan_states_floats(int64_t B, int64_t T, int64_t C) {
   if (B < 0 || T < 0 || C < 0) return -1;
   return B * tp::ceil_div(T, (int64_t)tp::GATED_SCAN_CHUNK) * C;
@@ -756,7 +778,8 @@ int64_t tp_gated_scan_states_floats(int64_t B, int64_t T, int64_t C) {
 int tp_gated_scan_fwd(int dtype, int form, int64_t B, int64_t T, int64_t C, const void* gate,
                       int64_t gate_sb, int64_t gate_st, const void* x, int64_t x_sb,
                       int64_t x_st, const float* h0, const int32_t* lengths, void* h,
-                      float* h_last, float* states, void* stream) {
+                      float* h_last, float* states, void* workspace, int64_t workspace_bytes,
+                      void* stream) {
   tp::GatedScanArgs a{};
   const int st = gated_scan_args(a, dtype, form, B, T, C, gate, gate_sb, gate_st, x, x_sb, x_st,
                                  lengths);
@@ -769,6 +792,8 @@ int tp_gated_scan_fwd(int dtype, int form, int64_t B, int64_t T, int64_t C, cons
   a.h = h;
   a.h_last = h_last;
   a.states = states;
+  const int ws = gated_scan_workspace(a, false, workspace, workspace_bytes);
+  if (ws != TP_OK) return ws;
   return tp::launch_gated_scan_fwd(a, as_stream(stream));
 }
 
@@ -776,7 +801,7 @@ int tp_gated_scan_bwd(int dtype, int form, int64_t B, int64_t T, int64_t C, cons
                       int64_t gate_sb, int64_t gate_st, const void* x, int64_t x_sb,
                       int64_t x_st, const int32_t* lengths, const float* states,
                       const void* dh, const float* dh_last, void* dgate, void* dx, float* dh0,
-                      void* stream) {
+                      void* workspace, int64_t workspace_bytes, void* stream) {
   tp::GatedScanBwdArgs g{};
   const int st = gated_scan_args(g.f, dtype, form, B, T, C, gate, gate_sb, gate_st, x, x_sb,
                                  x_st, lengths);
@@ -795,6 +820,8 @@ int tp_gated_scan_bwd(int dtype, int form, int64_t B, int64_t T, int64_t C, cons
   g.dgate = dgate;
   g.dx = dx;
   g.dh0 = dh0;
+  const int ws = gated_scan_workspace(g.f, true, workspace, workspace_bytes);
+  if (ws != TP_OK) return ws;
   return tp::launch_gated_scan_bwd(g, as_stream(stream));
 }
 

@@ -10,17 +10,20 @@
 // Steps compose: a run of steps maps h -> A h + H with A the product of its
 // gates and H its result from a zero state.  One warp owns 32 lanes of channels
 // (two per lane where the layout allows: 128 or 256 bytes a row, and packed
-// fp32 pairs in the arithmetic) and L consecutive steps; the W warps of a block
-// own consecutive runs, and the S blocks of a thread-block cluster consecutive
-// groups of those.  An iteration of S * W * L steps forms every warp's (A, H),
-// exchanges them through shared memory (between the cluster's blocks through
-// distributed shared memory, one cluster barrier), applies the runs in order to
-// the carried state, and runs each warp's steps again from its own starting
+// fp32 pairs in the arithmetic) and L consecutive steps, in registers; the W
+// warps of a block own consecutive runs.  An iteration of W * L steps forms every
+// warp's (A, H), exchanges them through shared memory, applies the runs in order
+// to the carried state, and runs each warp's steps again from its own starting
 // state.  So the inputs are read once, the order of every operation is fixed
-// (the same bits on each call), and few channels still spread over many SMs.
-// The inputs of the next iterations are on their way meanwhile: each thread
-// copies its own elements asynchronously into shared memory, one or two
-// iterations ahead, and reads only those, so the copies need no barrier.
+// (the same bits on each call).  The inputs of the next iterations are on their
+// way meanwhile: asynchronous 16-byte copies into shared memory, a warp's own
+// rows only, so that they need no block barrier.
+//
+// Too few rows and channels to fill the GPU that way: time is cut into segments
+// with a block each.  A first kernel forms the run of every segment (each warp a
+// part of it, nothing to wait for), and the second starts each segment from the
+// runs before it, composed in order.  The inputs are then read twice, the second
+// time from L2 as far as it holds them.
 //
 // The backward walks the iterations from the end with the mirrored recurrence
 //   g_t = dh_t + c_{t+1},  c_t = a_t g_t   (c_t: gradient of h_{t-1})
@@ -36,26 +39,6 @@ namespace tp {
 
 namespace {
 
-#ifndef GS_MINB
-#define GS_MINB 2
-#endif
-#ifndef GS_WANT
-#define GS_WANT 1.0
-#endif
-constexpr int GS_MAX_CLUSTER = 16;
-
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-
-__device__ __forceinline__ void cluster_arrive() {
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void cluster_wait() {
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
 
 // One or two channels of a lane.
 template <int CPL>
@@ -87,35 +70,6 @@ __device__ __forceinline__ Lane<2> mul_(Lane<2> a, Lane<2> b) { return {tp_mul2(
 __device__ __forceinline__ Lane<1> add_(Lane<1> a, Lane<1> b) { return {__fadd_rn(a.v, b.v)}; }
 __device__ __forceinline__ Lane<2> add_(Lane<2> a, Lane<2> b) { return {tp_add2(a.v, b.v)}; }
 
-// The run (A, H) of a block, sent into the same shared-memory place of the
-// cluster's block `rank`; the bytes count on that block's barrier, so the
-// receiver needs no fence, and the sender does not wait for its global stores
-// as a cluster barrier's release would.
-template <int CPL>
-struct __align__(8 * CPL) Run {
-  Lane<CPL> a, h;
-};
-__device__ __forceinline__ uint32_t at_rank(const void* p, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
-               : "=r"(r)
-               : "r"(tp_smem_addr(p)), "r"(rank));
-  return r;
-}
-__device__ __forceinline__ void send_run(Run<1>* to, uint64_t* bar, uint32_t rank, Run<1> r) {
-  asm volatile(
-      "st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::
-          "r"(at_rank(to, rank)), "f"(r.a.v), "f"(r.h.v), "r"(at_rank(bar, rank))
-      : "memory");
-}
-__device__ __forceinline__ void send_run(Run<2>* to, uint64_t* bar, uint32_t rank, Run<2> r) {
-  asm volatile(
-      "st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 "
-      "[%0], {%1, %2, %3, %4}, [%5];" ::"r"(at_rank(to, rank)),
-      "f"(r.a.v.x), "f"(r.a.v.y), "f"(r.h.v.x), "f"(r.h.v.y), "r"(at_rank(bar, rank))
-      : "memory");
-}
-
 // CPL channels in storage, as one word of shared memory or a register
 template <typename T, int CPL>
 __device__ __forceinline__ Lane<CPL> unpack(const RowVec<T, CPL>& r) {
@@ -143,21 +97,21 @@ __device__ __forceinline__ void store_lane(T* p, Lane<CPL> l) {
 template <typename T, int CPL, int L, bool WIDE>
 struct Rows {
   static constexpr int PER = 32 * CPL * (int)sizeof(T) / 16;   // 16-byte pieces of a row
-  // the element of the row at which this lane's copies begin
+  // the row and the channel at which this lane's copies begin
+  __device__ __forceinline__ static int first_row(int lane) { return WIDE ? lane / PER : 0; }
   __device__ __forceinline__ static int first_channel(int lane) {
     return WIDE ? (lane % PER) * (16 / (int)sizeof(T)) : lane * CPL;
   }
-  // p: this lane's element of the first row
+  // p: where this lane's copies begin
   __device__ __forceinline__ static void copy(RowVec<T, CPL>* s, const T* p, int64_t stride,
                                               int n, int lane) {
     if constexpr (WIDE) {
       constexpr int ROWS = 32 / PER;      // rows per instruction
       char* d = reinterpret_cast<char*>(s) + lane * 16;
-      const int r = lane / PER;
-      p += r * stride;
+      n -= lane / PER;
 #pragma unroll
       for (int i = 0; i < L; i += ROWS) {
-        if (i + r < n)
+        if (i < n)
           asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(tp_smem_addr(d + i * PER * 16)),
                        "l"(p)
                        : "memory");
@@ -211,12 +165,16 @@ __device__ __forceinline__ void gate_of(float z, float& a, float& rest) {
 }
 template <typename T, int FORM, int CPL>
 __device__ __forceinline__ void gates_of(Lane<CPL> z, Lane<CPL>& a, Lane<CPL>& rest) {
+  if constexpr (FORM == TP_GATE_SIGMOID && sizeof(T) == 2 && CPL == 2) {
+    fast_sigmoid_pair2(z.v, a.v, rest.v);
+  } else {
 #pragma unroll
-  for (int k = 0; k < CPL; ++k) {
-    float p, q;
-    gate_of<T, FORM>(z.at(k), p, q);
-    a.put(k, p);
-    rest.put(k, q);
+    for (int k = 0; k < CPL; ++k) {
+      float p, q;
+      gate_of<T, FORM>(z.at(k), p, q);
+      a.put(k, p);
+      rest.put(k, q);
+    }
   }
 }
 
@@ -225,10 +183,11 @@ struct Place {
   int64_t b, c;       // batch row, this lane's first channel
   bool in;            // the lane has channels
   int64_t len;        // live steps of the row
-  int rank;           // block of the cluster
-  __device__ __forceinline__ Place(const GatedScanArgs& a, int S, int64_t tiles) {
-    const int64_t id = blockIdx.x / S;
-    rank = S > 1 ? (int)cluster_rank() : 0;
+  int64_t begin, end; // steps of the block's segment
+  int seg;
+  __device__ __forceinline__ Place(const GatedScanArgs& a, int64_t tiles) {
+    const int64_t id = blockIdx.x / a.segs;
+    seg = (int)(blockIdx.x - id * a.segs);
     b = id / tiles;
     c = (id - b * tiles) * (32 * CPL) + (threadIdx.x & 31) * CPL;
     in = c < a.C;
@@ -237,6 +196,8 @@ struct Place {
       const int64_t n = a.lengths[b];
       len = n < 0 ? 0 : (n < a.T ? n : a.T);
     }
+    begin = seg * a.seg_len;
+    end = begin + a.seg_len < a.T ? begin + a.seg_len : a.T;
   }
   __device__ __forceinline__ Lane<CPL> load(const float* p, int64_t row, int64_t C) const {
     Lane<CPL> l = Lane<CPL>::all(0.0f);
@@ -261,62 +222,179 @@ __device__ __forceinline__ int steps_below(int64_t end, int64_t t0) {
   return n <= 0 ? 0 : (n < L ? (int)n : L);
 }
 
+// The run of every segment: runs [B][segs][2][C], products then results.  Each
+// of the block's warps takes an eighth of the segment, L steps at a time, with
+// the copies of the next steps on their way.  REVERSE: the backward's runs.
+template <typename T, int CPL, int FORM, int L, int W, int STAGES, bool WIDE, bool REVERSE>
+__global__ void __launch_bounds__(32 * W)
+    gated_scan_runs_kernel(const GatedScanArgs a, const T* dh, const int64_t tiles) {
+  using V = RowVec<T, CPL>;
+  using N = Lane<CPL>;
+  using R = Rows<T, CPL, L, WIDE>;
+  extern __shared__ __align__(16) unsigned char s_raw[];   // [STAGES][W][2][L][32] of V
+  __shared__ N s_a[W][32], s_h[W][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const Place<T, CPL> w(a, tiles);
+  if (w.seg == (REVERSE ? 0 : a.segs - 1)) return;      // nothing follows it
+  const int64_t part = a.seg_len / W;                   // a multiple of L
+  const int64_t lo = w.begin + warp * part;
+  const int64_t hi = min(lo + part, w.len);
+  const int batches = hi > lo ? (int)ceil_div(hi - lo, (int64_t)L) : 0;
+  const int64_t ost = REVERSE ? a.C : a.x_st;           // the other operand: dh or x
+  const bool has = !REVERSE || dh != nullptr;
+  const int64_t c0 = w.c - lane * CPL + R::first_channel(lane);
+  const int64_t r0 = lo + (REVERSE ? (int64_t)(batches - 1) * L : 0) + R::first_row(lane);
+  const T* gf = (const T*)a.gate + w.b * a.gate_sb + r0 * a.gate_st + c0;
+  const T* of = (REVERSE ? dh + w.b * a.T * a.C : (const T*)a.x + w.b * a.x_sb) + r0 * ost + c0;
+  const int64_t gate_step = (REVERSE ? -L : L) * a.gate_st, o_step = (REVERSE ? -L : L) * ost;
+  V* const raw = reinterpret_cast<V*>(s_raw) + warp * (2 * L * 32);
+  int next = 0, filling = 0, reading = 0;
+  // live steps of batch k: all but those of the last one are full
+  auto live = [&](int k) {
+    return steps_below<L>(hi, lo + (int64_t)(REVERSE ? batches - 1 - k : k) * L);
+  };
+  auto fetch = [&]() {
+    if (next < batches && c0 < a.C) {
+      V* s = raw + filling * (W * 2 * L * 32);
+      const int n = live(next);
+      R::copy(s, gf, a.gate_st, n, lane);
+      if (has) R::copy(s + L * 32, of, ost, n, lane);
+    }
+    tp_cp_async_commit();
+    ++next;
+    gf += gate_step;
+    of += o_step;
+    filling = filling + 1 == STAGES ? 0 : filling + 1;
+  };
+#pragma unroll
+  for (int k = 0; k < STAGES - 1; ++k) fetch();
+  N pa = N::all(1.0f), ph = N::all(0.0f);
+  for (int k = 0; k < batches; ++k) {
+    __syncwarp();
+    fetch();
+    tp_cp_async_wait<STAGES - 1>();
+    __syncwarp();
+    const V* s = raw + reading * (W * 2 * L * 32) + lane;
+    reading = reading + 1 == STAGES ? 0 : reading + 1;
+    const int n = live(k);
+    auto run = [&](auto all) {
+#pragma unroll
+      for (int j = 0; j < L; ++j) {
+        const int i = REVERSE ? L - 1 - j : j;
+        if (all.value || i < n) {
+          N A, rest, U = N::all(0.0f);
+          gates_of<T, FORM>(unpack<T, CPL>(s[i * 32]), A, rest);
+          if (has) U = unpack<T, CPL>(s[(L + i) * 32]);
+          if constexpr (REVERSE) {
+            ph = mul_(A, add_(U, ph));
+          } else {
+            if constexpr (FORM == TP_GATE_SIGMOID) U = mul_(rest, U);
+            ph = fma_(A, ph, U);
+          }
+          pa = mul_(pa, A);
+        }
+      }
+    };
+    if (n == L) run(std::true_type());
+    else run(std::false_type());
+  }
+  s_a[warp][lane] = finite(pa);
+  s_h[warp][lane] = ph;
+  __syncthreads();
+  if (warp != 0) return;
+  pa = N::all(1.0f);
+  ph = N::all(0.0f);
+#pragma unroll
+  for (int k = 0; k < W; ++k) {
+    const int q = REVERSE ? W - 1 - k : k;
+    ph = fma_(s_a[q][lane], ph, s_h[q][lane]);
+    pa = mul_(pa, s_a[q][lane]);
+  }
+  const int64_t row = (w.b * a.segs + w.seg) * 2;
+  w.store(a.runs, row, a.C, finite(pa));
+  w.store(a.runs, row + 1, a.C, ph);
+}
+
+// The state before (REVERSE: the gradient after) the block's segment: the runs of
+// the segments before (after) it applied to `carry`.  The warps compose an equal
+// share each, through `s_a`, `s_h`, and all apply the shares in order.
+template <typename T, int CPL, int W, bool REVERSE>
+__device__ __forceinline__ Lane<CPL> segment_start(const GatedScanArgs& a, const Place<T, CPL>& w,
+                                                   Lane<CPL> carry, Lane<CPL> (*s_a)[32],
+                                                   Lane<CPL> (*s_h)[32], int warp, int lane) {
+  using N = Lane<CPL>;
+  if (a.segs == 1) return carry;
+  const int n = REVERSE ? a.segs - 1 - w.seg : w.seg;    // segments to apply
+  const int per = (n + W - 1) / W;
+  const int lo = min(n, warp * per), hi = min(n, lo + per);
+  N pa = N::all(1.0f), ph = N::all(0.0f);
+#pragma unroll 4
+  for (int k = lo; k < hi; ++k) {
+    const int64_t row = (w.b * a.segs + (REVERSE ? a.segs - 1 - k : k)) * 2;
+    const N ra = w.load(a.runs, row, a.C), rh = w.load(a.runs, row + 1, a.C);
+    ph = fma_(ra, ph, rh);
+    pa = mul_(pa, ra);
+  }
+  s_a[warp][lane] = finite(pa);
+  s_h[warp][lane] = ph;
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < W; ++q) carry = fma_(s_a[q][lane], carry, s_h[q][lane]);
+  return carry;
+}
+
 template <typename T, int CPL, int FORM, int L, int W, int STAGES, bool WIDE>
-__global__ void __launch_bounds__(32 * W, GS_MINB)
-    gated_scan_fwd_kernel(const GatedScanArgs a, const int S, const int64_t tiles, int* err) {
+__global__ void __launch_bounds__(32 * W, 2)
+    gated_scan_fwd_kernel(const GatedScanArgs a, const int64_t tiles) {
   using V = RowVec<T, CPL>;
   using N = Lane<CPL>;
   extern __shared__ __align__(16) unsigned char s_raw[];   // [STAGES][2][W][L][32] of V
   __shared__ N s_a[2][W][32], s_h[2][W][32];               // runs of the warps
   V* const raw = reinterpret_cast<V*>(s_raw);
-  // runs of the cluster's blocks: [2][S][32], filled by the blocks themselves
-  Run<CPL>* const s_blk = reinterpret_cast<Run<CPL>*>(raw + STAGES * 2 * L * 32 * W);
-  __shared__ uint64_t s_bar[2];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const Place<T, CPL> w(a, S, tiles);
+  const Place<T, CPL> w(a, tiles);
   T* const hp = (T*)a.h + (w.b * a.T) * a.C + w.c;
   const int64_t chunks = ceil_div(a.T, (int64_t)GATED_SCAN_CHUNK);
-  const int64_t step = (int64_t)S * W * L;
-  const int64_t iters = ceil_div(a.T, step);
-  const int64_t mine0 = ((int64_t)w.rank * W + warp) * L;
+  constexpr int step = W * L;
+  const int64_t iters = ceil_div(w.end - w.begin, (int64_t)step);
+  const int64_t mine0 = w.begin + warp * L;
   N carry = w.load(a.h0, w.b, a.C);
 
   using R = Rows<T, CPL, L, WIDE>;
   const int64_t c0 = w.c - lane * CPL + R::first_channel(lane);   // this lane copies from here
-  const T* const gf = (const T*)a.gate + w.b * a.gate_sb + c0;
-  const T* const xf = (const T*)a.x + w.b * a.x_sb + c0;
-  const bool copies = c0 < a.C;
-  auto fetch = [&](int64_t it) {
-    if (it < iters && copies) {
-      const int64_t t0 = it * step + mine0;
-      const int n = steps_below<L>(w.len, t0);
-      V* s = raw + ((it % STAGES) * (2 * W) + warp) * (L * 32);
-      R::copy(s, gf + t0 * a.gate_st, a.gate_st, n, lane);
-      R::copy(s + W * L * 32, xf + t0 * a.x_st, a.x_st, n, lane);
+  const int64_t r0 = mine0 + R::first_row(lane);
+  const T* gf = (const T*)a.gate + w.b * a.gate_sb + r0 * a.gate_st + c0;
+  const T* xf = (const T*)a.x + w.b * a.x_sb + r0 * a.x_st + c0;
+  const int64_t gate_step = step * a.gate_st, x_step = step * a.x_st;
+  // live steps of the segment from the next copies on
+  int64_t left = c0 < a.C ? min(w.len, w.end) - mine0 : 0;
+  int filling = 0, reading = 0;                     // stages
+  auto fetch = [&]() {                              // one iteration further each time
+    const int n = left <= 0 ? 0 : (left < L ? (int)left : L);
+    V* s = raw + (filling * (2 * W) + warp) * (L * 32);
+    if (n > 0) {
+      R::copy(s, gf, a.gate_st, n, lane);
+      R::copy(s + W * L * 32, xf, a.x_st, n, lane);
     }
     tp_cp_async_commit();
+    gf += gate_step;
+    xf += x_step;
+    left -= step;
+    filling = filling + 1 == STAGES ? 0 : filling + 1;
   };
 #pragma unroll
-  for (int k = 0; k < STAGES - 1; ++k) fetch(k);
-  if (S > 1) {     // every block of the cluster has its barriers before the first run is sent
-    if (threadIdx.x == 0) {
-      tp_mbar_init(&s_bar[0], 1);
-      tp_mbar_init(&s_bar[1], 1);
-      tp_fence_mbar_init();
-    }
-    cluster_arrive();
-    cluster_wait();
-  }
-  bool ok = true;
+  for (int k = 0; k < STAGES - 1; ++k) fetch();
+  carry = segment_start<T, CPL, W, false>(a, w, carry, s_a[1], s_h[1], warp, lane);
   for (int64_t it = 0; it < iters; ++it) {
     __syncwarp();          // the warp has read the stage that is filled now
-    fetch(it + STAGES - 1);
+    fetch();
     const int par = (int)(it & 1);
-    const int64_t t0 = it * step + mine0;
+    const int64_t t0 = mine0 + it * step;
     const int n = steps_below<L>(w.len, t0);
     tp_cp_async_wait<STAGES - 1>();
     __syncwarp();          // and every lane's copies of this stage are there
-    const V* s = raw + ((it % STAGES) * (2 * W) + warp) * (L * 32) + lane;
+    const V* s = raw + (reading * (2 * W) + warp) * (L * 32) + lane;
+    reading = reading + 1 == STAGES ? 0 : reading + 1;
     N A[L], U[L];
     N pa = N::all(1.0f), ph = N::all(0.0f);
 #pragma unroll
@@ -342,50 +420,13 @@ __global__ void __launch_bounds__(32 * W, GS_MINB)
     s_a[par][warp][lane] = finite(pa);
     s_h[par][warp][lane] = ph;
     __syncthreads();
-    N mine;
-    if (S == 1) {
-      N h = carry;
-      mine = h;
+    N mine = carry, h = carry;
 #pragma unroll
-      for (int q = 0; q < W; ++q) {
-        if (q == warp) mine = h;
-        h = fma_(s_a[par][q][lane], h, s_h[par][q][lane]);
-      }
-      carry = h;
-    } else {
-      // the runs before this warp's, composed; the last warp has the block's
-      N qa = N::all(1.0f), qh = N::all(0.0f);
-#pragma unroll
-      for (int q = 0; q < W; ++q) {
-        if (q < warp || warp == W - 1) {
-          const N na = s_a[par][q][lane];
-          if (q == warp) {
-            mine = qh;     // (last warp: keep the composition up to itself)
-            pa = qa;
-          }
-          qh = fma_(na, qh, s_h[par][q][lane]);
-          qa = mul_(qa, na);
-        }
-      }
-      if (warp == W - 1) {
-        const Run<CPL> r = {finite(qa), qh};
-        for (int q = 0; q < S; ++q)
-          send_run(s_blk + (par * S + w.rank) * 32 + lane, &s_bar[par], q, r);
-        if (lane == 0) tp_mbar_arrive_expect_tx(&s_bar[par], S * 32 * (int)sizeof(Run<CPL>));
-        qa = pa;
-        qh = mine;
-      }
-      // (a wait that runs out is recorded; the blocks stay in step and finish)
-      ok = ok && tp_mbar_wait(&s_bar[par], (unsigned)(it >> 1) & 1u, err);
-      N h = carry, start = carry;
-      for (int q = 0; q < S; ++q) {
-        if (q == w.rank) start = h;
-        const Run<CPL> r = s_blk[(par * S + q) * 32 + lane];
-        h = fma_(r.a, h, r.h);
-      }
-      carry = h;
-      mine = fma_(finite(qa), start, qh);
+    for (int q = 0; q < W; ++q) {
+      if (q == warp) mine = h;
+      h = fma_(s_a[par][q][lane], h, s_h[par][q][lane]);
     }
+    carry = h;
     if (a.states && t0 < a.T && (t0 % GATED_SCAN_CHUNK) == 0)
       w.store(a.states, w.b * chunks + t0 / GATED_SCAN_CHUNK, a.C, mine);
     T* o = hp + t0 * a.C;
@@ -406,16 +447,12 @@ __global__ void __launch_bounds__(32 * W, GS_MINB)
       }
     }
   }
-  if (w.rank == 0 && warp == 0) w.store(a.h_last, w.b, a.C, carry);
-  if (S > 1) {     // no block leaves while another may still send to it
-    cluster_arrive();
-    cluster_wait();
-  }
+  if (w.seg == a.segs - 1 && warp == 0) w.store(a.h_last, w.b, a.C, carry);
 }
 
 template <typename T, int CPL, int FORM, int L, int W, int STAGES, bool WIDE>
-__global__ void __launch_bounds__(32 * W, GS_MINB)
-    gated_scan_bwd_kernel(const GatedScanBwdArgs g, const int S, const int64_t tiles, int* err) {
+__global__ void __launch_bounds__(32 * W, 2)
+    gated_scan_bwd_kernel(const GatedScanBwdArgs g, const int64_t tiles) {
   static_assert(GATED_SCAN_CHUNK % L == 0 && (W * L) % GATED_SCAN_CHUNK == 0, "");
   using V = RowVec<T, CPL>;
   using N = Lane<CPL>;
@@ -423,16 +460,14 @@ __global__ void __launch_bounds__(32 * W, GS_MINB)
   extern __shared__ __align__(16) unsigned char s_raw[];   // [STAGES][3][W][L][32] of V
   __shared__ N s_a[2][W][32], s_h[2][W][32], s_c[2][W][32];   // runs, forwards and backwards
   V* const raw = reinterpret_cast<V*>(s_raw);
-  Run<CPL>* const s_blk = reinterpret_cast<Run<CPL>*>(raw + STAGES * 3 * L * 32 * W);
-  __shared__ uint64_t s_bar[2];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const Place<T, CPL> w(a, S, tiles);
+  const Place<T, CPL> w(a, tiles);
   T* const dgp = (T*)g.dgate + (w.b * a.T) * a.C + w.c;
   T* const dxp = (T*)g.dx + (w.b * a.T) * a.C + w.c;
   const int64_t chunks = ceil_div(a.T, (int64_t)GATED_SCAN_CHUNK);
-  const int64_t step = (int64_t)S * W * L;
-  const int64_t iters = ceil_div(a.T, step);
-  const int64_t mine0 = ((int64_t)w.rank * W + warp) * L;
+  constexpr int step = W * L;
+  const int64_t iters = ceil_div(w.end - w.begin, (int64_t)step);
+  const int64_t mine0 = w.begin + warp * L;
   // the first warp of this warp's 64-step chunk, whose starting state is kept
   constexpr int WPC = GATED_SCAN_CHUNK / L;
   const int lead = warp - warp % WPC;
@@ -440,20 +475,30 @@ __global__ void __launch_bounds__(32 * W, GS_MINB)
 
   using R = Rows<T, CPL, L, WIDE>;
   const int64_t c0 = w.c - lane * CPL + R::first_channel(lane);
-  const T* const gf = (const T*)a.gate + w.b * a.gate_sb + c0;
-  const T* const xf = (const T*)a.x + w.b * a.x_sb + c0;
-  const T* const df = (const T*)g.dh + w.b * a.T * a.C + c0;
-  const bool copies = c0 < a.C, has_dh = g.dh != nullptr;
-  auto fetch = [&](int64_t it) {       // it counts from the end
-    if (it < iters && copies) {
-      const int64_t t0 = (iters - 1 - it) * step + mine0;
-      const int n = steps_below<L>(w.len, t0);
-      V* s = raw + ((it % STAGES) * (3 * W) + warp) * (L * 32);
-      R::copy(s, gf + t0 * a.gate_st, a.gate_st, n, lane);
-      R::copy(s + W * L * 32, xf + t0 * a.x_st, a.x_st, n, lane);
-      if (has_dh) R::copy(s + 2 * W * L * 32, df + t0 * a.C, a.C, n, lane);
+  const int64_t r0 = (iters - 1) * step + mine0 + R::first_row(lane);
+  const T* gf = (const T*)a.gate + w.b * a.gate_sb + r0 * a.gate_st + c0;
+  const T* xf = (const T*)a.x + w.b * a.x_sb + r0 * a.x_st + c0;
+  const T* df = (const T*)g.dh + (w.b * a.T + r0) * a.C + c0;
+  const int64_t gate_step = step * a.gate_st, x_step = step * a.x_st, d_step = step * a.C;
+  const bool has_dh = g.dh != nullptr;
+  // live steps from the next copies on, and copies left
+  int64_t left = w.len - ((iters - 1) * step + mine0), todo = c0 < a.C ? iters : 0;
+  int filling = 0, reading = 0;
+  auto fetch = [&]() {                 // one iteration towards the start each time
+    const int n = left <= 0 ? 0 : (left < L ? (int)left : L);
+    V* s = raw + (filling * (3 * W) + warp) * (L * 32);
+    if (n > 0 && todo > 0) {
+      R::copy(s, gf, a.gate_st, n, lane);
+      R::copy(s + W * L * 32, xf, a.x_st, n, lane);
+      if (has_dh) R::copy(s + 2 * W * L * 32, df, a.C, n, lane);
     }
     tp_cp_async_commit();
+    gf -= gate_step;
+    xf -= x_step;
+    df -= d_step;
+    left += step;
+    --todo;
+    filling = filling + 1 == STAGES ? 0 : filling + 1;
   };
   auto first_state = [&](int64_t it) {
     const int64_t t0 = (iters - 1 - it) * step + mine0;
@@ -461,21 +506,12 @@ __global__ void __launch_bounds__(32 * W, GS_MINB)
     return w.load(a.states, w.b * chunks + t0 / GATED_SCAN_CHUNK, a.C);
   };
 #pragma unroll
-  for (int k = 0; k < STAGES - 1; ++k) fetch(k);
+  for (int k = 0; k < STAGES - 1; ++k) fetch();
   N next = first_state(0);
-  if (S > 1) {     // every block of the cluster has its barriers before the first run is sent
-    if (threadIdx.x == 0) {
-      tp_mbar_init(&s_bar[0], 1);
-      tp_mbar_init(&s_bar[1], 1);
-      tp_fence_mbar_init();
-    }
-    cluster_arrive();
-    cluster_wait();
-  }
-  bool ok = true;
+  carry = segment_start<T, CPL, W, true>(a, w, carry, s_a[1], s_c[1], warp, lane);
   for (int64_t it = 0; it < iters; ++it) {
     __syncwarp();
-    fetch(it + STAGES - 1);
+    fetch();
     const N first = next;
     next = first_state(it + 1);
     const int par = (int)(it & 1);
@@ -483,7 +519,8 @@ __global__ void __launch_bounds__(32 * W, GS_MINB)
     const int n = steps_below<L>(w.len, t0);
     tp_cp_async_wait<STAGES - 1>();
     __syncwarp();
-    const V* s = raw + ((it % STAGES) * (3 * W) + warp) * (L * 32) + lane;
+    const V* s = raw + (reading * (3 * W) + warp) * (L * 32) + lane;
+    reading = reading + 1 == STAGES ? 0 : reading + 1;
     N A[L], O[L], U[L];      // gate, its complement, input
     N pa = N::all(1.0f), ph = N::all(0.0f);
     auto dh_at = [&](int i) {
@@ -515,49 +552,13 @@ __global__ void __launch_bounds__(32 * W, GS_MINB)
     s_h[par][warp][lane] = ph;
     s_c[par][warp][lane] = mul_(A[0], gr);
     __syncthreads();
-    N mine;
-    if (S == 1) {
-      N c = carry;
-      mine = c;
+    N mine = carry, c = carry;
 #pragma unroll
-      for (int q = W - 1; q >= 0; --q) {
-        if (q == warp) mine = c;
-        c = fma_(s_a[par][q][lane], c, s_c[par][q][lane]);
-      }
-      carry = c;
-    } else {
-      // the runs after this warp's, composed; the first warp has the block's
-      N qa = N::all(1.0f), qc = N::all(0.0f);
-#pragma unroll
-      for (int q = W - 1; q >= 0; --q) {
-        if (q > warp || warp == 0) {
-          const N na = s_a[par][q][lane];
-          if (q == warp) {
-            mine = qc;
-            pa = qa;
-          }
-          qc = fma_(na, qc, s_c[par][q][lane]);
-          qa = mul_(qa, na);
-        }
-      }
-      if (warp == 0) {
-        const Run<CPL> r = {finite(qa), qc};
-        for (int q = 0; q < S; ++q)
-          send_run(s_blk + (par * S + w.rank) * 32 + lane, &s_bar[par], q, r);
-        if (lane == 0) tp_mbar_arrive_expect_tx(&s_bar[par], S * 32 * (int)sizeof(Run<CPL>));
-        qa = pa;
-        qc = mine;
-      }
-      ok = ok && tp_mbar_wait(&s_bar[par], (unsigned)(it >> 1) & 1u, err);
-      N c = carry, start = carry;
-      for (int q = S - 1; q >= 0; --q) {
-        if (q == w.rank) start = c;
-        const Run<CPL> r = s_blk[(par * S + q) * 32 + lane];
-        c = fma_(r.a, c, r.h);
-      }
-      carry = c;
-      mine = fma_(finite(qa), start, qc);
+    for (int q = W - 1; q >= 0; --q) {
+      if (q == warp) mine = c;
+      c = fma_(s_a[par][q][lane], c, s_c[par][q][lane]);
     }
+    carry = c;
     N before[L];      // h_{t-1}
     {
       N h = first;
@@ -591,11 +592,7 @@ __global__ void __launch_bounds__(32 * W, GS_MINB)
       ox -= a.C;
     }
   }
-  if (w.rank == 0 && warp == 0) w.store(g.dh0, w.b, a.C, carry);
-  if (S > 1) {     // no block leaves while another may still send to it
-    cluster_arrive();
-    cluster_wait();
-  }
+  if (w.seg == 0 && warp == 0) w.store(g.dh0, w.b, a.C, carry);
 }
 
 // One step of every row, the state updated in place: a serving step.
@@ -624,41 +621,25 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// Blocks of a cluster: enough for two blocks per SM, no more than the steps
-// fill.  It goes by the sizes alone, as L does by the type, so that the order of
-// operations, and with it the bits, do not depend on strides and alignment.
-int cluster_size(int64_t B, int64_t T, int64_t C, int64_t steps_per_block) {
-  const int64_t want = (int64_t)(GS_WANT * num_sms()), blocks = B * ceil_div(C, (int64_t)64);
-  int S = 1;
-  while (S < GS_MAX_CLUSTER && blocks * S < want && T > S * steps_per_block) S *= 2;
-  return S;
-}
+// Warps of a block, and steps of a warp's run.  More steps per iteration spread
+// its fixed costs (exchange, barrier): forward 16 x 4096 x 1024 fp32 with 16
+// steps and two stages 131 us, with 8 steps and three stages 156 us.  The
+// backward holds twice the registers per step: 8 (16 spill or halve the blocks:
+// 232 against 238 us).
+constexpr int GS_W = 8;
+constexpr int GS_FWD_L = 16, GS_BWD_L = 8, GS_RUN_L = 8;
+constexpr int GS_RUN_STAGES = 3;
 
-template <typename K, typename A>
-int launch_clustered(K kernel, const A& args, int threads, size_t smem, size_t runs_bytes,
-                     int64_t B, int64_t tiles, int S, cudaStream_t stream) {
-  if (B * tiles > INT32_MAX / GS_MAX_CLUSTER) return TP_ERR_TOO_LARGE;
-  if (S > 1) smem += (size_t)2 * S * runs_bytes;
-  cudaError_t e = cudaFuncSetAttribute((const void*)kernel,
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e == cudaSuccess && S > 8)
-    e = cudaFuncSetAttribute((const void*)kernel,
-                             cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  if (e != cudaSuccess) return cuda_status(e);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(B * tiles * S));
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = S;
-  at[0].val.clusterDim.y = 1;
-  at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = S > 1 ? 1 : 0;
-  int* err = device_error_ptr();
-  return cuda_status(cudaLaunchKernelEx(&cfg, kernel, args, S, tiles, err));
+template <typename K, typename A, typename... More>
+int launch_blocks(K kernel, int64_t blocks, size_t smem, cudaStream_t stream, const A& args,
+                  More... more) {
+  if (smem > 24 * 1024) {      // beside up to 12 KB of the kernels' own
+    const cudaError_t e = cudaFuncSetAttribute(
+        (const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return cuda_status(e);
+  }
+  kernel<<<(unsigned)blocks, 32 * GS_W, smem, stream>>>(args, more...);
+  return launch_status();
 }
 
 // Whether rows, strides and bases are multiples of `bytes`.
@@ -675,30 +656,37 @@ bool rows_at(const GatedScanArgs& a, std::initializer_list<const void*> more, in
 
 template <typename T, int CPL, int FORM, bool WIDE>
 int fwd(const GatedScanArgs& a, cudaStream_t stream) {
-#ifdef GS_FL
-  constexpr int L = GS_FL, W = GS_FW, STAGES = GS_FS;
-#else
-  constexpr int L = sizeof(T) == 4 ? 8 : 16, W = 8, STAGES = 3;
-#endif
+  constexpr int L = GS_FWD_L, W = GS_W, STAGES = 2;
   const int64_t tiles = ceil_div(a.C, (int64_t)(32 * CPL));
-  const int S = cluster_size(a.B, a.T, a.C, L * W);
-  return launch_clustered(gated_scan_fwd_kernel<T, CPL, FORM, L, W, STAGES, WIDE>, a, 32 * W,
-                          (size_t)STAGES * 2 * L * 32 * W * CPL * sizeof(T),
-                          32 * sizeof(Run<CPL>), a.B, tiles, S, stream);
+  const int64_t blocks = a.B * tiles * a.segs;
+  if (blocks > INT32_MAX) return TP_ERR_TOO_LARGE;
+  if (a.segs > 1) {
+    constexpr int RL = GS_RUN_L, RS = GS_RUN_STAGES;
+    const int st =
+        launch_blocks(gated_scan_runs_kernel<T, CPL, FORM, RL, W, RS, WIDE, false>, blocks,
+                      (size_t)RS * 2 * RL * 32 * W * CPL * sizeof(T), stream, a,
+                      (const T*)nullptr, tiles);
+    if (st != TP_OK) return st;
+  }
+  return launch_blocks(gated_scan_fwd_kernel<T, CPL, FORM, L, W, STAGES, WIDE>, blocks,
+                       (size_t)STAGES * 2 * L * 32 * W * CPL * sizeof(T), stream, a, tiles);
 }
 
 template <typename T, int CPL, int FORM, bool WIDE>
 int bwd(const GatedScanBwdArgs& g, cudaStream_t stream) {
-#ifdef GS_BL
-  constexpr int L = GS_BL, W = GS_BW, STAGES = GS_BS;
-#else
-  constexpr int L = 8, W = 8, STAGES = sizeof(T) * CPL == 8 ? 2 : 3;
-#endif
+  constexpr int L = GS_BWD_L, W = GS_W, STAGES = sizeof(T) * CPL == 8 ? 2 : 3;
   const int64_t tiles = ceil_div(g.f.C, (int64_t)(32 * CPL));
-  const int S = cluster_size(g.f.B, g.f.T, g.f.C, L * W);
-  return launch_clustered(gated_scan_bwd_kernel<T, CPL, FORM, L, W, STAGES, WIDE>, g, 32 * W,
-                          (size_t)STAGES * 3 * L * 32 * W * CPL * sizeof(T),
-                          32 * sizeof(Run<CPL>), g.f.B, tiles, S, stream);
+  const int64_t blocks = g.f.B * tiles * g.f.segs;
+  if (blocks > INT32_MAX) return TP_ERR_TOO_LARGE;
+  if (g.f.segs > 1) {
+    constexpr int RL = GS_RUN_L, RS = GS_RUN_STAGES;
+    const int st = launch_blocks(gated_scan_runs_kernel<T, CPL, FORM, RL, W, RS, WIDE, true>,
+                                 blocks, (size_t)RS * 2 * RL * 32 * W * CPL * sizeof(T), stream,
+                                 g.f, (const T*)g.dh, tiles);
+    if (st != TP_OK) return st;
+  }
+  return launch_blocks(gated_scan_bwd_kernel<T, CPL, FORM, L, W, STAGES, WIDE>, blocks,
+                       (size_t)STAGES * 3 * L * 32 * W * CPL * sizeof(T), stream, g, tiles);
 }
 
 // Two channels per lane and 16-byte copies where rows are 16-byte aligned, else
@@ -715,6 +703,26 @@ int bwd_any(const GatedScanBwdArgs& g, cudaStream_t stream) {
 }
 
 }  // namespace
+
+// Segments of time.  A cut costs a second reading (three arrays forwards become
+// five, five backwards become seven), so only rows and channels for less than a
+// third of the SMs are cut forwards (4 x 8192 x 1024 fp32, 64 blocks: 95 us in
+// one piece, 121 us cut; 2 x 8192 x 1024: 95 and 69 us), less than a half
+// backwards (4 x 8192 x 1024: 209 us in one piece, 159 us cut), into about four
+// blocks per SM, of at least 256 steps.  The cut goes by the sizes alone, as L
+// does by the direction, so that the order of operations, and with it the bits,
+// do not depend on strides and alignment.
+GatedScanCut gated_scan_cut(int64_t B, int64_t T, int64_t C, bool backward) {
+  constexpr int64_t unit = GS_W * GS_FWD_L;       // a segment is a multiple of it
+  const int64_t blocks = B * ceil_div(C, (int64_t)64), sms = num_sms();
+  int64_t segs = 1;
+  if (blocks > 0 && blocks * (backward ? 2 : 3) < sms) segs = ceil_div(4 * sms, blocks);
+  const int64_t most = T / (2 * unit);
+  segs = segs < most ? segs : most;
+  if (segs <= 1) return {1, ceil_div(T > 0 ? T : 1, unit) * unit};
+  const int64_t len = ceil_div(ceil_div(T, segs), unit) * unit;
+  return {(int)ceil_div(T, len), len};
+}
 
 int launch_gated_scan_fwd(const GatedScanArgs& a, cudaStream_t stream) {
   const bool sig = a.form == TP_GATE_SIGMOID;

@@ -335,6 +335,9 @@ struct GatedScanArgs {
   void* h;               // [B, T, C]
   float* h_last;         // [B, C] or NULL
   float* states;         // [B, ceil(T / 64), C]: the state before each chunk, or NULL
+  int segs;              // segments of time with a block each (gated_scan_cut)
+  int64_t seg_len;       // steps of a segment
+  float* runs;           // [B][segs][2][C] when segs > 1
 };
 struct GatedScanBwdArgs {
   GatedScanArgs f;       // h, h_last unused; states from the forward
@@ -343,6 +346,11 @@ struct GatedScanBwdArgs {
   void *dgate, *dx;      // [B, T, C]
   float* dh0;            // [B, C] or NULL
 };
+struct GatedScanCut {
+  int segs;
+  int64_t seg_len;
+};
+GatedScanCut gated_scan_cut(int64_t B, int64_t T, int64_t C, bool backward);
 int launch_gated_scan_fwd(const GatedScanArgs& a, cudaStream_t stream);
 int launch_gated_scan_bwd(const GatedScanBwdArgs& a, cudaStream_t stream);
 int launch_gated_scan_step(int dtype, int form, int64_t B, int64_t C, const void* gate,

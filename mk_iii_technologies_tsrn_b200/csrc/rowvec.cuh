@@ -189,14 +189,27 @@ __device__ __forceinline__ void sigmoid_pair(float v, float& s, float& rest) {
 // two.  Relative error about (8 + 1.5 |v|) 2^-24 (argument rounded once, 2^x to
 // 2^-22, 1 + e, reciprocal and product).  The exponent is held at 126, so that
 // sigmoid(-inf) is 2^-126 and its complement exactly 1.
-__device__ __forceinline__ void fast_sigmoid_pair(float v, float& s, float& rest) {
-  float t = v * -1.442695041f;
+__device__ __forceinline__ float ex2_of_capped(float t) {
   asm("min.NaN.f32 %0, %0, 0f42FC0000;" : "+f"(t));   // 126
-  const float e = tp_ex2(t);
+  return tp_ex2(t);
+}
+__device__ __forceinline__ float rcp_approx(float v) {
   float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
-  s = r;
-  rest = e * r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ void fast_sigmoid_pair(float v, float& s, float& rest) {
+  const float e = ex2_of_capped(__fmul_rn(v, -1.442695041f));
+  s = rcp_approx(__fadd_rn(1.0f, e));
+  rest = __fmul_rn(e, s);
+}
+// two at once, the same bits
+__device__ __forceinline__ void fast_sigmoid_pair2(float2 v, float2& s, float2& rest) {
+  const float2 t = tp_mul2(v, make_float2(-1.442695041f, -1.442695041f));
+  const float2 e = make_float2(ex2_of_capped(t.x), ex2_of_capped(t.y));
+  const float2 d = tp_add2(make_float2(1.0f, 1.0f), e);
+  s = make_float2(rcp_approx(d.x), rcp_approx(d.y));
+  rest = tp_mul2(e, s);
 }
 
 }  // namespace tp

@@ -1524,6 +1524,12 @@ def _gated_scan_inputs(gate, x, h0, lengths):
     return dev, dtype, lengths
 
 
+def _gated_scan_workspace(dev, B, T, C):
+    with _on(dev):
+        need = _lib.load().tp_gated_scan_workspace_bytes(B, T, C)
+    return (torch.empty(need, device=dev, dtype=torch.uint8) if need > 0 else None), need
+
+
 def _gated_scan_run(dev, dtype, lengths, code, gate, x, h0, need_states, need_last):
     B, T, C = x.shape
     gate, x, h0 = _channels(gate), _channels(x), _contiguous(h0)
@@ -1531,9 +1537,10 @@ def _gated_scan_run(dev, dtype, lengths, code, gate, x, h0, need_states, need_la
     last = torch.empty((B, C), device=dev, dtype=torch.float32) if need_last else None
     states = (torch.empty((B, -(-T // 64), C), device=dev, dtype=torch.float32)
               if need_states else None)
+    ws, need = _gated_scan_workspace(dev, B, T, C)
     _launch("tp_gated_scan_fwd", dev, dtype, code, B, T, C, gate.data_ptr(), gate.stride(0),
             gate.stride(1), x.data_ptr(), x.stride(0), x.stride(1), _at(h0), _at(lengths),
-            h.data_ptr(), _at(last), _at(states))
+            h.data_ptr(), _at(last), _at(states), _at(ws), need)
     return h, last, states
 
 
@@ -1542,9 +1549,10 @@ def _gated_scan_back(dev, dtype, lengths, code, states, dh, dh_last, gate, x, ne
     gate, x, dh, dh_last = _channels(gate), _channels(x), _contiguous(dh), _contiguous(dh_last)
     dgate, dx = _empty_as(x), _empty_as(x)
     dh0 = torch.empty((B, C), device=dev, dtype=torch.float32) if need_dh0 else None
+    ws, need = _gated_scan_workspace(dev, B, T, C)
     _launch("tp_gated_scan_bwd", dev, dtype, code, B, T, C, gate.data_ptr(), gate.stride(0),
             gate.stride(1), x.data_ptr(), x.stride(0), x.stride(1), _at(lengths), _at(states),
-            _at(dh), _at(dh_last), dgate.data_ptr(), dx.data_ptr(), _at(dh0))
+            _at(dh), _at(dh_last), dgate.data_ptr(), dx.data_ptr(), _at(dh0), _at(ws), need)
     return dgate, dx, dh0
 
 

@@ -73,16 +73,22 @@ def test_residual_norm_entry_refuses(lib):
 def test_gated_scan_entries_refuse(lib):
     def fwd(dtype=0, form=0, B=1, T=2, C=4, gate=P, sb=8, h=P):
         return lib.tp_gated_scan_fwd(dtype, form, B, T, C, gate, sb, 4, P, 8, 4, None, None, h,
-                                     None, None, None)
+                                     None, None, None, 0, None)
 
     assert fwd(B=-1) == -1 and fwd(T=-1) == -1 and fwd(C=-1) == -1 and fwd(sb=-1) == -1
     assert fwd(dtype=2) == -4 and fwd(form=2) == -1 and fwd(gate=None) == -2 and fwd(h=None) == -2
     assert fwd(B=0, gate=None, h=None) == 0 and fwd(C=0, gate=None, h=None) == 0
     assert fwd(B=2 ** 40) == -5
+    # one row of few channels over a long time is cut in time: runs in a workspace
+    need = lib.tp_gated_scan_workspace_bytes(1, 65536, 8)
+    assert need > 0 and need % (2 * 8 * 4) == 0
+    assert lib.tp_gated_scan_workspace_bytes(64, 1024, 640) == 0
+    assert lib.tp_gated_scan_workspace_bytes(-1, 1, 1) == -1
+    assert fwd(T=65536, C=8) == -7
 
     def bwd(states=P, dgate=P, form=1):
         return lib.tp_gated_scan_bwd(0, form, 1, 2, 4, P, 8, 4, P, 8, 4, None, states, None, None,
-                                     dgate, P, None, None)
+                                     dgate, P, None, None, 0, None)
 
     assert bwd(states=None) == -2 and bwd(dgate=None) == -2 and bwd(form=-1) == -1
 
