@@ -15,10 +15,12 @@
 // serialise; instead the tokens are sorted by id (a stable counting sort, so
 // equal ids keep their order) and the sorted rows summed in that order:
 //
-// 1. sort: the id is cut into one or two digits of at most 11 bits.  Per
-//    digit, one kernel counts the digits of each tile of tokens and one
-//    places them: each warp ranks its run of tokens 32 at a time by digit
-//    match, on top of the counts of earlier bins, tiles and warps.
+// 1. sort: the id is cut into one or two digits (three above 2^20 rows).  Per
+//    digit the tokens are counted by warp, and placed: each warp ranks its run of
+//    tokens 32 at a time by digit match, on top of the counts of earlier bins,
+//    blocks and warps.  Up to 2^18 tokens one cluster of up to 16 blocks does all
+//    of it in one launch (131072 tokens of 131072 rows: see sort_cluster_kernel);
+//    more take two kernels a digit over all SMs.
 // 2. sum: tokens and table rows form one list of N + V items (the tokens of a
 //    row, then the row's end).  Each team of threads takes an equal share of
 //    it, found by bisection, whatever the distribution of the ids: it adds a
@@ -41,59 +43,74 @@ __device__ __forceinline__ int64_t load_index(const void* p, int is64, int64_t i
 }
 
 // ---------------------------------------------------------------- forward
-template <typename T, int VEC>
+// A team of `lanes` threads takes TOK tokens and UV vectors of each at a time, so
+// that their loads are under way together.
+template <typename T, int VEC, int TOK, int UV>
 __global__ void __launch_bounds__(128) embedding_fwd_kernel(const EmbeddingArgs a, int lanes,
                                                             int* err) {
   using V = RowVec<T, VEC>;
-  constexpr int U = 4;
   const int t = threadIdx.x % lanes, per = blockDim.x / lanes;
   const int64_t nv = a.D / VEC;
-  for (int64_t i = (int64_t)blockIdx.x * per + threadIdx.x / lanes; i < a.N;
-       i += (int64_t)gridDim.x * per) {
-    const int64_t id = load_index(a.ids, a.ids64, i);
-    int64_t at = 0;
-    bool ok = id >= 0 && id < a.V;
-    if (a.pos_weight) {
-      at = a.positions ? load_index(a.positions, a.ids64, i) : i % a.T;
-      ok = ok && at >= 0 && at < a.L;
-    }
-    if (!ok && t == 0) tp_record_device_error(err, TP_DEVERR_INDEX);
-    const T* wr = (const T*)a.weight + (ok ? id * a.ldw : 0);
-    const T* pr = a.pos_weight ? (const T*)a.pos_weight + (ok ? at * a.ldp : 0) : nullptr;
-    T* o = (T*)a.out + i * a.D;
-    for (int64_t v0 = t; v0 < nv; v0 += U * lanes) {
-      V w[U], p[U];
+  for (int64_t i0 = ((int64_t)blockIdx.x * per + threadIdx.x / lanes) * TOK; i0 < a.N;
+       i0 += (int64_t)gridDim.x * per * TOK) {
+    const T* wr[TOK];
+    const T* pr[TOK];
+    bool ok[TOK];
 #pragma unroll
-      for (int k = 0; k < U; ++k) {
-        const int64_t v = v0 + k * lanes;
-        if (ok && v < nv) {
-          w[k].load(wr + v * VEC);
-          if (pr) p[k].load(pr + v * VEC);
-        }
+    for (int k = 0; k < TOK; ++k) {
+      const int64_t i = i0 + k < a.N ? i0 + k : i0;
+      const int64_t id = load_index(a.ids, a.ids64, i);
+      int64_t at = 0;
+      ok[k] = id >= 0 && id < a.V;
+      if (a.pos_weight) {
+        at = a.positions ? load_index(a.positions, a.ids64, i) : i % a.T;
+        ok[k] = ok[k] && at >= 0 && at < a.L;
       }
+      if (!ok[k] && t == 0) tp_record_device_error(err, TP_DEVERR_INDEX);
+      wr[k] = (const T*)a.weight + (ok[k] ? id * a.ldw : 0);    // read only if ok
+      pr[k] = (const T*)a.pos_weight + (ok[k] ? at * a.ldp : 0);
+    }
+    for (int64_t v0 = t; v0 < nv; v0 += UV * lanes) {
+      V w[TOK][UV], p[TOK][UV];
 #pragma unroll
-      for (int k = 0; k < U; ++k) {
-        const int64_t v = v0 + k * lanes;
-        if (v >= nv) break;
-        float f[VEC];
-        w[k].get(f);
-        if (pr) {
-          float q[VEC];
-          p[k].get(q);
-          // product and sum rounded one by one, as the unfused expression
+      for (int k = 0; k < TOK; ++k)
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) f[j] = __fadd_rn(__fmul_rn(f[j], a.scale), q[j]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) f[j] = __fmul_rn(f[j], a.scale);
+        for (int u = 0; u < UV; ++u) {
+          const int64_t v = v0 + u * lanes;
+          w[k][u].zero();
+          p[k][u].zero();
+          if (ok[k] && v < nv) {
+            w[k][u].load(wr[k] + v * VEC);
+            if (a.pos_weight) p[k][u].load(pr[k] + v * VEC);
+          }
         }
-        if (!ok) {
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) f[j] = __int_as_float(0x7fc00000);
+      for (int k = 0; k < TOK; ++k) {
+        if (i0 + k >= a.N) break;
+#pragma unroll
+        for (int u = 0; u < UV; ++u) {
+          const int64_t v = v0 + u * lanes;
+          if (v >= nv) break;
+          float f[VEC];
+          w[k][u].get(f);
+          if (a.pos_weight) {
+            float q[VEC];
+            p[k][u].get(q);
+            // product and sum rounded one by one, as the unfused expression
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) f[j] = __fadd_rn(__fmul_rn(f[j], a.scale), q[j]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) f[j] = __fmul_rn(f[j], a.scale);
+          }
+          if (!ok[k]) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) f[j] = __int_as_float(0x7fc00000);
+          }
+          V r;
+          r.set(f);
+          r.store((T*)a.out + (i0 + k) * a.D + v * VEC);
         }
-        V r;
-        r.set(f);
-        r.store(o + v * VEC);
       }
     }
   }
@@ -105,7 +122,20 @@ constexpr int SORT_WARPS = SORT_THREADS / 32;
 constexpr int SORT_MAX_BITS = 11;
 constexpr int64_t SORT_MAX_TILES = 128;
 
+// Lanes of the warp whose token has this lane's digit (0 where `in` is false), by
+// one vote per bit: several times faster than __match_any_sync on many different
+// digits.
+__device__ __forceinline__ unsigned same_digit(bool in, int d, int bits) {
+  unsigned m = __ballot_sync(0xffffffffu, in);
+  for (int b = 0; b < bits; ++b) {
+    const unsigned set = __ballot_sync(0xffffffffu, (d >> b) & 1);
+    m &= (d >> b) & 1 ? set : ~set;
+  }
+  return in ? m : 0u;
+}
+
 struct SortPlan {
+  int cluster;      // blocks of sort_cluster_kernel (0: the two-kernel sort)
   int64_t tile;     // tokens per block, a multiple of 32 * SORT_WARPS
   int tiles;
   int passes, bits; // digits per key, bits per digit
@@ -115,7 +145,15 @@ SortPlan sort_plan(int64_t N, int64_t V) {
   SortPlan p;
   int bits = 1;
   while (((int64_t)1 << bits) <= V) ++bits;     // keys 0 .. V (V: not in the table)
-  p.passes = bits <= SORT_MAX_BITS ? 1 : (bits <= 2 * SORT_MAX_BITS ? 2 : 3);
+  p.cluster = 0;
+  const int most = N <= ((int64_t)1 << 18) ? 10 : SORT_MAX_BITS;
+  p.passes = (bits + most - 1) / most;
+  if (most == 10 && p.passes <= 3) {
+    p.cluster = 1;         // a block per 4096 tokens
+    while (p.cluster < 16 && (int64_t)p.cluster * 4096 < N) p.cluster *= 2;
+  } else {
+    p.passes = (bits + SORT_MAX_BITS - 1) / SORT_MAX_BITS;
+  }
   p.bits = (bits + p.passes - 1) / p.passes;
   const int64_t unit = 32 * SORT_WARPS;
   p.tile = 8 * unit;                            // 2048 tokens
@@ -129,20 +167,22 @@ struct SortArgs {
   const void* ids;        // first pass: the caller's ids
   int ids64;
   int64_t V, padding_idx;
-  const int* keys_in;     // later passes: keys and token numbers of the pass before
-  const int* toks_in;
-  int* keys_out;
-  int* toks_out;
+  const int2* in;         // later passes: (key, token) of the pass before
+  int2* out;
   int* hist;              // [tiles][bins]
   int64_t N, tile;
-  int tiles, shift, bins;
+  int tiles, shift, bins, bits;
   int first;
 };
 
+// V for what is not in the table or gets no gradient: sorted behind the rows
+__device__ __forceinline__ int key_of(int64_t id, int64_t V, int64_t padding_idx) {
+  return (id < 0 || id >= V || id == padding_idx) ? (int)V : (int)id;
+}
+
 __device__ __forceinline__ int sort_key(const SortArgs& s, int64_t i) {
-  if (!s.first) return s.keys_in[i];
-  const int64_t id = load_index(s.ids, s.ids64, i);
-  return (id < 0 || id >= s.V || id == s.padding_idx) ? (int)s.V : (int)id;
+  if (!s.first) return s.in[i].x;
+  return key_of(load_index(s.ids, s.ids64, i), s.V, s.padding_idx);
 }
 
 __global__ void __launch_bounds__(SORT_THREADS) sort_count_kernel(const SortArgs s) {
@@ -228,25 +268,179 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_place_kernel(const SortArgs
     const int64_t i = i0 + lane;
     const bool in = i < hi;
     const int key = in ? sort_key(s, i) : -1;
-    const int d = in ? (key >> s.shift) & (s.bins - 1) : -1;
-    const unsigned same = __match_any_sync(0xffffffffu, d);
+    const int d = in ? (key >> s.shift) & (s.bins - 1) : 0;
+    const unsigned same = same_digit(in, d, s.bits);
     const int rank = __popc(same & ((1u << lane) - 1u));
     int at = 0;
     if (in) at = mine[d] + rank;
     __syncwarp();
     if (in) {
       if (rank == 0) mine[d] += __popc(same);
-      s.keys_out[at] = key;
-      s.toks_out[at] = s.first ? (int)i : s.toks_in[i];
+      s.out[at] = make_int2(key, s.first ? (int)i : s.in[i].y);
     }
     __syncwarp();
   }
 }
 
+// The whole sort in one launch: a cluster of S blocks of 32 warps, each warp a
+// contiguous run of tokens.  The blocks exchange their counts and their output
+// through global memory (L2), with a cluster barrier between.
+constexpr int SC_THREADS = 1024, SC_WARPS = 32;
+constexpr int SC_MAX_BITS = 10;
+constexpr int SC_GROUPS = 4;
+
+struct ClusterSortArgs {
+  const void* ids;
+  int ids64;
+  int64_t V, padding_idx;
+  int2* pairs[2];         // (key, token)
+  int* hist;              // [passes][S][bins]
+  int64_t N;
+  int passes, bits, S;
+};
+
+__device__ __forceinline__ void sc_cluster_sync(int S) {
+  if (S > 1)
+    asm volatile(
+        "barrier.cluster.arrive.release.aligned;\n\t"
+        "barrier.cluster.wait.acquire.aligned;" ::
+            : "memory");
+  else
+    __syncthreads();
+}
+
+__global__ void __launch_bounds__(SC_THREADS) sort_cluster_kernel(const ClusterSortArgs s) {
+  extern __shared__ uint16_t s_runs[];          // [SC_WARPS][bins]: of a warp, then before it
+  __shared__ int s_base[1 << SC_MAX_BITS], s_warp[SC_WARPS];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int bins = 1 << s.bits;
+  const int64_t share = ceil_div(s.N, (int64_t)s.S);
+  const int64_t run = ceil_div(share, (int64_t)(32 * SC_WARPS)) * 32;   // tokens of a warp
+  const int64_t lo = min(s.N, ((int64_t)blockIdx.x * SC_WARPS + warp) * run);
+  const int64_t hi = min(s.N, lo + run);
+  uint16_t* const mine = s_runs + warp * bins;
+  for (int pass = 0; pass < s.passes; ++pass) {
+    const int2* const in_pairs = s.pairs[(pass & 1) ^ 1];
+    int2* const out_pairs = s.pairs[pass & 1];
+    const int shift = pass * s.bits;
+    auto pair_at = [&](int64_t i) {
+      if (pass > 0) return __ldcg(in_pairs + i);
+      return make_int2(key_of(load_index(s.ids, s.ids64, i), s.V, s.padding_idx), (int)i);
+    };
+    for (int b = threadIdx.x; b < SC_WARPS * bins / 2; b += SC_THREADS)
+      reinterpret_cast<unsigned*>(s_runs)[b] = 0;
+    __syncthreads();
+    // counts of this warp's run (16 bits each, two in a word)
+    for (int64_t i0 = lo; i0 < hi; i0 += 32 * SC_GROUPS) {
+      int key[SC_GROUPS];
+#pragma unroll
+      for (int k = 0; k < SC_GROUPS; ++k)
+        key[k] = i0 + k * 32 + lane < hi ? pair_at(i0 + k * 32 + lane).x : -1;
+#pragma unroll
+      for (int k = 0; k < SC_GROUPS; ++k) {
+        const int d = (key[k] >> shift) & (bins - 1);
+        if (key[k] >= 0)
+          atomicAdd(reinterpret_cast<unsigned*>(mine) + (d >> 1), 1u << ((d & 1) * 16));
+      }
+    }
+    __syncthreads();
+    int* const hist = s.hist + (int64_t)pass * s.S * bins;
+    for (int b = threadIdx.x; b < bins; b += SC_THREADS) {
+      int n = 0;
+#pragma unroll 8
+      for (int w = 0; w < SC_WARPS; ++w) {
+        const int c = s_runs[w * bins + b];
+        s_runs[w * bins + b] = (uint16_t)n;     // at most 2^18 / 16 tokens in a block
+        n += c;
+      }
+      __stcg(hist + blockIdx.x * bins + b, n);
+    }
+    sc_cluster_sync(s.S);
+    // start of each bin: all tokens of lower bins, then this bin's of earlier blocks
+    // (at most as many bins as threads)
+    int all = 0, earlier = 0;
+    if (threadIdx.x < bins) {
+#pragma unroll 4
+      for (int q = 0; q < s.S; ++q) {
+        const int n = __ldcg(hist + q * bins + threadIdx.x);
+        all += n;
+        if (q < (int)blockIdx.x) earlier += n;
+      }
+    }
+    int inc = all;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int n = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += n;
+    }
+    if (lane == 31) s_warp[warp] = inc;
+    __syncthreads();
+    if (warp == 0) {
+      int v = s_warp[lane];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int n = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += n;
+      }
+      s_warp[lane] = v;
+    }
+    __syncthreads();
+    if (threadIdx.x < bins)
+      s_base[threadIdx.x] = (warp > 0 ? s_warp[warp - 1] : 0) + inc - all + earlier;
+    __syncthreads();
+    // place this warp's run in order
+    for (int64_t i0 = lo; i0 < hi; i0 += 32 * SC_GROUPS) {
+      int2 pair[SC_GROUPS];
+#pragma unroll
+      for (int k = 0; k < SC_GROUPS; ++k) {
+        const int64_t i = i0 + k * 32 + lane;
+        pair[k] = i < hi ? pair_at(i) : make_int2(-1, 0);
+      }
+#pragma unroll
+      for (int k = 0; k < SC_GROUPS; ++k) {
+        if (i0 + k * 32 >= hi) break;
+        const bool in = pair[k].x >= 0;
+        const int d = in ? (pair[k].x >> shift) & (bins - 1) : 0;
+        const unsigned same = same_digit(in, d, s.bits);
+        const int rank = __popc(same & ((1u << lane) - 1u));
+        int at = 0;
+        if (in) at = s_base[d] + mine[d] + rank;
+        __syncwarp();
+        if (in) {
+          if (rank == 0) mine[d] += (uint16_t)__popc(same);
+          __stcg(out_pairs + at, pair[k]);
+        }
+        __syncwarp();
+      }
+    }
+    if (pass + 1 < s.passes) sc_cluster_sync(s.S);
+  }
+}
+
+// Up to 1024 tokens: one block, each thread counts the tokens before its own.
+constexpr int64_t SMALL_TOKENS = 1024;
+__global__ void __launch_bounds__(SMALL_TOKENS) sort_small_kernel(const void* ids, int ids64,
+                                                                  int N, int64_t V,
+                                                                  int64_t padding_idx,
+                                                                  int2* out) {
+  __shared__ __align__(16) int s_key[SMALL_TOKENS];
+  const int i = threadIdx.x;
+  const int key = i < N ? key_of(load_index(ids, ids64, i), V, padding_idx) : 0x7fffffff;
+  s_key[i] = key;
+  __syncthreads();
+  if (i >= N) return;
+  int rank = 0;
+  for (int j = 0; j < N; j += 4) {        // (places behind N hold the largest key)
+    const int4 k = *reinterpret_cast<const int4*>(s_key + j);
+    rank += (k.x < key || (k.x == key && j < i)) + (k.y < key || (k.y == key && j + 1 < i)) +
+            (k.z < key || (k.z == key && j + 2 < i)) + (k.w < key || (k.w == key && j + 3 < i));
+  }
+  out[rank] = make_int2(key, i);
+}
+
 // ---------------------------------------------------------------- sum
 struct SumArgs {
-  const int* keys;      // sorted; V: dropped
-  const int* toks;
+  const int2* pairs;    // (key, token), sorted by key; V: dropped
   int64_t N, V, D;
   const void* dout;
   float scale;
@@ -256,21 +450,30 @@ struct SumArgs {
   int lanes;            // threads of a team
   float* head;          // [shares][D]: end of a row begun in an earlier share
   float* tail;          // [shares][D]: begin of a row that ends in a later share
+  int64_t* rows;        // [shares]: the first row of the share
   int* flags;           // [shares]: bit 0 the first row began earlier, bit 1 an end lies inside
 };
 
 // Tokens among the first `d` items of the list (the tokens of row 0, the end of
 // row 0, the tokens of row 1, ...): the smallest j with keys[j] + j >= d, as
-// token j is item keys[j] + j.
-__device__ __forceinline__ int64_t tokens_before(const int* keys, int64_t N, int64_t d) {
-  int64_t lo = 0, hi = min(N, d);
+// token j is item keys[j] + j.  A whole warp searches, 32 places at a time.
+__device__ __forceinline__ int64_t tokens_before(const int2* pairs, int64_t N, int64_t d) {
+  const int lane = threadIdx.x & 31;
+  int64_t lo = 0, hi = min(N, d);            // the answer lies in [lo, hi]
   while (lo < hi) {
-    const int64_t mid = (lo + hi) >> 1;
-    if ((int64_t)__ldg(keys + mid) + mid >= d) hi = mid;
-    else lo = mid + 1;
+    const int64_t step = (hi - lo + 31) / 32;
+    const int64_t at = lo + lane * step;     // 32 places cover [lo, hi)
+    const bool below = at < hi && (int64_t)__ldg(pairs + at).x + at < d;
+    const int n = __popc(__ballot_sync(0xffffffffu, below));   // below for the first n lanes
+    if (n == 0) return lo;
+    const int64_t last = lo + (n - 1) * step;                  // the last place known below
+    hi = min(hi, last + step);
+    lo = last + 1;
   }
   return lo;
 }
+
+constexpr int SUM_CHUNK = 128;
 
 // A team's share of the columns [blockIdx.y * lanes * VEC, ...) of its items.
 template <typename T, int VEC>
@@ -282,15 +485,18 @@ __global__ void __launch_bounds__(256) embedding_sum_kernel(const SumArgs s) {
   if (share >= s.shares) return;
   const int64_t items = s.N + s.V;
   const int64_t d0 = share * s.share, d1 = min(items, d0 + s.share);
-  int64_t j = tokens_before(s.keys, s.N, d0);
-  const int64_t j1 = tokens_before(s.keys, s.N, d1);
+  int64_t j = tokens_before(s.pairs, s.N, d0);
+  const int64_t j1 = tokens_before(s.pairs, s.N, d1);
   int64_t v = d0 - j;
   const int64_t v1 = d1 - j1;          // rows whose end lies before d1
   const int64_t c = ((int64_t)blockIdx.y * s.lanes + t) * VEC;
   const bool in = c < s.D;
   // the first row continues one of an earlier share
-  bool open = j > 0 && v < s.V && s.keys[j - 1] == v;
-  if (t == 0 && blockIdx.y == 0) s.flags[share] = (open ? 1 : 0) | (v1 > v ? 2 : 0);
+  bool open = j > 0 && v < s.V && s.pairs[j - 1].x == v;
+  if (t == 0 && blockIdx.y == 0) {
+    s.flags[share] = (open ? 1 : 0) | (v1 > v ? 2 : 0);
+    s.rows[share] = v;
+  }
   const T* dout = (const T*)s.dout + c;
   T* dw = (T*)s.dweight + c;
   float acc[VEC];
@@ -314,30 +520,43 @@ __global__ void __launch_bounds__(256) embedding_sum_kernel(const SumArgs s) {
 #pragma unroll
     for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
   };
-  while (j < j1) {
-    V row[U];
-    int key[U];
-    const int n = (int)min((int64_t)U, j1 - j);
+  // pairs of 128 tokens at a time in shared memory, a copy for each warp
+  __shared__ int2 s_pairs[8][SUM_CHUNK];
+  int2* const pairs = s_pairs[threadIdx.x >> 5];
+  const int lane = threadIdx.x & 31;
+  for (; j < j1; j += SUM_CHUNK) {
+    const int m = (int)min((int64_t)SUM_CHUNK, j1 - j);
+    __syncwarp();
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (u < n) {
-        key[u] = __ldg(s.keys + j + u);
-        if (in && key[u] < s.V) row[u].load_stream(dout + (int64_t)__ldg(s.toks + j + u) * s.D);
+    for (int k = 0; k < SUM_CHUNK / 32; ++k)
+      if (k * 32 + lane < m) pairs[k * 32 + lane] = __ldg(s.pairs + j + k * 32 + lane);
+    __syncwarp();
+#pragma unroll 1
+    for (int i = 0; i < m; i += U) {
+      V row[U];
+      const int n = min(U, m - i);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (u < n) {
+          const int2 p = pairs[i + u];
+          if (in && p.x < s.V) row[u].load_stream(dout + (int64_t)p.y * s.D);
+        }
       }
-    }
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (u < n && key[u] < s.V) {
-        while (v < key[u]) end_row();
-        if (in) {
-          float f[VEC];
-          row[u].get(f);
+      for (int u = 0; u < U; ++u) {
+        if (u < n) {
+          const int key = pairs[i + u].x;
+          if (key >= s.V) break;             // dropped tokens come last
+          while (v < key) end_row();
+          if (in) {
+            float f[VEC];
+            row[u].get(f);
 #pragma unroll
-          for (int k = 0; k < VEC; ++k) acc[k] += f[k];
+            for (int k = 0; k < VEC; ++k) acc[k] += f[k];
+          }
         }
       }
     }
-    j += n;
   }
   while (v < v1) end_row();
   if (in) {
@@ -348,62 +567,113 @@ __global__ void __launch_bounds__(256) embedding_sum_kernel(const SumArgs s) {
 
 // Rows over several shares: the share that ends such a row (its first row is
 // open and it has an end) adds the tails of the shares before it, in order,
-// and its head.
+// and its head.  A block per share; a row over more than 16 shares takes one per
+// 256 columns, whose warps add contiguous parts of the shares.
 template <typename T>
-__global__ void __launch_bounds__(128) embedding_join_kernel(const SumArgs s) {
+__global__ void __launch_bounds__(256) embedding_join_kernel(const SumArgs s) {
   const int64_t share = blockIdx.x;
   if (s.flags[share] != 3) return;
-  __shared__ long long s_first;
-  if (threadIdx.x == 0) {
-    int64_t p = share - 1;
-    while (p > 0 && s.flags[p] == 1) --p;     // shares wholly inside the row
-    s_first = p;
+  __shared__ int s_first[8];
+  __shared__ float s_part[8][256];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // the share in which the row began: back over shares wholly inside it (flag 1)
+  int64_t first = share - 1;
+  for (int64_t p0 = share - 1;; p0 -= 256) {
+    const int64_t p = p0 - threadIdx.x;
+    const bool stop = p <= 0 || s.flags[p] != 1;
+    const unsigned any = __ballot_sync(0xffffffffu, stop);
+    if (lane == 0) s_first[warp] = any ? warp * 32 + __ffs(any) - 1 : 256;
+    __syncthreads();
+    int at = 256;
+#pragma unroll
+    for (int w = 7; w >= 0; --w) at = s_first[w] < 256 ? s_first[w] : at;
+    __syncthreads();
+    first = p0 - at;
+    if (at < 256) break;
   }
+  T* const out = (T*)s.dweight + s.rows[share] * s.D;
+  const float* const head = s.head + share * s.D;
+  RowVec<T, 1> r;
+  if (share - first <= 16) {
+    if (blockIdx.y > 0) return;
+    for (int64_t c = threadIdx.x; c < s.D; c += 256) {
+      float t = 0.f;
+#pragma unroll 4
+      for (int64_t p = first; p < share; ++p) t += s.tail[p * s.D + c];
+      t = (t + head[c]) * s.scale;
+      r.set(&t);
+      r.store(out + c);
+    }
+    return;
+  }
+  const int64_t c0 = (int64_t)blockIdx.y * 256;
+  const int64_t per = (share - first + 7) / 8;
+  const int64_t lo = min(share, first + warp * per), hi = min(share, lo + per);
+  float acc[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) acc[j] = 0.f;
+#pragma unroll 4
+  for (int64_t p = lo; p < hi; ++p)
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (c0 + j * 32 + lane < s.D) acc[j] += s.tail[p * s.D + c0 + j * 32 + lane];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) s_part[warp][j * 32 + lane] = acc[j];
   __syncthreads();
-  const int64_t first = s_first;
-  const int64_t j = tokens_before(s.keys, s.N, share * s.share);
-  const int64_t v = share * s.share - j;
-  for (int64_t c = threadIdx.x; c < s.D; c += blockDim.x) {
-    float acc = 0.f;
-#pragma unroll 8
-    for (int64_t p = first; p < share; ++p) acc += s.tail[p * s.D + c];
-    acc = (acc + s.head[share * s.D + c]) * s.scale;
-    RowVec<T, 1> r;
-    r.set(&acc);
-    r.store((T*)s.dweight + v * s.D + c);
-  }
+  const int64_t c = c0 + threadIdx.x;
+  if (c >= s.D) return;
+  float t = 0.f;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) t += s_part[w][threadIdx.x];
+  t = (t + head[c]) * s.scale;
+  r.set(&t);
+  r.store(out + c);
 }
 
 // ---------------------------------------------------------------- positions
-// dpos[t] = sum over the sequences of dout[., t]: 8 warps take contiguous
-// ranges of the sequences for 32 vectors of one position.
-template <typename T, int VEC>
-__global__ void __launch_bounds__(256) embedding_pos_kernel(int64_t B, int64_t steps, int64_t D,
-                                                            const T* __restrict__ dout, T* dpos) {
+// dpos[t] = sum over the sequences of dout[., t].  SPLIT: the block's 8 warps take
+// contiguous ranges of the sequences for 32 vectors of one position; else each
+// warp has 32 vectors of its own and adds all sequences.
+template <typename T, int VEC, bool SPLIT>
+__global__ void __launch_bounds__(256) embedding_pos_kernel(int64_t B, int64_t steps, int64_t L,
+                                                            int64_t D,
+                                                            const T* __restrict__ dout,
+                                                            T* dpos) {
   using V = RowVec<T, VEC>;
-  __shared__ float s[8][32 * VEC];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t t = blockIdx.x;
+  const int64_t t = SPLIT ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 8 + warp;
   const int64_t c = ((int64_t)blockIdx.y * 32 + lane) * VEC;
   float acc[VEC];
 #pragma unroll
   for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
+  const int64_t per = (B + 7) / 8, lo = SPLIT ? warp * per : 0;
+  const int64_t hi = SPLIT ? min(B, lo + per) : B;
   if (t < steps && c < D) {
-    const int64_t per = (B + 7) / 8, lo = warp * per, hi = min(B, lo + per);
-#pragma unroll 4
-    for (int64_t b = lo; b < hi; ++b) {
-      V r;
-      float f[VEC];
-      r.load(dout + (b * steps + t) * D + c);
-      r.get(f);
+    const T* p = dout + (lo * steps + t) * D + c;
+    for (int64_t b = lo; b < hi; b += 8) {
+      V r[8];
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) acc[k] += f[k];
+      for (int u = 0; u < 8; ++u) {
+        r[u].zero();
+        if (b + u < hi) r[u].load(p);
+        p += steps * D;
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        float f[VEC];
+        r[u].get(f);
+        if (b + u < hi)
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) acc[k] += f[k];
+      }
     }
   }
+  if constexpr (SPLIT) {
+    __shared__ float s[8][32 * VEC];
 #pragma unroll
-  for (int k = 0; k < VEC; ++k) s[warp][lane * VEC + k] = acc[k];
-  __syncthreads();
-  if (warp == 0 && c < D) {
+    for (int k = 0; k < VEC; ++k) s[warp][lane * VEC + k] = acc[k];
+    __syncthreads();
+    if (warp != 0) return;
 #pragma unroll
     for (int k = 0; k < VEC; ++k) {
       float v = 0.f;
@@ -411,6 +681,8 @@ __global__ void __launch_bounds__(256) embedding_pos_kernel(int64_t B, int64_t s
       for (int w = 0; w < 8; ++w) v += s[w][lane * VEC + k];
       acc[k] = v;
     }
+  }
+  if (t < L && c < D) {
     V r;
     r.set(acc);
     r.store(dpos + t * D + c);
@@ -431,29 +703,47 @@ bool vec_ok(int64_t D, std::initializer_list<const void*> ps,
 
 int64_t round16(int64_t n) { return (n + 15) & ~(int64_t)15; }
 
+// Threads of a team: whole warps over the row's vectors, at most 256 a column range.
+int sum_lanes(int64_t D, int vec, int64_t* ranges) {
+  const int64_t nv = ceil_div(D, (int64_t)vec);
+  *ranges = ceil_div(nv, (int64_t)256);
+  return (int)(ceil_div(ceil_div(nv, *ranges), (int64_t)32) * 32);
+}
+
+// Teams of a block: at least 128 threads.
+int sum_teams(int lanes) { return lanes >= 128 ? 1 : 128 / lanes; }
+
 struct SumPlan {
   int64_t share, shares;
 };
 
-// About twelve shares per SM (teams that wait on loads overlap), at least 16
-// items each so that partial sums stay few.
-SumPlan sum_plan(int64_t N, int64_t V) {
+// As many shares as teams fit at once (819 threads of 80 registers on an SM), so
+// that there is one wave of them and each searches its place once; at least 16
+// items each, so that partial sums stay few (two or four waves: the sums of 60 x 4096 tokens
+// 83, 85 and 92 us, their joins 8, 14 and 25 us).  By the sizes alone.
+SumPlan sum_plan(int64_t N, int64_t V, int64_t D, int esize) {
   const int64_t items = N + V;
-  const int64_t want = (int64_t)num_sms() * 12;
-  int64_t share = ceil_div(items, want);
+  int64_t ranges;
+  const int lanes = sum_lanes(D, 16 / esize, &ranges);
+  const int per = sum_teams(lanes);
+  int64_t teams = 819 / (lanes * per) * per / ranges;
+  if (teams < 1) teams = 1;
+  int64_t share = ceil_div(items, num_sms() * teams);
   if (share < 16) share = 16;
   return {share, ceil_div(items, share)};
 }
 
 struct Workspace {
-  int *keys[2], *toks[2], *hist, *flags;
+  int2* pairs[2];
+  int *hist, *flags;
+  int64_t* rows;
   float *head, *tail;
   int64_t bytes;
 };
 
-Workspace layout(int64_t N, int64_t V, int64_t D, void* base) {
+Workspace layout(int64_t N, int64_t V, int64_t D, int esize, void* base) {
   const SortPlan sp = sort_plan(N, V);
-  const SumPlan su = sum_plan(N, V);
+  const SumPlan su = sum_plan(N, V, D, esize);
   Workspace w;
   char* p = (char*)base;
   auto take = [&](int64_t bytes) {
@@ -461,46 +751,87 @@ Workspace layout(int64_t N, int64_t V, int64_t D, void* base) {
     p += round16(bytes);
     return (void*)q;
   };
-  for (int k = 0; k < 2; ++k) {
-    w.keys[k] = (int*)take(N * 4);
-    w.toks[k] = (int*)take(N * 4);
-  }
-  w.hist = (int*)take((int64_t)sp.tiles * (4 << sp.bits));
+  for (int k = 0; k < 2; ++k) w.pairs[k] = (int2*)take(N * 8);
+  w.hist = (int*)take((int64_t)(sp.cluster ? sp.cluster * sp.passes : sp.tiles) * (4 << sp.bits));
   w.flags = (int*)take(su.shares * 4);
+  w.rows = (int64_t*)take(su.shares * 8);
   w.head = (float*)take(su.shares * D * 4);
   w.tail = (float*)take(su.shares * D * 4);
   w.bytes = p - (char*)base;
   return w;
 }
 
+// Few tokens: a block per token, so that each row's loads are issued at once.
+// Many: a warp takes four rows of up to 64 vectors, or four vectors of a longer
+// row, at a time (32 x 4096 tokens of 1024 bf16 channels: 61 us against 70 us with
+// four rows; 16 x 2048 of 512: 18 and 15 us).
+template <typename T, int VEC>
+int fwd_rows(const EmbeddingArgs& a, int* err, cudaStream_t stream) {
+  const bool many = a.N >= 16 * (int64_t)num_sms(), rows = many && a.D / VEC <= 64;
+  const int lanes = many ? 32 : 128;
+  const int64_t want = ceil_div(a.N, rows ? (int64_t)16 : (many ? (int64_t)4 : (int64_t)1));
+  const int64_t cap = (int64_t)num_sms() * 64;
+  const unsigned grid = (unsigned)(want < cap ? want : cap);
+  if (rows) embedding_fwd_kernel<T, VEC, 4, 1><<<grid, 128, 0, stream>>>(a, lanes, err);
+  else embedding_fwd_kernel<T, VEC, 1, 4><<<grid, 128, 0, stream>>>(a, lanes, err);
+  return launch_status();
+}
+
 template <typename T>
 int fwd(const EmbeddingArgs& a, cudaStream_t stream) {
   int* err = device_error_ptr();
-  // a warp per token; few tokens: a block per token, so that each row's loads
-  // are issued at once
-  const int lanes = a.N >= 8 * (int64_t)num_sms() ? 32 : 128;
-  const int64_t want = ceil_div(a.N, (int64_t)(128 / lanes)), cap = (int64_t)num_sms() * 64;
-  const unsigned grid = (unsigned)(want < cap ? want : cap);
   constexpr int WIDE = 16 / sizeof(T);
   if (vec_ok<T, WIDE>(a.D, {a.weight, a.pos_weight, a.out}, {a.ldw, a.pos_weight ? a.ldp : 0}))
-    embedding_fwd_kernel<T, WIDE><<<grid, 128, 0, stream>>>(a, lanes, err);
-  else
-    embedding_fwd_kernel<T, 1><<<grid, 128, 0, stream>>>(a, lanes, err);
-  return launch_status();
+    return fwd_rows<T, WIDE>(a, err, stream);
+  return fwd_rows<T, 1>(a, err, stream);
 }
 
 template <typename T, int VEC>
 int sum(SumArgs s, cudaStream_t stream) {
-  const int64_t nv = ceil_div(s.D, (int64_t)VEC);
-  // whole warps over the row's vectors, at most 256 threads a column range
-  const int64_t ranges = ceil_div(nv, (int64_t)256);
-  s.lanes = (int)(ceil_div(ceil_div(nv, ranges), (int64_t)32) * 32);
-  const int per = s.lanes >= 128 ? 1 : 128 / s.lanes;
+  int64_t ranges;
+  s.lanes = sum_lanes(s.D, VEC, &ranges);
+  const int per = sum_teams(s.lanes);
   const int threads = s.lanes * per;
   const dim3 grid((unsigned)ceil_div(s.shares, (int64_t)per), (unsigned)ranges);
   embedding_sum_kernel<T, VEC><<<grid, threads, 0, stream>>>(s);
-  embedding_join_kernel<T><<<(unsigned)s.shares, 128, 0, stream>>>(s);
+  const dim3 join((unsigned)s.shares, (unsigned)ceil_div(s.D, (int64_t)256));
+  embedding_join_kernel<T><<<join, 256, 0, stream>>>(s);
   return launch_status();
+}
+
+int sort_in_cluster(const SortPlan& p, const Workspace& w, const void* ids, int ids64, int64_t N,
+                    int64_t V, int64_t padding_idx, cudaStream_t stream) {
+  ClusterSortArgs s;
+  s.ids = ids;
+  s.ids64 = ids64;
+  s.V = V;
+  s.padding_idx = padding_idx;
+  for (int k = 0; k < 2; ++k) s.pairs[k] = w.pairs[k];
+  s.hist = w.hist;
+  s.N = N;
+  s.passes = p.passes;
+  s.bits = p.bits;
+  s.S = p.cluster;
+  const size_t smem = sizeof(uint16_t) * SC_WARPS * ((size_t)1 << p.bits);
+  cudaError_t e = cudaFuncSetAttribute((const void*)sort_cluster_kernel,
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e == cudaSuccess && p.cluster > 8)
+    e = cudaFuncSetAttribute((const void*)sort_cluster_kernel,
+                             cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e != cudaSuccess) return cuda_status(e);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)p.cluster);
+  cfg.blockDim = dim3(SC_THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)p.cluster;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = p.cluster > 1 ? 1 : 0;
+  return cuda_status(cudaLaunchKernelEx(&cfg, sort_cluster_kernel, s));
 }
 
 template <typename T>
@@ -510,18 +841,29 @@ int sum_any(const SumArgs& s, cudaStream_t stream) {
   return sum<T, 1>(s, stream);
 }
 
+template <typename T, int VEC>
+int pos_rows(int64_t B, int64_t steps, int64_t D, const void* dout, int64_t L, void* dpos,
+             cudaStream_t stream) {
+  const unsigned columns = (unsigned)ceil_div(D, (int64_t)32 * VEC);
+  // few positions and many sequences: the sequences are shared out as well
+  if (B > 8 && steps * columns < 8 * (int64_t)num_sms())
+    embedding_pos_kernel<T, VEC, true><<<dim3((unsigned)L, columns), 256, 0, stream>>>(
+        B, steps, L, D, (const T*)dout, (T*)dpos);
+  else
+    embedding_pos_kernel<T, VEC, false>
+        <<<dim3((unsigned)ceil_div(L, (int64_t)8), columns), 256, 0, stream>>>(
+            B, steps, L, D, (const T*)dout, (T*)dpos);
+  return launch_status();
+}
+
 template <typename T>
 int pos(int64_t N, int64_t steps, int64_t D, const void* dout, int64_t L, void* dpos,
         cudaStream_t stream) {
   constexpr int WIDE = 16 / sizeof(T);
   const int64_t B = steps > 0 ? N / steps : 0;
   if (vec_ok<T, WIDE>(D, {dout, dpos}, {}))
-    embedding_pos_kernel<T, WIDE><<<dim3((unsigned)L, (unsigned)ceil_div(D, (int64_t)32 * WIDE)),
-                                    256, 0, stream>>>(B, steps, D, (const T*)dout, (T*)dpos);
-  else
-    embedding_pos_kernel<T, 1><<<dim3((unsigned)L, (unsigned)ceil_div(D, (int64_t)32)), 256, 0,
-                                 stream>>>(B, steps, D, (const T*)dout, (T*)dpos);
-  return launch_status();
+    return pos_rows<T, WIDE>(B, steps, D, dout, L, dpos, stream);
+  return pos_rows<T, 1>(B, steps, D, dout, L, dpos, stream);
 }
 
 }  // namespace
@@ -531,14 +873,16 @@ int launch_embedding_fwd(const EmbeddingArgs& a, cudaStream_t stream) {
 }
 
 int64_t embedding_bwd_workspace_bytes(int64_t N, int64_t V, int64_t D) {
-  return layout(N, V, D, nullptr).bytes;
+  const int64_t a = layout(N, V, D, 4, nullptr).bytes, b = layout(N, V, D, 2, nullptr).bytes;
+  return a > b ? a : b;
 }
 
 int launch_embedding_bwd(int dtype, int ids64, int64_t N, int64_t D, const void* ids,
                          const void* dout, int64_t V, float scale, int64_t padding_idx,
                          void* dweight, void* workspace, cudaStream_t stream) {
   const SortPlan p = sort_plan(N, V);
-  const Workspace w = layout(N, V, D, workspace);
+  const int esize = dtype == TP_DTYPE_F32 ? 4 : 2;
+  const Workspace w = layout(N, V, D, esize, workspace);
   const int bins = 1 << p.bits;
   const size_t place_smem = sizeof(int) * SORT_WARPS * bins;
   if (place_smem > 48 * 1024) {
@@ -547,33 +891,38 @@ int launch_embedding_bwd(int dtype, int ids64, int64_t N, int64_t D, const void*
                                                (int)place_smem);
     if (e != cudaSuccess) return cuda_status(e);
   }
-  int at = 0;
-  for (int pass = 0; pass < p.passes && N > 0; ++pass) {
+  int at = N <= SMALL_TOKENS ? 1 : (p.cluster ? (p.passes & 1) : 0);
+  if (N > 0 && N <= SMALL_TOKENS) {
+    sort_small_kernel<<<1, (unsigned)SMALL_TOKENS, 0, stream>>>(ids, ids64, (int)N, V,
+                                                               padding_idx, w.pairs[0]);
+  } else if (p.cluster && N > 0) {
+    const int st = sort_in_cluster(p, w, ids, ids64, N, V, padding_idx, stream);
+    if (st != TP_OK) return st;
+  }
+  for (int pass = 0; pass < p.passes && N > SMALL_TOKENS && !p.cluster; ++pass) {
     SortArgs s;
     s.ids = ids;
     s.ids64 = ids64;
     s.V = V;
     s.padding_idx = padding_idx;
     s.first = pass == 0;
-    s.keys_in = w.keys[at ^ 1];
-    s.toks_in = w.toks[at ^ 1];
-    s.keys_out = w.keys[at];
-    s.toks_out = w.toks[at];
+    s.in = w.pairs[at ^ 1];
+    s.out = w.pairs[at];
     s.hist = w.hist;
     s.N = N;
     s.tile = p.tile;
     s.tiles = p.tiles;
     s.shift = pass * p.bits;
     s.bins = bins;
+    s.bits = p.bits;
     if (p.tiles > 1)
       sort_count_kernel<<<(unsigned)p.tiles, SORT_THREADS, sizeof(int) * bins, stream>>>(s);
     sort_place_kernel<<<(unsigned)p.tiles, SORT_THREADS, place_smem, stream>>>(s);
     at ^= 1;
   }
-  const SumPlan su = sum_plan(N, V);
+  const SumPlan su = sum_plan(N, V, D, esize);
   SumArgs s;
-  s.keys = w.keys[at ^ 1];
-  s.toks = w.toks[at ^ 1];
+  s.pairs = w.pairs[at ^ 1];
   s.N = N;
   s.V = V;
   s.D = D;
@@ -585,6 +934,7 @@ int launch_embedding_bwd(int dtype, int ids64, int64_t N, int64_t D, const void*
   s.head = w.head;
   s.tail = w.tail;
   s.flags = w.flags;
+  s.rows = w.rows;
   return dtype == TP_DTYPE_F32 ? sum_any<float>(s, stream) : sum_any<bf16_t>(s, stream);
 }
 
