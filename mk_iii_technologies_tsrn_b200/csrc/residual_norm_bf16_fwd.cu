@@ -1,0 +1,21 @@
+// residual_norm_bf16_fwd.cu -- residual_norm.cu's forward for bf16 rows.
+#include "residual_norm.cuh"
+
+namespace tp {
+
+int launch_residual_norm_fwd_bf16(int vec, int nv, const ResNormArgs& a, size_t smem,
+                                  cudaStream_t s) {
+#define RN_WARP(VEC, NV)                              \
+  if (a.group == 32 && vec == VEC && nv == NV)       \
+    return launch_fwd_known<bf16_t, VEC, NV, 32, RN_STAGED>(a, smem, s);
+#define RN_BLOCK(VEC, NV)     \
+  if (vec == VEC && nv == NV) \
+    return launch_fwd_known<bf16_t, VEC, NV, 0, RN_F32>(a, smem, s);
+  RN_WARP_BF16(RN_WARP)
+  RN_BLOCK_BF16(RN_BLOCK)
+#undef RN_WARP
+#undef RN_BLOCK
+  return TP_ERR_UNSUPPORTED;
+}
+
+}  // namespace tp
