@@ -71,9 +71,16 @@ int* device_error_ptr() {
 }
 
 int num_sms() {
+  static std::atomic<int> known[64];
   int dev = 0, n = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess)
-    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  const bool got = cudaGetDevice(&dev) == cudaSuccess;
+  if (got && dev < 64) {
+    const int k = known[dev].load(std::memory_order_relaxed);
+    if (k > 0) return k;
+  }
+  if (got && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess &&
+      n > 0 && dev < 64)
+    known[dev].store(n, std::memory_order_relaxed);
   return n > 0 ? n : 148;
 }
 

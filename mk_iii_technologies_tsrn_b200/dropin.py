@@ -13,10 +13,13 @@ with the tropical parts on this library's kernels:
   scatter backward that autograd of ``.max(-1)`` gives (value-only kernel
   when no gradient is taken), also across a ``TropicalKVCache``;
 * ``TropicalHybridFFN`` (:288-328): in inference ``lf_act(trop_up(x))`` is one
-  kernel (the LF activation fused into the max-plus epilogue).
+  kernel (the LF activation fused into the max-plus epilogue);
+* the scaled token embedding with learned positions of the token models
+  (:616-720): one kernel, its gradient by sorted tokens (``ops.embedding``; the
+  values are those of the PyTorch expression bit for bit).
 
 Everything else (projections, gate, masks, Maslov softmax, layer norms,
-residuals, embeddings) is the reference's PyTorch expression.  The encoder /
+residuals) is the reference's PyTorch expression.  The encoder /
 decoder layers, stacks and models below only compose these, as the reference
 ones do; alternatively swap ``TropicalLinear``, ``TropicalMultiHeadAttention``
 and ``TropicalHybridFFN`` into the reference module before building a model.
@@ -325,6 +328,15 @@ def make_causal_mask(seq_len: int, device: torch.device) -> torch.Tensor:
     return torch.triu(torch.full((seq_len, seq_len), -1e9, device=device), diagonal=1)
 
 
+def _plain_table(m: nn.Module) -> bool:
+    # an nn.Embedding that is only its float32 table: no hooks, parametrisation, renormalisation
+    # or other gradient than the dense sum
+    return (type(m) is nn.Embedding and type(m.weight) in (nn.Parameter, torch.Tensor)
+            and m.weight.dtype == torch.float32 and m.weight.is_cuda and m.max_norm is None
+            and not m.sparse and not m.scale_grad_by_freq and not m._forward_hooks
+            and not m._forward_pre_hooks and not m._backward_hooks and not m._backward_pre_hooks)
+
+
 class _TokenModel(nn.Module):
     # token + learned position embeddings scaled by sqrt(d_model), then an
     # encoder stack with a final norm (the shared body of the two models below)
@@ -340,6 +352,13 @@ class _TokenModel(nn.Module):
         return TropicalEncoder(layer, num_layers, norm=nn.LayerNorm(d_model))
 
     def _embed(self, input_ids: torch.Tensor) -> torch.Tensor:
+        tok, pos = self.embed, self.pos_embed
+        if (input_ids.is_cuda and input_ids.dtype in (torch.int32, torch.int64)
+                and _plain_table(tok) and _plain_table(pos) and pos.padding_idx is None
+                and input_ids.device == tok.weight.device == pos.weight.device):
+            return self.embed_drop(ops.embedding(input_ids, tok.weight, self.embed_scale,
+                                                 pos_weight=pos.weight,
+                                                 padding_idx=tok.padding_idx))
         positions = torch.arange(input_ids.shape[1], device=input_ids.device)[None]
         return self.embed_drop(self.embed(input_ids) * self.embed_scale +
                                self.pos_embed(positions))

@@ -21,6 +21,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 from typing import Optional, Tuple
 
 import torch
@@ -1261,6 +1262,17 @@ NORMS = {"layer": _lib.TP_NORM_LAYER, "rms": _lib.TP_NORM_RMS}
 RESIDUAL_NORM_MAX_CHANNELS = 8192
 
 
+def _once(backward):
+    # torch's once_differentiable where a second derivative could be asked for (a backward that
+    # records); its wrapper costs every other backward a few microseconds
+    guarded = torch.autograd.function.once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
+
+
 def _launch(name: str, dev: torch.device, *args) -> None:
     # an entry point on the device's current stream.  These operators are also called for single
     # tokens, where the host's time is the call's: the device is switched only if it is another,
@@ -1306,8 +1318,7 @@ def _contiguous(t: Optional[torch.Tensor]):
 
 def _empty_as(t: torch.Tensor) -> torch.Tensor:
     # contiguous, of t's shape, dtype and device
-    return torch.empty_like(t) if t.is_contiguous() else torch.empty(
-        t.shape, device=t.device, dtype=t.dtype)
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
 
 
 def _floating(t: torch.Tensor, what: str) -> int:
@@ -1447,7 +1458,7 @@ class ResidualNormFunction(torch.autograd.Function):
         return y, n
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dy, dn):
         if dy is None and dn is None:
             return (None,) * 12
@@ -1596,7 +1607,7 @@ class GatedScanFunction(torch.autograd.Function):
         return h, last
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dh, dh_last):
         if dh is None and dh_last is None:
             return (None,) * 5
@@ -1694,7 +1705,7 @@ def embedding_fwd(ids, weight, scale: float = 1.0, *, pos_weight=None, positions
                 positions = positions.expand(ids.shape)
             positions = _contiguous(positions.to(ids.dtype))
     flat = _contiguous(ids)
-    out = torch.empty((*ids.shape, D), device=dev, dtype=w.dtype)
+    out = w.new_empty((*ids.shape, D))
     _launch("tp_embedding_fwd", dev, dtype, bits, flat.numel(), T, D, flat.data_ptr(),
             w.data_ptr(), V, w.stride(0), float(scale), _at(p), p.shape[0] if p is not None else 0,
             p.stride(0) if p is not None else 0, _at(positions), out.data_ptr())
@@ -1713,7 +1724,7 @@ def embedding_bwd(ids, dout, rows: int, scale: float = 1.0, *,
                          f"{tuple(ids.shape)}")
     D, N = dout.shape[-1], ids.numel()
     ids, dout = _contiguous(ids), _contiguous(dout)
-    dw = torch.empty((rows, D), device=dev, dtype=dout.dtype)
+    dw = dout.new_empty((rows, D))
     with _on(dev):
         need = _lib.load().tp_embedding_bwd_workspace_bytes(N, rows, D)
     if need < 0:
@@ -1732,7 +1743,7 @@ def embedding_pos_bwd(dout: torch.Tensor, rows: int) -> torch.Tensor:
     D = dout.shape[-1]
     T = dout.shape[-2] if dout.dim() > 1 else 1
     dout = _contiguous(dout)
-    dp = torch.empty((rows, D), device=dev, dtype=dout.dtype)
+    dp = dout.new_empty((rows, D))
     N = dout.numel() // D if D else 0
     _launch("tp_embedding_pos_bwd", dev, dtype, N, T, D, dout.data_ptr(), rows, dp.data_ptr())
     return dp
@@ -1749,7 +1760,7 @@ class EmbeddingFunction(torch.autograd.Function):
         return embedding_fwd(ids, weight, scale, pos_weight=pos_weight, positions=positions)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dout):
         ids, positions = ctx.saved_tensors
         dw = dp = None

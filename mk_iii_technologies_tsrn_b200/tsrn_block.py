@@ -17,7 +17,11 @@ under the block's own attribute names (``ln_attn``/``attn``, ``ln_res``/
 ``reservoir``, ``ln_ssm``/``tropical_ssm``), so the matching subset of a
 ``TSRNBlock`` state dict loads unchanged.  It runs the branches in the
 block's order without the non-tropical ones between them (sheaf diffusion,
-Clifford FFN, p-adic modules).  :func:`swap_into` instead puts this library's
+Clifford FFN, p-adic modules).  With ``fused_residual`` the residual sums, the
+SSM's output gate and mix, and the LayerNorms between the branches run as one
+kernel each (``ops.residual_norm``; the LayerNorms' rounding then differs from
+PyTorch's in the last bits).  ``ssm="gated"`` takes :class:`~.ssm.GatedSSM` in
+place of the tropical SSM.  :func:`swap_into` instead puts this library's
 modules into a reference ``TSRNBlock`` in place, with the same weights, so the
 reference model itself runs its tropical branches on these kernels.
 """
@@ -30,7 +34,7 @@ import torch.nn as nn
 
 from . import ops
 from .reservoir import EchoStateReservoir
-from .ssm import TropicalSSM
+from .ssm import GatedSSM, TropicalSSM
 from .tsrn_attention import TropicalAttention
 
 BRANCHES = ("attn", "reservoir", "tropical_ssm")
@@ -38,8 +42,12 @@ BRANCHES = ("attn", "reservoir", "tropical_ssm")
 
 class TSRNTropicalPath(nn.Module):
     def __init__(self, d_model: int, top_k: int, n_heads: int, *, use_reservoir: bool = True,
-                 use_tropical_ssm: bool = True, dropout: float = 0.0):
+                 use_tropical_ssm: bool = True, dropout: float = 0.0, ssm: str = "tropical",
+                 fused_residual: bool = False):
         super().__init__()
+        if ssm not in ("tropical", "gated"):
+            raise ValueError(f"ssm must be 'tropical' or 'gated', got {ssm!r}")
+        self.fused_residual = fused_residual
         self.ln_attn = nn.LayerNorm(d_model)
         self.attn = TropicalAttention(d_model, top_k=top_k, n_heads=n_heads, dropout=dropout)
         self.use_reservoir = use_reservoir
@@ -49,12 +57,15 @@ class TSRNTropicalPath(nn.Module):
         self.use_tropical_ssm = use_tropical_ssm
         if use_tropical_ssm:
             self.ln_ssm = nn.LayerNorm(d_model)
-            self.tropical_ssm = TropicalSSM(d_model)
+            self.tropical_ssm = (TropicalSSM if ssm == "tropical" else GatedSSM)(d_model)
 
     def forward(self, x: torch.Tensor,
                 events: Optional[Dict[str, tuple]] = None) -> torch.Tensor:
         """``events`` (optional): branch name -> (start, end) CUDA events recorded
         around that branch on the current stream, for per-branch timing."""
+        if self.fused_residual:
+            return self._forward_fused(x, events or {})
+
         def branch(name, ln, mod, h):
             if events is not None and name in events:
                 events[name][0].record()
@@ -68,6 +79,35 @@ class TSRNTropicalPath(nn.Module):
             x = branch("reservoir", self.ln_res, self.reservoir, x)
         if self.use_tropical_ssm:
             x = branch("tropical_ssm", self.ln_ssm, self.tropical_ssm, x)
+        return x
+
+    def _forward_fused(self, x: torch.Tensor, events: Dict[str, tuple]) -> torch.Tensor:
+        # each branch's residual sum together with the LayerNorm of the next one
+        todo = [("attn", self.ln_attn, self.attn)]
+        if self.use_reservoir:
+            todo.append(("reservoir", self.ln_res, self.reservoir))
+        if self.use_tropical_ssm:
+            todo.append(("tropical_ssm", self.ln_ssm, self.tropical_ssm))
+        n = None
+        for i, (name, ln, mod) in enumerate(todo):
+            if name in events:
+                events[name][0].record()
+            if n is None:
+                n = ops.layer_norm(x, ln.weight, ln.bias, ln.eps)
+            gate = scale = None
+            if name == "tropical_ssm":
+                out, gate = mod.branch(n)
+                scale = torch.sigmoid(mod.mix)
+            else:
+                out = mod(n)
+            after = todo[i + 1][1] if i + 1 < len(todo) else None
+            if after is not None:
+                x, n = ops.residual_norm(x, out, after.weight, after.bias, after.eps, gate=gate,
+                                         scale=scale)
+            else:
+                x, _ = ops.residual_norm(x, out, gate=gate, scale=scale, normalize=False)
+            if name in events:
+                events[name][1].record()
         return x
 
 

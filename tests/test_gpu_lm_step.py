@@ -1,0 +1,150 @@
+"""The embedding, the gated recurrence and the residual step together, as a small language model
+uses them: embedding -> blocks (attention, reservoir, gated SSM with fused residual steps) -> tied
+logits, trained and decoded, against the same model on the PyTorch expressions.
+
+Both run the same attention and reservoir kernels; the rest differs in the order and number of fp32
+roundings only.  Tolerances are those of the block's own fixture test (outputs 1e-4 relative, 5e-5
+absolute) and of the drop-ins' gradient test (1e-3 of the largest value); top_k covers every key,
+so that no rounding decides a selection."""
+import numpy as np
+import pytest
+import torch
+import torch.nn as nn
+
+pytestmark = pytest.mark.gpu
+
+V, D, T, B = 61, 64, 40, 3
+
+
+class TinyLM(nn.Module):
+    def __init__(self, fused: bool, ssm: str = "gated"):
+        super().__init__()
+        from mk_iii_technologies_tsrn_b200.tsrn_block import TSRNTropicalPath
+        self.fused = fused
+        self.embed = nn.Embedding(V, D, padding_idx=0)
+        self.pos = nn.Embedding(T, D)
+        self.blocks = nn.ModuleList(TSRNTropicalPath(D, top_k=T, n_heads=4, ssm=ssm,
+                                                     fused_residual=fused) for _ in range(2))
+
+    def forward(self, ids):
+        from mk_iii_technologies_tsrn_b200 import ops
+        # the reservoirs' power iteration starts from a drawn vector and moves it on with every
+        # call: one start for both models and all calls
+        for blk in self.blocks:
+            v = blk.reservoir._cached_v
+            v.copy_(torch.linspace(-1.0, 1.3, v.numel(), device=v.device))
+        if self.fused:
+            x = ops.embedding(ids, self.embed.weight, D ** 0.5, pos_weight=self.pos.weight,
+                              padding_idx=0)
+        else:
+            at = torch.arange(ids.shape[1], device=ids.device)
+            x = self.embed(ids) * D ** 0.5 + self.pos(at)
+        for blk in self.blocks:
+            x = blk(x)
+        return x @ self.embed.weight.t()
+
+
+def _pair(cuda, ssm):
+    torch.manual_seed(0)
+    a = TinyLM(True, ssm)
+    with torch.no_grad():
+        for p in a.parameters():                # zero-initialised projections would hide errors
+            p.add_(0.05 * torch.randn_like(p))
+    b = TinyLM(False, ssm)
+    b.load_state_dict(a.state_dict())
+    return a.to(cuda), b.to(cuda)
+
+
+def _ids(cuda):
+    g = torch.Generator(device=cuda).manual_seed(1)
+    ids = torch.randint(1, V, (B, T), device=cuda, generator=g)
+    ids[1, 30:] = 0                             # padding
+    return ids
+
+
+@pytest.mark.parametrize("ssm", ["gated", "tropical"])
+def test_training_step_matches_the_unfused_model(cuda, ssm):
+    a, b = _pair(cuda, ssm)
+    ids = _ids(cuda)
+    out = []
+    for m in (a, b):
+        logits = m(ids)
+        loss = nn.functional.cross_entropy(logits[:, :-1].reshape(-1, V), ids[:, 1:].reshape(-1),
+                                           ignore_index=0)
+        loss.backward()
+        out.append(logits.detach())
+    torch.testing.assert_close(out[0], out[1], rtol=1e-4, atol=5e-5 * float(out[1].abs().max()))
+    for (name, p), q in zip(a.named_parameters(), b.parameters()):
+        assert (p.grad is None) == (q.grad is None), name
+        if p.grad is not None:
+            np.testing.assert_allclose(p.grad.cpu().numpy(), q.grad.cpu().numpy(), rtol=1e-3,
+                                       atol=1e-3 * float(q.grad.abs().max()), err_msg=name)
+
+
+def test_inference_matches_and_repeats(cuda):
+    a, b = _pair(cuda, "gated")
+    ids = _ids(cuda)
+    with torch.no_grad():
+        y = a(ids)
+        torch.testing.assert_close(y, b(ids), rtol=1e-4, atol=5e-5 * float(y.abs().max()))
+        assert torch.equal(y, a(ids))
+
+
+def test_branch_events_of_the_fused_path(cuda):
+    a, _ = _pair(cuda, "tropical")
+    ev = {n: (torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True))
+          for n in ("attn", "reservoir", "tropical_ssm")}
+    with torch.no_grad():
+        a.blocks[0](torch.randn(B, T, D, device=cuda), events=ev)
+    torch.cuda.synchronize()
+    assert all(s.elapsed_time(e) > 0 for s, e in ev.values())
+
+
+def test_ssm_prefill_then_steps_equal_the_whole(cuda):
+    # a padded prefill, then one token at a time: the same recurrence on the same fp32 states; the
+    # projections' rows go through products of another size: 1e-5 of the values
+    from mk_iii_technologies_tsrn_b200.ssm import GatedSSM
+    torch.manual_seed(2)
+    m = GatedSSM(D, 96)
+    with torch.no_grad():
+        for p in m.parameters():
+            p.add_(0.1 * torch.randn_like(p))
+    m = m.to(cuda)
+    x = torch.randn(B, 30, D, device=cuda)
+    n = torch.tensor([20, 1, 13], device=cuda)
+    with torch.no_grad():
+        whole = m(x)
+        padded = x.clone()
+        for i, k in enumerate(n.tolist()):
+            padded[i, k:] = float("nan")        # nothing behind a row's end may matter
+        _, state = m(padded, lengths=n, return_state=True)
+        for t in range(8):
+            at = n + t
+            y = m.step(x[torch.arange(B, device=cuda), at], state)
+            torch.testing.assert_close(y, whole[torch.arange(B, device=cuda), at], rtol=1e-5,
+                                       atol=1e-5)
+        h0 = m.init_state(B)
+        assert h0.shape == (B, 96) and torch.all(h0 == 0)
+
+
+def test_decoder_model_embeds_with_the_kernel(cuda):
+    # the drop-in's embedding: bits of the PyTorch expression, gradients within the bound of a sum
+    # of n rows in fp32; a table with a hook takes the PyTorch path
+    from mk_iii_technologies_tsrn_b200 import dropin
+    m = dropin.TropicalDecoderModel(V, d_model=32, nhead=4, num_layers=1, dim_feedforward=64,
+                                    dropout=0.0, max_seq_len=T).to(cuda)
+    ids = _ids(cuda)
+    x = m._embed(ids)
+    want = m.embed(ids) * m.embed_scale + m.pos_embed(torch.arange(T, device=cuda))[None]
+    assert torch.equal(x, want) and x.grad_fn.name() == "EmbeddingFunctionBackward"
+    d = torch.randn_like(x)
+    for p, q in zip(torch.autograd.grad(x, (m.embed.weight, m.pos_embed.weight), d),
+                    torch.autograd.grad(want, (m.embed.weight, m.pos_embed.weight), d)):
+        n = B * T
+        size = float(d.abs().sum((0, 1)).max()) * m.embed_scale
+        assert float((p - q).abs().max()) <= 2 * (n + 2) * 2.0 ** -24 * size
+    h = m.embed.register_forward_hook(lambda mod, i, o: o * 2)
+    assert torch.equal(m._embed(ids), m.embed(ids) * m.embed_scale + m.pos_embed(
+        torch.arange(T, device=cuda))[None])
+    h.remove()
+    assert m(ids).shape == (B, T, V)
