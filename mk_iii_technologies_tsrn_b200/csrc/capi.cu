@@ -721,7 +721,7 @@ int tp_residual_norm_fwd(int dtype, int params_dtype, int norm, int64_t rows, in
 
 int64_t tp_residual_norm_bwd_workspace_bytes(int64_t rows, int64_t D) {
   if (rows < 0 || !tp::residual_norm_supported(D)) return -1;
-  return (int64_t)tp::residual_norm_bwd_blocks(rows, D) * (5 * D + 1) * (int64_t)sizeof(float);
+  return (int64_t)tp::residual_norm_bwd_blocks(rows, D) * (5 * D + 2) * (int64_t)sizeof(float);
 }
 
 int tp_residual_norm_bwd(int dtype, int params_dtype, int norm, int64_t rows, int64_t D,

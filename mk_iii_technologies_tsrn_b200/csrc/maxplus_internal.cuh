@@ -312,7 +312,7 @@ struct ResNormBwdArgs {
   const void* dn;        // optional
   void *dx, *dbranch, *dgate;
   float *dw, *db, *dscale, *dbw, *dbb;   // each optional
-  float* part;           // [blocks][sums * D + 1]
+  float* part;           // [blocks][sums * D + 2]
   int sums, slot_w, slot_b, slot_s, slot_bw, slot_bb;   // set by the launcher
 };
 bool residual_norm_supported(int64_t D);

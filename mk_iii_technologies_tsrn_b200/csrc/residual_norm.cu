@@ -37,30 +37,38 @@ namespace tp {
 namespace {
 
 // Column sums over the blocks' partials, in block order: 32 columns per block,
-// 8 warps each take a contiguous range of the partials.
+// 8 warps each take a contiguous range of the partials.  The last block adds the
+// single scale's, in 64 bits.
 __global__ void __launch_bounds__(256) residual_norm_sum_kernel(const ResNormBwdArgs g,
                                                                 int blocks) {
   __shared__ float s[8][32];
-  const int64_t width = (int64_t)g.sums * g.f.D + 1;
+  const int64_t columns = (int64_t)g.sums * g.f.D, width = columns + 2;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (blockIdx.x == gridDim.x - 1) {
+    if (g.f.scale_mode != 1 || g.dscale == nullptr || warp != 0) return;
+    double t = 0.0;
+    for (int i = lane; i < blocks; i += 32)
+      t += (double)g.part[(int64_t)i * width + columns] +
+           (double)g.part[(int64_t)i * width + columns + 1];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+    if (lane == 0) *g.dscale = (float)t;
+    return;
+  }
   const int64_t col = (int64_t)blockIdx.x * 32 + lane;
   const int per = (blocks + 7) / 8;
   const int lo = warp * per, hi = min(blocks, lo + per);
   float acc = 0.f;
-  if (col < width) {
+  if (col < columns) {
 #pragma unroll 8
     for (int i = lo; i < hi; ++i) acc += g.part[(int64_t)i * width + col];
   }
   s[warp][lane] = acc;
   __syncthreads();
-  if (warp != 0 || col >= width) return;
+  if (warp != 0 || col >= columns) return;
   float t = 0.f;
 #pragma unroll
   for (int w = 0; w < 8; ++w) t += s[w][lane];
-  if (col == width - 1) {
-    if (g.f.scale_mode == 1 && g.dscale) *g.dscale = t;
-    return;
-  }
   const int k = (int)(col / g.f.D);
   const int64_t c = col - (int64_t)k * g.f.D;
   if (k == g.slot_w) g.dw[c] = t;
@@ -196,8 +204,8 @@ int launch_residual_norm_bwd(const ResNormBwdArgs& args, cudaStream_t stream) {
                   : bwd_any<bf16_t, 1>(g, smem, blocks, stream);
   }
   if (st != TP_OK) return st;
-  const int64_t width = (int64_t)k * g.f.D + 1;
-  residual_norm_sum_kernel<<<(unsigned)ceil_div(width, (int64_t)32), 256, 0, stream>>>(g, blocks);
+  const unsigned sum_blocks = (unsigned)ceil_div((int64_t)k * g.f.D, (int64_t)32) + 1;
+  residual_norm_sum_kernel<<<sum_blocks, 256, 0, stream>>>(g, blocks);
   return launch_status();
 }
 

@@ -175,13 +175,9 @@ struct Param {
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
 // exp(-|g|) of a gate with the gate's sign: what the sigmoid and its complement
-// are formed from, twice in the backward.  bf16 storage takes one power of two.
-template <typename T>
-__device__ __forceinline__ float gate_exp(float g) {
-  const float a = fabsf(g);
-  const float e = sizeof(T) == 2 ? tp_ex2(a * -1.442695041f) : expf(-a);
-  return copysignf(e, g);
-}
+// are formed from, twice in the backward.  To fp32 accuracy for bf16 storage too:
+// the parameter gradients are fp32 sums of it.
+__device__ __forceinline__ float gate_exp(float g) { return copysignf(expf(-fabsf(g)), g); }
 // sigmoid and 1 - sigmoid: the larger one is 1 / (1 + e), the smaller e / (1 + e)
 __device__ __forceinline__ void gate_from(float signed_e, float& s, float& rest) {
   const float e = fabsf(signed_e);
@@ -356,8 +352,8 @@ __global__ void __launch_bounds__(MAXT) residual_norm_fwd_kernel(const ResNormAr
         for (int i = 0; i < P2; ++i) {
           float2 sg;
           float om;
-          gate_from(gate_exp<T>(f[i].x), sg.x, om);
-          gate_from(gate_exp<T>(f[i].y), sg.y, om);
+          gate_from(gate_exp(f[i].x), sg.x, om);
+          gate_from(gate_exp(f[i].y), sg.y, om);
           p[i] = tp_mul2(sg, p[i]);
         }
       }
@@ -453,7 +449,7 @@ __global__ void __launch_bounds__(MAXT, MAXT == 128 ? 3 : 1)
   float* const acc_s = g.slot_s >= 0 ? s_acc + g.slot_s * plane : nullptr;
   float* const acc_bw = g.slot_bw >= 0 ? s_acc + g.slot_bw * plane : nullptr;
   float* const acc_bb = g.slot_bb >= 0 ? s_acc + g.slot_bb * plane : nullptr;
-  float2 sum_scale = both(0.f);
+  double sum_scale = 0.0;    // of the single scale: a row in fp32, the rows in 64 bits
 
   for (int64_t row = (int64_t)blockIdx.x * teams + team; row < a.rows;
        row += (int64_t)gridDim.x * teams) {
@@ -517,7 +513,7 @@ __global__ void __launch_bounds__(MAXT, MAXT == 128 ? 3 : 1)
         vg[v].get(ev);
 #pragma unroll
         for (int i = 0; i < P2; ++i)
-          ev[i] = make_float2(gate_exp<T>(ev[i].x), gate_exp<T>(ev[i].y));
+          ev[i] = make_float2(gate_exp(ev[i].x), gate_exp(ev[i].y));
       }
       if (dnr == nullptr) continue;
       float2 p[P2], f[P2];
@@ -571,6 +567,7 @@ __global__ void __launch_bounds__(MAXT, MAXT == 128 ? 3 : 1)
       c2 = r.y * inv_d;
     }
     s1 = s2 = both(0.f);
+    float2 row_scale = both(0.f);
 #pragma unroll
     for (int v = 0; v < NG; ++v) {
       if (!V::any(v, t, G, D)) continue;
@@ -611,7 +608,7 @@ __global__ void __launch_bounds__(MAXT, MAXT == 128 ? 3 : 1)
         } else if (a.scale_mode == 1) {
 #pragma unroll
           for (int i = 0; i < P2; ++i) {
-            sum_scale = tp_fma2(d[i], aff[i], sum_scale);
+            row_scale = tp_fma2(d[i], aff[i], row_scale);
             d[i] = tp_mul2(d[i], both(one_scale));
           }
         }
@@ -631,7 +628,7 @@ __global__ void __launch_bounds__(MAXT, MAXT == 128 ? 3 : 1)
       } else if (a.scale_mode == 1) {
 #pragma unroll
         for (int i = 0; i < P2; ++i) {
-          sum_scale = tp_fma2(d[i], aff[i], sum_scale);
+          row_scale = tp_fma2(d[i], aff[i], row_scale);
           d[i] = tp_mul2(d[i], both(one_scale));
         }
       }
@@ -657,6 +654,7 @@ __global__ void __launch_bounds__(MAXT, MAXT == 128 ? 3 : 1)
         s2 = tp_fma2(d[i], phat[i], s2);
       }
     }
+    sum_scale += (double)(row_scale.x + row_scale.y);
     if (branch_norm) {
       const float2 r = team_sum<true>(s1.x + s1.y, s2.x + s2.y, G, slots, half);
       c1 = layer ? r.x * inv_d : 0.f;
@@ -676,7 +674,7 @@ __global__ void __launch_bounds__(MAXT, MAXT == 128 ? 3 : 1)
   }
   // this block's column sums: its teams in order
   __syncthreads();
-  const int64_t width = (int64_t)g.sums * a.D + 1;
+  const int64_t width = (int64_t)g.sums * a.D + 2;
   float* part = g.part + (int64_t)blockIdx.x * width;
   if (team == 0) {
     for (int k = 0; k < g.sums; ++k) {
@@ -693,17 +691,18 @@ __global__ void __launch_bounds__(MAXT, MAXT == 128 ? 3 : 1)
       }
     }
   }
-  // and its share of the single scale's gradient
-  float mine = sum_scale.x + sum_scale.y;
+  // and its share of the single scale's gradient, as two floats
+  __shared__ double s_scale[RN_MAX_WARPS];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5].x = mine;
+  for (int o = 16; o > 0; o >>= 1) sum_scale += __shfl_xor_sync(0xffffffffu, sum_scale, o);
+  if ((threadIdx.x & 31) == 0) s_scale[threadIdx.x >> 5] = sum_scale;
   __syncthreads();
   if (threadIdx.x == 0) {
-    float s = 0.f;
-    for (int w = 0; w < (int)(blockDim.x >> 5); ++w) s += slots[w].x;
-    part[width - 1] = s;
+    double s = 0.0;
+    for (int w = 0; w < (int)(blockDim.x >> 5); ++w) s += s_scale[w];
+    const float hi = (float)s;
+    part[width - 2] = hi;
+    part[width - 1] = isinf(hi) ? 0.f : (float)(s - (double)hi);
   }
 }
 

@@ -1361,6 +1361,12 @@ def _residual_norm_args(x, branch, weight, bias, norm, gate, scale, branch_norm,
     return dev, dtype, TP_DTYPE_BF16 if pd == torch.bfloat16 else TP_DTYPE_F32, D
 
 
+@functools.lru_cache(maxsize=1024)
+def _residual_norm_bytes(index: int, rows: int, D: int) -> int:
+    with _on(torch.device("cuda", index)):
+        return _lib.load().tp_residual_norm_bwd_workspace_bytes(rows, D)
+
+
 def _residual_norm_run(dev, dtype, pdtype, D, x, branch, weight, bias, eps, norm, gate, scale,
                        branch_norm, branch_weight, branch_bias, normalize, need_stats):
     (x2, ldx), (b2, ldb), (g2, ldg) = _rows_of(x, D), _rows_of(branch, D), _rows_of(gate, D)
@@ -1391,8 +1397,7 @@ def _residual_norm_back(dev, dtype, pdtype, D, stats, dy, dn, x, branch, weight,
     if any(wanted):
         views = torch.empty(sum(sizes), device=dev, dtype=torch.float32).split_with_sizes(sizes)
         params = [v if want else None for v, want in zip(views, wanted)]
-    with _on(dev):
-        need = _lib.load().tp_residual_norm_bwd_workspace_bytes(rows, D)
+    need = _residual_norm_bytes(dev.index, rows, D)
     ws = torch.empty(need, device=dev, dtype=torch.uint8)
     dsc, dw, db, dbw, dbb = params
     _launch("tp_residual_norm_bwd", dev, dtype, pdtype, NORMS[norm], rows, D, x2.data_ptr(), ldx,
@@ -1535,9 +1540,14 @@ def _gated_scan_inputs(gate, x, h0, lengths):
     return dev, dtype, lengths
 
 
+@functools.lru_cache(maxsize=1024)
+def _gated_scan_bytes(index: int, B: int, T: int, C: int) -> int:
+    with _on(torch.device("cuda", index)):
+        return _lib.load().tp_gated_scan_workspace_bytes(B, T, C)
+
+
 def _gated_scan_workspace(dev, B, T, C):
-    with _on(dev):
-        need = _lib.load().tp_gated_scan_workspace_bytes(B, T, C)
+    need = _gated_scan_bytes(dev.index, B, T, C)
     return (torch.empty(need, device=dev, dtype=torch.uint8) if need > 0 else None), need
 
 
@@ -1712,6 +1722,25 @@ def embedding_fwd(ids, weight, scale: float = 1.0, *, pos_weight=None, positions
     return out
 
 
+@functools.lru_cache(maxsize=1024)
+def _embedding_workspace(index: int, N: int, rows: int, D: int) -> int:
+    with _on(torch.device("cuda", index)):
+        return _lib.load().tp_embedding_bwd_workspace_bytes(N, rows, D)
+
+
+def _embedding_back(dev, dtype, bits, ids, dout, rows, D, scale, padding_idx):
+    N = ids.numel()
+    dw = dout.new_empty((rows, D))
+    need = _embedding_workspace(dev.index, N, rows, D)
+    if need < 0:
+        raise ValueError(f"embedding_bwd takes fewer than 2^31 tokens and rows, got {N} and {rows}")
+    ws = torch.empty(need or 16, device=dev, dtype=torch.uint8)
+    _launch("tp_embedding_bwd", dev, dtype, bits, N, D, ids.data_ptr(), dout.data_ptr(), rows,
+            scale, -1 if padding_idx is None else padding_idx, dw.data_ptr(), ws.data_ptr(),
+            need or 16)
+    return dw
+
+
 def embedding_bwd(ids, dout, rows: int, scale: float = 1.0, *,
                   padding_idx: Optional[int] = None) -> torch.Tensor:
     """Gradient [rows, D] of an embedding table from ``dout`` [*ids.shape, D]: row v is
@@ -1722,18 +1751,8 @@ def embedding_bwd(ids, dout, rows: int, scale: float = 1.0, *,
     if dout.shape[:-1] != ids.shape:
         raise ValueError(f"dout must be [*ids.shape, D], got {tuple(dout.shape)} for ids "
                          f"{tuple(ids.shape)}")
-    D, N = dout.shape[-1], ids.numel()
-    ids, dout = _contiguous(ids), _contiguous(dout)
-    dw = dout.new_empty((rows, D))
-    with _on(dev):
-        need = _lib.load().tp_embedding_bwd_workspace_bytes(N, rows, D)
-    if need < 0:
-        raise ValueError(f"embedding_bwd takes fewer than 2^31 tokens and rows, got {N} and {rows}")
-    ws = torch.empty(max(need, 16), device=dev, dtype=torch.uint8)
-    _launch("tp_embedding_bwd", dev, dtype, bits, N, D, ids.data_ptr(), dout.data_ptr(), rows,
-            float(scale), -1 if padding_idx is None else padding_idx, dw.data_ptr(), ws.data_ptr(),
-            ws.numel())
-    return dw
+    return _embedding_back(dev, dtype, bits, _contiguous(ids), _contiguous(dout), rows,
+                           dout.shape[-1], float(scale), padding_idx)
 
 
 def embedding_pos_bwd(dout: torch.Tensor, rows: int) -> torch.Tensor:
@@ -1764,12 +1783,19 @@ class EmbeddingFunction(torch.autograd.Function):
     def backward(ctx, dout):
         ids, positions = ctx.saved_tensors
         dw = dp = None
-        dout = dout.contiguous()
+        dout = _contiguous(dout)
+        dev, D = dout.device, dout.shape[-1]
+        dtype = _floating(dout, "dout")
         if ctx.needs_input_grad[1]:
-            dw = embedding_bwd(ids, dout, ctx.rows[0], ctx.scale, padding_idx=ctx.padding_idx)
+            dw = _embedding_back(dev, dtype, _index_bits(ids, "ids"), _contiguous(ids), dout,
+                                 ctx.rows[0], D, ctx.scale, ctx.padding_idx)
         if ctx.needs_input_grad[2]:
-            dp = (embedding_pos_bwd(dout, ctx.rows[1]) if positions is None
-                  else embedding_bwd(positions.expand(ids.shape), dout, ctx.rows[1]))
+            if positions is None:
+                dp = embedding_pos_bwd(dout, ctx.rows[1])
+            else:
+                at = _contiguous(positions.expand(ids.shape))
+                dp = _embedding_back(dev, dtype, _index_bits(at, "positions"), at, dout,
+                                     ctx.rows[1], D, 1.0, None)
         return None, dw, dp, None, None, None
 
 
