@@ -81,32 +81,38 @@ __global__ void __launch_bounds__(256) residual_norm_sum_kernel(const ResNormBwd
 struct Plan {
   int vec, nv, group;
   bool known;       // gate, branch norm and parameters known at compile time
-  bool warp;        // a team is a warp (parameters staged), else a block
+  bool warp;        // a team is a warp, else a block
+  bool shift;       // rows begin inside 16 bytes
+  bool staged;      // parameters in shared memory
 };
 
 // Vectors per thread and threads per row.  A warp as long as its registers hold
 // the row (20 fp32 or 24 bf16 elements per thread), else a block of whole warps
 // around it (16 elements per thread; 8 or 4 fp32: 16384 x 2048 bf16 forward 82
 // against 59 us, backward 202 against 157 us).
-Plan plan_row(bool bf16, int vec, int64_t D, bool params_f32) {
+Plan plan_row(bool bf16, bool shift, int vec, int64_t D, bool params_f32) {
   Plan p;
   p.vec = vec;
-  const int64_t n = ceil_div(D, (int64_t)vec);
+  p.shift = shift;
+  const int64_t n = shift ? shifted_vectors((int)D, vec) : ceil_div(D, (int64_t)vec);
   p.warp = vec == (bf16 ? 8 : 4) && n <= 32 * (bf16 ? 3 : 5);
+  p.staged = p.warp || shift;
   if (p.warp) {
     p.known = true;
     p.group = 32;
     p.nv = (int)ceil_div(n, (int64_t)32);
+    if (shift && p.nv % 2 == 0) ++p.nv;      // 1, 3 or 5
     return p;
   }
-  p.known = params_f32 && (vec > 1 || D <= 4096);
-  p.nv = p.known && vec == 1 ? 8 : 16 / vec;
+  p.known = shift || (params_f32 && vec > 1);
+  p.nv = shift && !bf16 ? 2 : 16 / vec;
   p.group = (int)ceil_div(ceil_div(n, (int64_t)p.nv), (int64_t)32) * 32;
   // (the dispatch tells warps by a group of 32: a block of one warp takes two)
   if (p.known && p.group == 32) p.group = 64;
   return p;
 }
 
+// vectors of rows that begin on a vector's bytes
 bool vec_ok(const ResNormArgs& a, int vec, int esize) {
   const int64_t m = (int64_t)vec * esize - 1;   // 8- or 16-byte vectors
   auto al = [&](const void* q) { return q == nullptr || (((uintptr_t)q) & m) == 0; };
@@ -116,6 +122,14 @@ bool vec_ok(const ResNormArgs& a, int vec, int esize) {
          al16(a.w) && al16(a.b) && al16(a.bw) && al16(a.bb) &&
          (a.scale_mode != 2 || al16(a.scale));
 }
+// and of rows whose first channels lie at the same element of 16 bytes in all tensors.
+// (Above 4096 channels the backward's sums and parameters outgrow shared memory.)
+bool shift_ok(const ResNormArgs& a, int vec) {
+  auto al = [](const void* q) { return q == nullptr || aligned16(q); };
+  auto ld = [&](int64_t l) { return l >= a.D && l % vec == a.D % vec; };
+  return a.D <= 4080 && a.D % RN_RESIDUES != 0 && al(a.x) && al(a.branch) && al(a.gate) && al(a.y) && al(a.n) &&
+         ld(a.ldx) && ld(a.ldb) && (a.gate == nullptr || ld(a.ldg));
+}
 
 int common_align(std::initializer_list<const void*> ps) {
   uintptr_t m = 16;
@@ -123,27 +137,32 @@ int common_align(std::initializer_list<const void*> ps) {
   return (int)(m & (~m + 1));
 }
 
-int vector_width(const ResNormArgs& a, int align_of_grads) {
+Plan plan(const ResNormArgs& a, int align_of_grads) {
   const bool bf16 = a.dtype == TP_DTYPE_BF16;
   const int esize = bf16 ? 2 : 4;
-  for (int vec : {bf16 ? 8 : 4, bf16 ? 4 : 1})
-    if (vec == 1 || (vec_ok(a, vec, esize) && align_of_grads % (vec * esize) == 0)) return vec;
-  return 1;
+  for (int vec : {bf16 ? 8 : 4, 4})
+    if (align_of_grads % (vec * esize) == 0 && vec_ok(a, vec, esize))
+      return plan_row(bf16, false, vec, a.D, !a.params_bf16);
+  if (align_of_grads == 16 && shift_ok(a, 16 / esize))
+    return plan_row(bf16, true, 16 / esize, a.D, !a.params_bf16);
+  return plan_row(bf16, false, 1, a.D, !a.params_bf16);
 }
 
-int staged_floats(const ResNormArgs& a, bool backward) {
-  return ((a.w != nullptr) + (!backward && a.b != nullptr) + (a.scale_mode == 2) +
-          (a.bw != nullptr) + (a.bb != nullptr)) * (int)a.D;
+size_t staged_bytes(const ResNormArgs& a, const Plan& p, bool backward) {
+  if (!p.staged) return 0;
+  const int n = (a.w != nullptr) + (!backward && a.b != nullptr) + (a.scale_mode == 2) +
+                (a.bw != nullptr) + (a.bb != nullptr);
+  return sizeof(float) * (size_t)n * (p.shift ? staged_size((int)a.D, p.vec) : (int)a.D);
 }
 
 // the kernels that look everything up: other alignments, bf16 parameters of long rows
 template <typename T, int VEC>
 int fwd_any(const ResNormArgs& a, cudaStream_t s) {
-  return launch_fwd_kernel<T, VEC, 16 / VEC, 0, RN_ANY, 2, 2>(a, 0, s);
+  return launch_fwd_kernel<T, VEC, 16 / VEC, 0, RN_ANY, 2, 2, false>(a, 0, s);
 }
 template <typename T, int VEC>
 int bwd_any(const ResNormBwdArgs& g, size_t smem, int blocks, cudaStream_t s) {
-  return launch_bwd_kernel<T, VEC, 16 / VEC, 0, RN_ANY, 2, 2>(g, smem, blocks, s);
+  return launch_bwd_kernel<T, VEC, 16 / VEC, 0, RN_ANY, 2, 2, false>(g, smem, blocks, s);
 }
 
 }  // namespace
@@ -152,23 +171,26 @@ bool residual_norm_supported(int64_t D) { return D >= 1 && D <= 8192; }
 
 int residual_norm_bwd_blocks(int64_t rows, int64_t D) {
   // what an SM holds at once: three blocks of four rows, or rows in 512 threads of
-  // 128 registers (at most four); each block keeps a set of column sums
+  // 128 registers (at most four); each block keeps a set of column sums.  Rows that
+  // may begin inside 16 bytes want a multiple of the residues.
   const int64_t threads = ceil_div(D, (int64_t)512) * 32;
   const int64_t per_sm = D <= 640 ? 3 : (threads <= 128 ? 4 : (threads <= 256 ? 2 : 1));
-  const int64_t cap = (int64_t)num_sms() * per_sm;
-  return (int)(rows < cap ? (rows > 0 ? rows : 1) : cap);
+  const int64_t r = D % RN_RESIDUES ? RN_RESIDUES : 1;
+  const int64_t cap = (int64_t)num_sms() * per_sm / r * r;
+  const int64_t want = ceil_div(rows > 0 ? rows : 1, r) * r;
+  return (int)(want < cap ? want : cap);
 }
 
 int launch_residual_norm_fwd(const ResNormArgs& args, cudaStream_t stream) {
   ResNormArgs a = args;
   const bool bf16 = a.dtype == TP_DTYPE_BF16;
-  const Plan p = plan_row(bf16, vector_width(a, 16), a.D, !a.params_bf16);
+  const Plan p = plan(a, 16);
   a.group = p.group;
-  if (p.known) {
-    const size_t smem = p.warp ? sizeof(float) * staged_floats(a, false) : 0;
+  const size_t smem = staged_bytes(a, p, false);
+  if (p.shift) return launch_residual_norm_fwd_shift(p.nv, a, smem, stream);
+  if (p.known)
     return bf16 ? launch_residual_norm_fwd_bf16(p.vec, p.nv, a, smem, stream)
                 : launch_residual_norm_fwd_f32(p.vec, p.nv, a, smem, stream);
-  }
   if (!bf16) return p.vec == 4 ? fwd_any<float, 4>(a, stream) : fwd_any<float, 1>(a, stream);
   if (p.vec == 8) return fwd_any<bf16_t, 8>(a, stream);
   return p.vec == 4 ? fwd_any<bf16_t, 4>(a, stream) : fwd_any<bf16_t, 1>(a, stream);
@@ -184,24 +206,29 @@ int launch_residual_norm_bwd(const ResNormBwdArgs& args, cudaStream_t stream) {
   g.slot_bw = g.dbw ? k++ : -1;
   g.slot_bb = g.dbb ? k++ : -1;
   g.sums = k;
-  const int vec = vector_width(g.f, common_align({g.dy, g.dn, g.dx, g.dbranch, g.dgate}));
-  const int blocks = residual_norm_bwd_blocks(g.f.rows, g.f.D);
-  const Plan p = plan_row(bf16, vec, g.f.D, !g.f.params_bf16);
+  int blocks = residual_norm_bwd_blocks(g.f.rows, g.f.D);
+  const Plan p = plan(g.f, common_align({g.dy, g.dn, g.dx, g.dbranch, g.dgate}));
   g.f.group = p.group;
-  size_t smem = sizeof(float) * (size_t)k * p.vec * p.nv * (p.warp ? 128 : p.group);
+  const size_t smem = sizeof(float) * (size_t)k * p.vec * p.nv * (p.warp ? 128 : p.group) +
+                      staged_bytes(g.f, p, true);
   int st;
-  if (p.known) {
-    if (p.warp) smem += sizeof(float) * staged_floats(g.f, true);
+  if (p.shift) {
+    // one wave where rows take more threads than that count supposes
+    const int fit = num_sms() * (p.warp ? 4 : max(512 / p.group, 1)) / RN_RESIDUES * RN_RESIDUES;
+    blocks = min(blocks, fit);
+    st = bf16 ? launch_residual_norm_bwd_shift_bf16(p.nv, g, smem, blocks, stream)
+              : launch_residual_norm_bwd_shift_f32(p.nv, g, smem, blocks, stream);
+  } else if (p.known) {
     st = bf16 ? launch_residual_norm_bwd_bf16(p.vec, p.nv, g, smem, blocks, stream)
               : launch_residual_norm_bwd_f32(p.vec, p.nv, g, smem, blocks, stream);
   } else if (!bf16) {
-    st = vec == 4 ? bwd_any<float, 4>(g, smem, blocks, stream)
-                  : bwd_any<float, 1>(g, smem, blocks, stream);
-  } else if (vec == 8) {
+    st = p.vec == 4 ? bwd_any<float, 4>(g, smem, blocks, stream)
+                    : bwd_any<float, 1>(g, smem, blocks, stream);
+  } else if (p.vec == 8) {
     st = bwd_any<bf16_t, 8>(g, smem, blocks, stream);
   } else {
-    st = vec == 4 ? bwd_any<bf16_t, 4>(g, smem, blocks, stream)
-                  : bwd_any<bf16_t, 1>(g, smem, blocks, stream);
+    st = p.vec == 4 ? bwd_any<bf16_t, 4>(g, smem, blocks, stream)
+                    : bwd_any<bf16_t, 1>(g, smem, blocks, stream);
   }
   if (st != TP_OK) return st;
   const unsigned sum_blocks = (unsigned)ceil_div((int64_t)k * g.f.D, (int64_t)32) + 1;

@@ -7,10 +7,10 @@ int launch_residual_norm_bwd_bf16(int vec, int nv, const ResNormBwdArgs& g, size
                                   int blocks, cudaStream_t s) {
 #define RN_WARP(VEC, NV)                              \
   if (g.f.group == 32 && vec == VEC && nv == NV)       \
-    return launch_bwd_known<bf16_t, VEC, NV, 32, RN_STAGED>(g, smem, blocks, s);
+    return launch_bwd_known<bf16_t, VEC, NV, 32, RN_STAGED, false>(g, smem, blocks, s);
 #define RN_BLOCK(VEC, NV)     \
   if (vec == VEC && nv == NV) \
-    return launch_bwd_known<bf16_t, VEC, NV, 0, RN_F32>(g, smem, blocks, s);
+    return launch_bwd_known<bf16_t, VEC, NV, 0, RN_F32, false>(g, smem, blocks, s);
   RN_WARP_BF16(RN_WARP)
   RN_BLOCK_BF16(RN_BLOCK)
 #undef RN_WARP

@@ -7,10 +7,10 @@ int launch_residual_norm_fwd_bf16(int vec, int nv, const ResNormArgs& a, size_t 
                                   cudaStream_t s) {
 #define RN_WARP(VEC, NV)                              \
   if (a.group == 32 && vec == VEC && nv == NV)       \
-    return launch_fwd_known<bf16_t, VEC, NV, 32, RN_STAGED>(a, smem, s);
+    return launch_fwd_known<bf16_t, VEC, NV, 32, RN_STAGED, false>(a, smem, s);
 #define RN_BLOCK(VEC, NV)     \
   if (vec == VEC && nv == NV) \
-    return launch_fwd_known<bf16_t, VEC, NV, 0, RN_F32>(a, smem, s);
+    return launch_fwd_known<bf16_t, VEC, NV, 0, RN_F32, false>(a, smem, s);
   RN_WARP_BF16(RN_WARP)
   RN_BLOCK_BF16(RN_BLOCK)
 #undef RN_WARP

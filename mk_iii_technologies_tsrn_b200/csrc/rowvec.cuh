@@ -39,6 +39,7 @@ struct RowVec<float, 4> {
     f[0] = r.x; f[1] = r.y; f[2] = r.z; f[3] = r.w;
   }
   __device__ __forceinline__ void set(const float* f) { r = make_float4(f[0], f[1], f[2], f[3]); }
+  __device__ __forceinline__ void pack(const float* e) { set(e); }
   __device__ __forceinline__ void store(float* p) const { *reinterpret_cast<float4*>(p) = r; }
   __device__ __forceinline__ void store_stream(float* p) const {
     __stcs(reinterpret_cast<float4*>(p), r);
@@ -98,6 +99,10 @@ struct RowVec<bf16_t, 8> {
     r.y = f32x2_to_bf16x2_bits(f[2], f[3]);
     r.z = f32x2_to_bf16x2_bits(f[4], f[5]);
     r.w = f32x2_to_bf16x2_bits(f[6], f[7]);
+  }
+  __device__ __forceinline__ void pack(const bf16_t* e) {
+    r = make_uint4(e[0].v | (uint32_t)e[1].v << 16, e[2].v | (uint32_t)e[3].v << 16,
+                   e[4].v | (uint32_t)e[5].v << 16, e[6].v | (uint32_t)e[7].v << 16);
   }
   __device__ __forceinline__ void store(bf16_t* p) const { *reinterpret_cast<uint4*>(p) = r; }
   __device__ __forceinline__ void store_stream(bf16_t* p) const {
