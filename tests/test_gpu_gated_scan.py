@@ -3,8 +3,11 @@
 Error bound.  With u = 2^-24, a term u_s of h_t passes t - s products with gates; each product and
 each addition on the way (a step's multiply-add, or a run's product and its application) loses at
 most u of a value not above M_t = |a_t| M_{t-1} + |u_t|.  A sigmoid gate adds its own error: the
-exponential 1 ulp, 1 + e half, the quotient 2, the product half: at most 4 ulp = 8 u.  So with
-K = 2 (decay) or 12 (sigmoid) the error stays below u N_t, N_t = |a_t| (N_{t-1} + K M_{t-1}) +
+exponential 1 ulp, 1 + e half, the quotient 2, the product half: at most 4 ulp = 8 u.  Gates in bf16
+take e as one power of two, and the rounded argument adds to it: the constant log2(e) is off by
+0.23 u of itself and the product by u, so the exponent by 1.5 u |z| log2(e) and e by 1.5 |z| u; the
+power itself 4 u, 1 + e one u, the reciprocal 2 u, the product e / (1 + e) one u: (8 + 1.5 |z|) u.
+So with K = 2 (decay), 12 (sigmoid) or 12 + 1.5 |z| (sigmoid of bf16) the error stays below u N_t, N_t = |a_t| (N_{t-1} + K M_{t-1}) +
 K |u_t|, computed in 64 bits beside the recurrence; the gradients' bounds follow from those of g
 (the same recurrence backwards) and h.  A result is rounded once to its type: half a step more."""
 import pytest
@@ -37,9 +40,9 @@ def _reference(gate, x, h0, dh, dl, lengths, form):
     z, xx = gate.double().cpu(), x.double().cpu()
     n = [T] * B if lengths is None else [min(max(int(k), 0), T) for k in lengths]
     live = (torch.arange(T)[None] < torch.tensor(n)[:, None])[..., None].expand(B, T, C)
-    K = 2.0
+    K = torch.full_like(z, 2.0)
     if form == "sigmoid":
-        K = 12.0
+        K = 12.0 + (1.5 * z.abs() if gate.dtype == torch.bfloat16 else 0 * z)
         a, rest = torch.sigmoid(z), torch.sigmoid(-z)
         u = rest * xx
     else:
@@ -49,8 +52,8 @@ def _reference(gate, x, h0, dh, dl, lengths, form):
     H, HM, HN, P, PN = [], [], [], [], []
     for t in range(T):
         P.append(h), PN.append(N + 2 * M)
-        aa, uu = a[:, t].abs(), u[:, t].abs()
-        hn, Nn, Mn = a[:, t] * h + u[:, t], aa * (N + K * M) + K * uu, aa * M + uu
+        aa, uu, k = a[:, t].abs(), u[:, t].abs(), K[:, t]
+        hn, Nn, Mn = a[:, t] * h + u[:, t], aa * (N + k * M) + k * uu, aa * M + uu
         h, N, M = (torch.where(live[:, t], *p) for p in ((hn, h), (Nn, N), (Mn, M)))
         H.append(h), HM.append(M), HN.append(N)
     last = (h, U * (N + M))
@@ -61,8 +64,8 @@ def _reference(gate, x, h0, dh, dl, lengths, form):
         g, gM = d[:, t] + c, d[:, t].abs() + cM
         gN = cN + gM
         G[t], GN[t] = g, gN
-        aa = a[:, t].abs()
-        cn, cNn, cMn = a[:, t] * g, aa * (gN + K * gM), aa * gM
+        aa, k = a[:, t].abs(), K[:, t]
+        cn, cNn, cMn = a[:, t] * g, aa * (gN + k * gM), aa * gM
         c, cN, cM = (torch.where(live[:, t], *p) for p in ((cn, c), (cNn, cN), (cMn, cM)))
     out = {"last": last, "dh0": (c, U * (cN + cM))}
     if T:

@@ -285,3 +285,52 @@ def test_captured_and_replayed(cuda):
     graph.replay()
     for p, q in zip(out, step()):
         assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("R,D", [(1, 3), (2, 1), (9, 5), (3, 7), (17, 9), (50, 11), (33, 333),
+                                 (2000, 101), (21, 641), (13, 767), (19, 1001), (9, 2001),
+                                 (9, 4079), (5, 4081), (10, 1028)])
+def test_rows_that_begin_inside_16_bytes(cuda, dtype, R, D):
+    for how in (dict(), dict(norm="rms", gate=False, branch_norm=False, scale="one")):
+        _check(*_make(cuda, R, D, dtype, seed=R, **how))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("more", [3, 8, 24])
+def test_odd_rows_of_a_wider_buffer(cuda, dtype, more):
+    for D in (43, 901):
+        t, how, dy, dn = _make(cuda, 18, D, dtype, seed=7)
+        for k in ("x", "branch", "gate"):
+            wide = torch.full((18, D + more), float("nan"), device=cuda, dtype=dtype)
+            wide[:, :D] = t[k]
+            t[k] = wide[:, :D]
+        _check(t, how, dy, dn)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_bad_row_leaves_its_neighbours(cuda, dtype):
+    # rows of odd lengths share 16 bytes with their neighbours
+    for D in (5, 333, 1001):
+        t, how, dy, dn = _make(cuda, 20, D, dtype, seed=8)
+        bad = {k: (a.clone() if a is not None and a.dim() == 2 else a) for k, a in t.items()}
+        bdy, bdn = dy.clone(), dn.clone()
+        for a, v in zip((bad["x"], bad["branch"], bad["gate"], bdy, bdn),
+                        (float("nan"), float("inf"), float("nan"), float("inf"), float("nan"))):
+            a[1::2] = v
+        good, hit = _call(t, how, dy, dn), _call(bad, how, bdy, bdn)
+        for p, q in ((good[0], hit[0]), (good[1], hit[1]),
+                     *((good[2][k], hit[2][k]) for k in ("x", "branch", "gate"))):
+            assert torch.equal(p[::2], q[::2])
+            assert not torch.any(torch.isfinite(q[1::2]))
+
+
+def test_the_single_scale_sums_rows_in_64_bits(cuda):
+    # every term is 1 + 2^-10 and a row's sum of three exact: what is left is one rounding
+    from mk_iii_technologies_tsrn_b200 import ops
+    R = 100001
+    b = torch.full((R, 3), 1 + 2.0 ** -10, device=cuda)
+    scale = torch.ones(1, device=cuda, requires_grad=True)
+    y, _ = ops.residual_norm(torch.zeros_like(b), b, scale=scale, normalize=False)
+    y.backward(torch.ones_like(y))
+    assert scale.grad.item() == torch.tensor(3 * R * (1 + 2.0 ** -10), dtype=torch.float64).float()
