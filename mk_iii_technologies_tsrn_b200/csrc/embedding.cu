@@ -19,16 +19,22 @@
 //    digit the tokens are counted by warp, and placed: each warp ranks its run of
 //    tokens 32 at a time by digit match, on top of the counts of earlier bins,
 //    blocks and warps.  Up to 2^18 tokens one cluster of up to 16 blocks does all
-//    of it in one launch (131072 tokens of 131072 rows: see sort_cluster_kernel);
-//    more take two kernels a digit over all SMs.
+//    of it in one launch (65536 tokens of 256 rows 13 us, 131072 of 131072 rows
+//    34 us); more take two kernels a digit over all SMs.
 // 2. sum: tokens and table rows form one list of N + V items (the tokens of a
-//    row, then the row's end).  Each team of threads takes an equal share of
-//    it, found by bisection, whatever the distribution of the ids: it adds a
+//    row, then the row's end), tokens with twice the weight.  Each team of threads
+//    takes an equal share of it, found by bisection, whatever the ids: it adds a
 //    row of dout per token and writes a row of the gradient (zeros for an
 //    absent id) per end.  So every dout row is read once and every gradient
 //    row written once: the bytes the result needs.
 // 3. join: a table row whose tokens reach over several shares left fp32
 //    partial sums in the workspace; they are added in order.
+//
+// Measured, of the bytes each has to move at the card's copy rate: the forward of
+// 32 x 4096 tokens of 1024 bf16 channels 59 us, its gradient for 131072 rows 150 us
+// (sum 111), together 149 us of bytes; 64 x 1024 tokens of 640 fp32 channels with
+// 256 rows 32 and 74 us (sum 53), 52 us of bytes.  The sort is a chain of
+// exchanges over few blocks, and the sum's rows come in the order of the ids.
 #include <initializer_list>
 
 #include "maxplus_internal.cuh"
@@ -454,16 +460,23 @@ struct SumArgs {
   int* flags;           // [shares]: bit 0 the first row began earlier, bit 1 an end lies inside
 };
 
-// Tokens among the first `d` items of the list (the tokens of row 0, the end of
-// row 0, the tokens of row 1, ...): the smallest j with keys[j] + j >= d, as
-// token j is item keys[j] + j.  A whole warp searches, 32 places at a time.
+// The list of the tokens of row 0, the end of row 0, the tokens of row 1, ..., a token
+// TOKEN_COST places long and a row end one: token j begins at keys[j] + cost * j.  A
+// token is a row read, mostly one latency after the other within a team, an end a row
+// written: where frequent ids leave some teams with tokens alone and others with absent
+// rows, shares of equal counts wait for the former (8604 tokens of 132453 rows of 1096
+// fp32 channels, Zipf's law: 181 us at 1, 136 us at 2; 32 x 4096 of 131072 rows of 1024
+// bf16 channels: 126 and 111 us).
+constexpr int64_t TOKEN_COST = 2;
+// Tokens that begin before place `d`: the smallest j with keys[j] + cost * j >= d.  A
+// whole warp searches, 32 places at a time.
 __device__ __forceinline__ int64_t tokens_before(const int2* pairs, int64_t N, int64_t d) {
   const int lane = threadIdx.x & 31;
   int64_t lo = 0, hi = min(N, d);            // the answer lies in [lo, hi]
   while (lo < hi) {
     const int64_t step = (hi - lo + 31) / 32;
     const int64_t at = lo + lane * step;     // 32 places cover [lo, hi)
-    const bool below = at < hi && (int64_t)__ldg(pairs + at).x + at < d;
+    const bool below = at < hi && (int64_t)__ldg(pairs + at).x + TOKEN_COST * at < d;
     const int n = __popc(__ballot_sync(0xffffffffu, below));   // below for the first n lanes
     if (n == 0) return lo;
     const int64_t last = lo + (n - 1) * step;                  // the last place known below
@@ -475,6 +488,23 @@ __device__ __forceinline__ int64_t tokens_before(const int2* pairs, int64_t N, i
 
 constexpr int SUM_CHUNK = 128;
 
+// Zeros to elements [lo, hi) of out with `lanes` threads: whole 16 bytes wherever the
+// range holds them, since rows of absent tokens lie one behind the other.
+template <typename T>
+__device__ __forceinline__ void fill_zeros(T* out, int64_t lo, int64_t hi, int t, int lanes) {
+  constexpr int W = 16 / sizeof(T);
+  T* p = out + lo;
+  int64_t n = hi - lo;
+  const int64_t head =
+      min(n, (int64_t)((16 - ((uintptr_t)p & 15)) & 15) / (int64_t)sizeof(T));
+  if (t < head) p[t] = T{};
+  p += head;
+  n -= head;
+  for (int64_t i = t; i < n / W; i += lanes)
+    __stcs(reinterpret_cast<uint4*>(p) + i, make_uint4(0, 0, 0, 0));
+  if (t < n % W) p[n / W * W + t] = T{};
+}
+
 // A team's share of the columns [blockIdx.y * lanes * VEC, ...) of its items.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256) embedding_sum_kernel(const SumArgs s) {
@@ -483,12 +513,13 @@ __global__ void __launch_bounds__(256) embedding_sum_kernel(const SumArgs s) {
   const int per = blockDim.x / s.lanes, t = threadIdx.x % s.lanes;
   const int64_t share = (int64_t)blockIdx.x * per + threadIdx.x / s.lanes;
   if (share >= s.shares) return;
-  const int64_t items = s.N + s.V;
+  const int64_t items = TOKEN_COST * s.N + s.V;
   const int64_t d0 = share * s.share, d1 = min(items, d0 + s.share);
   int64_t j = tokens_before(s.pairs, s.N, d0);
   const int64_t j1 = tokens_before(s.pairs, s.N, d1);
-  int64_t v = d0 - j;
-  const int64_t v1 = d1 - j1;          // rows whose end lies before d1
+  // rows whose end lies before d0 and d1 (a place inside a token counts as behind it)
+  int64_t v = max(d0 - TOKEN_COST * j, j > 0 ? (int64_t)s.pairs[j - 1].x : 0);
+  const int64_t v1 = max(d1 - TOKEN_COST * j1, j1 > 0 ? (int64_t)s.pairs[j1 - 1].x : 0);
   const int64_t c = ((int64_t)blockIdx.y * s.lanes + t) * VEC;
   const bool in = c < s.D;
   // the first row continues one of an earlier share
@@ -520,6 +551,19 @@ __global__ void __launch_bounds__(256) embedding_sum_kernel(const SumArgs s) {
 #pragma unroll
     for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
   };
+  // row ends up to row `to`: this row's, then absent ones.  Longer runs of those are one
+  // range of zeros, of which each column range takes its part (8604 tokens of 132453 rows
+  // of 1095 fp32 channels: 222 us against 339 us row by row; runs of two rows lose by it).
+  auto end_rows = [&](int64_t to) {
+    end_row();
+    if (to - v >= 4) {
+      const int64_t first = v * s.D, n = (to - v) * s.D;
+      const int64_t part = (n + gridDim.y - 1) / gridDim.y, lo = min(n, blockIdx.y * part);
+      fill_zeros((T*)s.dweight, first + lo, first + min(n, lo + part), t, s.lanes);
+      v = to;
+    }
+    while (v < to) end_row();
+  };
   // pairs of 128 tokens at a time in shared memory, a copy for each warp
   __shared__ int2 s_pairs[8][SUM_CHUNK];
   int2* const pairs = s_pairs[threadIdx.x >> 5];
@@ -547,7 +591,7 @@ __global__ void __launch_bounds__(256) embedding_sum_kernel(const SumArgs s) {
         if (u < n) {
           const int key = pairs[i + u].x;
           if (key >= s.V) break;             // dropped tokens come last
-          while (v < key) end_row();
+          if (v < key) end_rows(key);
           if (in) {
             float f[VEC];
             row[u].get(f);
@@ -558,7 +602,7 @@ __global__ void __launch_bounds__(256) embedding_sum_kernel(const SumArgs s) {
       }
     }
   }
-  while (v < v1) end_row();
+  if (v < v1) end_rows(v1);
   if (in) {
 #pragma unroll
     for (int k = 0; k < VEC; ++k) s.tail[share * s.D + c + k] = acc[k];
@@ -722,14 +766,14 @@ struct SumPlan {
 // items each, so that partial sums stay few (two or four waves: the sums of 60 x 4096 tokens
 // 83, 85 and 92 us, their joins 8, 14 and 25 us).  By the sizes alone.
 SumPlan sum_plan(int64_t N, int64_t V, int64_t D, int esize) {
-  const int64_t items = N + V;
+  const int64_t items = TOKEN_COST * N + V;
   int64_t ranges;
   const int lanes = sum_lanes(D, 16 / esize, &ranges);
   const int per = sum_teams(lanes);
   int64_t teams = 819 / (lanes * per) * per / ranges;
   if (teams < 1) teams = 1;
   int64_t share = ceil_div(items, num_sms() * teams);
-  if (share < 16) share = 16;
+  if (share < 16 * TOKEN_COST) share = 16 * TOKEN_COST;
   return {share, ceil_div(items, share)};
 }
 

@@ -218,3 +218,27 @@ def test_captured_and_replayed(cuda):
         ids.copy_(torch.randint(0, 500, (8, 300), device=cuda, generator=_gen(cuda, seed)))
         graph.replay()
         assert torch.equal(dw, ops.embedding_bwd(ids, dout, 500))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D", [33, 40, 1095, 2056])
+def test_every_row_of_a_sparse_gradient_is_written(cuda, dtype, D):
+    # runs of absent rows of all lengths, before, between and behind the tokens' rows, over a
+    # buffer of NaN; one id very often, so that some shares hold tokens alone
+    from mk_iii_technologies_tsrn_b200 import _lib
+    lib = _lib.load()
+    g = torch.Generator(device=cuda).manual_seed(3)
+    V, rows = 4000, torch.tensor([3, 4, 6, 9, 13, 18, 30, 700, 701, 3990], device=cuda)
+    ids = torch.cat((rows, rows[4].expand(3000), rows[torch.randint(0, 10, (90,), device=cuda,
+                                                                    generator=g)]))
+    N = ids.numel()
+    dout = torch.randint(-8, 9, (N, D), device=cuda, generator=g).to(dtype)    # sums are exact
+    dw = torch.full((V * D + 8,), float("nan"), device=cuda, dtype=dtype)
+    need = lib.tp_embedding_bwd_workspace_bytes(N, V, D)
+    ws = torch.full((need,), 255, device=cuda, dtype=torch.uint8)
+    st = lib.tp_embedding_bwd(0 if dtype == torch.float32 else 1, 64, N, D, ids.data_ptr(),
+                              dout.data_ptr(), V, 1.0, -1, dw.data_ptr(), ws.data_ptr(), need,
+                              torch.cuda.current_stream().cuda_stream)
+    assert st == 0
+    want = torch.zeros(V, D, device=cuda, dtype=torch.float64).index_add_(0, ids, dout.double())
+    assert torch.equal(dw[:V * D].view(V, D), want.to(dtype)) and torch.all(dw[V * D:].isnan())
