@@ -298,6 +298,25 @@ def load(path: str | None = None) -> ctypes.CDLL:
         return lib
 
 
+_host = None
+
+
+def host():
+    """The host module of the language-model operators over the library (once)."""
+    global _host
+    if _host is None:
+        load()
+        with _lock:
+            try:
+                from . import _tropical_b200_torch as module
+            except ImportError as e:
+                raise RuntimeError(
+                    f"the host module _tropical_b200_torch.so does not load ({e}); build it with "
+                    "`python -m mk_iii_technologies_tsrn_b200.build`") from e
+            _host = module
+    return _host
+
+
 def status_text(status: int) -> str:
     return load().tp_status_string(status).decode()
 

@@ -3,8 +3,10 @@
 Compiles every ``csrc/*.cu`` with nvcc for ``sm_100a`` only and links them
 into one shared library next to this file.  The library exposes the C ABI
 declared in ``include/tropical_b200.h``; Python reaches it through ctypes
-(``_lib.py``).  Rebuilds only when a source or header is newer than the
-library.  Run ``python -m mk_iii_technologies_tsrn_b200.build`` or call
+(``_lib.py``).  ``csrc/torch_host.cpp``, the host side of the language-model
+operators over that ABI (outputs, workspaces, autograd nodes), becomes the Python
+module ``_tropical_b200_torch.so`` beside it.  Rebuilds only what is older than
+its sources and headers.  Run ``python -m mk_iii_technologies_tsrn_b200.build`` or call
 :func:`build`.
 """
 from __future__ import annotations
@@ -22,6 +24,9 @@ INCLUDE = os.path.join(REPO_DIR, "include")
 LIB_NAME = "_tropical_b200.so"
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
 BUILD_DIR = os.path.join(PKG_DIR, "_build")
+HOST_SOURCE = os.path.join(CSRC, "torch_host.cpp")
+HOST_MODULE = "_tropical_b200_torch"
+HOST_PATH = os.path.join(PKG_DIR, HOST_MODULE + ".so")
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = [
@@ -63,16 +68,53 @@ def needs_build() -> bool:
     return any(os.path.getmtime(p) > lib_mtime for p in _deps())
 
 
+def needs_host_build() -> bool:
+    if not os.path.exists(HOST_PATH):
+        return True
+    built = os.path.getmtime(HOST_PATH)
+    return any(os.path.getmtime(p) > built for p in
+               [HOST_SOURCE, os.path.abspath(__file__), *glob.glob(os.path.join(INCLUDE, "*.h"))])
+
+
+def build_host(verbose: bool = False) -> str:
+    """Compile ``torch_host.cpp`` against the installed torch and link it to the library."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    cuda = os.path.dirname(os.path.dirname(_nvcc()))
+    libs = os.path.join(os.path.dirname(torch.__file__), "lib")
+    includes = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"],
+                os.path.join(cuda, "include"), INCLUDE]
+    tmp = HOST_PATH + ".tmp"
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+           "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f"-DTORCH_EXTENSION_NAME={HOST_MODULE}", *(f"-isystem{i}" for i in includes),
+           HOST_SOURCE, "-o", tmp, f"-L{libs}", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10",
+           "-lc10_cuda", "-ltorch_python", f"-L{PKG_DIR}", f"-l:{LIB_NAME}",
+           "-Wl,-rpath,$ORIGIN"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"the host module failed to build:\n{res.stdout}\n{res.stderr}")
+    os.replace(tmp, HOST_PATH)
+    return HOST_PATH
+
+
 def build(force: bool = False, verbose: bool = False, ptxas_verbose: bool = False,
           extra_flags: list[str] | None = None, lib_path: str | None = None,
           build_dir: str | None = None) -> str:
-    """Compile the library if needed and return its path.
+    """Compile the library and its host module if needed and return the library's path.
 
     ``extra_flags`` (e.g. ``-DTP_TMA_TM=8``) and ``lib_path``/``build_dir`` build a
     variant library elsewhere without touching the in-tree one."""
     out_path = lib_path or LIB_PATH
     bdir = build_dir or BUILD_DIR
     if lib_path is None and not force and not needs_build():
+        if needs_host_build():
+            build_host(verbose)
         return LIB_PATH
     nvcc = _nvcc()
     os.makedirs(bdir, exist_ok=True)
@@ -107,6 +149,8 @@ def build(force: bool = False, verbose: bool = False, ptxas_verbose: bool = Fals
     if res.returncode != 0:
         raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
     os.replace(tmp, out_path)
+    if lib_path is None and (force or needs_host_build()):
+        build_host(verbose)
     return out_path
 
 

@@ -15,19 +15,35 @@
 //
 // Both directions are bound by memory: the forward reads x, branch, gate once
 // and writes y and n; the backward reads x, branch, gate, dy, dn once and
-// writes dx, dbranch, dgate.  A team of G threads (a warp, or up to 16 warps
-// for long rows) holds a whole row in registers, so the statistics cost no
-// second read; all loads of a row are issued before the first use.  The
-// backward recomputes y from x (the same bytes as reading y, and exact where
-// the stored y is rounded to bf16) and takes the row statistics (mean and
-// 1 / deviation of y and branch) from the forward.
+// writes dx, dbranch, dgate.  A team of G threads (a warp, or a block of up to
+// 16 warps for long rows) holds a whole row in registers, so the statistics cost
+// no second read; all loads of a row are issued before the first use, and the
+// team's next row is asked into L2 meanwhile.  The backward recomputes y from x
+// (the same bytes as reading y, and exact where the stored y is rounded to bf16)
+// and takes the row statistics (mean and 1 / deviation of y and branch) from the
+// forward.
+//
+// Rows of an odd length begin inside 16 bytes, each at another element; rows
+// eight apart begin at the same one.  So a block takes rows that are alike modulo
+// eight, and its vectors lie on 16 bytes in all of them, each with channels of its
+// own for good (the column sums need that): only the first and the last vector of
+// a row are cut.  42919 x 1031 bf16: 168 and 372 us against 594 and 1199 us with
+// single channels.
 //
 // Parameter gradients are column sums.  Up to five of them run at once (w, b,
 // channel scale, bw, bb), too many to stay in registers beside the row, so
 // each thread keeps those of its own columns in shared memory (16-byte
 // read-add-writes without conflicts, no synchronisation); a block adds its
 // teams in order and a second kernel adds the blocks in order, so the same
-// inputs give the same bits.
+// inputs give the same bits.  A single scale's gradient is one sum over all
+// elements, whose terms may cancel: a row of it is added in fp32, the rows in
+// 64 bits.
+//
+// Measured (forward, backward), in the bytes above: 65536 x 640 fp32 with gate and
+// LayerNorm 139 us (6.0 TB/s) and 241 us (5.6); 16384 x 2048 fp32 with a branch
+// norm and a channel scale 94 (5.7) and 200 us (4.0), bf16 59 (4.5) and 159 us
+// (2.5): bf16 rows have the same arithmetic for half the bytes, and the backward's
+// 128 registers a thread leave 16 warps on an SM to hide it.
 #include <initializer_list>
 
 #include "residual_norm.cuh"

@@ -16,12 +16,20 @@ Reference expressions each op replaces (Mediocr3Mik3/MK_III_Technologies_TSRN):
   tropical attention score (``research/tsrn_dml.py:438-460``).
 * :func:`tropical_scan` -- the ``TropicalSSM`` max-plus recurrence
   (``research/tsrn_dml.py:961-972``), evaluated as the exact sequential recurrence.
+
+Operators around them in a language model, with their gradients:
+
+* :func:`embedding` -- ``embed(ids) * scale + pos_embed(positions)``
+  (``tropformer_dropin.py:616-720``), the gradient by sorted tokens.
+* :func:`residual_norm` -- the branch's norm, gate and scale, the residual sum and the next
+  block's norm in one pass (``research/tsrn_dml.py:975-980,1096-1106``).
+* :func:`gated_scan`, :func:`gated_scan_step` -- the gated linear recurrence, the (plus, times)
+  counterpart of :func:`tropical_scan`, over sequences and for one token.
 """
 from __future__ import annotations
 
 import contextlib
 import ctypes
-import functools
 from typing import Optional, Tuple
 
 import torch
@@ -1262,78 +1270,16 @@ NORMS = {"layer": _lib.TP_NORM_LAYER, "rms": _lib.TP_NORM_RMS}
 RESIDUAL_NORM_MAX_CHANNELS = 8192
 
 
-def _once(backward):
-    # torch's once_differentiable where a second derivative could be asked for (a backward that
-    # records); its wrapper costs every other backward a few microseconds
-    guarded = torch.autograd.function.once_differentiable(backward)
-
-    @functools.wraps(backward)
-    def run(ctx, *grads):
-        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
-    return run
-
-
-def _launch(name: str, dev: torch.device, *args) -> None:
-    # an entry point on the device's current stream.  These operators are also called for single
-    # tokens, where the host's time is the call's: the device is switched only if it is another,
-    # and addresses and the stream go through as plain integers
-    fn = getattr(_lib.load(), name)
-    if torch._C._cuda_getDevice() == dev.index:
-        st = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
-    else:
-        with torch.cuda.device(dev):
-            st = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
-    if st:
-        _lib.check(st, name)
-
-
-def _on(dev: torch.device):
-    # the device as the current one (for a size that depends on it)
-    return (contextlib.nullcontext() if torch._C._cuda_getDevice() == dev.index
-            else torch.cuda.device(dev))
-
-
-def _at(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
-
-
-def _channels(t: torch.Tensor) -> torch.Tensor:
-    # the last dimension contiguous; the others at any strides
-    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
-
-
-def _rows_of(t: Optional[torch.Tensor], D: int):
-    # t as rows of D channels, and their stride
-    if t is None:
-        return None, 0
-    if t.is_contiguous():
-        return t, D
-    t = _channels(t.reshape(-1, D))
-    return t, t.stride(0)
-
-
-def _contiguous(t: Optional[torch.Tensor]):
-    return t if t is None or t.is_contiguous() else t.contiguous()
-
-
-def _empty_as(t: torch.Tensor) -> torch.Tensor:
-    # contiguous, of t's shape, dtype and device
-    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
-
-
-def _floating(t: torch.Tensor, what: str) -> int:
-    if t.dtype == torch.float32:
-        return TP_DTYPE_F32
-    if t.dtype == torch.bfloat16:
-        return TP_DTYPE_BF16
-    raise TypeError(f"{what} must be float32 or bfloat16, got {t.dtype}")
+def _floating(t: torch.Tensor, what: str) -> None:
+    if t.dtype != torch.float32 and t.dtype != torch.bfloat16:
+        raise TypeError(f"{what} must be float32 or bfloat16, got {t.dtype}")
 
 
 def _residual_norm_args(x, branch, weight, bias, norm, gate, scale, branch_norm, branch_weight,
                         branch_bias, normalize):
-    """Checks; (device, dtype code, parameters' dtype code, D)."""
+    """Checks; (device, D)."""
     dev = _require_cuda(x, branch, weight, bias, gate, scale, branch_weight, branch_bias)
-    dtype = _floating(x, "residual_norm inputs")
+    _floating(x, "residual_norm inputs")
     D = x.shape[-1] if x.dim() else 0
     if not 1 <= D <= RESIDUAL_NORM_MAX_CHANNELS:
         raise ValueError(f"residual_norm takes 1 to {RESIDUAL_NORM_MAX_CHANNELS} channels, got {D}")
@@ -1358,54 +1304,7 @@ def _residual_norm_args(x, branch, weight, bias, norm, gate, scale, branch_norm,
         if t.dtype not in (torch.float32, x.dtype) or t.dtype != (pd or t.dtype):
             raise TypeError("residual_norm parameters must share a dtype: float32 or that of x")
         pd = t.dtype
-    return dev, dtype, TP_DTYPE_BF16 if pd == torch.bfloat16 else TP_DTYPE_F32, D
-
-
-@functools.lru_cache(maxsize=1024)
-def _residual_norm_bytes(index: int, rows: int, D: int) -> int:
-    with _on(torch.device("cuda", index)):
-        return _lib.load().tp_residual_norm_bwd_workspace_bytes(rows, D)
-
-
-def _residual_norm_run(dev, dtype, pdtype, D, x, branch, weight, bias, eps, norm, gate, scale,
-                       branch_norm, branch_weight, branch_bias, normalize, need_stats):
-    (x2, ldx), (b2, ldb), (g2, ldg) = _rows_of(x, D), _rows_of(branch, D), _rows_of(gate, D)
-    w, b, bw, bb, sc = (_contiguous(t) for t in (weight, bias, branch_weight, branch_bias, scale))
-    rows = x.numel() // D
-    y = _empty_as(x)
-    n = torch.empty_like(y) if normalize else None
-    stats = torch.empty((rows, 4), device=dev, dtype=torch.float32) if need_stats else None
-    _launch("tp_residual_norm_fwd", dev, dtype, pdtype, NORMS[norm], rows, D, x2.data_ptr(), ldx,
-            b2.data_ptr(), ldb, _at(g2), ldg, _at(sc), sc is not None and sc.numel() > 1,
-            branch_norm, _at(bw), _at(bb), _at(w), _at(b), eps, y.data_ptr(), _at(n), _at(stats))
-    return y, n, stats
-
-
-def _residual_norm_back(dev, dtype, pdtype, D, stats, dy, dn, x, branch, weight, bias, eps, norm,
-                        gate, scale, branch_norm, branch_weight, branch_bias, wanted):
-    """(dx, dbranch, dgate, [dscale, dweight, dbias, dbranch_weight, dbranch_bias]); the parameter
-    gradients that are ``wanted`` are float32 views of one buffer."""
-    (x2, ldx), (b2, ldb), (g2, ldg) = _rows_of(x, D), _rows_of(branch, D), _rows_of(gate, D)
-    w, b, bw, bb, sc = (_contiguous(t) for t in (weight, bias, branch_weight, branch_bias, scale))
-    dy, dn = _contiguous(dy), _contiguous(dn)
-    rows = x.numel() // D
-    dx, dbranch = _empty_as(x), _empty_as(branch)
-    dgate = _empty_as(gate) if gate is not None else None
-    params = [None] * 5
-    sizes = [t.numel() if want else 0 for t, want in zip((scale, weight, bias, branch_weight,
-                                                          branch_bias), wanted)]
-    if any(wanted):
-        views = torch.empty(sum(sizes), device=dev, dtype=torch.float32).split_with_sizes(sizes)
-        params = [v if want else None for v, want in zip(views, wanted)]
-    need = _residual_norm_bytes(dev.index, rows, D)
-    ws = torch.empty(need, device=dev, dtype=torch.uint8)
-    dsc, dw, db, dbw, dbb = params
-    _launch("tp_residual_norm_bwd", dev, dtype, pdtype, NORMS[norm], rows, D, x2.data_ptr(), ldx,
-            b2.data_ptr(), ldb, _at(g2), ldg, _at(sc), sc is not None and sc.numel() > 1,
-            branch_norm, _at(bw), _at(bb), _at(w), _at(b), eps, stats.data_ptr(), _at(dy), _at(dn),
-            dx.data_ptr(), dbranch.data_ptr(), _at(dgate), _at(dsc), _at(dbw), _at(dbb), _at(dw),
-            _at(db), ws.data_ptr(), need)
-    return dx, dbranch, dgate, params
+    return dev, D
 
 
 def residual_norm_fwd(x, branch, weight=None, bias=None, eps: float = 1e-5, *, norm: str = "layer",
@@ -1413,10 +1312,11 @@ def residual_norm_fwd(x, branch, weight=None, bias=None, eps: float = 1e-5, *, n
                       branch_bias=None, normalize: bool = True, need_stats: bool = False):
     """Forward of :func:`residual_norm` without autograd: (y, n | None, stats | None), stats
     [rows, 4] fp32 for :func:`residual_norm_bwd`."""
-    head = _residual_norm_args(x, branch, weight, bias, norm, gate, scale, branch_norm,
-                               branch_weight, branch_bias, normalize)
-    return _residual_norm_run(*head, x, branch, weight, bias, eps, norm, gate, scale, branch_norm,
-                              branch_weight, branch_bias, normalize, need_stats)
+    _residual_norm_args(x, branch, weight, bias, norm, gate, scale, branch_norm, branch_weight,
+                        branch_bias, normalize)
+    return _lib.host().residual_norm_fwd(x, branch, gate, scale, weight, bias, branch_weight,
+                                         branch_bias, eps, NORMS[norm], branch_norm, normalize,
+                                         need_stats)
 
 
 def residual_norm_bwd(stats, dy, dn, x, branch, weight=None, bias=None, eps: float = 1e-5, *,
@@ -1426,61 +1326,21 @@ def residual_norm_bwd(stats, dy, dn, x, branch, weight=None, bias=None, eps: flo
     a dict with the gradients of x, branch, gate (in their dtype) and of scale, weight, bias,
     branch_weight, branch_bias (float32); None for what is not there.  Parameter gradients are
     summed in a fixed order (the same bits on every call)."""
-    head = _residual_norm_args(x, branch, weight, bias, norm, gate, scale, branch_norm,
-                               branch_weight, branch_bias, normalize)
+    dev, D = _residual_norm_args(x, branch, weight, bias, norm, gate, scale, branch_norm,
+                                 branch_weight, branch_bias, normalize)
     for t, what in ((dy, "dy"), (dn, "dn")):
-        if t is not None and (t.shape != x.shape or t.dtype != x.dtype or t.device != head[0]):
+        if t is not None and (t.shape != x.shape or t.dtype != x.dtype or t.device != dev):
             raise ValueError(f"{what} must have the shape, dtype and device of x")
     if dn is not None and not normalize:
         raise ValueError("dn needs normalize=True")
-    if (stats is None or stats.shape != (x.numel() // head[3], 4) or stats.device != head[0]
+    if (stats is None or stats.shape != (x.numel() // D, 4) or stats.device != dev
             or stats.dtype != torch.float32 or not stats.is_contiguous()):
         raise ValueError("stats must be the forward's [rows, 4] float32 tensor")
-    given = (scale, weight, bias, branch_weight, branch_bias)
-    dx, dbranch, dgate, ps = _residual_norm_back(
-        *head, stats, dy, dn, x, branch, weight, bias, eps, norm, gate, scale, branch_norm,
-        branch_weight, branch_bias, [t is not None for t in given])
-    ps = [g.view(t.shape) if t is not None else None for g, t in zip(ps, given)]
+    grads = _lib.host().residual_norm_bwd(stats, dy, dn, x, branch, gate, scale, weight, bias,
+                                          branch_weight, branch_bias, eps, NORMS[norm],
+                                          branch_norm)
     return dict(zip(("x", "branch", "gate", "scale", "weight", "bias", "branch_weight",
-                     "branch_bias"), (dx, dbranch, dgate, *ps)))
-
-
-class ResidualNormFunction(torch.autograd.Function):
-    """(y, n) of :func:`residual_norm`; the backward recomputes y from x and takes the row
-    statistics from the forward."""
-
-    @staticmethod
-    def forward(ctx, x, branch, gate, scale, weight, bias, branch_weight, branch_bias, eps, norm,
-                branch_norm, normalize):
-        ctx.set_materialize_grads(False)
-        head = _residual_norm_args(x, branch, weight, bias, norm, gate, scale, branch_norm,
-                                   branch_weight, branch_bias, normalize)
-        y, n, stats = _residual_norm_run(*head, x, branch, weight, bias, eps, norm, gate, scale,
-                                         branch_norm, branch_weight, branch_bias, normalize, True)
-        ctx.save_for_backward(x, branch, gate, scale, weight, bias, branch_weight, branch_bias,
-                              stats)
-        ctx.how = (head, eps, norm, branch_norm)
-        return y, n
-
-    @staticmethod
-    @_once
-    def backward(ctx, dy, dn):
-        if dy is None and dn is None:
-            return (None,) * 12
-        x, branch, gate, scale, weight, bias, bw, bb, stats = ctx.saved_tensors
-        head, eps, norm, branch_norm = ctx.how
-        need = ctx.needs_input_grad
-        dx, dbranch, dgate, ps = _residual_norm_back(
-            *head, stats, dy, dn, x, branch, weight, bias, eps, norm, gate, scale, branch_norm,
-            bw, bb, need[3:8])
-        for i, t in enumerate((scale, weight, bias, bw, bb)):
-            if ps[i] is not None:
-                if t.dtype != torch.float32:
-                    ps[i] = ps[i].to(t.dtype)
-                if t.dim() != 1:
-                    ps[i] = ps[i].view(t.shape)
-        return (dx if need[0] else None, dbranch if need[1] else None, dgate if need[2] else None,
-                *ps, None, None, None, None)
+                     "branch_bias"), grads))
 
 
 def residual_norm(x: torch.Tensor, branch: torch.Tensor, weight: Optional[torch.Tensor] = None,
@@ -1500,14 +1360,10 @@ def residual_norm(x: torch.Tensor, branch: torch.Tensor, weight: Optional[torch.
     biases are float32 or of x's dtype.  Differentiable in all tensors.  It is the TSRN block's
     ``x + branch(ln(x))`` (research/tsrn_dml.py:1096-1106) with TropicalSSM's gate and mix
     (:975-980) and the next LayerNorm."""
-    ts = (x, branch, gate, scale, weight, bias, branch_weight, branch_bias)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
-        return ResidualNormFunction.apply(*ts, float(eps), norm, bool(branch_norm),
-                                          bool(normalize))
-    y, n, _ = residual_norm_fwd(x, branch, weight, bias, eps, norm=norm, gate=gate, scale=scale,
-                                branch_norm=branch_norm, branch_weight=branch_weight,
-                                branch_bias=branch_bias, normalize=normalize)
-    return y, n
+    _residual_norm_args(x, branch, weight, bias, norm, gate, scale, branch_norm, branch_weight,
+                        branch_bias, normalize)
+    return _lib.host().residual_norm(x, branch, gate, scale, weight, bias, branch_weight,
+                                     branch_bias, eps, NORMS[norm], branch_norm, normalize)
 
 
 # --------------------------------------------------------------------------- gated scan
@@ -1521,9 +1377,9 @@ def _gate_form(form: str) -> int:
 
 
 def _gated_scan_inputs(gate, x, h0, lengths):
-    """Checks; (device, dtype code, lengths as int32 | None)."""
+    """Checks; (device, lengths as int32 | None)."""
     dev = _require_cuda(gate, x, h0, lengths)
-    dtype = _floating(x, "gated_scan inputs")
+    _floating(x, "gated_scan inputs")
     if x.dim() != 3 or gate.shape != x.shape or gate.dtype != x.dtype:
         raise ValueError("gate and x must be [B, T, C] of one shape and dtype, got "
                          f"{tuple(gate.shape)} {gate.dtype} and {tuple(x.shape)} {x.dtype}")
@@ -1537,44 +1393,7 @@ def _gated_scan_inputs(gate, x, h0, lengths):
         if lengths.dtype == torch.int64:
             lengths = lengths.clamp(0, T).to(torch.int32)
         lengths = lengths.contiguous()
-    return dev, dtype, lengths
-
-
-@functools.lru_cache(maxsize=1024)
-def _gated_scan_bytes(index: int, B: int, T: int, C: int) -> int:
-    with _on(torch.device("cuda", index)):
-        return _lib.load().tp_gated_scan_workspace_bytes(B, T, C)
-
-
-def _gated_scan_workspace(dev, B, T, C):
-    need = _gated_scan_bytes(dev.index, B, T, C)
-    return (torch.empty(need, device=dev, dtype=torch.uint8) if need > 0 else None), need
-
-
-def _gated_scan_run(dev, dtype, lengths, code, gate, x, h0, need_states, need_last):
-    B, T, C = x.shape
-    gate, x, h0 = _channels(gate), _channels(x), _contiguous(h0)
-    h = _empty_as(x)
-    last = torch.empty((B, C), device=dev, dtype=torch.float32) if need_last else None
-    states = (torch.empty((B, -(-T // 64), C), device=dev, dtype=torch.float32)
-              if need_states else None)
-    ws, need = _gated_scan_workspace(dev, B, T, C)
-    _launch("tp_gated_scan_fwd", dev, dtype, code, B, T, C, gate.data_ptr(), gate.stride(0),
-            gate.stride(1), x.data_ptr(), x.stride(0), x.stride(1), _at(h0), _at(lengths),
-            h.data_ptr(), _at(last), _at(states), _at(ws), need)
-    return h, last, states
-
-
-def _gated_scan_back(dev, dtype, lengths, code, states, dh, dh_last, gate, x, need_dh0):
-    B, T, C = x.shape
-    gate, x, dh, dh_last = _channels(gate), _channels(x), _contiguous(dh), _contiguous(dh_last)
-    dgate, dx = _empty_as(x), _empty_as(x)
-    dh0 = torch.empty((B, C), device=dev, dtype=torch.float32) if need_dh0 else None
-    ws, need = _gated_scan_workspace(dev, B, T, C)
-    _launch("tp_gated_scan_bwd", dev, dtype, code, B, T, C, gate.data_ptr(), gate.stride(0),
-            gate.stride(1), x.data_ptr(), x.stride(0), x.stride(1), _at(lengths), _at(states),
-            _at(dh), _at(dh_last), dgate.data_ptr(), dx.data_ptr(), _at(dh0), _at(ws), need)
-    return dgate, dx, dh0
+    return dev, lengths
 
 
 def gated_scan_fwd(gate, x, h0=None, *, form: str = "decay", lengths=None,
@@ -1582,8 +1401,8 @@ def gated_scan_fwd(gate, x, h0=None, *, form: str = "decay", lengths=None,
     """Forward of :func:`gated_scan` without autograd: (h, h_last | None, states | None), states
     [B, ceil(T / 64), C] fp32 for :func:`gated_scan_bwd`."""
     code = _gate_form(form)
-    head = _gated_scan_inputs(gate, x, h0, lengths)
-    return _gated_scan_run(*head, code, gate, x, h0, need_states, need_last)
+    _, lengths = _gated_scan_inputs(gate, x, h0, lengths)
+    return _lib.host().gated_scan_fwd(gate, x, h0, lengths, code, need_states, need_last)
 
 
 def gated_scan_bwd(states, dh, dh_last, gate, x, *, form: str = "decay", lengths=None,
@@ -1591,42 +1410,16 @@ def gated_scan_bwd(states, dh, dh_last, gate, x, *, form: str = "decay", lengths
     """Backward of :func:`gated_scan` from the gradients of h and h_last (either may be None) and
     the forward's states: (dgate, dx, dh0 | None)."""
     code = _gate_form(form)
-    head = _gated_scan_inputs(gate, x, None, lengths)
+    dev, lengths = _gated_scan_inputs(gate, x, None, lengths)
     B, T, C = x.shape
     if (states is None or states.shape != (B, -(-T // 64), C) or states.dtype != torch.float32
-            or states.device != head[0] or not states.is_contiguous()):
+            or states.device != dev or not states.is_contiguous()):
         raise ValueError("states must be the forward's [B, ceil(T / 64), C] float32 tensor")
-    if dh is not None and (dh.shape != x.shape or dh.dtype != x.dtype or dh.device != head[0]):
+    if dh is not None and (dh.shape != x.shape or dh.dtype != x.dtype or dh.device != dev):
         raise ValueError("dh must have the shape, dtype and device of x")
-    if dh_last is not None and (_f32(dh_last).shape != (B, C) or dh_last.device != head[0]):
+    if dh_last is not None and (_f32(dh_last).shape != (B, C) or dh_last.device != dev):
         raise ValueError(f"dh_last must be [{B}, {C}] on the inputs' device")
-    return _gated_scan_back(*head, code, states, dh, dh_last, gate, x, need_dh0)
-
-
-class GatedScanFunction(torch.autograd.Function):
-    """(h, h_last) of :func:`gated_scan`; keeps gate, x and one fp32 state per 64 steps."""
-
-    @staticmethod
-    def forward(ctx, gate, x, h0, form: str, lengths):
-        ctx.set_materialize_grads(False)
-        code = _gate_form(form)
-        dev, dtype, lengths = _gated_scan_inputs(gate, x, h0, lengths)
-        h, last, states = _gated_scan_run(dev, dtype, lengths, code, gate, x, h0, True, True)
-        ctx.save_for_backward(gate, x, lengths, states)
-        ctx.how = (dev, dtype, code)
-        return h, last
-
-    @staticmethod
-    @_once
-    def backward(ctx, dh, dh_last):
-        if dh is None and dh_last is None:
-            return (None,) * 5
-        gate, x, lengths, states = ctx.saved_tensors
-        dev, dtype, code = ctx.how
-        need = ctx.needs_input_grad
-        dgate, dx, dh0 = _gated_scan_back(dev, dtype, lengths, code, states, dh, dh_last, gate, x,
-                                          need[2])
-        return dgate if need[0] else None, dx if need[1] else None, dh0, None, None
+    return _lib.host().gated_scan_bwd(states, dh, dh_last, gate, x, lengths, code, need_dh0)
 
 
 def gated_scan(gate: torch.Tensor, x: torch.Tensor, h0: Optional[torch.Tensor] = None, *,
@@ -1644,11 +1437,9 @@ def gated_scan(gate: torch.Tensor, x: torch.Tensor, h0: Optional[torch.Tensor] =
     there is read.  Returns h [B, T, C] in x's dtype, with ``return_state`` also the float32
     state [B, C] at each row's end (for :func:`gated_scan_step`, or to go on with the next
     segment).  States are float32 throughout.  Meant for gates of magnitude at most 1."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (gate, x, h0)):
-        h, last = GatedScanFunction.apply(gate, x, h0, form, lengths)
-    else:
-        h, last, _ = gated_scan_fwd(gate, x, h0, form=form, lengths=lengths,
-                                    need_last=return_state)
+    code = _gate_form(form)
+    _, lengths = _gated_scan_inputs(gate, x, h0, lengths)
+    h, last = _lib.host().gated_scan(gate, x, h0, lengths, code, return_state)
     return (h, last) if return_state else h
 
 
@@ -1658,8 +1449,8 @@ def gated_scan_step(gate: torch.Tensor, x: torch.Tensor, state: torch.Tensor, *,
     of at least C) is updated in place and the new h [B, C] returned in x's dtype.  ``gate``,
     ``x``: [B, C].  Not differentiable."""
     code = _gate_form(form)
-    dev = _require_cuda(gate, x, state)
-    dtype = _floating(x, "gated_scan_step inputs")
+    _require_cuda(gate, x, state)
+    _floating(x, "gated_scan_step inputs")
     if x.dim() != 2 or gate.shape != x.shape or gate.dtype != x.dtype:
         raise ValueError("gate and x must be [B, C] of one shape and dtype, got "
                          f"{tuple(gate.shape)} {gate.dtype} and {tuple(x.shape)} {x.dtype}")
@@ -1671,74 +1462,46 @@ def gated_scan_step(gate: torch.Tensor, x: torch.Tensor, state: torch.Tensor, *,
     if torch.is_grad_enabled() and (gate.requires_grad or x.requires_grad or state.requires_grad):
         raise RuntimeError("gated_scan_step is not differentiable; use gated_scan, or call it "
                            "under torch.no_grad()")
-    gate, x = _channels(gate), _channels(x)
-    h = _empty_as(x)
-    _launch("tp_gated_scan_step", dev, dtype, code, B, C, gate.data_ptr(), gate.stride(0),
-            x.data_ptr(), x.stride(0), state.data_ptr(), state.stride(0), h.data_ptr())
-    torch.autograd.graph.increment_version(state)
-    return h
+    return _lib.host().gated_scan_step(gate, x, state, code)
 
 
 # --------------------------------------------------------------------------- embedding
-def _index_bits(t: torch.Tensor, what: str) -> int:
-    if t.dtype not in (torch.int32, torch.int64):
+def _index(t: torch.Tensor, what: str) -> None:
+    if t.dtype != torch.int32 and t.dtype != torch.int64:
         raise TypeError(f"{what} must be int32 or int64, got {t.dtype}")
-    return 32 if t.dtype == torch.int32 else 64
 
 
-def _table(t: torch.Tensor, what: str) -> torch.Tensor:
-    if t.dim() != 2:
-        raise ValueError(f"{what} must be [rows, channels], got {tuple(t.shape)}")
-    return _channels(t)
+def _embedding_inputs(ids, weight, pos_weight, positions):
+    """Checks; positions as the kernel reads them (of ids' shape and type, contiguous)."""
+    _require_cuda(ids, weight, pos_weight, positions)
+    _floating(weight, "embedding tables")
+    _index(ids, "ids")
+    if weight.dim() != 2:
+        raise ValueError(f"weight must be [rows, channels], got {tuple(weight.shape)}")
+    if pos_weight is None:
+        if positions is not None:
+            raise ValueError("positions need pos_weight")
+        return None
+    if pos_weight.dim() != 2:
+        raise ValueError(f"pos_weight must be [rows, channels], got {tuple(pos_weight.shape)}")
+    if pos_weight.shape[1] != weight.shape[1] or pos_weight.dtype != weight.dtype:
+        raise ValueError("pos_weight must have weight's channels and dtype, got "
+                         f"{tuple(pos_weight.shape)} {pos_weight.dtype}")
+    if positions is None:
+        T = ids.shape[-1] if ids.dim() else 1
+        if T > pos_weight.shape[0]:
+            raise ValueError(f"{T} positions do not fit a table of {pos_weight.shape[0]}")
+        return None
+    _index(positions, "positions")
+    if positions.shape != ids.shape:
+        positions = positions.expand(ids.shape)
+    return positions.to(ids.dtype).contiguous()
 
 
 def embedding_fwd(ids, weight, scale: float = 1.0, *, pos_weight=None, positions=None):
     """Forward of :func:`embedding` without autograd."""
-    dev = _require_cuda(ids, weight, pos_weight, positions)
-    dtype, bits = _floating(weight, "embedding tables"), _index_bits(ids, "ids")
-    w = _table(weight, "weight")
-    V, D = w.shape
-    if positions is not None and pos_weight is None:
-        raise ValueError("positions need pos_weight")
-    p, T = None, ids.shape[-1] if ids.dim() else 1
-    if pos_weight is not None:
-        p = _table(pos_weight, "pos_weight")
-        if p.shape[1] != D or p.dtype != w.dtype:
-            raise ValueError("pos_weight must have weight's channels and dtype, got "
-                             f"{tuple(p.shape)} {p.dtype}")
-        if positions is None:
-            if T > p.shape[0]:
-                raise ValueError(f"{T} positions do not fit a table of {p.shape[0]}")
-        else:
-            _index_bits(positions, "positions")
-            if positions.shape != ids.shape:
-                positions = positions.expand(ids.shape)
-            positions = _contiguous(positions.to(ids.dtype))
-    flat = _contiguous(ids)
-    out = w.new_empty((*ids.shape, D))
-    _launch("tp_embedding_fwd", dev, dtype, bits, flat.numel(), T, D, flat.data_ptr(),
-            w.data_ptr(), V, w.stride(0), float(scale), _at(p), p.shape[0] if p is not None else 0,
-            p.stride(0) if p is not None else 0, _at(positions), out.data_ptr())
-    return out
-
-
-@functools.lru_cache(maxsize=1024)
-def _embedding_workspace(index: int, N: int, rows: int, D: int) -> int:
-    with _on(torch.device("cuda", index)):
-        return _lib.load().tp_embedding_bwd_workspace_bytes(N, rows, D)
-
-
-def _embedding_back(dev, dtype, bits, ids, dout, rows, D, scale, padding_idx):
-    N = ids.numel()
-    dw = dout.new_empty((rows, D))
-    need = _embedding_workspace(dev.index, N, rows, D)
-    if need < 0:
-        raise ValueError(f"embedding_bwd takes fewer than 2^31 tokens and rows, got {N} and {rows}")
-    ws = torch.empty(need or 16, device=dev, dtype=torch.uint8)
-    _launch("tp_embedding_bwd", dev, dtype, bits, N, D, ids.data_ptr(), dout.data_ptr(), rows,
-            scale, -1 if padding_idx is None else padding_idx, dw.data_ptr(), ws.data_ptr(),
-            need or 16)
-    return dw
+    positions = _embedding_inputs(ids, weight, pos_weight, positions)
+    return _lib.host().embedding_fwd(ids, weight, pos_weight, positions, scale)
 
 
 def embedding_bwd(ids, dout, rows: int, scale: float = 1.0, *,
@@ -1746,57 +1509,21 @@ def embedding_bwd(ids, dout, rows: int, scale: float = 1.0, *,
     """Gradient [rows, D] of an embedding table from ``dout`` [*ids.shape, D]: row v is
     ``scale`` times the float32 sum of the rows of dout whose id is v, in the order of the tokens
     (the same bits on every call); absent rows and ``padding_idx`` are zero."""
-    dev = _require_cuda(ids, dout)
-    dtype, bits = _floating(dout, "dout"), _index_bits(ids, "ids")
+    _require_cuda(ids, dout)
+    _floating(dout, "dout")
+    _index(ids, "ids")
     if dout.shape[:-1] != ids.shape:
         raise ValueError(f"dout must be [*ids.shape, D], got {tuple(dout.shape)} for ids "
                          f"{tuple(ids.shape)}")
-    return _embedding_back(dev, dtype, bits, _contiguous(ids), _contiguous(dout), rows,
-                           dout.shape[-1], float(scale), padding_idx)
+    return _lib.host().embedding_bwd(ids, dout, rows, scale,
+                                     -1 if padding_idx is None else padding_idx)
 
 
 def embedding_pos_bwd(dout: torch.Tensor, rows: int) -> torch.Tensor:
     """Gradient [rows, D] of a position table whose row t was added to ``dout[..., t, :]``."""
-    dev = _require_cuda(dout)
-    dtype = _floating(dout, "dout")
-    D = dout.shape[-1]
-    T = dout.shape[-2] if dout.dim() > 1 else 1
-    dout = _contiguous(dout)
-    dp = dout.new_empty((rows, D))
-    N = dout.numel() // D if D else 0
-    _launch("tp_embedding_pos_bwd", dev, dtype, N, T, D, dout.data_ptr(), rows, dp.data_ptr())
-    return dp
-
-
-class EmbeddingFunction(torch.autograd.Function):
-    """:func:`embedding`; the gradients of the tables are dense."""
-
-    @staticmethod
-    def forward(ctx, ids, weight, pos_weight, positions, scale: float, padding_idx):
-        ctx.save_for_backward(ids, positions)
-        ctx.rows = (weight.shape[0], pos_weight.shape[0] if pos_weight is not None else 0)
-        ctx.scale, ctx.padding_idx = scale, padding_idx
-        return embedding_fwd(ids, weight, scale, pos_weight=pos_weight, positions=positions)
-
-    @staticmethod
-    @_once
-    def backward(ctx, dout):
-        ids, positions = ctx.saved_tensors
-        dw = dp = None
-        dout = _contiguous(dout)
-        dev, D = dout.device, dout.shape[-1]
-        dtype = _floating(dout, "dout")
-        if ctx.needs_input_grad[1]:
-            dw = _embedding_back(dev, dtype, _index_bits(ids, "ids"), _contiguous(ids), dout,
-                                 ctx.rows[0], D, ctx.scale, ctx.padding_idx)
-        if ctx.needs_input_grad[2]:
-            if positions is None:
-                dp = embedding_pos_bwd(dout, ctx.rows[1])
-            else:
-                at = _contiguous(positions.expand(ids.shape))
-                dp = _embedding_back(dev, dtype, _index_bits(at, "positions"), at, dout,
-                                     ctx.rows[1], D, 1.0, None)
-        return None, dw, dp, None, None, None
+    _require_cuda(dout)
+    _floating(dout, "dout")
+    return _lib.host().embedding_pos_bwd(dout, rows)
 
 
 def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, *,
@@ -1819,11 +1546,9 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, *,
         if not -V <= padding_idx < V:
             raise ValueError(f"padding_idx {padding_idx} is outside a table of {V} rows")
         padding_idx %= V
-    if torch.is_grad_enabled() and (weight.requires_grad or (
-            pos_weight is not None and pos_weight.requires_grad)):
-        return EmbeddingFunction.apply(ids, weight, pos_weight, positions, float(scale),
-                                       padding_idx)
-    return embedding_fwd(ids, weight, scale, pos_weight=pos_weight, positions=positions)
+    positions = _embedding_inputs(ids, weight, pos_weight, positions)
+    return _lib.host().embedding(ids, weight, pos_weight, positions, scale,
+                                 -1 if padding_idx is None else padding_idx)
 
 
 def tsrn_attention_host(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor,
