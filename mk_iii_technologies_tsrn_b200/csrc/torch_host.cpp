@@ -18,6 +18,8 @@
 #include <torch/extension.h>
 
 #include <optional>
+#include <stdexcept>
+#include <string>
 #include <tuple>
 
 #include "tropical_b200.h"
@@ -38,9 +40,16 @@ float* floats(const Tensor& t) { return static_cast<float*>(at_(t)); }
 void* stream_of(const Tensor& t) {
   return c10::cuda::getCurrentCUDAStream(t.device().index()).stream();
 }
+// a status of the C ABI; _lib.TropicalLibraryError in Python
+struct LibraryError : std::runtime_error {
+  const char* what_failed;
+  int status;
+  LibraryError(const char* name, int st)
+      : std::runtime_error(std::string(name) + " failed: " + tp_status_string(st)),
+        what_failed(name), status(st) {}
+};
 void check(int status, const char* what) {
-  TORCH_CHECK(status == TP_OK, what, " failed: ", tp_status_string(status), " (status ", status,
-              ")");
+  if (status != TP_OK) throw LibraryError(what, status);
 }
 Tensor contiguous(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
 // the last dimension contiguous, the others at any strides
@@ -437,6 +446,15 @@ Tensor embedding_fwd(Tensor ids, Tensor weight, Maybe pos_weight, Maybe position
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  py::register_exception_translator([](std::exception_ptr p) {
+    try {
+      if (p) std::rethrow_exception(p);
+    } catch (const LibraryError& e) {
+      const py::object cls = py::module_::import("mk_iii_technologies_tsrn_b200._lib")
+                                 .attr("TropicalLibraryError");
+      PyErr_SetObject(cls.ptr(), cls(e.what_failed, e.status, tp_status_string(e.status)).ptr());
+    }
+  });
   m.def("residual_norm", &residual_norm);
   m.def("residual_norm_fwd", &residual_norm_fwd);
   m.def("residual_norm_bwd", &residual_norm_bwd);

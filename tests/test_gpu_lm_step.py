@@ -166,3 +166,75 @@ def test_second_derivatives_are_refused(cuda):
             once.sum().backward()
         (free,) = torch.autograd.grad(out, leaf, d.detach(), create_graph=True)
         assert torch.equal(free, plain) and not free.requires_grad
+
+
+def test_a_refusal_of_the_library_is_its_error(cuda):
+    from mk_iii_technologies_tsrn_b200 import _lib, ops
+    x = torch.randn(4, 8, device=cuda)
+    for t in (x, x.clone().requires_grad_()):
+        with pytest.raises(_lib.TropicalLibraryError) as e:
+            ops.residual_norm(t, t, eps=-1.0)
+        assert e.value.status == -1
+
+
+def test_captured_forward_and_backward(cuda):
+    # whole calls with their autograd nodes in one graph, replayed on new values; an eager call of
+    # the same tensors in between leaves the graph's results alone
+    from mk_iii_technologies_tsrn_b200 import ops
+    g = torch.Generator(device=cuda).manual_seed(11)
+    B, T, V, D = 3, 70, 40, 33
+    ids = torch.randint(0, V, (B, T), device=cuda, generator=g)
+    w, z, s, p = (torch.randn(n, device=cuda, generator=g).requires_grad_()
+                  for n in ((V, D), (B, T, D), (D,), (T, D)))
+    d = torch.randn(B, T, D, device=cuda, generator=g)
+
+    def step():
+        e = ops.embedding(ids, w, 1.5, pos_weight=p)
+        h = ops.gated_scan(z, e, form="sigmoid")
+        y, n = ops.residual_norm(e, h, gate=z, scale=s)
+        return torch.autograd.grad((y, n), (w, z, s, p), (d, d))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for seed in (1, 2):
+        with torch.no_grad():
+            for t in (w, z, s, d, p):
+                t.copy_(torch.randn(t.shape, device=cuda, generator=g))
+            ids.copy_(torch.randint(0, V, (B, T), device=cuda, generator=g))
+        eager = step()
+        graph.replay()
+        for a, b in zip(out, eager):
+            assert torch.equal(a, b)
+
+
+def test_two_streams_at_once(cuda):
+    from mk_iii_technologies_tsrn_b200 import ops
+    g = torch.Generator(device=cuda).manual_seed(12)
+    x = [torch.randn(2, 400, 96, device=cuda, generator=g).requires_grad_() for _ in range(2)]
+    ids = [torch.randint(0, 50, (3000,), device=cuda, generator=g) for _ in range(2)]
+    d = torch.randn(3000, 96, device=cuda, generator=g)
+
+    def work(i):
+        h = ops.gated_scan(x[i], x[i], form="sigmoid")
+        y, n = ops.residual_norm(x[i], h, gate=x[i])
+        return (*torch.autograd.grad((y, n), x[i], (y.detach(), n.detach())),
+                ops.embedding_bwd(ids[i], d, 50))
+
+    want = [work(0), work(1)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(work(i))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for r in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(r, want[i]))
