@@ -187,10 +187,12 @@ bool residual_norm_supported(int64_t D) { return D >= 1 && D <= 8192; }
 
 int residual_norm_bwd_blocks(int64_t rows, int64_t D) {
   // what an SM holds at once: three blocks of four rows, or rows in 512 threads of
-  // 128 registers (at most four); each block keeps a set of column sums.  Rows that
-  // may begin inside 16 bytes want a multiple of the residues.
+  // 128 registers.  Each block keeps a set of column sums, so more than four only where
+  // each then still has 16 rows.  Rows that may begin inside 16 bytes want a multiple of
+  // the residues.
   const int64_t threads = ceil_div(D, (int64_t)512) * 32;
-  const int64_t per_sm = D <= 640 ? 3 : (threads <= 128 ? 4 : (threads <= 256 ? 2 : 1));
+  int64_t per_sm = D <= 640 ? 3 : (threads <= 256 ? 512 / threads : 1);
+  if (per_sm > 4 && rows < 16 * per_sm * num_sms()) per_sm = 4;
   const int64_t r = D % RN_RESIDUES ? RN_RESIDUES : 1;
   const int64_t cap = (int64_t)num_sms() * per_sm / r * r;
   const int64_t want = ceil_div(rows > 0 ? rows : 1, r) * r;
@@ -228,10 +230,11 @@ int launch_residual_norm_bwd(const ResNormBwdArgs& args, cudaStream_t stream) {
   const size_t smem = sizeof(float) * (size_t)k * p.vec * p.nv * (p.warp ? 128 : p.group) +
                       staged_bytes(g.f, p, true);
   int st;
+  // one wave, where rows take more threads than that count supposes
+  const int r = p.shift ? RN_RESIDUES : 1;
+  const int fit = num_sms() * (p.warp ? 3 : max(512 / p.group, 1)) / r * r;
+  blocks = min(blocks, fit);
   if (p.shift) {
-    // one wave where rows take more threads than that count supposes
-    const int fit = num_sms() * (p.warp ? 4 : max(512 / p.group, 1)) / RN_RESIDUES * RN_RESIDUES;
-    blocks = min(blocks, fit);
     st = bf16 ? launch_residual_norm_bwd_shift_bf16(p.nv, g, smem, blocks, stream)
               : launch_residual_norm_bwd_shift_f32(p.nv, g, smem, blocks, stream);
   } else if (p.known) {
