@@ -419,8 +419,6 @@ __global__ void __launch_bounds__(MAXT) residual_norm_fwd_kernel(const ResNormAr
           for (int i = 0; i < P2; ++i) p[i] = tp_add2(p[i], f[i]);
         }
       }
-      // products and the residual sum are rounded one by one, as the unfused
-      // expression rounds them
       if (has_gate) {
         vg[g].get(f, g, L);
 #pragma unroll

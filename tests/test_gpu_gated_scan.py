@@ -296,3 +296,21 @@ def test_captured_and_replayed(cuda):
     graph.replay()
     for p, q in zip(out, step()):
         assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B,T,C", [(2, 300, 36), (3, 65, 2), (1, 2500, 70), (1, 2500, 68)])
+def test_rows_that_begin_on_pairs(cuda, form, dtype, B, T, C):
+    # channels of an even number that is no multiple of 16 bytes, and the same bits from buffers
+    # whose rows begin elsewhere
+    gate, x, h0, dh, dl, n = _make(cuda, B, T, C, dtype, form, 13, lengths=[T, T - 7, 1][:B])
+    got = _check(cuda, gate, x, h0, dh, dl, n, form)
+    for shift in (1, 2):
+        views = []
+        for t in (gate, x):
+            wide = torch.full((B, T, C + 5), float("nan"), device=cuda, dtype=dtype)
+            wide[..., shift:shift + C] = t
+            views.append(wide[..., shift:shift + C])
+        same = _check(cuda, *views, h0, dh, dl, n, form)
+        assert all(torch.equal(got[k], same[k]) for k in got)
