@@ -33,7 +33,7 @@
 // Measured, of the bytes each has to move at the card's copy rate: the forward of
 // 32 x 4096 tokens of 1024 bf16 channels 59 us, its gradient for 131072 rows 150 us
 // (sum 111), together 149 us of bytes; 64 x 1024 tokens of 640 fp32 channels with
-// 256 rows 32 and 74 us (sum 53), 52 us of bytes.  The sort is a chain of
+// 256 rows 32 and 67 us, 52 us of bytes.  The sort is a chain of
 // exchanges over few blocks, and the sum's rows come in the order of the ids.
 #include <initializer_list>
 
@@ -486,7 +486,10 @@ __device__ __forceinline__ int64_t tokens_before(const int2* pairs, int64_t N, i
   return lo;
 }
 
-constexpr int SUM_CHUNK = 128;
+// Rows under way to a team: SUM_STAGES batches of SUM_BATCH, a thread's 16 bytes of each
+// in shared memory of its own.
+constexpr int SUM_BATCH = 4, SUM_STAGES = 4;
+constexpr int SUM_CHUNK = 128;     // pairs at a time, of rows loaded to registers
 
 // Zeros to elements [lo, hi) of out with `lanes` threads: whole 16 bytes wherever the
 // range holds them, since rows of absent tokens lie one behind the other.
@@ -564,39 +567,91 @@ __global__ void __launch_bounds__(256) embedding_sum_kernel(const SumArgs s) {
     }
     while (v < to) end_row();
   };
-  // pairs of 128 tokens at a time in shared memory, a copy for each warp
-  __shared__ int2 s_pairs[8][SUM_CHUNK];
-  int2* const pairs = s_pairs[threadIdx.x >> 5];
   const int lane = threadIdx.x & 31;
-  for (; j < j1; j += SUM_CHUNK) {
-    const int m = (int)min((int64_t)SUM_CHUNK, j1 - j);
-    __syncwarp();
-#pragma unroll
-    for (int k = 0; k < SUM_CHUNK / 32; ++k)
-      if (k * 32 + lane < m) pairs[k * 32 + lane] = __ldg(s.pairs + j + k * 32 + lane);
-    __syncwarp();
-#pragma unroll 1
-    for (int i = 0; i < m; i += U) {
-      V row[U];
-      const int n = min(U, m - i);
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (u < n) {
-          const int2 p = pairs[i + u];
-          if (in && p.x < s.V) row[u].load_stream(dout + (int64_t)p.y * s.D);
-        }
+  if constexpr (VEC * sizeof(T) == 16) {
+    // Each thread copies its own pieces of the rows and reads only those, so that no
+    // thread waits for another; the pairs come 32 at a time, a copy for each warp.
+    extern __shared__ __align__(16) uint4 s_rows[];      // [SUM_STAGES * SUM_BATCH][blockDim.x]
+    __shared__ int2 s_ring[8][64];
+    int2* const ring = s_ring[threadIdx.x >> 5];
+    V* const rows = reinterpret_cast<V*>(s_rows) + threadIdx.x;
+    const int n = (int)(j1 - j);
+    const int2* const src = s.pairs + j;
+    int2 ahead = lane < n ? __ldg(src + lane) : make_int2(0, 0);
+    auto fetch = [&](int i0) {
+      if ((i0 & 31) == 0 && i0 < n) {
+        __syncwarp();
+        ring[(i0 & 63) + lane] = ahead;
+        __syncwarp();
+        if (i0 + 32 + lane < n) ahead = __ldg(src + i0 + 32 + lane);
       }
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (u < n) {
-          const int key = pairs[i + u].x;
-          if (key >= s.V) break;             // dropped tokens come last
-          if (v < key) end_rows(key);
-          if (in) {
-            float f[VEC];
-            row[u].get(f);
+      for (int u = 0; u < SUM_BATCH; ++u) {
+        const int i = i0 + u;
+        if (i < n) {
+          const int2 p = ring[i & 63];
+          if (in && p.x < s.V)
+            tp_cp_async16(rows + (i % (SUM_STAGES * SUM_BATCH)) * blockDim.x,
+                          dout + (int64_t)p.y * s.D, 16);
+        }
+      }
+      tp_cp_async_commit();
+    };
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) acc[k] += f[k];
+    for (int k = 0; k < SUM_STAGES - 1; ++k) fetch(k * SUM_BATCH);
+#pragma unroll 1
+    for (int i0 = 0; i0 < n; i0 += SUM_BATCH) {
+      fetch(i0 + (SUM_STAGES - 1) * SUM_BATCH);
+      tp_cp_async_wait<SUM_STAGES - 1>();
+#pragma unroll
+      for (int u = 0; u < SUM_BATCH; ++u) {
+        const int i = i0 + u;
+        const int key = i < n ? ring[i & 63].x : (int)s.V;
+        if (key >= s.V) break;               // dropped tokens come last
+        if (v < key) end_rows(key);
+        if (in) {
+          const V row = rows[(i % (SUM_STAGES * SUM_BATCH)) * blockDim.x];
+          float f[VEC];
+          row.get(f);
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) acc[k] += f[k];
+        }
+      }
+    }
+  } else {
+    // pairs of 128 tokens at a time in shared memory, a copy for each warp
+    __shared__ int2 s_pairs[8][SUM_CHUNK];
+    int2* const pairs = s_pairs[threadIdx.x >> 5];
+    for (; j < j1; j += SUM_CHUNK) {
+      const int m = (int)min((int64_t)SUM_CHUNK, j1 - j);
+      __syncwarp();
+  #pragma unroll
+      for (int k = 0; k < SUM_CHUNK / 32; ++k)
+        if (k * 32 + lane < m) pairs[k * 32 + lane] = __ldg(s.pairs + j + k * 32 + lane);
+      __syncwarp();
+  #pragma unroll 1
+      for (int i = 0; i < m; i += U) {
+        V row[U];
+        const int n = min(U, m - i);
+  #pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (u < n) {
+            const int2 p = pairs[i + u];
+            if (in && p.x < s.V) row[u].load_stream(dout + (int64_t)p.y * s.D);
+          }
+        }
+  #pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (u < n) {
+            const int key = pairs[i + u].x;
+            if (key >= s.V) break;             // dropped tokens come last
+            if (v < key) end_rows(key);
+            if (in) {
+              float f[VEC];
+              row[u].get(f);
+  #pragma unroll
+              for (int k = 0; k < VEC; ++k) acc[k] += f[k];
+            }
           }
         }
       }
@@ -761,7 +816,7 @@ struct SumPlan {
   int64_t share, shares;
 };
 
-// As many shares as teams fit at once (819 threads of 80 registers on an SM), so
+// As many shares as teams fit at once (768 threads with their 256 bytes of rows on an SM), so
 // that there is one wave of them and each searches its place once; at least 16
 // items each, so that partial sums stay few (two or four waves: the sums of 60 x 4096 tokens
 // 83, 85 and 92 us, their joins 8, 14 and 25 us).  By the sizes alone.
@@ -770,7 +825,7 @@ SumPlan sum_plan(int64_t N, int64_t V, int64_t D, int esize) {
   int64_t ranges;
   const int lanes = sum_lanes(D, 16 / esize, &ranges);
   const int per = sum_teams(lanes);
-  int64_t teams = 819 / (lanes * per) * per / ranges;
+  int64_t teams = 768 / (lanes * per) * per / ranges;
   if (teams < 1) teams = 1;
   int64_t share = ceil_div(items, num_sms() * teams);
   if (share < 16 * TOKEN_COST) share = 16 * TOKEN_COST;
@@ -837,7 +892,14 @@ int sum(SumArgs s, cudaStream_t stream) {
   const int per = sum_teams(s.lanes);
   const int threads = s.lanes * per;
   const dim3 grid((unsigned)ceil_div(s.shares, (int64_t)per), (unsigned)ranges);
-  embedding_sum_kernel<T, VEC><<<grid, threads, 0, stream>>>(s);
+  const size_t smem = VEC * sizeof(T) == 16 ? (size_t)SUM_STAGES * SUM_BATCH * 16 * threads : 0;
+  if (smem > 40 * 1024) {
+    const cudaError_t e =
+        cudaFuncSetAttribute((const void*)embedding_sum_kernel<T, VEC>,
+                             cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return cuda_status(e);
+  }
+  embedding_sum_kernel<T, VEC><<<grid, threads, smem, stream>>>(s);
   const dim3 join((unsigned)s.shares, (unsigned)ceil_div(s.D, (int64_t)256));
   embedding_join_kernel<T><<<join, 256, 0, stream>>>(s);
   return launch_status();
