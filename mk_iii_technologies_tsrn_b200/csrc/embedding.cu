@@ -486,9 +486,15 @@ __device__ __forceinline__ int64_t tokens_before(const int2* pairs, int64_t N, i
   return lo;
 }
 
-// Rows under way to a team: SUM_STAGES batches of SUM_BATCH, a thread's 16 bytes of each
-// in shared memory of its own.
+// fp32 rows come through shared memory: SUM_STAGES batches of SUM_BATCH under way, a
+// thread's 16 bytes of each in a place of its own (64 x 1024 tokens of 256 rows of 640
+// channels, the gradient with its sort: 67 us, against 82 us with eight rows at a time
+// in registers, 70 with three batches and more threads, 73 with six and fewer).  bf16
+// rows have half the bytes for the same steps and take eight at a time in registers
+// (the same tokens: 56 us against 71; 60 x 4096 of 32000 rows of 768: 149 against 195).
 constexpr int SUM_BATCH = 4, SUM_STAGES = 4;
+template <typename T, int VEC>
+constexpr bool SUM_ASYNC = VEC * sizeof(T) == 16 && sizeof(T) == 4;
 constexpr int SUM_CHUNK = 128;     // pairs at a time, of rows loaded to registers
 
 // Zeros to elements [lo, hi) of out with `lanes` threads: whole 16 bytes wherever the
@@ -568,7 +574,7 @@ __global__ void __launch_bounds__(256) embedding_sum_kernel(const SumArgs s) {
     while (v < to) end_row();
   };
   const int lane = threadIdx.x & 31;
-  if constexpr (VEC * sizeof(T) == 16) {
+  if constexpr (SUM_ASYNC<T, VEC>) {
     // Each thread copies its own pieces of the rows and reads only those, so that no
     // thread waits for another; the pairs come 32 at a time, a copy for each warp.
     extern __shared__ __align__(16) uint4 s_rows[];      // [SUM_STAGES * SUM_BATCH][blockDim.x]
@@ -816,7 +822,8 @@ struct SumPlan {
   int64_t share, shares;
 };
 
-// As many shares as teams fit at once (768 threads with their 256 bytes of rows on an SM), so
+// As many shares as teams fit at once (768 threads with their 256 bytes of rows on an SM,
+// 819 of 80 registers where rows stay in those), so
 // that there is one wave of them and each searches its place once; at least 16
 // items each, so that partial sums stay few (two or four waves: the sums of 60 x 4096 tokens
 // 83, 85 and 92 us, their joins 8, 14 and 25 us).  By the sizes alone.
@@ -825,7 +832,7 @@ SumPlan sum_plan(int64_t N, int64_t V, int64_t D, int esize) {
   int64_t ranges;
   const int lanes = sum_lanes(D, 16 / esize, &ranges);
   const int per = sum_teams(lanes);
-  int64_t teams = 768 / (lanes * per) * per / ranges;
+  int64_t teams = (esize == 4 ? 768 : 819) / (lanes * per) * per / ranges;
   if (teams < 1) teams = 1;
   int64_t share = ceil_div(items, num_sms() * teams);
   if (share < 16 * TOKEN_COST) share = 16 * TOKEN_COST;
@@ -892,7 +899,7 @@ int sum(SumArgs s, cudaStream_t stream) {
   const int per = sum_teams(s.lanes);
   const int threads = s.lanes * per;
   const dim3 grid((unsigned)ceil_div(s.shares, (int64_t)per), (unsigned)ranges);
-  const size_t smem = VEC * sizeof(T) == 16 ? (size_t)SUM_STAGES * SUM_BATCH * 16 * threads : 0;
+  const size_t smem = SUM_ASYNC<T, VEC> ? (size_t)SUM_STAGES * SUM_BATCH * 16 * threads : 0;
   if (smem > 40 * 1024) {
     const cudaError_t e =
         cudaFuncSetAttribute((const void*)embedding_sum_kernel<T, VEC>,
