@@ -84,6 +84,10 @@ TP_API int tp_abi_version(void);
  * is device memory of the current device (cudaPointerGetAttributes).  Enabled
  * by default.  Returns the previous setting. */
 TP_API int tp_set_pointer_checks(int enable);
+/* The same for the calling thread's calls alone (they are checked where both are
+ * on): for callers that know what their pointers are, as a check is about a
+ * microsecond each.  Returns the thread's previous setting. */
+TP_API int tp_set_thread_pointer_checks(int enable);
 
 /* ======================================================================== *
  *  Max-plus GEMM forward

@@ -25,6 +25,7 @@ SIGNATURES: dict[str, tuple] = {
     "tp_status_string": (ctypes.c_char_p, [_c_int]),
     "tp_abi_version": (_c_int, []),
     "tp_set_pointer_checks": (_c_int, [_c_int]),
+    "tp_set_thread_pointer_checks": (_c_int, [_c_int]),
     "tp_maxplus_fwd": (
         _c_int,
         [_c_int, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_p, _c_i64, _c_p, _c_p, _c_i64, _c_p,

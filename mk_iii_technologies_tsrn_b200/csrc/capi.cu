@@ -21,9 +21,12 @@ namespace {
 std::atomic<int> g_pointer_checks{1};
 std::atomic<int> g_smooth_fused{1};
 thread_local int g_last_error = TP_OK;
+thread_local int g_thread_pointer_checks = 1;
 }  // namespace
 
-bool pointer_checks_enabled() { return g_pointer_checks.load(std::memory_order_relaxed) != 0; }
+bool pointer_checks_enabled() {
+  return g_thread_pointer_checks != 0 && g_pointer_checks.load(std::memory_order_relaxed) != 0;
+}
 
 int check_device_pointer(const void* p) {
   cudaPointerAttributes attr;
@@ -258,6 +261,12 @@ const char* tp_status_string(int status) {
 }
 
 int tp_abi_version(void) { return 1; }
+
+int tp_set_thread_pointer_checks(int enable) {
+  const int old = tp::g_thread_pointer_checks;
+  tp::g_thread_pointer_checks = enable ? 1 : 0;
+  return old;
+}
 
 int tp_set_pointer_checks(int enable) {
   return g_pointer_checks.exchange(enable ? 1 : 0);

@@ -5,11 +5,13 @@
 // These operators are also called on single tokens and small batches, where the
 // host's time is the call's.  A node written in Python takes the interpreter lock
 // in the autograd engine's thread and builds its objects there: forward and
-// backward of a 64 x 640 residual step 163 us so and 107 us here, of 32 tokens'
-// embedding 96 and 64 us (a node that does nothing: 41 us); a decoding step of the
-// embedding 15 and 10 us.
+// backward of a 64 x 640 residual step 163 us so and 96 us here, of 32 tokens'
+// embedding 96 and 60 us (a node that does nothing: 41 us); a decoding step of the
+// embedding 15 and 6 us.
 //
-// Arguments are checked by the callers in ops.py.
+// The calls below return None for arguments that are not as the kernels take them;
+// ops.py then converts them or raises what is wrong with them.  The other entries
+// are called with checked arguments.
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -51,6 +53,13 @@ struct LibraryError : std::runtime_error {
 void check(int status, const char* what) {
   if (status != TP_OK) throw LibraryError(what, status);
 }
+// The device as the current one, and pointers taken for what they are: torch's.
+struct On {
+  c10::cuda::CUDAGuard guard;
+  const int checks = tp_set_thread_pointer_checks(0);
+  explicit On(const Tensor& t) : guard(t.device()) {}
+  ~On() { tp_set_thread_pointer_checks(checks); }
+};
 Tensor contiguous(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
 // the last dimension contiguous, the others at any strides
 Tensor channels(const Tensor& t) {
@@ -65,6 +74,18 @@ bool any_needs_grad(std::initializer_list<const Tensor*> ts) {
   for (const Tensor* t : ts)
     if (t->defined() && t->requires_grad()) return true;
   return false;
+}
+
+bool is_float(const Tensor& t) {
+  return t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16;
+}
+bool is_index(const Tensor& t) {
+  return t.scalar_type() == at::kInt || t.scalar_type() == at::kLong;
+}
+// t, where there is one: on `like`'s device, of its shape and type
+bool alike(const Tensor& t, const Tensor& like) {
+  return !t.defined() || (t.device() == like.device() &&
+                          t.scalar_type() == like.scalar_type() && t.sizes() == like.sizes());
 }
 
 // The gradients that `make` returns, which cannot be differentiated again.
@@ -114,7 +135,7 @@ int params_code(const ResidualIn& a) {
 
 std::tuple<Tensor, Tensor, Tensor> residual_run(const ResidualIn& a, bool normalize,
                                                 bool need_stats) {
-  c10::cuda::CUDAGuard guard(a.x.device());
+  const On device(a.x);
   const int64_t D = a.x.size(-1), rows = a.x.numel() / D;
   const Rows x = rows_of(a.x, D), b = rows_of(a.branch, D), g = rows_of(a.gate, D);
   const Tensor w = contiguous(a.weight), bias = contiguous(a.bias), bw = contiguous(a.bw),
@@ -135,7 +156,7 @@ std::tuple<Tensor, Tensor, Tensor> residual_run(const ResidualIn& a, bool normal
 // branch weight and branch bias (views of one buffer)
 variable_list residual_back(const ResidualIn& a, const Tensor& stats, const Tensor& dy_,
                             const Tensor& dn_, const std::array<bool, 5>& wanted) {
-  c10::cuda::CUDAGuard guard(a.x.device());
+  const On device(a.x);
   const int64_t D = a.x.size(-1), rows = a.x.numel() / D;
   const Rows x = rows_of(a.x, D), b = rows_of(a.branch, D), g = rows_of(a.gate, D);
   const Tensor w = contiguous(a.weight), bias = contiguous(a.bias), bw = contiguous(a.bw),
@@ -213,18 +234,37 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
   }
 };
 
-std::tuple<Tensor, Tensor> residual_norm(Tensor x, Tensor branch, Maybe gate, Maybe scale,
+bool residual_ok(const ResidualIn& a, bool normalize) {
+  if (!a.x.is_cuda() || !is_float(a.x) || a.x.dim() == 0) return false;
+  const int64_t D = a.x.size(-1);
+  if (D < 1 || D > 8192 || !alike(a.branch, a.x) || !alike(a.gate, a.x)) return false;
+  if (!a.branch_norm && (a.bw.defined() || a.bb.defined())) return false;
+  if (!normalize && (a.weight.defined() || a.bias.defined())) return false;
+  const Tensor* one = nullptr;      // the parameters' type
+  for (const Tensor* t : {&a.scale, &a.weight, &a.bias, &a.bw, &a.bb}) {
+    if (!t->defined()) continue;
+    if (!(t->dim() == 1 && t->size(0) == D) && !(t == &a.scale && t->numel() == 1)) return false;
+    if (t->device() != a.x.device()) return false;
+    if (t->scalar_type() != at::kFloat && t->scalar_type() != a.x.scalar_type()) return false;
+    if (one != nullptr && one->scalar_type() != t->scalar_type()) return false;
+    one = t;
+  }
+  return true;
+}
+
+std::optional<std::tuple<Tensor, Tensor>> residual_norm(Tensor x, Tensor branch, Maybe gate, Maybe scale,
                                          Maybe weight, Maybe bias, Maybe bw, Maybe bb, double eps,
                                          int64_t norm, bool branch_norm, bool normalize) {
   const ResidualIn a{x, branch, or_none(gate), or_none(scale), or_none(weight), or_none(bias),
                      or_none(bw), or_none(bb), eps, norm, branch_norm};
+  if (!residual_ok(a, normalize)) return std::nullopt;
   if (any_needs_grad({&a.x, &a.branch, &a.gate, &a.scale, &a.weight, &a.bias, &a.bw, &a.bb})) {
     variable_list out = ResidualNorm::apply(x, branch, gate, scale, weight, bias, bw, bb, eps,
                                             norm, branch_norm, normalize);
-    return {out[0], normalize ? out[1] : Tensor()};
+    return std::make_tuple(out[0], normalize ? out[1] : Tensor());
   }
   auto [y, n, stats] = residual_run(a, normalize, false);
-  return {y, n};
+  return std::make_tuple(y, n);
 }
 
 std::tuple<Tensor, Tensor, Tensor> residual_norm_fwd(
@@ -255,7 +295,7 @@ Tensor scan_workspace(const Tensor& x, int64_t& need) {
 std::tuple<Tensor, Tensor, Tensor> scan_run(const Tensor& gate_, const Tensor& x_,
                                             const Tensor& h0_, const Tensor& lengths, int64_t form,
                                             bool need_states, bool need_last) {
-  c10::cuda::CUDAGuard guard(x_.device());
+  const On device(x_);
   const int64_t B = x_.size(0), T = x_.size(1), C = x_.size(2);
   const Tensor gate = channels(gate_), x = channels(x_), h0 = contiguous(h0_);
   const auto f32 = x_.options().dtype(at::kFloat);
@@ -276,7 +316,7 @@ std::tuple<Tensor, Tensor, Tensor> scan_back(const Tensor& states, const Tensor&
                                              const Tensor& dlast_, const Tensor& gate_,
                                              const Tensor& x_, const Tensor& lengths, int64_t form,
                                              bool need_dh0) {
-  c10::cuda::CUDAGuard guard(x_.device());
+  const On device(x_);
   const int64_t B = x_.size(0), T = x_.size(1), C = x_.size(2);
   const Tensor gate = channels(gate_), x = channels(x_), dh = contiguous(dh_),
                dlast = contiguous(dlast_);
@@ -317,15 +357,25 @@ struct GatedScan : torch::autograd::Function<GatedScan> {
   }
 };
 
-std::tuple<Tensor, Tensor> gated_scan(Tensor gate, Tensor x, Maybe h0, Maybe lengths, int64_t form,
-                                      bool need_last) {
+std::optional<std::tuple<Tensor, Tensor>> gated_scan(Tensor gate, Tensor x, Maybe h0,
+                                                     Maybe lengths, int64_t form,
+                                                     bool need_last) {
   const Tensor first = or_none(h0), ends = or_none(lengths);
+  if (!x.is_cuda() || !is_float(x) || x.dim() != 3 || !alike(gate, x)) return std::nullopt;
+  if (first.defined() &&
+      (first.device() != x.device() || first.scalar_type() != at::kFloat || first.dim() != 2 ||
+       first.size(0) != x.size(0) || first.size(1) != x.size(2)))
+    return std::nullopt;
+  if (ends.defined() &&
+      (ends.device() != x.device() || ends.scalar_type() != at::kInt || ends.dim() != 1 ||
+       ends.size(0) != x.size(0) || !ends.is_contiguous()))
+    return std::nullopt;
   if (any_needs_grad({&gate, &x, &first})) {
     variable_list out = GatedScan::apply(gate, x, h0, lengths, form);
-    return {out[0], out[1]};
+    return std::make_tuple(out[0], out[1]);
   }
   auto [h, last, states] = scan_run(gate, x, first, ends, form, false, need_last);
-  return {h, last};
+  return std::make_tuple(h, last);
 }
 
 std::tuple<Tensor, Tensor, Tensor> gated_scan_fwd(Tensor gate, Tensor x, Maybe h0, Maybe lengths,
@@ -341,9 +391,15 @@ std::tuple<Tensor, Tensor, Tensor> gated_scan_bwd(Tensor states, Maybe dh, Maybe
   return scan_back(states, or_none(dh), or_none(dlast), gate, x, or_none(lengths), form, need_dh0);
 }
 
-Tensor gated_scan_step(Tensor gate_, Tensor x_, Tensor state, int64_t form) {
+Maybe gated_scan_step(Tensor gate_, Tensor x_, Tensor state, int64_t form) {
+  if (!x_.is_cuda() || !is_float(x_) || x_.dim() != 2 || !alike(gate_, x_)) return std::nullopt;
+  if (state.device() != x_.device() || state.scalar_type() != at::kFloat ||
+      state.sizes() != x_.sizes() || (x_.size(1) > 1 && state.stride(1) != 1) ||
+      (x_.size(0) > 1 && state.stride(0) < x_.size(1)))
+    return std::nullopt;
+  if (any_needs_grad({&gate_, &x_, &state})) return std::nullopt;
   at::NoGradGuard off;
-  c10::cuda::CUDAGuard guard(x_.device());
+  const On device(x_);
   const Tensor gate = channels(gate_), x = channels(x_);
   Tensor h = empty_as(x_);
   check(tp_gated_scan_step(code_of(x), (int)form, x.size(0), x.size(1), at_(gate), gate.stride(0),
@@ -359,7 +415,7 @@ int bits_of(const Tensor& t) { return t.scalar_type() == at::kInt ? 32 : 64; }
 
 Tensor embed_run(const Tensor& ids_, const Tensor& weight, const Tensor& pos, const Tensor& at,
                  double scale) {
-  c10::cuda::CUDAGuard guard(weight.device());
+  const On device(weight);
   const Tensor ids = ids_.contiguous(), w = channels(weight),
                p = pos.defined() ? channels(pos) : pos;
   const int64_t D = w.size(1), T = ids.dim() ? ids.size(-1) : 1;
@@ -375,7 +431,7 @@ Tensor embed_run(const Tensor& ids_, const Tensor& weight, const Tensor& pos, co
 
 Tensor embed_back(const Tensor& ids_, const Tensor& dout_, int64_t rows, double scale,
                   int64_t padding) {
-  c10::cuda::CUDAGuard guard(dout_.device());
+  const On device(dout_);
   const Tensor ids = ids_.contiguous(), dout = dout_.contiguous();
   const int64_t N = ids.numel(), D = dout.size(-1);
   const int64_t need = tp_embedding_bwd_workspace_bytes(N, rows, D);
@@ -390,7 +446,7 @@ Tensor embed_back(const Tensor& ids_, const Tensor& dout_, int64_t rows, double 
 }
 
 Tensor embed_pos_back(const Tensor& dout_, int64_t rows) {
-  c10::cuda::CUDAGuard guard(dout_.device());
+  const On device(dout_);
   const Tensor dout = dout_.contiguous();
   const int64_t D = dout.size(-1), T = dout.dim() > 1 ? dout.size(-2) : 1;
   Tensor dp = at::empty({rows, D}, dout.options());
@@ -430,9 +486,20 @@ struct Embedding : torch::autograd::Function<Embedding> {
   }
 };
 
-Tensor embedding(Tensor ids, Tensor weight, Maybe pos_weight, Maybe positions, double scale,
-                 int64_t padding) {
+Maybe embedding(Tensor ids, Tensor weight, Maybe pos_weight, Maybe positions, double scale,
+                int64_t padding) {
   const Tensor pos = or_none(pos_weight), at = or_none(positions);
+  if (!weight.is_cuda() || !is_float(weight) || weight.dim() != 2 || !is_index(ids) ||
+      ids.device() != weight.device())
+    return std::nullopt;
+  if (pos.defined() &&
+      (pos.device() != weight.device() || pos.scalar_type() != weight.scalar_type() ||
+       pos.dim() != 2 || pos.size(1) != weight.size(1)))
+    return std::nullopt;
+  if (at.defined() && (!pos.defined() || !alike(at, ids) || !at.is_contiguous()))
+    return std::nullopt;
+  if (pos.defined() && !at.defined() && (ids.dim() ? ids.size(-1) : 1) > pos.size(0))
+    return std::nullopt;
   if (any_needs_grad({&weight, &pos}))
     return Embedding::apply(weight, pos_weight, ids, positions, scale, padding);
   return embed_run(ids, weight, pos, at, scale);

@@ -1270,6 +1270,11 @@ NORMS = {"layer": _lib.TP_NORM_LAYER, "rms": _lib.TP_NORM_RMS}
 RESIDUAL_NORM_MAX_CHANNELS = 8192
 
 
+def _refused():
+    # the host module's checks found something that those of this file let through
+    raise RuntimeError("these arguments are not as the kernel takes them")
+
+
 def _floating(t: torch.Tensor, what: str) -> None:
     if t.dtype != torch.float32 and t.dtype != torch.bfloat16:
         raise TypeError(f"{what} must be float32 or bfloat16, got {t.dtype}")
@@ -1360,10 +1365,14 @@ def residual_norm(x: torch.Tensor, branch: torch.Tensor, weight: Optional[torch.
     biases are float32 or of x's dtype.  Differentiable in all tensors.  It is the TSRN block's
     ``x + branch(ln(x))`` (research/tsrn_dml.py:1096-1106) with TropicalSSM's gate and mix
     (:975-980) and the next LayerNorm."""
+    if norm in NORMS:
+        out = _lib.host().residual_norm(x, branch, gate, scale, weight, bias, branch_weight,
+                                        branch_bias, eps, NORMS[norm], branch_norm, normalize)
+        if out is not None:
+            return out
     _residual_norm_args(x, branch, weight, bias, norm, gate, scale, branch_norm, branch_weight,
                         branch_bias, normalize)
-    return _lib.host().residual_norm(x, branch, gate, scale, weight, bias, branch_weight,
-                                     branch_bias, eps, NORMS[norm], branch_norm, normalize)
+    _refused()
 
 
 # --------------------------------------------------------------------------- gated scan
@@ -1437,10 +1446,12 @@ def gated_scan(gate: torch.Tensor, x: torch.Tensor, h0: Optional[torch.Tensor] =
     there is read.  Returns h [B, T, C] in x's dtype, with ``return_state`` also the float32
     state [B, C] at each row's end (for :func:`gated_scan_step`, or to go on with the next
     segment).  States are float32 throughout.  Meant for gates of magnitude at most 1."""
-    code = _gate_form(form)
-    _, lengths = _gated_scan_inputs(gate, x, h0, lengths)
-    h, last = _lib.host().gated_scan(gate, x, h0, lengths, code, return_state)
-    return (h, last) if return_state else h
+    code, call = _gate_form(form), _lib.host().gated_scan
+    out = call(gate, x, h0, lengths, code, return_state)
+    if out is None:      # 64-bit lengths, or something wrong
+        _, lengths = _gated_scan_inputs(gate, x, h0, lengths)
+        out = call(gate, x, h0, lengths, code, return_state) or _refused()
+    return out if return_state else out[0]
 
 
 def gated_scan_step(gate: torch.Tensor, x: torch.Tensor, state: torch.Tensor, *,
@@ -1448,7 +1459,9 @@ def gated_scan_step(gate: torch.Tensor, x: torch.Tensor, state: torch.Tensor, *,
     """One step of :func:`gated_scan` for serving: ``state`` [B, C] float32 (rows at any stride
     of at least C) is updated in place and the new h [B, C] returned in x's dtype.  ``gate``,
     ``x``: [B, C].  Not differentiable."""
-    code = _gate_form(form)
+    h = _lib.host().gated_scan_step(gate, x, state, _gate_form(form))
+    if h is not None:
+        return h
     _require_cuda(gate, x, state)
     _floating(x, "gated_scan_step inputs")
     if x.dim() != 2 or gate.shape != x.shape or gate.dtype != x.dtype:
@@ -1462,7 +1475,7 @@ def gated_scan_step(gate: torch.Tensor, x: torch.Tensor, state: torch.Tensor, *,
     if torch.is_grad_enabled() and (gate.requires_grad or x.requires_grad or state.requires_grad):
         raise RuntimeError("gated_scan_step is not differentiable; use gated_scan, or call it "
                            "under torch.no_grad()")
-    return _lib.host().gated_scan_step(gate, x, state, code)
+    _refused()
 
 
 # --------------------------------------------------------------------------- embedding
@@ -1546,9 +1559,12 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, *,
         if not -V <= padding_idx < V:
             raise ValueError(f"padding_idx {padding_idx} is outside a table of {V} rows")
         padding_idx %= V
-    positions = _embedding_inputs(ids, weight, pos_weight, positions)
-    return _lib.host().embedding(ids, weight, pos_weight, positions, scale,
-                                 -1 if padding_idx is None else padding_idx)
+    padding, call = -1 if padding_idx is None else padding_idx, _lib.host().embedding
+    out = call(ids, weight, pos_weight, positions, scale, padding)
+    if out is None:      # positions to be expanded or converted, or something wrong
+        positions = _embedding_inputs(ids, weight, pos_weight, positions)
+        out = call(ids, weight, pos_weight, positions, scale, padding)
+    return out if out is not None else _refused()
 
 
 def tsrn_attention_host(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor,

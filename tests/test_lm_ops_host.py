@@ -153,3 +153,15 @@ def test_sorted_order_of_the_item_list():
         at = [k + i for i, k in enumerate(keys)]
         for d in range(n + V + 1):
             assert bisect.bisect_left(at, d) == items[:d].count("token")
+
+
+def test_pointer_checks_of_one_thread():
+    import threading
+    lib = _lib.load()
+    assert lib.tp_set_thread_pointer_checks(0) == 1
+    other = []
+    t = threading.Thread(target=lambda: other.append(lib.tp_set_thread_pointer_checks(1)))
+    t.start()
+    t.join()
+    assert other == [1]                                   # another thread's are on
+    assert lib.tp_set_thread_pointer_checks(1) == 0
