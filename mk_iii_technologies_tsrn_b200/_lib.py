@@ -308,6 +308,8 @@ def host():
     if _host is None:
         load()
         with _lock:
+            import torch  # noqa: F401  (the module links to torch's libraries: loaded first)
+
             try:
                 from . import _tropical_b200_torch as module
             except ImportError as e:
