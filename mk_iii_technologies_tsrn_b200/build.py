@@ -6,8 +6,8 @@ declared in ``include/tropical_b200.h``; Python reaches it through ctypes
 (``_lib.py``).  ``csrc/torch_host.cpp``, the host side of the language-model
 operators over that ABI (outputs, workspaces, autograd nodes), becomes the Python
 module ``_tropical_b200_torch.so`` beside it.  Rebuilds only what is older than
-its sources and headers.  Run ``python -m mk_iii_technologies_tsrn_b200.build`` or call
-:func:`build`.
+its sources and headers, and the host module for another torch or Python.  Run
+``python -m mk_iii_technologies_tsrn_b200.build`` or call :func:`build`.
 """
 from __future__ import annotations
 
@@ -27,6 +27,7 @@ BUILD_DIR = os.path.join(PKG_DIR, "_build")
 HOST_SOURCE = os.path.join(CSRC, "torch_host.cpp")
 HOST_MODULE = "_tropical_b200_torch"
 HOST_PATH = os.path.join(PKG_DIR, HOST_MODULE + ".so")
+HOST_STAMP = os.path.join(BUILD_DIR, HOST_MODULE + ".for")   # what the module was compiled against
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = [
@@ -68,9 +69,19 @@ def needs_build() -> bool:
     return any(os.path.getmtime(p) > lib_mtime for p in _deps())
 
 
+def _host_target() -> str:
+    """The torch and Python whose headers and ABI the host module is compiled against."""
+    from importlib import metadata
+
+    return f"torch {metadata.version('torch')} {sys.implementation.cache_tag}\n"
+
+
 def needs_host_build() -> bool:
-    if not os.path.exists(HOST_PATH):
+    if not os.path.exists(HOST_PATH) or not os.path.exists(HOST_STAMP):
         return True
+    with open(HOST_STAMP) as f:
+        if f.read() != _host_target():
+            return True
     built = os.path.getmtime(HOST_PATH)
     return any(os.path.getmtime(p) > built for p in
                [HOST_SOURCE, os.path.abspath(__file__), *glob.glob(os.path.join(INCLUDE, "*.h"))])
@@ -100,6 +111,9 @@ def build_host(verbose: bool = False) -> str:
     if res.returncode != 0:
         raise RuntimeError(f"the host module failed to build:\n{res.stdout}\n{res.stderr}")
     os.replace(tmp, HOST_PATH)
+    os.makedirs(BUILD_DIR, exist_ok=True)
+    with open(HOST_STAMP, "w") as f:
+        f.write(_host_target())
     return HOST_PATH
 
 
