@@ -7,7 +7,9 @@
 // (the ctypes calls that fed them).
 #include <atomic>
 #include <initializer_list>
+#include <map>
 #include <mutex>
+#include <utility>
 
 #include "maxplus_internal.cuh"
 
@@ -85,6 +87,20 @@ int num_sms() {
       n > 0 && dev < 64)
     known[dev].store(n, std::memory_order_relaxed);
   return n > 0 ? n : 148;
+}
+
+int allow_smem(const void* kernel, size_t bytes) {
+  static std::mutex mu;
+  static std::map<std::pair<const void*, int>, size_t> most;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_status(e);
+  std::lock_guard<std::mutex> lock(mu);
+  size_t& known = most[{kernel, dev}];
+  const size_t want = bytes > known ? bytes : known;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)want);
+  if (e == cudaSuccess) known = want;
+  return cuda_status(e);
 }
 
 int check_scan_bwd_pointers(int64_t T, const float* gh, const float* bb, const float* xx,

@@ -268,6 +268,12 @@ __host__ __device__ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + 
 
 int num_sms();
 
+// Lets `kernel` be launched on the current device with `bytes` of dynamic shared memory:
+// TP_OK or a cudaError_t.  The limit belongs to the kernel, not to the launch, so it only
+// ever rises: another thread's smaller call between this and the launch would otherwise
+// have the launch refused.
+int allow_smem(const void* kernel, size_t bytes);
+
 // Device address of the library's error word on the current device (resolved
 // once per device with cudaGetSymbolAddress); nullptr if unavailable.
 int* device_error_ptr();

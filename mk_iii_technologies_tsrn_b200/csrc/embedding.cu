@@ -901,12 +901,14 @@ int sum(SumArgs s, cudaStream_t stream) {
   const dim3 grid((unsigned)ceil_div(s.shares, (int64_t)per), (unsigned)ranges);
   const size_t smem = SUM_ASYNC<T, VEC> ? (size_t)SUM_STAGES * SUM_BATCH * 16 * threads : 0;
   if (smem > 40 * 1024) {
-    const cudaError_t e =
-        cudaFuncSetAttribute((const void*)embedding_sum_kernel<T, VEC>,
-                             cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return cuda_status(e);
+    const int st = allow_smem((const void*)embedding_sum_kernel<T, VEC>, smem);
+    if (st != TP_OK) return st;
   }
   embedding_sum_kernel<T, VEC><<<grid, threads, smem, stream>>>(s);
+  // (each launch that the next one's indices come from is asked for, so that none runs on
+  // what a refused one left in the workspace)
+  const int st = launch_status();
+  if (st != TP_OK) return st;
   const dim3 join((unsigned)s.shares, (unsigned)ceil_div(s.D, (int64_t)256));
   embedding_join_kernel<T><<<join, 256, 0, stream>>>(s);
   return launch_status();
@@ -926,12 +928,13 @@ int sort_in_cluster(const SortPlan& p, const Workspace& w, const void* ids, int 
   s.bits = p.bits;
   s.S = p.cluster;
   const size_t smem = sizeof(uint16_t) * SC_WARPS * ((size_t)1 << p.bits);
-  cudaError_t e = cudaFuncSetAttribute((const void*)sort_cluster_kernel,
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e == cudaSuccess && p.cluster > 8)
-    e = cudaFuncSetAttribute((const void*)sort_cluster_kernel,
-                             cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  if (e != cudaSuccess) return cuda_status(e);
+  const int st = allow_smem((const void*)sort_cluster_kernel, smem);
+  if (st != TP_OK) return st;
+  if (p.cluster > 8) {
+    const cudaError_t e = cudaFuncSetAttribute((const void*)sort_cluster_kernel,
+                                               cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return cuda_status(e);
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)p.cluster);
   cfg.blockDim = dim3(SC_THREADS);
@@ -1000,15 +1003,15 @@ int launch_embedding_bwd(int dtype, int ids64, int64_t N, int64_t D, const void*
   const int bins = 1 << p.bits;
   const size_t place_smem = sizeof(int) * SORT_WARPS * bins;
   if (place_smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute((const void*)sort_place_kernel,
-                                               cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               (int)place_smem);
-    if (e != cudaSuccess) return cuda_status(e);
+    const int st = allow_smem((const void*)sort_place_kernel, place_smem);
+    if (st != TP_OK) return st;
   }
   int at = N <= SMALL_TOKENS ? 1 : (p.cluster ? (p.passes & 1) : 0);
   if (N > 0 && N <= SMALL_TOKENS) {
     sort_small_kernel<<<1, (unsigned)SMALL_TOKENS, 0, stream>>>(ids, ids64, (int)N, V,
                                                                padding_idx, w.pairs[0]);
+    const int st = launch_status();
+    if (st != TP_OK) return st;
   } else if (p.cluster && N > 0) {
     const int st = sort_in_cluster(p, w, ids, ids64, N, V, padding_idx, stream);
     if (st != TP_OK) return st;
@@ -1029,9 +1032,14 @@ int launch_embedding_bwd(int dtype, int ids64, int64_t N, int64_t D, const void*
     s.shift = pass * p.bits;
     s.bins = bins;
     s.bits = p.bits;
-    if (p.tiles > 1)
+    if (p.tiles > 1) {
       sort_count_kernel<<<(unsigned)p.tiles, SORT_THREADS, sizeof(int) * bins, stream>>>(s);
+      const int st = launch_status();
+      if (st != TP_OK) return st;
+    }
     sort_place_kernel<<<(unsigned)p.tiles, SORT_THREADS, place_smem, stream>>>(s);
+    const int st = launch_status();
+    if (st != TP_OK) return st;
     at ^= 1;
   }
   const SumPlan su = sum_plan(N, V, D, esize);

@@ -556,11 +556,11 @@ struct EsnKernel<true, kGru, kSmemW, RB> {
 template <class Kn>
 int esn_configure(const EsnPlan& pl, cudaLaunchConfig_t* cfg, cudaLaunchAttribute* attr) {
   auto kern = Kn::fn;
-  cudaError_t e =
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pl.smem);
-  if (e != cudaSuccess) return (int)e;
+  const int st = allow_smem((const void*)kern, pl.smem);
+  if (st != TP_OK) return st;
   if (pl.CS > 8) {
-    e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    const cudaError_t e =
+        cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return (int)e;
   }
   *cfg = cudaLaunchConfig_t{};

@@ -637,9 +637,8 @@ template <typename K, typename A, typename... More>
 int launch_blocks(K kernel, int64_t blocks, size_t smem, cudaStream_t stream, const A& args,
                   More... more) {
   if (smem > 24 * 1024) {      // beside up to 12 KB of the kernels' own
-    const cudaError_t e = cudaFuncSetAttribute(
-        (const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return cuda_status(e);
+    const int st = allow_smem((const void*)kernel, smem);
+    if (st != TP_OK) return st;
   }
   kernel<<<(unsigned)blocks, 32 * GS_W, smem, stream>>>(args, more...);
   return launch_status();

@@ -799,9 +799,8 @@ int launch_fwd_kernel(const ResNormArgs& a, size_t smem, cudaStream_t stream) {
   auto* kernel = residual_norm_fwd_kernel<T, VEC, NV, TG, PM, GATE, BN, SH, MAXT>;
   const int threads = TG == 32 ? 128 : a.group;
   if (smem > 40 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(
-        (const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return cuda_status(e);
+    const int st = allow_smem((const void*)kernel, smem);
+    if (st != TP_OK) return st;
   }
   const int64_t want = ceil_div(a.rows, (int64_t)(threads / a.group));
   const int64_t cap = (int64_t)num_sms() * (2048 / threads < 32 ? 2048 / threads : 32);
@@ -817,9 +816,8 @@ int launch_bwd_kernel(const ResNormBwdArgs& g, size_t smem, int blocks, cudaStre
   constexpr int MAXT = TG == 32 ? 128 : 512;
   auto* kernel = residual_norm_bwd_kernel<T, VEC, NV, TG, PM, GATE, BN, SH, MAXT>;
   if (smem > 40 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(
-        (const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return cuda_status(e);
+    const int st = allow_smem((const void*)kernel, smem);
+    if (st != TP_OK) return st;
   }
   kernel<<<(unsigned)blocks, TG == 32 ? 128 : g.f.group, smem, stream>>>(g);
   return launch_status();

@@ -494,9 +494,8 @@ template <int R, int PL>
 int launch_att(const AttArgs& a, cudaStream_t stream) {
   const int tkv_pad = (int)((a.Tkv + 3) & ~(int64_t)3);
   const size_t smem = ((size_t)a.dh * R + 2 * (size_t)a.dh * ATT_KT + (size_t)R * tkv_pad) * 4;
-  cudaError_t e = cudaFuncSetAttribute(att_fwd_kernel<R, PL>,
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e != cudaSuccess) return (int)e;
+  const int st = allow_smem((const void*)att_fwd_kernel<R, PL>, smem);
+  if (st != TP_OK) return st;
   dim3 grid((unsigned)ceil_div(a.T, (int64_t)R), (unsigned)a.H, (unsigned)a.B);
   att_fwd_kernel<R, PL><<<grid, ATT_THREADS, smem, stream>>>(a);
   return launch_status();

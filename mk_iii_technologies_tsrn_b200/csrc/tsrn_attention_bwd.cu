@@ -313,9 +313,8 @@ int launch_tsrn_attention_bwd_group(int64_t S, int64_t T, int64_t Tkv, const int
   if (S > INT32_MAX || S * T * AB_L > INT32_MAX) return TP_ERR_TOO_LARGE;
   const size_t smem = (size_t)3 * Tkv * sizeof(int);
   if (smem > 200 * 1024) return TP_ERR_TOO_LARGE;   // Tkv up to ~17000 keys
-  cudaError_t e = cudaFuncSetAttribute(att_bwd_group_kernel,
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e != cudaSuccess) return cuda_status(e);
+  const int st = allow_smem((const void*)att_bwd_group_kernel, smem);
+  if (st != TP_OK) return st;
   att_bwd_group_kernel<<<(unsigned)S, AB_GROUP_THREADS, smem, stream>>>(T, Tkv, kj, order,
                                                                       key_begin, key_count);
   return launch_status();
