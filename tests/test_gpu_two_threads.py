@@ -8,7 +8,7 @@ import torch
 
 pytestmark = pytest.mark.gpu
 
-CALLS = 1500
+CALLS = 20000
 
 
 def _both(works):
