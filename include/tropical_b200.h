@@ -414,7 +414,7 @@ TP_API int tp_gated_scan_step(int dtype, int form, int64_t B, int64_t C, const v
  *  positions [N] of index_bits (32 or 64).  positions NULL: p_i = i % T (T <= L).
  *  fp32: product and sum rounded one by one, as tropformer_dropin.py:616-720
  *  rounds them; bf16: rounded once.  An id or position outside its table is not
- *  read: its row of out is NaN and TP_DEVERR_INDEX is recorded
+ *  read: the token's row of out is NaN and TP_DEVERR_INDEX is recorded
  *  (tp_device_error).
  *
  *  tp_embedding_bwd: dweight[v] = scale * sum of dout[i] over ids[i] = v, every
@@ -426,6 +426,12 @@ TP_API int tp_gated_scan_step(int dtype, int form, int64_t B, int64_t C, const v
  *
  *  tp_embedding_pos_bwd: dpos[t] = sum of dout[b * T + t] over b for t < T, zeros
  *  in the other rows of [L, D] (positions NULL).
+ *
+ *  These two look at one table's indices.  With both tables a token outside
+ *  either one must add to neither gradient (its row of out was NaN, and so is its
+ *  row of dout as a rule): tp_embedding_bwd_both and tp_embedding_pos_bwd_both
+ *  also leave out the tokens whose index in the other table (other [N] of
+ *  index_bits, other_rows rows; ids [N], V rows; NULL: all are in it) is outside.
  * ======================================================================== */
 TP_API int tp_embedding_fwd(int dtype, int index_bits, int64_t N, int64_t T, int64_t D,
                             const void* ids, const void* weight, int64_t V, int64_t ldw,
@@ -436,8 +442,16 @@ TP_API int tp_embedding_bwd(int dtype, int index_bits, int64_t N, int64_t D, con
                             const void* dout, int64_t V, float scale, int64_t padding_idx,
                             void* dweight, void* workspace, int64_t workspace_bytes,
                             void* stream);
+TP_API int tp_embedding_bwd_both(int dtype, int index_bits, int64_t N, int64_t D,
+                                 const void* ids, const void* dout, int64_t V, float scale,
+                                 int64_t padding_idx, const void* other, int64_t other_rows,
+                                 void* dweight, void* workspace, int64_t workspace_bytes,
+                                 void* stream);
 TP_API int tp_embedding_pos_bwd(int dtype, int64_t N, int64_t T, int64_t D, const void* dout,
                                 int64_t L, void* dpos, void* stream);
+TP_API int tp_embedding_pos_bwd_both(int dtype, int64_t N, int64_t T, int64_t D,
+                                     const void* dout, int64_t L, const void* ids,
+                                     int index_bits, int64_t V, void* dpos, void* stream);
 
 /* Backward of tp_tsrn_attention_prologue (training): from the gradients of Q,
  * K, V ([B, H, T, dh] contiguous) and the projections qkv, the gradient of qkv

@@ -187,9 +187,18 @@ SIGNATURES: dict[str, tuple] = {
         [_c_int, _c_int, _c_i64, _c_i64, _c_p, _c_p, _c_i64, _c_f, _c_i64, _c_p, _c_p, _c_i64,
          _c_p],
     ),
+    "tp_embedding_bwd_both": (
+        _c_int,
+        [_c_int, _c_int, _c_i64, _c_i64, _c_p, _c_p, _c_i64, _c_f, _c_i64, _c_p, _c_i64, _c_p,
+         _c_p, _c_i64, _c_p],
+    ),
     "tp_embedding_pos_bwd": (
         _c_int,
         [_c_int, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_p, _c_p],
+    ),
+    "tp_embedding_pos_bwd_both": (
+        _c_int,
+        [_c_int, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_p, _c_int, _c_i64, _c_p, _c_p],
     ),
     "tp_tsrn_attention_fwd": (
         _c_int,

@@ -917,10 +917,11 @@ int64_t tp_embedding_bwd_workspace_bytes(int64_t N, int64_t V, int64_t D) {
   return tp::embedding_bwd_workspace_bytes(N, V, D);
 }
 
-int tp_embedding_bwd(int dtype, int index_bits, int64_t N, int64_t D, const void* ids,
-                     const void* dout, int64_t V, float scale, int64_t padding_idx,
-                     void* dweight, void* workspace, int64_t workspace_bytes, void* stream) {
-  TP_RETURN_IF(N < 0 || D < 0 || V < 0, TP_ERR_INVALID_ARG);
+int tp_embedding_bwd_both(int dtype, int index_bits, int64_t N, int64_t D, const void* ids,
+                          const void* dout, int64_t V, float scale, int64_t padding_idx,
+                          const void* other, int64_t other_rows, void* dweight, void* workspace,
+                          int64_t workspace_bytes, void* stream) {
+  TP_RETURN_IF(N < 0 || D < 0 || V < 0 || other_rows < 0, TP_ERR_INVALID_ARG);
   TP_RETURN_IF(dtype != TP_DTYPE_F32 && dtype != TP_DTYPE_BF16, TP_ERR_UNSUPPORTED);
   TP_RETURN_IF(index_bits != 32 && index_bits != 64, TP_ERR_INVALID_ARG);
   TP_RETURN_IF(N > INT32_MAX || V >= INT32_MAX, TP_ERR_TOO_LARGE);
@@ -929,6 +930,7 @@ int tp_embedding_bwd(int dtype, int index_bits, int64_t N, int64_t D, const void
   if (N > 0) {
     TP_CHECK_PTR(ids);
     TP_CHECK_PTR(dout);
+    TP_CHECK_OPT_PTR(other);
   }
   TP_RETURN_IF(workspace == nullptr ||
                    workspace_bytes < tp_embedding_bwd_workspace_bytes(N, V, D),
@@ -936,20 +938,38 @@ int tp_embedding_bwd(int dtype, int index_bits, int64_t N, int64_t D, const void
   TP_CHECK_PTR(workspace);
   TP_RETURN_IF(!aligned16(workspace), TP_ERR_MISALIGNED);
   return tp::launch_embedding_bwd(dtype, index_bits == 64, N, D, ids, dout, V, scale,
-                                  padding_idx, dweight, workspace, as_stream(stream));
+                                  padding_idx, other, other_rows, dweight, workspace,
+                                  as_stream(stream));
 }
 
-int tp_embedding_pos_bwd(int dtype, int64_t N, int64_t T, int64_t D, const void* dout,
-                         int64_t L, void* dpos, void* stream) {
-  TP_RETURN_IF(N < 0 || T < 0 || D < 0 || L < 0, TP_ERR_INVALID_ARG);
+int tp_embedding_bwd(int dtype, int index_bits, int64_t N, int64_t D, const void* ids,
+                     const void* dout, int64_t V, float scale, int64_t padding_idx,
+                     void* dweight, void* workspace, int64_t workspace_bytes, void* stream) {
+  return tp_embedding_bwd_both(dtype, index_bits, N, D, ids, dout, V, scale, padding_idx, nullptr,
+                               0, dweight, workspace, workspace_bytes, stream);
+}
+
+int tp_embedding_pos_bwd_both(int dtype, int64_t N, int64_t T, int64_t D, const void* dout,
+                              int64_t L, const void* ids, int index_bits, int64_t V, void* dpos,
+                              void* stream) {
+  TP_RETURN_IF(N < 0 || T < 0 || D < 0 || L < 0 || V < 0, TP_ERR_INVALID_ARG);
   TP_RETURN_IF(dtype != TP_DTYPE_F32 && dtype != TP_DTYPE_BF16, TP_ERR_UNSUPPORTED);
+  TP_RETURN_IF(ids != nullptr && index_bits != 32 && index_bits != 64, TP_ERR_INVALID_ARG);
   TP_RETURN_IF(N > 0 && (T < 1 || N % T != 0 || T > L), TP_ERR_INVALID_ARG);
   TP_RETURN_IF(L > INT32_MAX || D > (int64_t)65535 * 32, TP_ERR_TOO_LARGE);
   if (L == 0 || D == 0) return TP_OK;
   TP_CHECK_PTR(dpos);
-  if (N > 0) TP_CHECK_PTR(dout);
-  return tp::launch_embedding_pos_bwd(dtype, N, N > 0 ? T : 0, D, dout, L, dpos,
-                                      as_stream(stream));
+  if (N > 0) {
+    TP_CHECK_PTR(dout);
+    TP_CHECK_OPT_PTR(ids);
+  }
+  return tp::launch_embedding_pos_bwd(dtype, N, N > 0 ? T : 0, D, dout, L, ids, index_bits == 64,
+                                      V, dpos, as_stream(stream));
+}
+
+int tp_embedding_pos_bwd(int dtype, int64_t N, int64_t T, int64_t D, const void* dout,
+                         int64_t L, void* dpos, void* stream) {
+  return tp_embedding_pos_bwd_both(dtype, N, T, D, dout, L, nullptr, 64, 0, dpos, stream);
 }
 
 int tp_tsrn_attention_fwd(int64_t B, int64_t H, int64_t T, int64_t Tkv, int64_t Tc, int64_t dh,

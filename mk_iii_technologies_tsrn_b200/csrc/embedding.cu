@@ -5,8 +5,8 @@
 //
 // as `embed(ids) * sqrt(d_model) + pos_embed(positions)` of the token models
 // (tropformer_dropin.py:616-720).  An id or position outside its table is
-// never read: its row of `out` is NaN, it adds to no gradient, and
-// TP_DEVERR_INDEX is recorded in the device error word.
+// never read: the token's row of `out` is NaN, its row of dout adds to neither
+// table's gradient, and TP_DEVERR_INDEX is recorded in the device error word.
 //
 // The forward is a row gather: bound by the rows read and written.
 //
@@ -169,10 +169,16 @@ SortPlan sort_plan(int64_t N, int64_t V) {
   return p;
 }
 
+// A token's index in this table, and in the other one where it has one.
+struct Keys {
+  const void* ids;
+  const void* other;      // NULL: no other table
+  int ids64;              // of both
+  int64_t V, padding_idx, other_rows;
+};
+
 struct SortArgs {
-  const void* ids;        // first pass: the caller's ids
-  int ids64;
-  int64_t V, padding_idx;
+  Keys keys;              // first pass
   const int2* in;         // later passes: (key, token) of the pass before
   int2* out;
   int* hist;              // [tiles][bins]
@@ -181,14 +187,19 @@ struct SortArgs {
   int first;
 };
 
-// V for what is not in the table or gets no gradient: sorted behind the rows
-__device__ __forceinline__ int key_of(int64_t id, int64_t V, int64_t padding_idx) {
-  return (id < 0 || id >= V || id == padding_idx) ? (int)V : (int)id;
+// V for a token that is not in both tables or gets no gradient: sorted behind the rows
+__device__ __forceinline__ int key_of(const Keys& k, int64_t i) {
+  const int64_t id = load_index(k.ids, k.ids64, i);
+  bool in = id >= 0 && id < k.V && id != k.padding_idx;
+  if (k.other != nullptr) {
+    const int64_t o = load_index(k.other, k.ids64, i);
+    in = in && o >= 0 && o < k.other_rows;
+  }
+  return in ? (int)id : (int)k.V;
 }
 
 __device__ __forceinline__ int sort_key(const SortArgs& s, int64_t i) {
-  if (!s.first) return s.in[i].x;
-  return key_of(load_index(s.ids, s.ids64, i), s.V, s.padding_idx);
+  return s.first ? key_of(s.keys, i) : s.in[i].x;
 }
 
 __global__ void __launch_bounds__(SORT_THREADS) sort_count_kernel(const SortArgs s) {
@@ -296,9 +307,7 @@ constexpr int SC_MAX_BITS = 10;
 constexpr int SC_GROUPS = 4;
 
 struct ClusterSortArgs {
-  const void* ids;
-  int ids64;
-  int64_t V, padding_idx;
+  Keys keys;
   int2* pairs[2];         // (key, token)
   int* hist;              // [passes][S][bins]
   int64_t N;
@@ -331,7 +340,7 @@ __global__ void __launch_bounds__(SC_THREADS) sort_cluster_kernel(const ClusterS
     const int shift = pass * s.bits;
     auto pair_at = [&](int64_t i) {
       if (pass > 0) return __ldcg(in_pairs + i);
-      return make_int2(key_of(load_index(s.ids, s.ids64, i), s.V, s.padding_idx), (int)i);
+      return make_int2(key_of(s.keys, i), (int)i);
     };
     for (int b = threadIdx.x; b < SC_WARPS * bins / 2; b += SC_THREADS)
       reinterpret_cast<unsigned*>(s_runs)[b] = 0;
@@ -425,13 +434,11 @@ __global__ void __launch_bounds__(SC_THREADS) sort_cluster_kernel(const ClusterS
 
 // Up to 1024 tokens: one block, each thread counts the tokens before its own.
 constexpr int64_t SMALL_TOKENS = 1024;
-__global__ void __launch_bounds__(SMALL_TOKENS) sort_small_kernel(const void* ids, int ids64,
-                                                                  int N, int64_t V,
-                                                                  int64_t padding_idx,
+__global__ void __launch_bounds__(SMALL_TOKENS) sort_small_kernel(const Keys keys, int N,
                                                                   int2* out) {
   __shared__ __align__(16) int s_key[SMALL_TOKENS];
   const int i = threadIdx.x;
-  const int key = i < N ? key_of(load_index(ids, ids64, i), V, padding_idx) : 0x7fffffff;
+  const int key = i < N ? key_of(keys, i) : 0x7fffffff;
   s_key[i] = key;
   __syncthreads();
   if (i >= N) return;
@@ -736,15 +743,17 @@ __global__ void __launch_bounds__(256) embedding_join_kernel(const SumArgs s) {
 }
 
 // ---------------------------------------------------------------- positions
-// dpos[t] = sum over the sequences of dout[., t].  SPLIT: the block's 8 warps take
+// dpos[t] = sum over the sequences of dout[., t] (ids: without the tokens whose id is
+// outside [0, V)).  SPLIT: the block's 8 warps take
 // contiguous ranges of the sequences for 32 vectors of one position; else each
 // warp has 32 vectors of its own and adds all sequences.
 template <typename T, int VEC, bool SPLIT>
 __global__ void __launch_bounds__(256) embedding_pos_kernel(int64_t B, int64_t steps, int64_t L,
                                                             int64_t D,
                                                             const T* __restrict__ dout,
-                                                            T* dpos) {
-  using V = RowVec<T, VEC>;
+                                                            const void* ids, int ids64,
+                                                            int64_t V, T* dpos) {
+  using R = RowVec<T, VEC>;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t t = SPLIT ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 8 + warp;
   const int64_t c = ((int64_t)blockIdx.y * 32 + lane) * VEC;
@@ -756,18 +765,26 @@ __global__ void __launch_bounds__(256) embedding_pos_kernel(int64_t B, int64_t s
   if (t < steps && c < D) {
     const T* p = dout + (lo * steps + t) * D + c;
     for (int64_t b = lo; b < hi; b += 8) {
-      V r[8];
+      R r[8];
+      bool in[8];
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
         r[u].zero();
-        if (b + u < hi) r[u].load(p);
+        in[u] = b + u < hi;
+        if (in[u]) {
+          r[u].load(p);
+          if (ids != nullptr) {
+            const int64_t id = load_index(ids, ids64, (b + u) * steps + t);
+            in[u] = id >= 0 && id < V;
+          }
+        }
         p += steps * D;
       }
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
         float f[VEC];
         r[u].get(f);
-        if (b + u < hi)
+        if (in[u])
 #pragma unroll
           for (int k = 0; k < VEC; ++k) acc[k] += f[k];
       }
@@ -788,7 +805,7 @@ __global__ void __launch_bounds__(256) embedding_pos_kernel(int64_t B, int64_t s
     }
   }
   if (t < L && c < D) {
-    V r;
+    R r;
     r.set(acc);
     r.store(dpos + t * D + c);
   }
@@ -914,13 +931,10 @@ int sum(SumArgs s, cudaStream_t stream) {
   return launch_status();
 }
 
-int sort_in_cluster(const SortPlan& p, const Workspace& w, const void* ids, int ids64, int64_t N,
-                    int64_t V, int64_t padding_idx, cudaStream_t stream) {
+int sort_in_cluster(const SortPlan& p, const Workspace& w, const Keys& keys, int64_t N,
+                    cudaStream_t stream) {
   ClusterSortArgs s;
-  s.ids = ids;
-  s.ids64 = ids64;
-  s.V = V;
-  s.padding_idx = padding_idx;
+  s.keys = keys;
   for (int k = 0; k < 2; ++k) s.pairs[k] = w.pairs[k];
   s.hist = w.hist;
   s.N = N;
@@ -957,30 +971,34 @@ int sum_any(const SumArgs& s, cudaStream_t stream) {
   return sum<T, 1>(s, stream);
 }
 
+struct PosArgs {
+  int64_t B, steps, L, D;
+  const void *dout, *ids;
+  int ids64;
+  int64_t V;
+  void* dpos;
+};
+
 template <typename T, int VEC>
-int pos_rows(int64_t B, int64_t steps, int64_t D, const void* dout, int64_t L, void* dpos,
-             cudaStream_t stream) {
-  const unsigned columns = (unsigned)ceil_div(D, (int64_t)32 * VEC);
+int pos_rows(const PosArgs& a, cudaStream_t stream) {
+  const unsigned columns = (unsigned)ceil_div(a.D, (int64_t)32 * VEC);
   // few positions for the GPU, or long sums: the sequences are shared out as well (114
   // sequences of 205 x 1152 fp32: 29 us against 65; 32 of 4096 x 1024 bf16: 59 against 47)
-  if (B > 8 && steps * columns < (B > 64 ? 64 : 8) * (int64_t)num_sms())
-    embedding_pos_kernel<T, VEC, true><<<dim3((unsigned)L, columns), 256, 0, stream>>>(
-        B, steps, L, D, (const T*)dout, (T*)dpos);
+  if (a.B > 8 && a.steps * columns < (a.B > 64 ? 64 : 8) * (int64_t)num_sms())
+    embedding_pos_kernel<T, VEC, true><<<dim3((unsigned)a.L, columns), 256, 0, stream>>>(
+        a.B, a.steps, a.L, a.D, (const T*)a.dout, a.ids, a.ids64, a.V, (T*)a.dpos);
   else
     embedding_pos_kernel<T, VEC, false>
-        <<<dim3((unsigned)ceil_div(L, (int64_t)8), columns), 256, 0, stream>>>(
-            B, steps, L, D, (const T*)dout, (T*)dpos);
+        <<<dim3((unsigned)ceil_div(a.L, (int64_t)8), columns), 256, 0, stream>>>(
+            a.B, a.steps, a.L, a.D, (const T*)a.dout, a.ids, a.ids64, a.V, (T*)a.dpos);
   return launch_status();
 }
 
 template <typename T>
-int pos(int64_t N, int64_t steps, int64_t D, const void* dout, int64_t L, void* dpos,
-        cudaStream_t stream) {
+int pos(const PosArgs& a, cudaStream_t stream) {
   constexpr int WIDE = 16 / sizeof(T);
-  const int64_t B = steps > 0 ? N / steps : 0;
-  if (vec_ok<T, WIDE>(D, {dout, dpos}, {}))
-    return pos_rows<T, WIDE>(B, steps, D, dout, L, dpos, stream);
-  return pos_rows<T, 1>(B, steps, D, dout, L, dpos, stream);
+  if (vec_ok<T, WIDE>(a.D, {a.dout, a.dpos}, {})) return pos_rows<T, WIDE>(a, stream);
+  return pos_rows<T, 1>(a, stream);
 }
 
 }  // namespace
@@ -996,7 +1014,9 @@ int64_t embedding_bwd_workspace_bytes(int64_t N, int64_t V, int64_t D) {
 
 int launch_embedding_bwd(int dtype, int ids64, int64_t N, int64_t D, const void* ids,
                          const void* dout, int64_t V, float scale, int64_t padding_idx,
-                         void* dweight, void* workspace, cudaStream_t stream) {
+                         const void* other, int64_t other_rows, void* dweight, void* workspace,
+                         cudaStream_t stream) {
+  const Keys keys = {ids, other, ids64, V, padding_idx, other_rows};
   const SortPlan p = sort_plan(N, V);
   const int esize = dtype == TP_DTYPE_F32 ? 4 : 2;
   const Workspace w = layout(N, V, D, esize, workspace);
@@ -1008,20 +1028,16 @@ int launch_embedding_bwd(int dtype, int ids64, int64_t N, int64_t D, const void*
   }
   int at = N <= SMALL_TOKENS ? 1 : (p.cluster ? (p.passes & 1) : 0);
   if (N > 0 && N <= SMALL_TOKENS) {
-    sort_small_kernel<<<1, (unsigned)SMALL_TOKENS, 0, stream>>>(ids, ids64, (int)N, V,
-                                                               padding_idx, w.pairs[0]);
+    sort_small_kernel<<<1, (unsigned)SMALL_TOKENS, 0, stream>>>(keys, (int)N, w.pairs[0]);
     const int st = launch_status();
     if (st != TP_OK) return st;
   } else if (p.cluster && N > 0) {
-    const int st = sort_in_cluster(p, w, ids, ids64, N, V, padding_idx, stream);
+    const int st = sort_in_cluster(p, w, keys, N, stream);
     if (st != TP_OK) return st;
   }
   for (int pass = 0; pass < p.passes && N > SMALL_TOKENS && !p.cluster; ++pass) {
     SortArgs s;
-    s.ids = ids;
-    s.ids64 = ids64;
-    s.V = V;
-    s.padding_idx = padding_idx;
+    s.keys = keys;
     s.first = pass == 0;
     s.in = w.pairs[at ^ 1];
     s.out = w.pairs[at];
@@ -1061,9 +1077,10 @@ int launch_embedding_bwd(int dtype, int ids64, int64_t N, int64_t D, const void*
 }
 
 int launch_embedding_pos_bwd(int dtype, int64_t N, int64_t T, int64_t D, const void* dout,
-                             int64_t L, void* dpos, cudaStream_t stream) {
-  return dtype == TP_DTYPE_F32 ? pos<float>(N, T, D, dout, L, dpos, stream)
-                               : pos<bf16_t>(N, T, D, dout, L, dpos, stream);
+                             int64_t L, const void* ids, int ids64, int64_t V, void* dpos,
+                             cudaStream_t stream) {
+  const PosArgs a = {T > 0 ? N / T : 0, T, L, D, dout, ids, ids64, V, dpos};
+  return dtype == TP_DTYPE_F32 ? pos<float>(a, stream) : pos<bf16_t>(a, stream);
 }
 
 }  // namespace tp

@@ -374,12 +374,16 @@ struct EmbeddingArgs {
 };
 int launch_embedding_fwd(const EmbeddingArgs& a, cudaStream_t stream);
 int64_t embedding_bwd_workspace_bytes(int64_t N, int64_t V, int64_t D);
-// gradient of a table of V rows from dout [N, D] and the row index of each token
+// gradient of a table of V rows from dout [N, D] and the row index of each token; other: the
+// tokens' indices in another table of other_rows rows (or NULL), in which they must lie too
 int launch_embedding_bwd(int dtype, int ids64, int64_t N, int64_t D, const void* ids,
                          const void* dout, int64_t V, float scale, int64_t padding_idx,
-                         void* dweight, void* workspace, cudaStream_t stream);
-// gradient of the first T rows of a position table of L rows (the others are zeros)
+                         const void* other, int64_t other_rows, void* dweight, void* workspace,
+                         cudaStream_t stream);
+// gradient of the first T rows of a position table of L rows (the others are zeros); ids: the
+// tokens' indices in a table of V rows (or NULL), in which they must lie
 int launch_embedding_pos_bwd(int dtype, int64_t N, int64_t T, int64_t D, const void* dout,
-                             int64_t L, void* dpos, cudaStream_t stream);
+                             int64_t L, const void* ids, int ids64, int64_t V, void* dpos,
+                             cudaStream_t stream);
 
 }  // namespace tp

@@ -429,40 +429,45 @@ Tensor embed_run(const Tensor& ids_, const Tensor& weight, const Tensor& pos, co
   return out;
 }
 
+// other: the tokens' indices in the other table, of other_rows rows, where there is one
 Tensor embed_back(const Tensor& ids_, const Tensor& dout_, int64_t rows, double scale,
-                  int64_t padding) {
+                  int64_t padding, const Tensor& other_, int64_t other_rows) {
   const On device(dout_);
-  const Tensor ids = ids_.contiguous(), dout = dout_.contiguous();
+  const Tensor ids = ids_.contiguous(), dout = dout_.contiguous(), other = contiguous(other_);
   const int64_t N = ids.numel(), D = dout.size(-1);
   const int64_t need = tp_embedding_bwd_workspace_bytes(N, rows, D);
   TORCH_CHECK_VALUE(need >= 0, "embedding_bwd takes fewer than 2^31 tokens and rows, got ", N,
                     " and ", rows);
   Tensor dw = at::empty({rows, D}, dout.options());
   const Tensor ws = bytes_on(dout, need);
-  check(tp_embedding_bwd(code_of(dout), bits_of(ids), N, D, at_(ids), at_(dout), rows,
-                         (float)scale, padding, at_(dw), at_(ws), ws.numel(), stream_of(dout)),
-        "tp_embedding_bwd");
+  check(tp_embedding_bwd_both(code_of(dout), bits_of(ids), N, D, at_(ids), at_(dout), rows,
+                              (float)scale, padding, at_(other), other_rows, at_(dw), at_(ws),
+                              ws.numel(), stream_of(dout)),
+        "tp_embedding_bwd_both");
   return dw;
 }
 
-Tensor embed_pos_back(const Tensor& dout_, int64_t rows) {
+// ids: the tokens' rows in a table of id_rows, where there is one
+Tensor embed_pos_back(const Tensor& dout_, int64_t rows, const Tensor& ids_, int64_t id_rows) {
   const On device(dout_);
-  const Tensor dout = dout_.contiguous();
+  const Tensor dout = dout_.contiguous(), ids = contiguous(ids_);
   const int64_t D = dout.size(-1), T = dout.dim() > 1 ? dout.size(-2) : 1;
   Tensor dp = at::empty({rows, D}, dout.options());
-  check(tp_embedding_pos_bwd(code_of(dout), D ? dout.numel() / D : 0, T, D, at_(dout), rows,
-                             at_(dp), stream_of(dout)),
-        "tp_embedding_pos_bwd");
+  check(tp_embedding_pos_bwd_both(code_of(dout), D ? dout.numel() / D : 0, T, D, at_(dout), rows,
+                                  at_(ids), ids.defined() ? bits_of(ids) : 64, id_rows, at_(dp),
+                                  stream_of(dout)),
+        "tp_embedding_pos_bwd_both");
   return dp;
 }
 
-// the gradients of the tables are dense
+// the gradients of the tables are dense; a token outside either table adds to neither
 struct Embedding : torch::autograd::Function<Embedding> {
   static Tensor forward(AutogradContext* ctx, Tensor weight, Maybe pos_weight, Tensor ids,
                         Maybe positions, double scale, int64_t padding) {
     const Tensor pos = or_none(pos_weight), at = or_none(positions);
     ctx->save_for_backward({ids, at});
     ctx->saved_data["rows"] = weight.size(0);
+    ctx->saved_data["pos"] = pos.defined();
     ctx->saved_data["positions"] = pos.defined() ? pos.size(0) : 0;
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["padding"] = padding;
@@ -473,14 +478,14 @@ struct Embedding : torch::autograd::Function<Embedding> {
       const variable_list s = ctx->get_saved_variables();
       const Tensor dout = grads[0].contiguous();
       variable_list out(6);
+      const int64_t rows = ctx->saved_data["rows"].toInt(),
+                    positions = ctx->saved_data["positions"].toInt();
       if (ctx->needs_input_grad(0))
-        out[0] = embed_back(s[0], dout, ctx->saved_data["rows"].toInt(),
-                            ctx->saved_data["scale"].toDouble(),
-                            ctx->saved_data["padding"].toInt());
-      const int64_t rows = ctx->saved_data["positions"].toInt();
-      if (rows > 0 && ctx->needs_input_grad(1))
-        out[1] = s[1].defined() ? embed_back(s[1], dout, rows, 1.0, -1)
-                                : embed_pos_back(dout, rows);
+        out[0] = embed_back(s[0], dout, rows, ctx->saved_data["scale"].toDouble(),
+                            ctx->saved_data["padding"].toInt(), s[1], positions);
+      if (ctx->saved_data["pos"].toBool() && ctx->needs_input_grad(1))
+        out[1] = s[1].defined() ? embed_back(s[1], dout, positions, 1.0, -1, s[0], rows)
+                                : embed_pos_back(dout, positions, s[0], rows);
       return out;
     });
   }
@@ -533,10 +538,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("embedding_fwd", &embedding_fwd);
   m.def("embedding_bwd", [](Tensor ids, Tensor dout, int64_t rows, double scale, int64_t padding) {
     at::NoGradGuard off;
-    return embed_back(ids, dout, rows, scale, padding);
+    return embed_back(ids, dout, rows, scale, padding, Tensor(), 0);
   });
   m.def("embedding_pos_bwd", [](Tensor dout, int64_t rows) {
     at::NoGradGuard off;
-    return embed_pos_back(dout, rows);
+    return embed_pos_back(dout, rows, Tensor(), 0);
   });
 }

@@ -77,7 +77,7 @@ class DeviceWaitTimeout(RuntimeError):
 
 class DeviceIndexError(IndexError):
     """A token id or position given to :func:`embedding` was outside its table;
-    its row of the output is NaN and it added to no gradient."""
+    the token's row of the output is NaN and it added to no gradient."""
 
     def __init__(self, device):
         super().__init__(f"an id or position given to ops.embedding on {device} is outside its "
@@ -1521,7 +1521,8 @@ def embedding_bwd(ids, dout, rows: int, scale: float = 1.0, *,
                   padding_idx: Optional[int] = None) -> torch.Tensor:
     """Gradient [rows, D] of an embedding table from ``dout`` [*ids.shape, D]: row v is
     ``scale`` times the float32 sum of the rows of dout whose id is v, in the order of the tokens
-    (the same bits on every call); absent rows and ``padding_idx`` are zero."""
+    (the same bits on every call); absent rows and ``padding_idx`` are zero.  Ids outside the table
+    add nothing (a token left out for its position is the caller's to mask)."""
     _require_cuda(ids, dout)
     _floating(dout, "dout")
     _index(ids, "ids")
@@ -1551,9 +1552,9 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, *,
     [L, D] of the same dtype.  ``positions`` (None: the index along the last dimension of ids;
     else integers that expand to ids' shape, as in a decoding step).  ``padding_idx``: a row that
     gets no gradient, as in ``F.embedding``.  float32 rounds the product and the sum one by one,
-    as the unfused expression; bfloat16 rounds once.  An id or position outside its table gives a
-    row of NaN and no gradient, and :func:`check_device_error` raises
-    :class:`DeviceIndexError`."""
+    as the unfused expression; bfloat16 rounds once.  A token whose id or position is outside its
+    table gets a row of NaN and adds to neither table's gradient, and :func:`check_device_error`
+    raises :class:`DeviceIndexError`."""
     if padding_idx is not None:
         V = weight.shape[0]
         if not -V <= padding_idx < V:

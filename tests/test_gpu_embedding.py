@@ -242,3 +242,36 @@ def test_every_row_of_a_sparse_gradient_is_written(cuda, dtype, D):
     assert st == 0
     want = torch.zeros(V, D, device=cuda, dtype=torch.float64).index_add_(0, ids, dout.double())
     assert torch.equal(dw[:V * D].view(V, D), want.to(dtype)) and torch.all(dw[V * D:].isnan())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("index", [torch.int32, torch.int64])
+@pytest.mark.parametrize("B,T,D", [(2, 3, 12), (5, 40, 33), (12, 7, 8), (70, 60, 16),
+                                   (1100, 250, 4)])
+def test_token_outside_one_table_adds_to_neither_gradient(cuda, dtype, index, B, T, D):
+    # bad ids at good positions and good ids at bad positions, with the NaN that their rows of the
+    # output send back; the tokens left in sum as if the others were not there
+    from mk_iii_technologies_tsrn_b200 import ops
+    g = _gen(cuda, B)
+    V, L, scale = 19, T + 2, 2.0
+    ids = torch.randint(0, V, (B, T), device=cuda, generator=g).to(index)
+    at = torch.randint(0, L, (B, T), device=cuda, generator=g).to(index)
+    bad_id = torch.rand(B, T, device=cuda, generator=g) < 0.2
+    bad_at = torch.rand(B, T, device=cuda, generator=g) < 0.2
+    bad_id[0, 1], bad_at[0, 0], bad_id[0, 0] = True, True, False
+    ids[bad_id] = torch.where(ids[bad_id] % 2 == 0, -1, V).to(index)
+    w = torch.randn(V, D, device=cuda, generator=g).to(dtype).requires_grad_()
+    p = torch.randn(L, D, device=cuda, generator=g).to(dtype).requires_grad_()
+    dout = torch.randn(B, T, D, device=cuda, generator=g).to(dtype)
+    rows = torch.arange(T, device=cuda).expand(B, T)
+    for positions, where, bad in ((None, rows, bad_id),
+                                  (torch.where(bad_at, L + 3, at.long()).to(index), at,
+                                   bad_id | bad_at)):
+        out = ops.embedding(ids, w, scale, pos_weight=p, positions=positions)
+        with pytest.raises(ops.DeviceIndexError):
+            ops.check_device_error(cuda)
+        assert torch.equal(out.isnan().any(-1), bad)
+        d = torch.where(bad[..., None], float("nan"), dout)
+        gw, gp = torch.autograd.grad(out, (w, p), d)
+        _check_grad(gw, torch.where(bad, -1, ids.long()), dout, V, scale)
+        _check_grad(gp, torch.where(bad, -1, where.long()), dout, L, 1.0)
