@@ -140,14 +140,23 @@ struct Rows {
   }
 };
 
-// A product of gates kept finite: gates above 1 may overflow it, and a zero
-// state must stay zero.  (A NaN gate is NaN in the run's result as well.)
+// Gates above 1 may overflow a run's product, which the recurrence itself need not do:
+// its states may be small, or zero, or end at a gate of 0.  A product that met a zero
+// gate after its overflow (inf * 0) is 0.  (A NaN gate is NaN in the run's result as
+// well, whatever the product.)  One that stays infinite makes the state so, except a
+// zero state, which stays what the run's result is.
 template <int CPL>
-__device__ __forceinline__ Lane<CPL> finite(Lane<CPL> a) {
+__device__ __forceinline__ Lane<CPL> product(Lane<CPL> a) {
 #pragma unroll
-  for (int k = 0; k < CPL; ++k)
-    a.put(k, fminf(fmaxf(a.at(k), -3.402823466e38f), 3.402823466e38f));
+  for (int k = 0; k < CPL; ++k) a.put(k, a.at(k) != a.at(k) ? 0.0f : a.at(k));
   return a;
+}
+// the run of product `a` (not NaN) and result `r` applied to a state
+template <int CPL>
+__device__ __forceinline__ Lane<CPL> apply(Lane<CPL> a, Lane<CPL> state, Lane<CPL> r) {
+#pragma unroll
+  for (int k = 0; k < CPL; ++k) a.put(k, state.at(k) == 0.0f ? 0.0f : a.at(k));
+  return fma_(a, state, r);
 }
 
 // Gate as the recurrence's a, and 1 - a in the sigmoid form.  bf16 storage: the
@@ -301,7 +310,7 @@ __global__ void __launch_bounds__(32 * W)
     if (n == L) run(std::true_type());
     else run(std::false_type());
   }
-  s_a[warp][lane] = finite(pa);
+  s_a[warp][lane] = product(pa);
   s_h[warp][lane] = REVERSE ? mul_(ga, ph) : ph;
   __syncthreads();
   if (warp != 0) return;
@@ -310,11 +319,11 @@ __global__ void __launch_bounds__(32 * W)
 #pragma unroll
   for (int k = 0; k < W; ++k) {
     const int q = REVERSE ? W - 1 - k : k;
-    ph = fma_(s_a[q][lane], ph, s_h[q][lane]);
+    ph = apply(s_a[q][lane], ph, s_h[q][lane]);
     pa = mul_(pa, s_a[q][lane]);
   }
   const int64_t row = (w.b * a.segs + w.seg) * 2;
-  w.store(a.runs, row, a.C, finite(pa));
+  w.store(a.runs, row, a.C, product(pa));
   w.store(a.runs, row + 1, a.C, ph);
 }
 
@@ -335,14 +344,14 @@ __device__ __forceinline__ Lane<CPL> segment_start(const GatedScanArgs& a, const
   for (int k = lo; k < hi; ++k) {
     const int64_t row = (w.b * a.segs + (REVERSE ? a.segs - 1 - k : k)) * 2;
     const N ra = w.load(a.runs, row, a.C), rh = w.load(a.runs, row + 1, a.C);
-    ph = fma_(ra, ph, rh);
+    ph = apply(ra, ph, rh);
     pa = mul_(pa, ra);
   }
-  s_a[warp][lane] = finite(pa);
+  s_a[warp][lane] = product(pa);
   s_h[warp][lane] = ph;
   __syncthreads();
 #pragma unroll
-  for (int q = 0; q < W; ++q) carry = fma_(s_a[q][lane], carry, s_h[q][lane]);
+  for (int q = 0; q < W; ++q) carry = apply(s_a[q][lane], carry, s_h[q][lane]);
   return carry;
 }
 
@@ -420,14 +429,14 @@ __global__ void __launch_bounds__(32 * W, 2)
       ph = fma_(A[i], ph, U[i]);
       pa = mul_(pa, A[i]);
     }
-    s_a[par][warp][lane] = finite(pa);
+    s_a[par][warp][lane] = product(pa);
     s_h[par][warp][lane] = ph;
     __syncthreads();
     N mine = carry, h = carry;
 #pragma unroll
     for (int q = 0; q < W; ++q) {
       if (q == warp) mine = h;
-      h = fma_(s_a[par][q][lane], h, s_h[par][q][lane]);
+      h = apply(s_a[par][q][lane], h, s_h[par][q][lane]);
     }
     carry = h;
     if (a.states && t0 < a.T && (t0 % GATED_SCAN_CHUNK) == 0)
@@ -551,7 +560,7 @@ __global__ void __launch_bounds__(32 * W, 2)
     N gr = dh_at(L - 1);      // g of the run alone
 #pragma unroll
     for (int i = L - 2; i >= 0; --i) gr = fma_(A[i + 1], gr, dh_at(i));
-    s_a[par][warp][lane] = finite(pa);
+    s_a[par][warp][lane] = product(pa);
     s_h[par][warp][lane] = ph;
     s_c[par][warp][lane] = mul_(A[0], gr);
     __syncthreads();
@@ -559,13 +568,13 @@ __global__ void __launch_bounds__(32 * W, 2)
 #pragma unroll
     for (int q = W - 1; q >= 0; --q) {
       if (q == warp) mine = c;
-      c = fma_(s_a[par][q][lane], c, s_c[par][q][lane]);
+      c = apply(s_a[par][q][lane], c, s_c[par][q][lane]);
     }
     carry = c;
     N before[L];      // h_{t-1}
     {
       N h = first;
-      for (int q = lead; q < warp; ++q) h = fma_(s_a[par][q][lane], h, s_h[par][q][lane]);
+      for (int q = lead; q < warp; ++q) h = apply(s_a[par][q][lane], h, s_h[par][q][lane]);
 #pragma unroll
       for (int i = 0; i < L; ++i) {
         before[i] = h;

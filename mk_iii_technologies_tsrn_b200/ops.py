@@ -1445,7 +1445,10 @@ def gated_scan(gate: torch.Tensor, x: torch.Tensor, h0: Optional[torch.Tensor] =
     ``lengths`` [B]: row b ends after lengths[b] steps; h is zero behind the end and nothing
     there is read.  Returns h [B, T, C] in x's dtype, with ``return_state`` also the float32
     state [B, C] at each row's end (for :func:`gated_scan_step`, or to go on with the next
-    segment).  States are float32 throughout.  Meant for gates of magnitude at most 1."""
+    segment).  States are float32 throughout.  Meant for gates of magnitude at most 1: steps are
+    joined by the products of their gates.  Larger gates are right as long as the products of
+    consecutive gates stay within float32's range; where one overflows, states behind it are right,
+    infinite or NaN, and one that underflows counts as 0."""
     code, call = _gate_form(form), _lib.host().gated_scan
     out = call(gate, x, h0, lengths, code, return_state)
     if out is None:      # 64-bit lengths, or something wrong

@@ -314,3 +314,59 @@ def test_rows_that_begin_on_pairs(cuda, form, dtype, B, T, C):
             views.append(wide[..., shift:shift + C])
         same = _check(cuda, *views, h0, dh, dl, n, form)
         assert all(torch.equal(got[k], same[k]) for k in got)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,C,per", [(64, 8, 8), (300, 33, 8), (2600, 6, 8), (3000, 7, 100)])
+def test_products_of_gates_that_overflow_meet_a_zero_gate(cuda, dtype, T, C, per):
+    # in every `per` steps, gates whose product leaves fp32's range, on states small enough for the
+    # recurrence to stay within it, and then a gate of 0, behind which the state is the input alone.
+    # The bound of the docstring counts roundings of normal numbers; dgate's products g h of two
+    # values near 1e-32 are below the type's least normal number, where a rounding is off by at most
+    # half of the least subnormal one (2^-149 in fp32, 2^-133 in bf16; fp32 underflow as well: twice).
+    # 64 steps are whole periods in every run of 8 or 16 steps: all values are the recurrence's.  In
+    # the others some runs end between the large gates and the zero: 1e10^4 > 2^128 stays infinite
+    # there, and what follows is right, infinite or NaN
+    from mk_iii_technologies_tsrn_b200 import ops
+    gate, x, h0, dh, dl, _ = _make(cuda, 2, T, C, dtype, "decay", 14)
+    n, big = (4, 1e10) if per == 8 else (39, 10.0)
+    gate = torch.where(gate.abs() < 0.5, gate, 0.5)
+    for k in range(per):
+        if k < n:
+            gate[:, k::per] = big
+        elif k == n:
+            gate[:, k::per] = 0
+    tiny = 1e-32
+    x, h0, dh, dl = x * tiny, h0 * tiny, dh * tiny, dl * tiny
+    ins = [t.detach().requires_grad_() for t in (gate, x, h0)]
+    h, last = ops.gated_scan(*ins, return_state=True)
+    got = dict(zip(("dgate", "dx", "dh0"), torch.autograd.grad((h, last), ins, (dh, dl))))
+    got.update(h=h.detach(), last=last.detach())
+    for k, (value, bound) in _reference(gate, x, h0, dh, dl, None, "decay").items():
+        tol = bound * 1.02 + HALF[got[k].dtype] * (value.abs() + bound) * 1.01
+        tol = tol + 2.0 ** -149 + (2.0 ** -134 if got[k].dtype == torch.bfloat16 else 0.0)
+        close = (got[k].double().cpu() - value).abs() <= tol
+        assert torch.all(close | ~got[k].cpu().isfinite()), k
+        assert T > 64 or torch.all(close), k
+
+
+@pytest.mark.parametrize("T", [64, 2600])
+def test_products_of_gates_that_stay_infinite_say_so(cuda, T):
+    # products that overflow before small gates bring them back: where the state behind a run is
+    # not the recurrence's, it is infinite or NaN, never another number
+    from mk_iii_technologies_tsrn_b200 import ops
+    gate = torch.full((1, T, 8), 0.5, device=cuda)
+    for k in range(4):
+        gate[:, k::32], gate[:, k + 4::32] = 1e10, 1e-10
+    h0 = torch.full((1, 8), 1e-32, device=cuda)
+    x = torch.zeros_like(gate)
+    h, last = ops.gated_scan(gate, x, h0, return_state=True)
+    want, state = [], h0.double()
+    for t in range(T):
+        state = state * gate[:, t].double()
+        want.append(state)
+    want = torch.stack(want, 1)
+    close = (h.double() - want).abs() <= 2 * T * U * want.abs() + 2.0 ** -149
+    assert torch.all(close | ~h.isfinite())
+    assert torch.all((last - h[:, -1] == 0) | ~last.isfinite())
+    assert torch.all(ops.gated_scan(gate, x) == 0)
