@@ -144,18 +144,22 @@ struct Rows {
 // its states may be small, or zero, or end at a gate of 0.  A product that met a zero
 // gate after its overflow (inf * 0) is 0.  (A NaN gate is NaN in the run's result as
 // well, whatever the product.)  One that stays infinite makes the state so, except a
-// zero state, which stays what the run's result is.
-template <int CPL>
+// zero state, which stays what the run's result is.  (Sigmoids are at most 1.)
+template <int FORM, int CPL>
 __device__ __forceinline__ Lane<CPL> product(Lane<CPL> a) {
+  if constexpr (FORM == TP_GATE_DECAY) {
 #pragma unroll
-  for (int k = 0; k < CPL; ++k) a.put(k, a.at(k) != a.at(k) ? 0.0f : a.at(k));
+    for (int k = 0; k < CPL; ++k) a.put(k, a.at(k) != a.at(k) ? 0.0f : a.at(k));
+  }
   return a;
 }
-// the run of product `a` (not NaN) and result `r` applied to a state
-template <int CPL>
+// the run of product `a` and result `r` applied to a state
+template <int FORM, int CPL>
 __device__ __forceinline__ Lane<CPL> apply(Lane<CPL> a, Lane<CPL> state, Lane<CPL> r) {
+  if constexpr (FORM == TP_GATE_DECAY) {
 #pragma unroll
-  for (int k = 0; k < CPL; ++k) a.put(k, state.at(k) == 0.0f ? 0.0f : a.at(k));
+    for (int k = 0; k < CPL; ++k) a.put(k, state.at(k) == 0.0f ? 0.0f : a.at(k));
+  }
   return fma_(a, state, r);
 }
 
@@ -310,7 +314,7 @@ __global__ void __launch_bounds__(32 * W)
     if (n == L) run(std::true_type());
     else run(std::false_type());
   }
-  s_a[warp][lane] = product(pa);
+  s_a[warp][lane] = product<FORM>(pa);
   s_h[warp][lane] = REVERSE ? mul_(ga, ph) : ph;
   __syncthreads();
   if (warp != 0) return;
@@ -319,18 +323,18 @@ __global__ void __launch_bounds__(32 * W)
 #pragma unroll
   for (int k = 0; k < W; ++k) {
     const int q = REVERSE ? W - 1 - k : k;
-    ph = apply(s_a[q][lane], ph, s_h[q][lane]);
+    ph = apply<FORM>(s_a[q][lane], ph, s_h[q][lane]);
     pa = mul_(pa, s_a[q][lane]);
   }
   const int64_t row = (w.b * a.segs + w.seg) * 2;
-  w.store(a.runs, row, a.C, product(pa));
+  w.store(a.runs, row, a.C, product<FORM>(pa));
   w.store(a.runs, row + 1, a.C, ph);
 }
 
 // The state before (REVERSE: the gradient after) the block's segment: the runs of
 // the segments before (after) it applied to `carry`.  The warps compose an equal
 // share each, through `s_a`, `s_h`, and all apply the shares in order.
-template <typename T, int CPL, int W, bool REVERSE>
+template <typename T, int CPL, int FORM, int W, bool REVERSE>
 __device__ __forceinline__ Lane<CPL> segment_start(const GatedScanArgs& a, const Place<T, CPL>& w,
                                                    Lane<CPL> carry, Lane<CPL> (*s_a)[32],
                                                    Lane<CPL> (*s_h)[32], int warp, int lane) {
@@ -344,14 +348,14 @@ __device__ __forceinline__ Lane<CPL> segment_start(const GatedScanArgs& a, const
   for (int k = lo; k < hi; ++k) {
     const int64_t row = (w.b * a.segs + (REVERSE ? a.segs - 1 - k : k)) * 2;
     const N ra = w.load(a.runs, row, a.C), rh = w.load(a.runs, row + 1, a.C);
-    ph = apply(ra, ph, rh);
+    ph = apply<FORM>(ra, ph, rh);
     pa = mul_(pa, ra);
   }
-  s_a[warp][lane] = product(pa);
+  s_a[warp][lane] = product<FORM>(pa);
   s_h[warp][lane] = ph;
   __syncthreads();
 #pragma unroll
-  for (int q = 0; q < W; ++q) carry = apply(s_a[q][lane], carry, s_h[q][lane]);
+  for (int q = 0; q < W; ++q) carry = apply<FORM>(s_a[q][lane], carry, s_h[q][lane]);
   return carry;
 }
 
@@ -396,7 +400,7 @@ __global__ void __launch_bounds__(32 * W, 2)
   };
 #pragma unroll
   for (int k = 0; k < STAGES - 1; ++k) fetch();
-  carry = segment_start<T, CPL, W, false>(a, w, carry, s_a[1], s_h[1], warp, lane);
+  carry = segment_start<T, CPL, FORM, W, false>(a, w, carry, s_a[1], s_h[1], warp, lane);
   for (int64_t it = 0; it < iters; ++it) {
     __syncwarp();          // the warp has read the stage that is filled now
     fetch();
@@ -429,14 +433,14 @@ __global__ void __launch_bounds__(32 * W, 2)
       ph = fma_(A[i], ph, U[i]);
       pa = mul_(pa, A[i]);
     }
-    s_a[par][warp][lane] = product(pa);
+    s_a[par][warp][lane] = product<FORM>(pa);
     s_h[par][warp][lane] = ph;
     __syncthreads();
     N mine = carry, h = carry;
 #pragma unroll
     for (int q = 0; q < W; ++q) {
       if (q == warp) mine = h;
-      h = apply(s_a[par][q][lane], h, s_h[par][q][lane]);
+      h = apply<FORM>(s_a[par][q][lane], h, s_h[par][q][lane]);
     }
     carry = h;
     if (a.states && t0 < a.T && (t0 % GATED_SCAN_CHUNK) == 0)
@@ -520,7 +524,7 @@ __global__ void __launch_bounds__(32 * W, 2)
 #pragma unroll
   for (int k = 0; k < STAGES - 1; ++k) fetch();
   N next = first_state(0);
-  carry = segment_start<T, CPL, W, true>(a, w, carry, s_a[1], s_c[1], warp, lane);
+  carry = segment_start<T, CPL, FORM, W, true>(a, w, carry, s_a[1], s_c[1], warp, lane);
   for (int64_t it = 0; it < iters; ++it) {
     __syncwarp();
     fetch();
@@ -560,7 +564,7 @@ __global__ void __launch_bounds__(32 * W, 2)
     N gr = dh_at(L - 1);      // g of the run alone
 #pragma unroll
     for (int i = L - 2; i >= 0; --i) gr = fma_(A[i + 1], gr, dh_at(i));
-    s_a[par][warp][lane] = product(pa);
+    s_a[par][warp][lane] = product<FORM>(pa);
     s_h[par][warp][lane] = ph;
     s_c[par][warp][lane] = mul_(A[0], gr);
     __syncthreads();
@@ -568,13 +572,13 @@ __global__ void __launch_bounds__(32 * W, 2)
 #pragma unroll
     for (int q = W - 1; q >= 0; --q) {
       if (q == warp) mine = c;
-      c = apply(s_a[par][q][lane], c, s_c[par][q][lane]);
+      c = apply<FORM>(s_a[par][q][lane], c, s_c[par][q][lane]);
     }
     carry = c;
     N before[L];      // h_{t-1}
     {
       N h = first;
-      for (int q = lead; q < warp; ++q) h = apply(s_a[par][q][lane], h, s_h[par][q][lane]);
+      for (int q = lead; q < warp; ++q) h = apply<FORM>(s_a[par][q][lane], h, s_h[par][q][lane]);
 #pragma unroll
       for (int i = 0; i < L; ++i) {
         before[i] = h;
