@@ -163,10 +163,12 @@ __device__ __forceinline__ Lane<CPL> apply(Lane<CPL> a, Lane<CPL> state, Lane<CP
   return fma_(a, state, r);
 }
 
-// Gate as the recurrence's a, and 1 - a in the sigmoid form.  bf16 storage: the
-// gate comes from 2^x with the argument rounded once, relative error about
-// (8 + 1.5 |z|) 2^-24, far below the 2^-9 of the stored result; fp32: to fp32
-// accuracy.
+// Gate as the recurrence's a, and 1 - a in the sigmoid form.  bf16 storage: from
+// 2^x with the argument rounded once, the smaller of the two to a relative
+// (8 + 1.5 |z|) 2^-24; fp32: to fp32 accuracy.  Either way the larger one is 1 less
+// the smaller, off by half a step and little more: states at the rows' ends, those
+// kept for the backward and the gradient of h0 are fp32 sums over many steps, and
+// have the error of the recurrence in fp32 with rounded gates, or less.
 template <typename T, int FORM>
 __device__ __forceinline__ void gate_of(float z, float& a, float& rest) {
   if constexpr (FORM == TP_GATE_SIGMOID) {

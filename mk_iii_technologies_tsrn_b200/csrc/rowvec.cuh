@@ -179,42 +179,52 @@ struct RowVec<bf16_t, 1> {
   }
 };
 
-// sigmoid(v) and 1 - sigmoid(v), both to fp32 accuracy: from e = exp(-|v|) the
-// larger one is 1 / (1 + e) and the smaller e / (1 + e), with no cancellation
-// and no overflow (NaN stays NaN).
-__device__ __forceinline__ void sigmoid_pair(float v, float& s, float& rest) {
-  const float e = expf(-fabsf(v));
-  const float big = __fdividef(1.0f, 1.0f + e);
-  const float small = e * big;
-  s = v >= 0.0f ? big : small;
-  rest = v >= 0.0f ? small : big;
-}
-
-// The same for results that are rounded to bf16: e = exp(-v) as one power of
-// two.  Relative error about (8 + 1.5 |v|) 2^-24 (argument rounded once, 2^x to
-// 2^-22, 1 + e, reciprocal and product).  The exponent is held at 126, so that
-// sigmoid(-inf) is 2^-126 and its complement exactly 1.
-__device__ __forceinline__ float ex2_of_capped(float t) {
-  asm("min.NaN.f32 %0, %0, 0f42FC0000;" : "+f"(t));   // 126
-  return tp_ex2(t);
-}
 __device__ __forceinline__ float rcp_approx(float v) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
+
+// sigmoid(v) and 1 - sigmoid(v), both to fp32 accuracy: with e = exp(-|v|) the
+// smaller one is e / (1 + e), with no cancellation and no overflow (NaN stays NaN),
+// and the larger one is 1 less that.  The quotient 1 / (1 + e) instead is off by up to
+// an ulp, always to the same side for like arguments: a gate of a long memory applies
+// that error once a step (h_last of 1536 steps at gates around sigmoid(6): root mean
+// square error 2.8 times that of correctly rounded gates).
+__device__ __forceinline__ void sigmoid_pair(float v, float& s, float& rest) {
+  const float e = expf(-fabsf(v));
+  const float small = e * rcp_approx(1.0f + e);
+  const float big = 1.0f - small;
+  s = v >= 0.0f ? big : small;
+  rest = v >= 0.0f ? small : big;
+}
+
+// The same for bf16 storage: e = exp(-v) as one power of two.  Relative error of
+// what comes from it about (8 + 1.5 |v|) 2^-24 (argument rounded once, 2^x to
+// 2^-22, 1 + e, reciprocal and product); a gate above 1/2 is 1 less its complement,
+// off by that of the complement and a rounding.  The exponent is held at 126, so that
+// sigmoid(-inf) is 2^-126 and its complement exactly 1.
+__device__ __forceinline__ float ex2_of_capped(float t) {
+  asm("min.NaN.f32 %0, %0, 0f42FC0000;" : "+f"(t));   // 126
+  return tp_ex2(t);
+}
 __device__ __forceinline__ void fast_sigmoid_pair(float v, float& s, float& rest) {
   const float e = ex2_of_capped(__fmul_rn(v, -1.442695041f));
-  s = rcp_approx(__fadd_rn(1.0f, e));
-  rest = __fmul_rn(e, s);
+  const float r = rcp_approx(__fadd_rn(1.0f, e));
+  rest = __fmul_rn(e, r);
+  const float big = __fsub_rn(1.0f, rest);
+  s = v > 0.0f ? big : r;
 }
 // two at once, the same bits
 __device__ __forceinline__ void fast_sigmoid_pair2(float2 v, float2& s, float2& rest) {
+  const float2 one = make_float2(1.0f, 1.0f);
   const float2 t = tp_mul2(v, make_float2(-1.442695041f, -1.442695041f));
   const float2 e = make_float2(ex2_of_capped(t.x), ex2_of_capped(t.y));
-  const float2 d = tp_add2(make_float2(1.0f, 1.0f), e);
-  s = make_float2(rcp_approx(d.x), rcp_approx(d.y));
-  rest = tp_mul2(e, s);
+  const float2 d = tp_add2(one, e);
+  const float2 r = make_float2(rcp_approx(d.x), rcp_approx(d.y));
+  rest = tp_mul2(e, r);
+  const float2 big = tp_fma2(rest, make_float2(-1.0f, -1.0f), one);
+  s = make_float2(v.x > 0.0f ? big.x : r.x, v.y > 0.0f ? big.y : r.y);
 }
 
 }  // namespace tp

@@ -370,3 +370,35 @@ def test_products_of_gates_that_stay_infinite_say_so(cuda, T):
     assert torch.all(close | ~h.isfinite())
     assert torch.all((last - h[:, -1] == 0) | ~last.isfinite())
     assert torch.all(ops.gated_scan(gate, x) == 0)
+
+
+@pytest.mark.parametrize("mean", [2.0, 6.0])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_fp32_results_have_fp32_gates(cuda, dtype, mean):
+    # the state at the end and the gradient of h0 are fp32 whatever the storage: their root mean
+    # square error is near that of the recurrence step by step in fp32 with fp32 sigmoids.  In units
+    # of a last place the plain complement of a gate has an exponential (0.4), a sum and a quotient
+    # (0.29 each, half a step at most), the kernel's a quotient of up to 2 (0.5) and a product (0.29)
+    # more: sqrt(0.58 / 0.33) = 1.33 times, less with the roundings that both share
+    from mk_iii_technologies_tsrn_b200 import ops
+    B, T, C = 4, 1536, 320
+    g = torch.Generator(device=cuda).manual_seed(15)
+    gate = (torch.randn(B, T, C, device=cuda, generator=g) + mean).to(dtype)
+    x, dh = (torch.randn(B, T, C, device=cuda, generator=g).to(dtype) for _ in range(2))
+    h0 = torch.randn(B, C, device=cuda, generator=g).requires_grad_()
+    h, last = ops.gated_scan(gate, x, h0, form="sigmoid", return_state=True)
+    dh0, = torch.autograd.grad(h, h0, dh)
+
+    def plain(to):
+        f, r = torch.sigmoid(gate.to(to)), torch.sigmoid(-gate.to(to))
+        u, d, s = r * x.to(to), dh.to(to), h0.detach().to(to)
+        c = torch.zeros_like(s)
+        for t in range(T):
+            s = f[:, t] * s + u[:, t]
+        for t in range(T - 1, -1, -1):
+            c = f[:, t] * (d[:, t] + c)
+        return s, c
+
+    rms = lambda v, e: float((v.detach().double() - e).square().mean().sqrt())  # noqa: E731
+    for got, one, exact in zip((last, dh0), plain(torch.float32), plain(torch.float64)):
+        assert rms(got, exact) <= 1.4 * rms(one, exact)
