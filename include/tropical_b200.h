@@ -850,14 +850,16 @@ TP_API int tp_last_error(void);
  * exchange, the stream-K merge flags) is bounded by a budget of %globaltimer
  * time.  A wait that runs out records a code in the device error word of its
  * GPU and the kernel returns early (its outputs are then incomplete), so the
- * context stays usable.  The word keeps the FIRST code recorded. */
+ * context stays usable.  The word keeps the FIRST code recorded.  An index outside
+ * its table has a word of its own. */
 #define TP_DEVERR_BARRIER_TIMEOUT 1   /* an mbarrier wait ran out of budget  */
 #define TP_DEVERR_FLAG_TIMEOUT 2      /* a flag wait ran out of budget       */
 #define TP_DEVERR_INDEX 3             /* an id or position outside its table */
 
 /* Device-side error word of the current device: 0 when no kernel reported a
  * problem, else a TP_DEVERR_* code.  Synchronises with the device (it reads
- * device memory).  reset != 0 clears the word afterwards.  Returns
+ * device memory).  A wait that ran out comes before an index; reset != 0 clears
+ * what was returned afterwards, so that the next call returns the other one.  Returns
  * -cudaError_t on failure.  The word's address is cached per device for the
  * life of the process: do not call the library after cudaDeviceReset in the
  * same process. */

@@ -1339,15 +1339,20 @@ int tp_set_smooth_fused(int enable) { return g_smooth_fused.exchange(enable ? 1 
 int tp_last_error(void) { return last_error(); }
 
 int tp_device_error(int reset) {
-  int v = 0;
-  cudaError_t e = cudaMemcpyFromSymbol(&v, g_tp_status, sizeof(int), offsetof(TpDeviceStatus, error));
+  int v[2] = {0, 0};
+  static_assert(offsetof(TpDeviceStatus, index_error) ==
+                    offsetof(TpDeviceStatus, error) + sizeof(int), "");
+  cudaError_t e =
+      cudaMemcpyFromSymbol(v, g_tp_status, sizeof(v), offsetof(TpDeviceStatus, error));
   if (e != cudaSuccess) return -(int)e;
-  if (reset) {
+  if (reset && (v[0] || v[1])) {        // the word that is returned, not the other one
     const int zero = 0;
-    e = cudaMemcpyToSymbol(g_tp_status, &zero, sizeof(int), offsetof(TpDeviceStatus, error));
+    e = cudaMemcpyToSymbol(g_tp_status, &zero, sizeof(int),
+                           v[0] ? offsetof(TpDeviceStatus, error)
+                                : offsetof(TpDeviceStatus, index_error));
     if (e != cudaSuccess) return -(int)e;
   }
-  return v;
+  return v[0] ? v[0] : v[1];
 }
 
 int tp_set_wait_budget_ns(int64_t ns, int64_t* previous) {

@@ -25,8 +25,9 @@
 // change it at run time (tp_set_wait_budget_ns).  Error codes
 // TP_DEVERR_BARRIER_TIMEOUT / TP_DEVERR_FLAG_TIMEOUT are in tropical_b200.h.
 struct TpDeviceStatus {
-  int error;                          // 0, or the first TP_DEVERR_* recorded
-  int reserved;
+  int error;                          // 0, or the first TP_DEVERR_* of a wait recorded
+  int index_error;                    // 0 or TP_DEVERR_INDEX (a word of its own: a bad index
+                                      // must not hide a wait that ran out later)
   unsigned long long wait_budget_ns;  // %globaltimer budget of one bounded wait
 };
 
@@ -41,6 +42,9 @@ __device__ __forceinline__ uint64_t tp_globaltimer() {
 
 __device__ __forceinline__ void tp_record_device_error(int* err, int code) {
   if (err) atomicCAS(err, 0, code);
+}
+__device__ __forceinline__ void tp_record_index_error(int* err) {
+  if (err) atomicExch(&reinterpret_cast<TpDeviceStatus*>(err)->index_error, TP_DEVERR_INDEX);
 }
 
 // The wait budget of the status block that `err` belongs to (read when a wait

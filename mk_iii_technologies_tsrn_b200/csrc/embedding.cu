@@ -72,7 +72,7 @@ __global__ void __launch_bounds__(128) embedding_fwd_kernel(const EmbeddingArgs 
         at = a.positions ? load_index(a.positions, a.ids64, i) : i % a.T;
         ok[k] = ok[k] && at >= 0 && at < a.L;
       }
-      if (!ok[k] && t == 0) tp_record_device_error(err, TP_DEVERR_INDEX);
+      if (!ok[k] && t == 0) tp_record_index_error(err);
       wr[k] = (const T*)a.weight + (ok[k] ? id * a.ldw : 0);    // read only if ok
       pr[k] = (const T*)a.pos_weight + (ok[k] ? at * a.ldp : 0);
     }

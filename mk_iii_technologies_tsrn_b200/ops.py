@@ -93,7 +93,8 @@ def check_device_error(device=None, reset: bool = True) -> None:
     Synchronises with the device.  The library's kernels never hang: a wait that
     cannot complete ends after the budget (:func:`set_wait_budget`) and leaves a
     code here, which this call turns into an exception (and clears, unless
-    ``reset`` is False)."""
+    ``reset`` is False).  Where both happened, the wait is raised first and the id
+    by the next call."""
     lib = _lib.load()
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None \
         else torch.device(device)

@@ -79,3 +79,29 @@ def test_wait_budget_bounds(cuda):
     with pytest.raises(RuntimeError):
         ops.set_wait_budget(0.0)
     assert ops.set_wait_budget(2.0) == pytest.approx(2.0)
+
+
+@pytest.mark.parametrize("index_first", [True, False])
+def test_bad_index_and_timed_out_wait_hide_neither(cuda, index_first):
+    """An id outside its table and a wait that ran out are both reported, the wait first."""
+    from mk_iii_technologies_tsrn_b200 import _lib, ops
+    lib = _lib.load()
+    prev = ops.set_wait_budget(1e-3)
+    try:
+        def wait():
+            assert lib.tp_selftest_bounded_wait(0, None, _stream()) == 0
+
+        def index():
+            ops.embedding(torch.tensor([0, 7], device=cuda), torch.ones(3, 4, device=cuda))
+
+        for call in ((index, wait) if index_first else (wait, index)):
+            call()
+        with pytest.raises(ops.DeviceWaitTimeout):
+            ops.check_device_error(cuda, reset=False)
+        with pytest.raises(ops.DeviceWaitTimeout):
+            ops.check_device_error(cuda)
+        with pytest.raises(ops.DeviceIndexError):
+            ops.check_device_error(cuda)
+        ops.check_device_error(cuda)
+    finally:
+        ops.set_wait_budget(prev)
