@@ -865,6 +865,11 @@ TP_API int tp_last_error(void);
  * same process. */
 TP_API int tp_device_error(int reset);
 
+/* TP_DEVERR_INDEX if a kernel on `device` has met an index outside its table since
+ * tp_device_error last returned (and cleared) that, as far as the host has seen,
+ * else 0.  Reads host memory: no CUDA call, no wait.  (No reference counterpart.) */
+TP_API int tp_index_error_seen(int device);
+
 /* Budget of every bounded device-side wait on the current device, in ns of
  * %globaltimer (default 2e9 = 2 s; accepted range [1e3, 6e10]).  Stores the
  * previous budget in *previous when it is not NULL.  Synchronous (a copy to

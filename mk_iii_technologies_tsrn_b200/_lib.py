@@ -248,6 +248,7 @@ SIGNATURES: dict[str, tuple] = {
     ),
     "tp_last_error": (_c_int, []),
     "tp_device_error": (_c_int, [_c_int]),
+    "tp_index_error_seen": (_c_int, [_c_int]),
     "tp_set_wait_budget_ns": (_c_int, [_c_i64, ctypes.POINTER(_c_i64)]),
     "tp_selftest_bounded_wait": (_c_int, [_c_int, _c_p, _c_p]),
 }

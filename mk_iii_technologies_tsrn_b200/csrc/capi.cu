@@ -75,6 +75,34 @@ int* device_error_ptr() {
   return ptrs[dev];
 }
 
+namespace {
+std::atomic<int*> g_index_seen[64];
+}
+
+int* index_error_seen() {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
+  int* p = g_index_seen[dev].load(std::memory_order_acquire);
+  if (p != nullptr) return p;
+  static std::mutex mu;
+  std::lock_guard<std::mutex> lock(mu);
+  p = g_index_seen[dev].load(std::memory_order_acquire);
+  if (p != nullptr) return p;
+  // (the first call may be one that is captured: an allocation that no graph sees)
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) return nullptr;
+  void* q = nullptr;
+  if (cudaHostAlloc(&q, sizeof(int), cudaHostAllocPortable) == cudaSuccess) {
+    p = static_cast<int*>(q);
+    *p = 0;
+    g_index_seen[dev].store(p, std::memory_order_release);
+  } else {
+    cudaGetLastError();
+  }
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  return p;
+}
+
 int num_sms() {
   static std::atomic<int> known[64];
   int dev = 0, n = 148;
@@ -1351,8 +1379,16 @@ int tp_device_error(int reset) {
                            v[0] ? offsetof(TpDeviceStatus, error)
                                 : offsetof(TpDeviceStatus, index_error));
     if (e != cudaSuccess) return -(int)e;
+    int* const seen = v[0] ? nullptr : tp::index_error_seen();
+    if (seen != nullptr) *(volatile int*)seen = 0;
   }
   return v[0] ? v[0] : v[1];
+}
+
+int tp_index_error_seen(int device) {
+  if (device < 0 || device >= 64) return 0;
+  const int* p = tp::g_index_seen[device].load(std::memory_order_acquire);
+  return p != nullptr ? *(const volatile int*)p : 0;
 }
 
 int tp_set_wait_budget_ns(int64_t ns, int64_t* previous) {

@@ -43,8 +43,10 @@ __device__ __forceinline__ uint64_t tp_globaltimer() {
 __device__ __forceinline__ void tp_record_device_error(int* err, int code) {
   if (err) atomicCAS(err, 0, code);
 }
-__device__ __forceinline__ void tp_record_index_error(int* err) {
+// `seen`: a word of host memory (index_error_seen), or NULL
+__device__ __forceinline__ void tp_record_index_error(int* err, int* seen) {
   if (err) atomicExch(&reinterpret_cast<TpDeviceStatus*>(err)->index_error, TP_DEVERR_INDEX);
+  if (seen) *(volatile int*)seen = TP_DEVERR_INDEX;
 }
 
 // The wait budget of the status block that `err` belongs to (read when a wait
@@ -281,6 +283,10 @@ int allow_smem(const void* kernel, size_t bytes);
 // Device address of the library's error word on the current device (resolved
 // once per device with cudaGetSymbolAddress); nullptr if unavailable.
 int* device_error_ptr();
+
+// A word of pinned host memory for the current device, where kernels note a bad index for a
+// host that does not wait for them; nullptr if unavailable.
+int* index_error_seen();
 
 }  // namespace tp
 

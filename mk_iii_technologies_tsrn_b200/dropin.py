@@ -16,7 +16,9 @@ with the tropical parts on this library's kernels:
   kernel (the LF activation fused into the max-plus epilogue);
 * the scaled token embedding with learned positions of the token models
   (:616-720): one kernel, its gradient by sorted tokens (``ops.embedding``; the
-  values are those of the PyTorch expression bit for bit).
+  values are those of the PyTorch expression bit for bit).  An id outside the
+  table makes its rows NaN, and a later call of the model raises
+  ``ops.DeviceIndexError``, where PyTorch's embedding ends the CUDA context.
 
 Everything else (projections, gate, masks, Maslov softmax, layer norms,
 residuals) is the reference's PyTorch expression.  The encoder /
@@ -356,6 +358,7 @@ class _TokenModel(nn.Module):
         if (input_ids.is_cuda and input_ids.dtype in (torch.int32, torch.int64)
                 and _plain_table(tok) and _plain_table(pos) and pos.padding_idx is None
                 and input_ids.device == tok.weight.device == pos.weight.device):
+            ops.raise_seen_index_error(input_ids.device)      # of an earlier call
             return self.embed_drop(ops.embedding(input_ids, tok.weight, self.embed_scale,
                                                  pos_weight=pos.weight,
                                                  padding_idx=tok.padding_idx))

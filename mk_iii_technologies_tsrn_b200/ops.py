@@ -108,6 +108,15 @@ def check_device_error(device=None, reset: bool = True) -> None:
         raise DeviceWaitTimeout(code, dev)
 
 
+def raise_seen_index_error(device: torch.device) -> None:
+    """Raise :class:`DeviceIndexError` (and clear it) if the host has seen by now that an earlier
+    call met an id outside its table.  Waits for nothing unless it raises, and leaves a stream
+    that is being captured alone: for a program's next step, as PyTorch's embedding reports it."""
+    if _lib.load().tp_index_error_seen(device.index or 0) and \
+            not torch.cuda.is_current_stream_capturing():
+        check_device_error(device)
+
+
 def set_wait_budget(seconds: float, device=None) -> float:
     """Set the budget of every bounded device-side wait on ``device`` (default
     2 s) and return the previous one, in seconds.  Synchronous; not during

@@ -238,3 +238,23 @@ def test_two_streams_at_once(cuda):
     for i in range(2):
         for r in got[i]:
             assert all(torch.equal(a, b) for a, b in zip(r, want[i]))
+
+
+def test_bad_ids_stop_a_token_model(cuda):
+    # the call that meets them returns NaN rows; once the device has run it, the next call raises
+    from mk_iii_technologies_tsrn_b200 import dropin, ops
+    m = dropin.TropicalDecoderModel(V, d_model=32, nhead=4, num_layers=1, dim_feedforward=64,
+                                    dropout=0.0, max_seq_len=T).to(cuda)
+    ids = _ids(cuda)
+    bad = ids.clone()
+    bad[1, 3] = V
+    with torch.no_grad():
+        want = m._embed(ids)
+        assert m._embed(bad)[1, 3].isnan().all()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):                  # a capture is left alone
+            m._embed(ids)
+        with pytest.raises(ops.DeviceIndexError):
+            m._embed(ids)
+        assert torch.equal(m._embed(ids), want)
