@@ -762,29 +762,27 @@ __global__ void __launch_bounds__(256) embedding_pos_kernel(int64_t B, int64_t s
   for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
   const int64_t per = (B + 7) / 8, lo = SPLIT ? warp * per : 0;
   const int64_t hi = SPLIT ? min(B, lo + per) : B;
-  if (t < steps && c < D) {
+  if (t < steps) {
     const T* p = dout + (lo * steps + t) * D + c;
     for (int64_t b = lo; b < hi; b += 8) {
+      // eight tokens' ids by one load, a lane each, on their way with the rows
+      int64_t id = 0;
+      if (ids != nullptr && lane < 8 && b + lane < hi)
+        id = load_index(ids, ids64, (b + lane) * steps + t);
       R r[8];
-      bool in[8];
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
         r[u].zero();
-        in[u] = b + u < hi;
-        if (in[u]) {
-          r[u].load(p);
-          if (ids != nullptr) {
-            const int64_t id = load_index(ids, ids64, (b + u) * steps + t);
-            in[u] = id >= 0 && id < V;
-          }
-        }
+        if (b + u < hi && c < D) r[u].load(p);
         p += steps * D;
       }
+      const unsigned in = __ballot_sync(
+          0xffffffffu, b + lane < hi && (ids == nullptr || (id >= 0 && id < V)));
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
         float f[VEC];
         r[u].get(f);
-        if (in[u])
+        if ((in >> u) & 1)
 #pragma unroll
           for (int k = 0; k < VEC; ++k) acc[k] += f[k];
       }
