@@ -69,6 +69,21 @@ Tensor empty_as(const Tensor& t) { return at::empty(t.sizes(), t.options()); }
 Tensor bytes_on(const Tensor& t, int64_t n) {
   return at::empty({n > 16 ? n : 16}, t.options().dtype(at::kByte));
 }
+// Tensors that a transform looks into -- tangents of forward-mode derivatives, and the
+// wrappers of torch.func -- would lose what it puts there: the nodes below know reverse
+// mode alone.
+void no_transforms(std::initializer_list<const Tensor*> ts, const char* what) {
+  const bool forward_mode = c10::AutogradState::get_tls_state().get_fw_grad_mode();
+  for (const Tensor* t : ts) {
+    if (!t->defined()) continue;
+    TORCH_CHECK_NOT_IMPLEMENTED(!forward_mode || !t->_fw_grad(/*level=*/0).defined(), what,
+                                " has no forward-mode derivative");
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->key_set().has_any(c10::DispatchKeySet(
+                                    {c10::DispatchKey::FuncTorchBatched,
+                                     c10::DispatchKey::FuncTorchGradWrapper})),
+                                what, " does not run under the transforms of torch.func");
+  }
+}
 bool any_needs_grad(std::initializer_list<const Tensor*> ts) {
   if (!at::GradMode::is_enabled()) return false;
   for (const Tensor* t : ts)
@@ -257,6 +272,8 @@ std::optional<std::tuple<Tensor, Tensor>> residual_norm(Tensor x, Tensor branch,
                                          int64_t norm, bool branch_norm, bool normalize) {
   const ResidualIn a{x, branch, or_none(gate), or_none(scale), or_none(weight), or_none(bias),
                      or_none(bw), or_none(bb), eps, norm, branch_norm};
+  no_transforms({&a.x, &a.branch, &a.gate, &a.scale, &a.weight, &a.bias, &a.bw, &a.bb},
+                "residual_norm");
   if (!residual_ok(a, normalize)) return std::nullopt;
   if (any_needs_grad({&a.x, &a.branch, &a.gate, &a.scale, &a.weight, &a.bias, &a.bw, &a.bb})) {
     variable_list out = ResidualNorm::apply(x, branch, gate, scale, weight, bias, bw, bb, eps,
@@ -361,6 +378,7 @@ std::optional<std::tuple<Tensor, Tensor>> gated_scan(Tensor gate, Tensor x, Mayb
                                                      Maybe lengths, int64_t form,
                                                      bool need_last) {
   const Tensor first = or_none(h0), ends = or_none(lengths);
+  no_transforms({&gate, &x, &first, &ends}, "gated_scan");
   if (!x.is_cuda() || !is_float(x) || x.dim() != 3 || !alike(gate, x)) return std::nullopt;
   if (first.defined() &&
       (first.device() != x.device() || first.scalar_type() != at::kFloat || first.dim() != 2 ||
@@ -392,6 +410,7 @@ std::tuple<Tensor, Tensor, Tensor> gated_scan_bwd(Tensor states, Maybe dh, Maybe
 }
 
 Maybe gated_scan_step(Tensor gate_, Tensor x_, Tensor state, int64_t form) {
+  no_transforms({&gate_, &x_, &state}, "gated_scan_step");
   if (!x_.is_cuda() || !is_float(x_) || x_.dim() != 2 || !alike(gate_, x_)) return std::nullopt;
   if (state.device() != x_.device() || state.scalar_type() != at::kFloat ||
       state.sizes() != x_.sizes() || (x_.size(1) > 1 && state.stride(1) != 1) ||
@@ -494,6 +513,7 @@ struct Embedding : torch::autograd::Function<Embedding> {
 Maybe embedding(Tensor ids, Tensor weight, Maybe pos_weight, Maybe positions, double scale,
                 int64_t padding) {
   const Tensor pos = or_none(pos_weight), at = or_none(positions);
+  no_transforms({&ids, &weight, &pos, &at}, "embedding");
   if (!weight.is_cuda() || !is_float(weight) || weight.dim() != 2 || !is_index(ids) ||
       ids.device() != weight.device())
     return std::nullopt;

@@ -36,6 +36,7 @@ from typing import Optional
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 
 from . import ops
 from . import tropical
@@ -339,6 +340,12 @@ def _plain_table(m: nn.Module) -> bool:
             and not m._forward_pre_hooks and not m._backward_hooks and not m._backward_pre_hooks)
 
 
+def _transformed(t: torch.Tensor) -> bool:
+    # carries the tangent of a forward-mode derivative, or a wrapper of torch.func
+    return (forward_ad.unpack_dual(t).tangent is not None
+            or torch._C._functorch.is_functorch_wrapped_tensor(t))
+
+
 class _TokenModel(nn.Module):
     # token + learned position embeddings scaled by sqrt(d_model), then an
     # encoder stack with a final norm (the shared body of the two models below)
@@ -357,7 +364,8 @@ class _TokenModel(nn.Module):
         tok, pos = self.embed, self.pos_embed
         if (input_ids.is_cuda and input_ids.dtype in (torch.int32, torch.int64)
                 and _plain_table(tok) and _plain_table(pos) and pos.padding_idx is None
-                and input_ids.device == tok.weight.device == pos.weight.device):
+                and input_ids.device == tok.weight.device == pos.weight.device
+                and not any(map(_transformed, (input_ids, tok.weight, pos.weight)))):
             ops.raise_seen_index_error(input_ids.device)      # of an earlier call
             return self.embed_drop(ops.embedding(input_ids, tok.weight, self.embed_scale,
                                                  pos_weight=pos.weight,

@@ -258,3 +258,85 @@ def test_bad_ids_stop_a_token_model(cuda):
         with pytest.raises(ops.DeviceIndexError):
             m._embed(ids)
         assert torch.equal(m._embed(ids), want)
+
+
+def _calls(cuda):
+    """name -> (call, its differentiable arguments)"""
+    from mk_iii_technologies_tsrn_b200 import ops
+    g = torch.Generator(device=cuda).manual_seed(21)
+    r = lambda *s: torch.randn(*s, device=cuda, generator=g)  # noqa: E731
+    ids = torch.randint(0, 7, (2, 3), device=cuda, generator=g)
+    return {
+        "embedding": (lambda w, p: ops.embedding(ids, w, 2.0, pos_weight=p), (r(7, 8), r(4, 8))),
+        "scan": (lambda z, x, h: ops.gated_scan(z, x, h, form="sigmoid"),
+                 (r(2, 5, 8), r(2, 5, 8), r(2, 8))),
+        "step": (lambda z, x, h: ops.gated_scan_step(z, x, h), (r(2, 8), r(2, 8), r(2, 8))),
+        "residual": (lambda x, b, z, s, w, c, bw, bc: ops.residual_norm(
+            x, b, w, c, gate=z, scale=s, branch_norm=True, branch_weight=bw, branch_bias=bc)[1],
+            (r(3, 8), r(3, 8), r(3, 8), r(8), r(8), r(8), r(8), r(8))),
+    }
+
+
+@pytest.mark.parametrize("name", ["embedding", "scan", "step", "residual"])
+@pytest.mark.parametrize("needs_grad", [False, True])
+def test_forward_mode_is_refused(cuda, name, needs_grad):
+    # a tangent of any argument, of a leaf or not, is never dropped
+    from torch.autograd import forward_ad
+    call, args = _calls(cuda)[name]
+    for i, t in enumerate(args):
+        with forward_ad.dual_level():
+            dual = forward_ad.make_dual(t.clone().requires_grad_(needs_grad), torch.ones_like(t))
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call(*args[:i], dual, *args[i + 1:])
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+                call(*args[:i], dual, *args[i + 1:])
+    call(*args)
+
+
+@pytest.mark.parametrize("name", ["embedding", "scan", "step", "residual"])
+def test_transforms_of_torch_func_are_refused(cuda, name):
+    call, args = _calls(cuda)[name]
+    with pytest.raises(NotImplementedError, match="torch.func"):
+        torch.func.vmap(call)(*(t[None] for t in args))
+    with pytest.raises(NotImplementedError, match="torch.func|forward-mode"):
+        torch.func.jvp(call, args, tuple(torch.ones_like(t) for t in args))
+    with pytest.raises(NotImplementedError, match="torch.func"):
+        torch.func.grad(lambda *a: call(*a).sum())(*args)
+
+
+def test_token_models_keep_the_transforms_of_the_plain_embedding(cuda):
+    # tangents of the tables, vmap over ids, and functional gradients, as the PyTorch expression
+    from torch.autograd import forward_ad
+    from mk_iii_technologies_tsrn_b200 import dropin
+    m = dropin.TropicalDecoderModel(V, d_model=32, nhead=4, num_layers=1, dim_feedforward=64,
+                                    dropout=0.0, max_seq_len=T).to(cuda).eval()
+    ids = _ids(cuda)
+    at = torch.arange(T, device=cuda)
+    w, p = m.embed.weight.detach(), m.pos_embed.weight.detach()
+    plain = lambda w, p, i=ids: w[i] * m.embed_scale + p[at][None]  # noqa: E731
+
+    def functional(w, p, i=ids):
+        old = m.embed.weight, m.pos_embed.weight
+        del m.embed.weight, m.pos_embed.weight
+        m.embed.weight, m.pos_embed.weight = w, p
+        try:
+            return m._embed(i)
+        finally:
+            del m.embed.weight, m.pos_embed.weight
+            m.embed.weight, m.pos_embed.weight = old
+
+    g = torch.Generator(device=cuda).manual_seed(22)
+    tw, tp = (torch.randn(t.shape, device=cuda, generator=g) for t in (w, p))
+    with forward_ad.dual_level():
+        out = functional(forward_ad.make_dual(w, tw), forward_ad.make_dual(p, tp))
+        tangent = forward_ad.unpack_dual(out).tangent
+        assert tangent is not None
+        torch.testing.assert_close(tangent, plain(tw, tp), rtol=1e-6, atol=1e-5)
+    out, tangent = torch.func.jvp(functional, (w, p), (tw, tp))
+    torch.testing.assert_close(tangent, plain(tw, tp), rtol=1e-6, atol=1e-5)
+    got = torch.func.vmap(lambda i: m._embed(i[None])[0])(ids)
+    assert torch.equal(got, plain(w, p))
+    d = torch.randn_like(out)
+    for a, b in zip(torch.func.grad(lambda w, p: (functional(w, p) * d).sum(), (0, 1))(w, p),
+                    torch.func.grad(lambda w, p: (plain(w, p) * d).sum(), (0, 1))(w, p)):
+        torch.testing.assert_close(a, b, rtol=1e-4, atol=1e-4)
