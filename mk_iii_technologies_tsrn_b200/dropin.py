@@ -37,6 +37,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 from torch.autograd import forward_ad
+from torch.nn.modules import module as _module
 
 from . import ops
 from . import tropical
@@ -332,12 +333,19 @@ def make_causal_mask(seq_len: int, device: torch.device) -> torch.Tensor:
 
 
 def _plain_table(m: nn.Module) -> bool:
-    # an nn.Embedding that is only its float32 table: no hooks, parametrisation, renormalisation
-    # or other gradient than the dense sum
+    # an nn.Embedding that is only its float32 table: no hooks, own forward, parametrisation,
+    # renormalisation or other gradient than the dense sum
     return (type(m) is nn.Embedding and type(m.weight) in (nn.Parameter, torch.Tensor)
             and m.weight.dtype == torch.float32 and m.weight.is_cuda and m.max_norm is None
             and not m.sparse and not m.scale_grad_by_freq and not m._forward_hooks
-            and not m._forward_pre_hooks and not m._backward_hooks and not m._backward_pre_hooks)
+            and not m._forward_pre_hooks and not m._backward_hooks and not m._backward_pre_hooks
+            and "forward" not in m.__dict__)
+
+
+def _global_hooks() -> bool:
+    # hooks on every module (module trackers, counters): they want the modules themselves run
+    return bool(_module._global_forward_hooks or _module._global_forward_pre_hooks
+                or _module._global_backward_hooks or _module._global_backward_pre_hooks)
 
 
 def _transformed(t: torch.Tensor) -> bool:
@@ -365,6 +373,7 @@ class _TokenModel(nn.Module):
         if (input_ids.is_cuda and input_ids.dtype in (torch.int32, torch.int64)
                 and _plain_table(tok) and _plain_table(pos) and pos.padding_idx is None
                 and input_ids.device == tok.weight.device == pos.weight.device
+                and not _global_hooks()
                 and not any(map(_transformed, (input_ids, tok.weight, pos.weight)))):
             ops.raise_seen_index_error(input_ids.device)      # of an earlier call
             return self.embed_drop(ops.embedding(input_ids, tok.weight, self.embed_scale,

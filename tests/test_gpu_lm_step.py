@@ -340,3 +340,31 @@ def test_token_models_keep_the_transforms_of_the_plain_embedding(cuda):
     for a, b in zip(torch.func.grad(lambda w, p: (functional(w, p) * d).sum(), (0, 1))(w, p),
                     torch.func.grad(lambda w, p: (plain(w, p) * d).sum(), (0, 1))(w, p)):
         torch.testing.assert_close(a, b, rtol=1e-4, atol=1e-4)
+
+
+@pytest.mark.parametrize("kind", ["forward", "forward_pre", "full_backward", "full_backward_pre"])
+def test_global_module_hooks_see_the_token_models_tables(cuda, kind):
+    from mk_iii_technologies_tsrn_b200 import dropin
+    from torch.nn.modules import module
+    m = dropin.TropicalDecoderModel(V, d_model=32, nhead=4, num_layers=1, dim_feedforward=64,
+                                    dropout=0.0, max_seq_len=T).to(cuda)
+    ids, seen = _ids(cuda), []
+    want = m._embed(ids)
+    h = getattr(module, f"register_module_{kind}_hook")(lambda mod, *a: seen.append(mod) and None)
+    try:
+        x = m._embed(ids)
+        x.sum().backward()
+    finally:
+        h.remove()
+    assert torch.equal(x, want) and m.embed in seen and m.pos_embed in seen
+
+
+def test_a_table_with_a_forward_of_its_own_runs_it(cuda):
+    from mk_iii_technologies_tsrn_b200 import dropin
+    m = dropin.TropicalDecoderModel(V, d_model=32, nhead=4, num_layers=1, dim_feedforward=64,
+                                    dropout=0.0, max_seq_len=T).to(cuda)
+    ids = _ids(cuda)
+    plain = m.embed.forward
+    m.embed.forward = lambda i: plain(i) * 3
+    want = plain(ids) * 3 * m.embed_scale + m.pos_embed(torch.arange(T, device=cuda))[None]
+    assert torch.equal(m._embed(ids), want)
