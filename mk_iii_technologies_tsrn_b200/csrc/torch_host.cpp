@@ -103,12 +103,18 @@ bool alike(const Tensor& t, const Tensor& like) {
                           t.scalar_type() == like.scalar_type() && t.sizes() == like.sizes());
 }
 
-// The gradients that `make` returns, which cannot be differentiated again.
+// The gradients that `make` returns, which cannot be differentiated again.  They depend on
+// the incoming gradients, and on inputs that require a gradient if `on_inputs`: where
+// create_graph=True records a graph of the former, differentiating it raises; of constant
+// incoming gradients no graph is kept, and a warning says so where one was due.
 template <typename F>
-variable_list once(const variable_list& grads, F make) {
+variable_list once(const char* what, const variable_list& grads, bool on_inputs, F make) {
   bool record = false;
   for (const Tensor& g : grads)
     record |= at::GradMode::is_enabled() && g.defined() && g.requires_grad();
+  if (at::GradMode::is_enabled() && on_inputs && !record)
+    TORCH_WARN(what, " has first derivatives only: its gradients, asked for with "
+               "create_graph=True, count as constants in what is differentiated next");
   at::NoGradGuard off;
   variable_list out = make();
   if (!record) return out;
@@ -222,21 +228,38 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
     ctx->saved_data["eps"] = eps;
     ctx->saved_data["norm"] = norm;
     ctx->saved_data["branch_norm"] = branch_norm;
+    // bit i: input i is there; bit 8 + i: it requires a gradient
+    int64_t bits = 0, i = 0;
+    for (const Tensor* t : {&a.x, &a.branch, &a.gate, &a.scale, &a.weight, &a.bias, &a.bw, &a.bb}) {
+      if (t->defined()) bits |= (int64_t)1 << i | (int64_t)t->requires_grad() << (8 + i);
+      ++i;
+    }
+    ctx->saved_data["inputs"] = bits;
     return normalize ? variable_list{y, n} : variable_list{y};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    return once(grads, [&] {
+    const int64_t bits = ctx->saved_data["inputs"].toInt();
+    std::array<bool, 8> need, grad;
+    for (int i = 0, place = 0; i < 8; ++i) {      // (what is not there has no place)
+      need[i] = (bits >> i & 1) && ctx->needs_input_grad(place++);
+      grad[i] = bits >> (8 + i) & 1;
+    }
+    // x, branch, gate, scale, bw and bb enter the second norm's derivative; without it the
+    // product scale * sigmoid(gate) * (N(branch) * bw + bb) is left, linear in each but the
+    // gate and a normalised branch
+    const bool branch_norm = ctx->saved_data["branch_norm"].toBool();
+    const bool in_norm = grads.size() > 1 && grads[1].defined() &&
+                         (grad[0] || grad[1] || grad[2] || grad[3] || grad[6] || grad[7]);
+    const bool in_product = grad[2] || (grad[1] && branch_norm) ||
+                            (grad[3] && (grad[1] || grad[6] || grad[7]));
+    return once("residual_norm", grads, in_norm || in_product, [&] {
       const Tensor dy = grads[0], dn = grads.size() > 1 ? grads[1] : Tensor();
       if (!dy.defined() && !dn.defined()) return variable_list(12);
       const variable_list s = ctx->get_saved_variables();
-      // (tensors that are not there have no place among the inputs)
-      std::array<bool, 8> need;
-      for (int i = 0, place = 0; i < 8; ++i)
-        need[i] = s[i].defined() && ctx->needs_input_grad(place++);
       variable_list out =
           residual_back({s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7],
                          ctx->saved_data["eps"].toDouble(), ctx->saved_data["norm"].toInt(),
-                         ctx->saved_data["branch_norm"].toBool()}, s[8], dy, dn,
+                         branch_norm}, s[8], dy, dn,
                         {need[3], need[4], need[5], need[6], need[7]});
       for (int i = 0; i < 3; ++i)
         if (!need[i]) out[i] = Tensor();
@@ -359,10 +382,12 @@ struct GatedScan : torch::autograd::Function<GatedScan> {
     ctx->save_for_backward({gate, x, ends, states});
     ctx->saved_data["form"] = form;
     ctx->saved_data["h0"] = h0.has_value();
+    ctx->saved_data["gate"] = gate.requires_grad();
     return {h, last};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    return once(grads, [&] {
+    // (linear in x and h0: only the gate is in the others' derivatives)
+    return once("gated_scan", grads, ctx->saved_data["gate"].toBool(), [&] {
       if (!grads[0].defined() && !grads[1].defined()) return variable_list(5);
       const variable_list s = ctx->get_saved_variables();
       const bool need_h0 = ctx->saved_data["h0"].toBool() && ctx->needs_input_grad(2);
@@ -493,7 +518,7 @@ struct Embedding : torch::autograd::Function<Embedding> {
     return embed_run(ids, weight, pos, at, scale);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    return once(grads, [&] {
+    return once("embedding", grads, false, [&] {
       const variable_list s = ctx->get_saved_variables();
       const Tensor dout = grads[0].contiguous();
       variable_list out(6);

@@ -1372,7 +1372,9 @@ def residual_norm(x: torch.Tensor, branch: torch.Tensor, weight: Optional[torch.
     Returns (y, n); n is None with ``normalize=False``.  ``norm``: "layer" (LayerNorm) or
     "rms".  ``x``, ``branch``, ``gate``: [..., D] of one shape, float32 or bfloat16, D at most
     8192, rows at any stride.  ``scale``: None, one learnt number, or [D]; it and the weights and
-    biases are float32 or of x's dtype.  Differentiable in all tensors.  It is the TSRN block's
+    biases are float32 or of x's dtype.  Differentiable in all tensors, once and backwards: second
+    derivatives raise, or warn where ``create_graph=True`` of constant gradients asks for a graph
+    that is not kept; forward mode and torch.func are refused.  It is the TSRN block's
     ``x + branch(ln(x))`` (research/tsrn_dml.py:1096-1106) with TropicalSSM's gate and mix
     (:975-980) and the next LayerNorm."""
     if norm in NORMS:
@@ -1455,7 +1457,7 @@ def gated_scan(gate: torch.Tensor, x: torch.Tensor, h0: Optional[torch.Tensor] =
     ``lengths`` [B]: row b ends after lengths[b] steps; h is zero behind the end and nothing
     there is read.  Returns h [B, T, C] in x's dtype, with ``return_state`` also the float32
     state [B, C] at each row's end (for :func:`gated_scan_step`, or to go on with the next
-    segment).  States are float32 throughout.  Meant for gates of magnitude at most 1: steps are
+    segment).  Differentiable in gate, x and h0 as :func:`residual_norm` is.  States are float32 throughout.  Meant for gates of magnitude at most 1: steps are
     joined by the products of their gates.  Larger gates are right as long as the products of
     consecutive gates stay within float32's range; where one overflows, states behind it are right,
     infinite or NaN, and one that underflows counts as 0."""
@@ -1559,7 +1561,8 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, *,
               padding_idx: Optional[int] = None) -> torch.Tensor:
     """``weight[ids] * scale (+ pos_weight[positions])``, the token embedding of
     ``TropicalEncoderModel`` / ``TropicalDecoderModel`` (tropformer_dropin.py:616-720), in one
-    kernel; differentiable in both tables.
+    kernel; differentiable in both tables (once and backwards; forward mode and torch.func are
+    refused).
 
     ``ids``: int32 or int64 of any shape; ``weight`` [V, D] float32 or bfloat16; ``pos_weight``
     [L, D] of the same dtype.  ``positions`` (None: the index along the last dimension of ids;

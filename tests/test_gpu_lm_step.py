@@ -368,3 +368,52 @@ def test_a_table_with_a_forward_of_its_own_runs_it(cuda):
     m.embed.forward = lambda i: plain(i) * 3
     want = plain(ids) * 3 * m.embed_scale + m.pos_embed(torch.arange(T, device=cuda))[None]
     assert torch.equal(m._embed(ids), want)
+
+
+def test_gradients_taken_as_constants_are_warned_of(cuda):
+    # create_graph=True of constant incoming gradients: a gradient that depends on what requires a
+    # gradient comes without its graph, and a penalty on it would add nothing without a word
+    import warnings
+    from mk_iii_technologies_tsrn_b200 import ops
+    g = torch.Generator(device=cuda).manual_seed(23)
+    shape = (2, 5, 8)
+
+    def ask(call, args, of):
+        ts = [torch.randn(s, device=cuda, generator=g).requires_grad_(k in of)
+              for k, s in enumerate(args)]
+        out = call(*ts)
+        with warnings.catch_warnings(record=True) as seen:
+            warnings.simplefilter("always")
+            torch.autograd.grad(out, [t for t in ts if t.requires_grad], torch.ones_like(out),
+                                create_graph=True, retain_graph=True)
+            torch.autograd.grad(out, [t for t in ts if t.requires_grad][-1:],
+                                torch.ones_like(out), create_graph=True, retain_graph=True)
+            said = sum("first derivatives only" in str(w.message) for w in seen)
+            torch.autograd.grad(out, [t for t in ts if t.requires_grad], torch.ones_like(out))
+            assert said == sum("first derivatives only" in str(w.message) for w in seen)
+        return said
+
+    def scan(z, x, h):
+        return ops.gated_scan(z, x, h, form="sigmoid")
+
+    def norm(x, b, w, c):
+        return ops.residual_norm(x, b, w, c)[1]
+
+    def product(x, b, z, s):
+        return ops.residual_norm(x, b, gate=z, scale=s, normalize=False)[0]
+
+    def normed(x, b, w):
+        return ops.residual_norm(x, b, branch_norm=True, branch_weight=w, normalize=False)[0]
+
+    sizes = (shape, shape, (2, 8))
+    assert ask(scan, sizes, {0}) == 2 and ask(scan, sizes, {0, 1}) == 2
+    assert ask(scan, sizes, {1, 2}) == 0                     # linear in x and h0
+    assert ask(norm, (shape, shape, (8,), (8,)), {0}) == 2
+    assert ask(norm, (shape, shape, (8,), (8,)), {1, 3}) == 2
+    assert ask(norm, (shape, shape, (8,), (8,)), {2, 3}) == 0
+    sizes = (shape, shape, shape, (8,))
+    assert ask(product, sizes, {2}) == 2 and ask(product, sizes, {1, 3}) == 2
+    assert ask(product, sizes, {0, 1}) == 0 and ask(product, sizes, {0, 3}) == 0
+    assert ask(normed, (shape, shape, (8,)), {1}) == 2 and ask(normed, (shape, shape, (8,)), {2}) == 0
+    ids = torch.randint(0, 7, (2, 3), device=cuda, generator=g)
+    assert ask(lambda w: ops.embedding(ids, w), ((7, 8),), {0}) == 0
