@@ -275,3 +275,12 @@ def test_token_outside_one_table_adds_to_neither_gradient(cuda, dtype, index, B,
         gw, gp = torch.autograd.grad(out, (w, p), d)
         _check_grad(gw, torch.where(bad, -1, ids.long()), dout, V, scale)
         _check_grad(gp, torch.where(bad, -1, where.long()), dout, L, 1.0)
+
+
+def test_padding_counted_from_the_end(cuda):
+    from mk_iii_technologies_tsrn_b200 import ops
+    g = _gen(cuda, 8)
+    ids = torch.randint(0, 6, (50,), device=cuda, generator=g)
+    dout = torch.randn(50, 8, device=cuda, generator=g)
+    for p in (-1, -6, -2):
+        _check_grad(ops.embedding_bwd(ids, dout, 6, padding_idx=p), ids, dout, 6, 1.0, p + 6)

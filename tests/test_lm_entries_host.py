@@ -31,3 +31,15 @@ def test_embedding_gradients_of_both_tables_refuse(lib):
 
     assert pos(V=-1) == -1 and pos(bits=8) == -1 and pos(T=3) == -1 and pos(L=1) == -1
     assert pos(dp=None) == -2 and pos(L=0, T=0) == -1
+
+
+def test_padding_of_the_table_gradient_is_checked():
+    import torch
+
+    from mk_iii_technologies_tsrn_b200 import ops
+    ids, dout = torch.zeros(2, dtype=torch.int64), torch.randn(2, 4)
+    for bad in (5, -6):
+        with pytest.raises(ValueError, match="padding_idx"):
+            ops.embedding_bwd(ids, dout, 5, padding_idx=bad)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        ops.embedding_bwd(ids, dout, 5, padding_idx=-5)
