@@ -284,3 +284,36 @@ def test_padding_counted_from_the_end(cuda):
     dout = torch.randn(50, 8, device=cuda, generator=g)
     for p in (-1, -6, -2):
         _check_grad(ops.embedding_bwd(ids, dout, 6, padding_idx=p), ids, dout, 6, 1.0, p + 6)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N,V", [(40000, 300), (40000, 70000), (40000, 4200000), (262144, 1023),
+                                 (262145, 1023), (300000, 300), (300000, 70000),
+                                 (300000, 4200000)])
+def test_gradient_of_many_tokens(cuda, dtype, N, V):
+    # sorts of one, two and three digits, by a cluster of 16 blocks and by two kernels a digit
+    from mk_iii_technologies_tsrn_b200 import ops
+    g = _gen(cuda, N + V)
+    ids = torch.randint(0, V, (N,), device=cuda, generator=g)
+    ids = torch.where(torch.rand(N, device=cuda, generator=g) < 0.25, V // 2, ids)
+    ids[::1001] = V + 5                                       # in no table
+    dout = torch.randn(N, 4, device=cuda, generator=g).to(dtype)
+    dw = ops.embedding_bwd(ids, dout, V, 1.7)
+    _check_grad(dw, ids, dout, V, 1.7)
+    assert torch.equal(dw, ops.embedding_bwd(ids.int(), dout, V, 1.7))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N", [2367, 2368, 40001])
+@pytest.mark.parametrize("D", [37, 40, 512, 1028])
+def test_forward_of_many_tokens(cuda, dtype, N, D):
+    # four rows at a time, four vectors of a longer row, single channels
+    from mk_iii_technologies_tsrn_b200 import ops
+    g = _gen(cuda, D)
+    ids = torch.randint(0, 999, (N,), device=cuda, generator=g)
+    at = torch.randint(0, 50, (N,), device=cuda, generator=g)
+    w = torch.randn(999, D, device=cuda, generator=g).to(dtype)
+    pos = torch.randn(50, D, device=cuda, generator=g).to(dtype)
+    assert torch.equal(ops.embedding(ids, w, 1.5), _plain(ids, w, 1.5))
+    assert torch.equal(ops.embedding(ids, w, 1.5, pos_weight=pos, positions=at),
+                       _plain(ids, w, 1.5, pos, at))

@@ -334,3 +334,12 @@ def test_the_single_scale_sums_rows_in_64_bits(cuda):
     y, _ = ops.residual_norm(torch.zeros_like(b), b, scale=scale, normalize=False)
     y.backward(torch.ones_like(y))
     assert scale.grad.item() == torch.tensor(3 * R * (1 + 2.0 ** -10), dtype=torch.float64).float()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("R,D", [(12000, 72), (12000, 71), (6000, 1000), (6000, 1001), (3000, 2048),
+                                 (1000, 4099), (1000, 5000)])
+def test_more_rows_than_teams(cuda, dtype, R, D):
+    # teams of a warp and of a block (aligned rows, rows that begin inside 16 bytes, single
+    # channels) take a second row, forwards and backwards: more rows than blocks of one wave
+    _check(*_make(cuda, R, D, dtype, seed=4))
