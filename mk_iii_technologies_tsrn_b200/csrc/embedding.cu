@@ -141,7 +141,9 @@ __device__ __forceinline__ unsigned same_digit(bool in, int d, int bits) {
 }
 
 struct SortPlan {
-  int cluster;      // blocks of sort_cluster_kernel (0: the two-kernel sort)
+  // blocks of sort_cluster_kernel; 0: the two-kernel sort, of more than 2^18 tokens or for
+  // a table of 2^30 rows
+  int cluster;
   int64_t tile;     // tokens per block, a multiple of 32 * SORT_WARPS
   int tiles;
   int passes, bits; // digits per key, bits per digit
@@ -162,9 +164,7 @@ SortPlan sort_plan(int64_t N, int64_t V) {
   }
   p.bits = (bits + p.passes - 1) / p.passes;
   const int64_t unit = 32 * SORT_WARPS;
-  p.tile = 8 * unit;                            // 2048 tokens
-  if (ceil_div(N, p.tile) > SORT_MAX_TILES)
-    p.tile = ceil_div(ceil_div(N, SORT_MAX_TILES), unit) * unit;
+  p.tile = N > 0 ? ceil_div(ceil_div(N, SORT_MAX_TILES), unit) * unit : unit;
   p.tiles = (int)ceil_div(N, p.tile);
   return p;
 }
@@ -255,16 +255,11 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_place_kernel(const SortArgs
     const int b = b0 + threadIdx.x;
     int all = 0, earlier = 0;
     if (b < s.bins) {
-      if (s.tiles == 1) {
-#pragma unroll
-        for (int w = 0; w < SORT_WARPS; ++w) all += s_mem[w * s.bins + b];
-      } else {
 #pragma unroll 8
-        for (int t = 0; t < s.tiles; ++t) {
-          const int n = s.hist[(int64_t)t * s.bins + b];
-          all += n;
-          if (t < (int)blockIdx.x) earlier += n;
-        }
+      for (int t = 0; t < s.tiles; ++t) {
+        const int n = s.hist[(int64_t)t * s.bins + b];
+        all += n;
+        if (t < (int)blockIdx.x) earlier += n;
       }
     }
     int total;
@@ -830,7 +825,7 @@ int sum_lanes(int64_t D, int vec, int64_t* ranges) {
   return (int)(ceil_div(ceil_div(nv, *ranges), (int64_t)32) * 32);
 }
 
-// Teams of a block: at least 128 threads.
+// Teams of a block: as many as make 128 threads, at least one.
 int sum_teams(int lanes) { return lanes >= 128 ? 1 : 128 / lanes; }
 
 struct SumPlan {
@@ -841,7 +836,8 @@ struct SumPlan {
 // 819 of 80 registers where rows stay in those), so
 // that there is one wave of them and each searches its place once; at least 16
 // items each, so that partial sums stay few (two or four waves: the sums of 60 x 4096 tokens
-// 83, 85 and 92 us, their joins 8, 14 and 25 us).  By the sizes alone.
+// 83, 85 and 92 us, their joins 8, 14 and 25 us).  By the sizes alone, for 16 bytes a
+// thread: rows of single channels take the same shares.
 SumPlan sum_plan(int64_t N, int64_t V, int64_t D, int esize) {
   const int64_t items = TOKEN_COST * N + V;
   int64_t ranges;
@@ -1046,13 +1042,11 @@ int launch_embedding_bwd(int dtype, int ids64, int64_t N, int64_t D, const void*
     s.shift = pass * p.bits;
     s.bins = bins;
     s.bits = p.bits;
-    if (p.tiles > 1) {
-      sort_count_kernel<<<(unsigned)p.tiles, SORT_THREADS, sizeof(int) * bins, stream>>>(s);
-      const int st = launch_status();
-      if (st != TP_OK) return st;
-    }
+    sort_count_kernel<<<(unsigned)p.tiles, SORT_THREADS, sizeof(int) * bins, stream>>>(s);
+    int st = launch_status();
+    if (st != TP_OK) return st;
     sort_place_kernel<<<(unsigned)p.tiles, SORT_THREADS, place_smem, stream>>>(s);
-    const int st = launch_status();
+    st = launch_status();
     if (st != TP_OK) return st;
     at ^= 1;
   }

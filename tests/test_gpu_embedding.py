@@ -317,3 +317,20 @@ def test_forward_of_many_tokens(cuda, dtype, N, D):
     assert torch.equal(ops.embedding(ids, w, 1.5), _plain(ids, w, 1.5))
     assert torch.equal(ops.embedding(ids, w, 1.5, pos_weight=pos, positions=at),
                        _plain(ids, w, 1.5, pos, at))
+
+
+def test_gradient_of_a_table_of_2_to_the_30_rows(cuda):
+    # keys of 31 bits: more digits than the cluster's sort takes, with few tokens too
+    from mk_iii_technologies_tsrn_b200 import ops
+    g = _gen(cuda, 9)
+    for N in (1500, 5000):
+        V = 2 ** 30 + 3
+        ids = torch.randint(0, V, (N,), device=cuda, generator=g)
+        ids[::3] = V - 1
+        dout = torch.randint(-8, 9, (N, 1), device=cuda, generator=g).bfloat16()
+        dw = ops.embedding_bwd(ids, dout, V)
+        rows, where = torch.unique(ids, return_inverse=True)
+        want = torch.zeros(len(rows), device=cuda).index_add_(0, where, dout[:, 0].float())
+        assert torch.equal(dw[rows, 0], want.bfloat16())
+        assert int(torch.count_nonzero(dw)) == int(torch.count_nonzero(want))
+        del dw
