@@ -79,28 +79,32 @@ namespace {
 std::atomic<int*> g_index_seen[64];
 }
 
-int* index_error_seen() {
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
-  int* p = g_index_seen[dev].load(std::memory_order_acquire);
-  if (p != nullptr) return p;
+IndexErrorWords index_error_words() {
   static std::mutex mu;
+  static std::atomic<int*> known[64];     // device_error_ptr's, set when both are there
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return {nullptr, nullptr};
+  int* err = known[dev].load(std::memory_order_acquire);
+  if (err != nullptr) return {err, g_index_seen[dev].load(std::memory_order_relaxed)};
+  err = device_error_ptr();
   std::lock_guard<std::mutex> lock(mu);
-  p = g_index_seen[dev].load(std::memory_order_acquire);
-  if (p != nullptr) return p;
-  // (the first call may be one that is captured: an allocation that no graph sees)
-  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-  if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) return nullptr;
-  void* q = nullptr;
-  if (cudaHostAlloc(&q, sizeof(int), cudaHostAllocPortable) == cudaSuccess) {
-    p = static_cast<int*>(q);
-    *p = 0;
-    g_index_seen[dev].store(p, std::memory_order_release);
-  } else {
-    cudaGetLastError();
+  int* seen = g_index_seen[dev].load(std::memory_order_acquire);
+  if (seen == nullptr) {
+    // (the first call may be one that is captured: an allocation that no graph sees)
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) return {err, nullptr};
+    void* q = nullptr;
+    if (cudaHostAlloc(&q, sizeof(int), cudaHostAllocPortable) == cudaSuccess) {
+      seen = static_cast<int*>(q);
+      *seen = 0;
+      g_index_seen[dev].store(seen, std::memory_order_release);
+    } else {
+      cudaGetLastError();
+    }
+    cudaThreadExchangeStreamCaptureMode(&mode);
   }
-  cudaThreadExchangeStreamCaptureMode(&mode);
-  return p;
+  if (seen != nullptr) known[dev].store(err, std::memory_order_release);
+  return {err, seen};
 }
 
 int num_sms() {
@@ -1379,7 +1383,7 @@ int tp_device_error(int reset) {
                            v[0] ? offsetof(TpDeviceStatus, error)
                                 : offsetof(TpDeviceStatus, index_error));
     if (e != cudaSuccess) return -(int)e;
-    int* const seen = v[0] ? nullptr : tp::index_error_seen();
+    int* const seen = v[0] ? nullptr : tp::index_error_words().seen;
     if (seen != nullptr) *(volatile int*)seen = 0;
   }
   return v[0] ? v[0] : v[1];

@@ -43,7 +43,7 @@ __device__ __forceinline__ uint64_t tp_globaltimer() {
 __device__ __forceinline__ void tp_record_device_error(int* err, int code) {
   if (err) atomicCAS(err, 0, code);
 }
-// `seen`: a word of host memory (index_error_seen), or NULL
+// `seen`: a word of host memory (index_error_words), or NULL
 __device__ __forceinline__ void tp_record_index_error(int* err, int* seen) {
   if (err) atomicExch(&reinterpret_cast<TpDeviceStatus*>(err)->index_error, TP_DEVERR_INDEX);
   if (seen) *(volatile int*)seen = TP_DEVERR_INDEX;
@@ -284,9 +284,13 @@ int allow_smem(const void* kernel, size_t bytes);
 // once per device with cudaGetSymbolAddress); nullptr if unavailable.
 int* device_error_ptr();
 
-// A word of pinned host memory for the current device, where kernels note a bad index for a
-// host that does not wait for them; nullptr if unavailable.
-int* index_error_seen();
+// device_error_ptr, and a word of pinned host memory for the current device, where kernels
+// note a bad index for a host that does not wait for them; nullptr if unavailable.
+struct IndexErrorWords {
+  int* error;
+  int* seen;
+};
+IndexErrorWords index_error_words();
 
 }  // namespace tp
 

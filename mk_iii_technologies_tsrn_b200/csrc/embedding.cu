@@ -53,7 +53,7 @@ __device__ __forceinline__ int64_t load_index(const void* p, int is64, int64_t i
 // that their loads are under way together.
 template <typename T, int VEC, int TOK, int UV>
 __global__ void __launch_bounds__(128) embedding_fwd_kernel(const EmbeddingArgs a, int lanes,
-                                                            int* err, int* seen) {
+                                                            const IndexErrorWords bad) {
   using V = RowVec<T, VEC>;
   const int t = threadIdx.x % lanes, per = blockDim.x / lanes;
   const int64_t nv = a.D / VEC;
@@ -72,7 +72,7 @@ __global__ void __launch_bounds__(128) embedding_fwd_kernel(const EmbeddingArgs 
         at = a.positions ? load_index(a.positions, a.ids64, i) : i % a.T;
         ok[k] = ok[k] && at >= 0 && at < a.L;
       }
-      if (!ok[k] && t == 0) tp_record_index_error(err, seen);
+      if (!ok[k] && t == 0) tp_record_index_error(bad.error, bad.seen);
       wr[k] = (const T*)a.weight + (ok[k] ? id * a.ldw : 0);    // read only if ok
       pr[k] = (const T*)a.pos_weight + (ok[k] ? at * a.ldp : 0);
     }
@@ -900,14 +900,14 @@ Workspace layout(int64_t N, int64_t V, int64_t D, int esize, void* base) {
 // four rows; 16 x 2048 of 512: 18 and 15 us).
 template <typename T, int VEC>
 int fwd_rows(const EmbeddingArgs& a, cudaStream_t stream) {
-  int *const err = device_error_ptr(), *const seen = index_error_seen();
+  const IndexErrorWords bad = index_error_words();
   const bool many = a.N >= 16 * (int64_t)num_sms(), rows = many && a.D / VEC <= 64;
   const int lanes = many ? 32 : 128;
   const int64_t want = ceil_div(a.N, rows ? (int64_t)16 : (many ? (int64_t)4 : (int64_t)1));
   const int64_t cap = (int64_t)num_sms() * 64;
   const unsigned grid = (unsigned)(want < cap ? want : cap);
-  if (rows) embedding_fwd_kernel<T, VEC, 4, 1><<<grid, 128, 0, stream>>>(a, lanes, err, seen);
-  else embedding_fwd_kernel<T, VEC, 1, 4><<<grid, 128, 0, stream>>>(a, lanes, err, seen);
+  if (rows) embedding_fwd_kernel<T, VEC, 4, 1><<<grid, 128, 0, stream>>>(a, lanes, bad);
+  else embedding_fwd_kernel<T, VEC, 1, 4><<<grid, 128, 0, stream>>>(a, lanes, bad);
   return launch_status();
 }
 

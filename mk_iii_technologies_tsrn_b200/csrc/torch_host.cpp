@@ -73,15 +73,16 @@ Tensor bytes_on(const Tensor& t, int64_t n) {
 // wrappers of torch.func -- would lose what it puts there: the nodes below know reverse
 // mode alone.
 void no_transforms(std::initializer_list<const Tensor*> ts, const char* what) {
-  const bool forward_mode = c10::AutogradState::get_tls_state().get_fw_grad_mode();
+  constexpr c10::DispatchKeySet wrapped =
+      c10::DispatchKeySet(c10::DispatchKey::FuncTorchBatched) |
+      c10::DispatchKeySet(c10::DispatchKey::FuncTorchGradWrapper);
   for (const Tensor* t : ts) {
     if (!t->defined()) continue;
-    TORCH_CHECK_NOT_IMPLEMENTED(!forward_mode || !t->_fw_grad(/*level=*/0).defined(), what,
-                                " has no forward-mode derivative");
-    TORCH_CHECK_NOT_IMPLEMENTED(!t->key_set().has_any(c10::DispatchKeySet(
-                                    {c10::DispatchKey::FuncTorchBatched,
-                                     c10::DispatchKey::FuncTorchGradWrapper})),
-                                what, " does not run under the transforms of torch.func");
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->key_set().has_any(wrapped), what,
+                                " does not run under the transforms of torch.func");
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->_fw_grad(/*level=*/0).defined() ||
+                                    !c10::AutogradState::get_tls_state().get_fw_grad_mode(),
+                                what, " has no forward-mode derivative");
   }
 }
 bool any_needs_grad(std::initializer_list<const Tensor*> ts) {

@@ -1499,10 +1499,8 @@ def _index(t: torch.Tensor, what: str) -> None:
         raise TypeError(f"{what} must be int32 or int64, got {t.dtype}")
 
 
-def _padding(padding_idx: Optional[int], rows: int) -> int:
-    """padding_idx counted from the front, -1 for none."""
-    if padding_idx is None:
-        return -1
+def _padding(padding_idx: int, rows: int) -> int:
+    """padding_idx counted from the front."""
     if not -rows <= padding_idx < rows:
         raise ValueError(f"padding_idx {padding_idx} is outside a table of {rows} rows")
     return padding_idx % rows
@@ -1547,7 +1545,7 @@ def embedding_bwd(ids, dout, rows: int, scale: float = 1.0, *,
     ``scale`` times the float32 sum of the rows of dout whose id is v, in the order of the tokens
     (the same bits on every call); absent rows and ``padding_idx`` are zero.  Ids outside the table
     add nothing (a token left out for its position is the caller's to mask)."""
-    padding = _padding(padding_idx, rows)
+    padding = -1 if padding_idx is None else _padding(padding_idx, rows)
     _require_cuda(ids, dout)
     _floating(dout, "dout")
     _index(ids, "ids")
@@ -1580,7 +1578,7 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, *,
     as the unfused expression; bfloat16 rounds once.  A token whose id or position is outside its
     table gets a row of NaN and adds to neither table's gradient, and :func:`check_device_error`
     raises :class:`DeviceIndexError`."""
-    padding = _padding(padding_idx, weight.shape[0] if weight.dim() else 0)
+    padding = -1 if padding_idx is None else _padding(padding_idx, weight.shape[0])
     call = _lib.host().embedding
     out = call(ids, weight, pos_weight, positions, scale, padding)
     if out is None:      # positions to be expanded or converted, or something wrong
