@@ -30,11 +30,12 @@
 // 3. join: a table row whose tokens reach over several shares left fp32
 //    partial sums in the workspace; they are added in order.
 //
-// Measured, of the bytes each has to move at the card's copy rate: the forward of
-// 32 x 4096 tokens of 1024 bf16 channels 59 us, its gradient for 131072 rows 150 us
-// (sum 111), together 149 us of bytes; 64 x 1024 tokens of 640 fp32 channels with
-// 256 rows 32 and 67 us, 52 us of bytes.  The sort is a chain of
-// exchanges over few blocks, and the sum's rows come in the order of the ids.
+// Measured: the forward of 32 x 4096 tokens of 1024 bf16 channels 59 us, its gradient
+// for 131072 rows 146 us (sum 111), together 133 us of bytes at the card's copy rate (of
+// ids that fall off as 1 / rank 32600 rows are met); 64 x 1024 tokens of 640 fp32
+// channels with 256 rows 33 and 65 us, 52 us of bytes.  There the sort (13 us) is a
+// chain of exchanges over 16 blocks, the sum runs at half of the DRAM's rate with 19
+// warps on an SM, and the join waits for its partial rows.
 #include <initializer_list>
 
 #include "maxplus_internal.cuh"

@@ -708,8 +708,8 @@ int bwd(const GatedScanBwdArgs& g, cudaStream_t stream) {
 
 // Two channels per lane where rows begin on a pair, with 16-byte copies where they
 // begin on 16 bytes, else one channel per lane (16 x 4096 bf16, sigmoid, forward and
-// backward: 1024 channels 76 and 160 us, 1020: 106 and 196,
-// 1023: 195 and 387 us; the backward of fp32 pairs copied one by one is slower than
+// backward: 1024 channels 80 and 166 us, 1020: 110 and 201,
+// 1023: 195 and 389 us; the backward of fp32 pairs copied one by one is slower than
 // single channels, 16 x 4096 x 1022: 368 against 324 us).
 template <typename T, int FORM>
 int fwd_any(const GatedScanArgs& a, cudaStream_t stream) {

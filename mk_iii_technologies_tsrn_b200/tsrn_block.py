@@ -20,10 +20,12 @@ block's order without the non-tropical ones between them (sheaf diffusion,
 Clifford FFN, p-adic modules).  With ``fused_residual`` the residual sums, the
 SSM's output gate and mix, and the LayerNorms between the branches run as one
 kernel each (``ops.residual_norm``; the LayerNorms' rounding then differs from
-PyTorch's in the last bits).  ``ssm="gated"`` takes :class:`~.ssm.GatedSSM` in
-place of the tropical SSM.  :func:`swap_into` instead puts this library's
-modules into a reference ``TSRNBlock`` in place, with the same weights, so the
-reference model itself runs its tropical branches on these kernels.
+PyTorch's in the last bits, and forward hooks on the LayerNorms and on the SSM
+do not run: their weights are read, the modules are not called).
+``ssm="gated"`` takes :class:`~.ssm.GatedSSM` in place of the tropical SSM.
+:func:`swap_into` instead puts this library's modules into a reference
+``TSRNBlock`` in place, with the same weights, so the reference model itself runs
+its tropical branches on these kernels.
 """
 from __future__ import annotations
 
