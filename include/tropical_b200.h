@@ -425,7 +425,7 @@ TP_API int tp_gated_scan_step(int dtype, int form, int64_t B, int64_t C, const v
  *  position table at given positions is the same call (scale 1).
  *
  *  tp_embedding_pos_bwd: dpos[t] = sum of dout[b * T + t] over b for t < T, zeros
- *  in the other rows of [L, D] (positions NULL).
+ *  in the other rows of [L, D] (positions NULL; fewer than 2^31 - 64 sequences).
  *
  *  These two look at one table's indices.  With both tables a token outside
  *  either one must add to neither gradient (its row of out was NaN, and so is its

@@ -73,7 +73,13 @@ def _host_target() -> str:
     """The torch and Python whose headers and ABI the host module is compiled against."""
     from importlib import metadata
 
-    return f"torch {metadata.version('torch')} {sys.implementation.cache_tag}\n"
+    try:
+        version = metadata.version("torch")
+    except metadata.PackageNotFoundError:      # a torch that was not installed as a package
+        import torch
+
+        version = torch.__version__
+    return f"torch {version} {sys.implementation.cache_tag}\n"
 
 
 def needs_host_build() -> bool:

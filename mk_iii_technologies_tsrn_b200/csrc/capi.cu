@@ -988,7 +988,8 @@ int tp_embedding_pos_bwd_both(int dtype, int64_t N, int64_t T, int64_t D, const 
   TP_RETURN_IF(dtype != TP_DTYPE_F32 && dtype != TP_DTYPE_BF16, TP_ERR_UNSUPPORTED);
   TP_RETURN_IF(ids != nullptr && index_bits != 32 && index_bits != 64, TP_ERR_INVALID_ARG);
   TP_RETURN_IF(N > 0 && (T < 1 || N % T != 0 || T > L), TP_ERR_INVALID_ARG);
-  TP_RETURN_IF(L > INT32_MAX || D > (int64_t)65535 * 32, TP_ERR_TOO_LARGE);
+  TP_RETURN_IF(L > INT32_MAX || D > (int64_t)65535 * 32 || (N > 0 && N / T > INT32_MAX - 64),
+               TP_ERR_TOO_LARGE);
   if (L == 0 || D == 0) return TP_OK;
   TP_CHECK_PTR(dpos);
   if (N > 0) {
@@ -1371,20 +1372,26 @@ int tp_set_smooth_fused(int enable) { return g_smooth_fused.exchange(enable ? 1 
 int tp_last_error(void) { return last_error(); }
 
 int tp_device_error(int reset) {
+  // (a kernel on a stream of its own may note an index between the two copies: what the
+  // host word says counts as well)
   int v[2] = {0, 0};
   static_assert(offsetof(TpDeviceStatus, index_error) ==
                     offsetof(TpDeviceStatus, error) + sizeof(int), "");
   cudaError_t e =
       cudaMemcpyFromSymbol(v, g_tp_status, sizeof(v), offsetof(TpDeviceStatus, error));
   if (e != cudaSuccess) return -(int)e;
+  int dev = 0;
+  int* const seen = cudaGetDevice(&dev) == cudaSuccess && dev < 64
+                        ? tp::g_index_seen[dev].load(std::memory_order_acquire)
+                        : nullptr;
+  if (seen != nullptr && *(const volatile int*)seen) v[1] = TP_DEVERR_INDEX;
   if (reset && (v[0] || v[1])) {        // the word that is returned, not the other one
     const int zero = 0;
     e = cudaMemcpyToSymbol(g_tp_status, &zero, sizeof(int),
                            v[0] ? offsetof(TpDeviceStatus, error)
                                 : offsetof(TpDeviceStatus, index_error));
     if (e != cudaSuccess) return -(int)e;
-    int* const seen = v[0] ? nullptr : tp::index_error_words().seen;
-    if (seen != nullptr) *(volatile int*)seen = 0;
+    if (seen != nullptr && !v[0]) *(volatile int*)seen = 0;
   }
   return v[0] ? v[0] : v[1];
 }

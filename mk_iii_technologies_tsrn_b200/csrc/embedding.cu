@@ -762,7 +762,7 @@ __global__ void __launch_bounds__(256, IDS ? 3 : 1) embedding_pos_kernel(int64_t
   // (IDS: lanes behind the row read its first channels, so that the warp stays together)
   if (t < steps && (IDS || c < D)) {
     const T* p = dout + (lo * steps + t) * D + (!IDS || c < D ? c : 0);
-    const int n = (int)max(hi - lo, (int64_t)0);
+    const int n = (int)max(hi - lo, (int64_t)0);      // (B is held below 2^31 - 64)
     // 32 sequences' ids by one load, a lane each, the next ones on their way with the rows
     int64_t at = (lo + lane) * steps + t;
     bool ahead = false;

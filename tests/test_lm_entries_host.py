@@ -31,6 +31,7 @@ def test_embedding_gradients_of_both_tables_refuse(lib):
 
     assert pos(V=-1) == -1 and pos(bits=8) == -1 and pos(T=3) == -1 and pos(L=1) == -1
     assert pos(dp=None) == -2 and pos(L=0, T=0) == -1
+    assert lib.tp_embedding_pos_bwd(0, 2 ** 31, 1, 8, P, 3, P, None) == -5
 
 
 def test_padding_of_the_table_gradient_is_checked():
