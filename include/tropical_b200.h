@@ -808,6 +808,95 @@ TP_API int tp_scan_bwd_noalloc(int64_t B, int64_t T, int64_t C,
 TP_API int tp_convert_bf16_to_f32(int64_t n, const void* src, float* dst, void* stream);
 
 /* ======================================================================== *
+ *  Decoding: attention of one new token over a paged key-value cache, prompts
+ *  written into it, eviction from it, and sampling of the next token.
+ *
+ *  A cache (tp_paged_cache, a struct in host memory that is read during the call)
+ *  is `pages` pages of `page_size` slots of [heads, channels] keys and as many
+ *  values; the strides of pages, slots and heads are free, channels contiguous.
+ *  Row b of `table` ([B] rows of `table_cols` int32, `table_row` elements apart)
+ *  lists the pages of sequence b: its slot j is slot j % page_size of page
+ *  table[b][j / page_size].  Pages may be read by several sequences; what is
+ *  written (a new token's slot, prompts, evicted rows) must be in pages of one
+ *  sequence.  A length, start or page outside its range is never followed:
+ *  TP_DEVERR_INDEX is noted, that row of an output is NaN (attention), nothing is
+ *  written (append), and the sequence, or a row whose page it is, stays (evict).
+ *
+ *  tp_paged_attention: for b in [0, B), query head h over key head
+ *  h / (H / heads) and the slots j < lengths[b]:
+ *    s_j = scale / tau[h] * ((1 - gate[b,h]) q.k_j + gate[b,h] max_f(q_f + k_jf))
+ *    out = sum_j softmax(s)_j v_j                      (zeros for a length of 0)
+ *  gate NULL: s_j = scale / tau[h] * q.k_j; tau NULL: 1.  key and value (both or
+ *  neither, [B, heads, channels]): the new token's, which count as slot
+ *  lengths[b] - 1 and are stored there.  mass ([B, heads, mass_slots] fp32, rows
+ *  mass_sb and mass_sh apart, or NULL): the softmax weights, summed over a key
+ *  head's query heads, are added to it; a new token's slot is set to its own.
+ *  Slots behind a length are neither read nor written.  H a multiple of heads; channels 1 to 256; fp32
+ *  or bf16 (statistics and sums in fp32).  Workspace: tp_paged_attention_workspace_bytes
+ *  bytes, 16-byte aligned.  The blended score of
+ *  tropformer_dropin.py:236-260 for one token; without a gate grouped-query
+ *  attention.
+ *
+ *  tp_paged_append: key and value [B, T, heads, channels]; token t < counts[b]
+ *  (NULL: T) goes to slot starts[b] + t.  (TropicalKVCache.update,
+ *  tropformer_dropin.py:143-164, without the copy of what is there.)
+ *
+ *  tp_cache_evict: of a sequence with more than `keep` slots, per key head, the
+ *  last `recent` slots stay and of the others those with the most mass, `keep` in
+ *  all (the lower slot of equals; NaN is the most).  Their rows of K and V move to
+ *  the front in order; kept [B, heads, keep] gets their slots (-1 behind a shorter
+ *  sequence's), out their mass (it may be mass).  Lengths are the caller's to lower
+ *  to `keep`: layers share them.  0 <= recent <= keep, keep >= 1.
+ *  (No reference counterpart.)
+ *
+ *  tp_sample_tokens: for each row of logits ([B, V] rows ld apart), with
+ *  w_i = exp((x_i - max) / temperature), in the order of falling x (the lower
+ *  index first of equals; NaN counts as -inf): the first top_k tokens (<= 0: all),
+ *  of those the ones with less than top_p of their weight before them (>= 1: all),
+ *  of those the ones with w >= min_p; the best one always.  token[b] is the first
+ *  kept token by index where the running sum of w passes uniform[b] (in [0, 1))
+ *  times the kept sum; logprob (or NULL) the log of its share of that sum.  A temperature that is not
+ *  above 0 takes the best token.  A row without a finite or +inf logit gives -1.
+ *  temperature, top_p and min_p come as numbers, or as [B] fp32 arrays where the
+ *  pointer is not NULL; top_k as a number or [B] int32.  uniform: fp32 or fp64
+ *  ([B], uniform_bits 32 or 64).  V < 2^19.  Weights below 2^-45 of the best's
+ *  count as 0.  Deterministic.  (No reference counterpart.)
+ * ======================================================================== */
+typedef struct tp_paged_cache {
+  void* k;
+  void* v;
+  int64_t pages, page_size, heads, channels;
+  int64_t k_page, k_slot, k_head; /* strides in elements */
+  int64_t v_page, v_slot, v_head;
+  const int32_t* table;
+  int64_t table_row, table_cols;
+} tp_paged_cache;
+
+TP_API int64_t tp_paged_attention_workspace_bytes(int dtype, int64_t B, int64_t H, int64_t heads,
+                                                  int64_t channels, int64_t slots, int mass);
+TP_API int tp_paged_attention(int dtype, int64_t B, int64_t H, const tp_paged_cache* cache,
+                              const int32_t* lengths, const void* q, int64_t q_sb, int64_t q_sh,
+                              const void* key, int64_t key_sb, int64_t key_sh, const void* value,
+                              int64_t value_sb, int64_t value_sh, const float* gate,
+                              const float* tau, float scale, float* mass, int64_t mass_sb,
+                              int64_t mass_sh, int64_t mass_slots, void* out, void* workspace,
+                              int64_t workspace_bytes, void* stream);
+TP_API int tp_paged_append(int dtype, int64_t B, int64_t T, const tp_paged_cache* cache,
+                           const int32_t* starts, const int32_t* counts, const void* key,
+                           int64_t key_sb, int64_t key_st, int64_t key_sh, const void* value,
+                           int64_t value_sb, int64_t value_st, int64_t value_sh, void* stream);
+TP_API int tp_cache_evict(int dtype, int64_t B, const tp_paged_cache* cache,
+                          const int32_t* lengths, const float* mass, int64_t mass_sb,
+                          int64_t mass_sh, int64_t mass_slots, float* out, int64_t out_sb,
+                          int64_t out_sh, int64_t keep, int64_t recent, int32_t* kept,
+                          void* stream);
+TP_API int tp_sample_tokens(int dtype, int64_t B, int64_t V, const void* logits, int64_t ld,
+                            int uniform_bits, const void* uniform, double temperature,
+                            const float* temperatures, int64_t top_k, const int32_t* top_ks,
+                            double top_p, const float* top_ps, double min_p, const float* min_ps,
+                            int64_t* token, float* logprob, void* stream);
+
+/* ======================================================================== *
  *  Roofline probe: register-only add+max loop measuring the CUDA-core
  *  max-plus term rate.  form 0: FADD + 2-input FMNMX per term;
  *  form 1: packed add.f32x2 + 3-input max per two terms; form 2: form 1 with

@@ -20,6 +20,20 @@ _c_f = ctypes.c_float
 _c_p = ctypes.c_void_p
 _c_bool = ctypes.c_bool
 
+
+
+class PagedCache(ctypes.Structure):
+    """``tp_paged_cache``: a paged key-value cache, strides in elements."""
+
+    _fields_ = [("k", _c_p), ("v", _c_p),
+                *((name, _c_i64) for name in ("pages", "page_size", "heads", "channels", "k_page",
+                                              "k_slot", "k_head", "v_page", "v_slot", "v_head")),
+                ("table", _c_p), ("table_row", _c_i64), ("table_cols", _c_i64)]
+
+
+_c_cache = ctypes.POINTER(PagedCache)
+_c_d = ctypes.c_double
+
 # name -> (restype, [argtypes])
 SIGNATURES: dict[str, tuple] = {
     "tp_status_string": (ctypes.c_char_p, [_c_int]),
@@ -199,6 +213,28 @@ SIGNATURES: dict[str, tuple] = {
     "tp_embedding_pos_bwd_both": (
         _c_int,
         [_c_int, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_p, _c_int, _c_i64, _c_p, _c_p],
+    ),
+    "tp_paged_attention_workspace_bytes": (
+        _c_i64, [_c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_int]),
+    "tp_paged_attention": (
+        _c_int,
+        [_c_int, _c_i64, _c_i64, _c_cache, _c_p, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p,
+         _c_i64, _c_i64, _c_p, _c_p, _c_f, _c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_p, _c_i64, _c_p],
+    ),
+    "tp_paged_append": (
+        _c_int,
+        [_c_int, _c_i64, _c_i64, _c_cache, _c_p, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_i64,
+         _c_i64, _c_i64, _c_p],
+    ),
+    "tp_cache_evict": (
+        _c_int,
+        [_c_int, _c_i64, _c_cache, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_i64,
+         _c_i64, _c_i64, _c_p, _c_p],
+    ),
+    "tp_sample_tokens": (
+        _c_int,
+        [_c_int, _c_i64, _c_i64, _c_p, _c_i64, _c_int, _c_p, _c_d, _c_p, _c_i64, _c_p, _c_d, _c_p,
+         _c_d, _c_p, _c_p, _c_p, _c_p],
     ),
     "tp_tsrn_attention_fwd": (
         _c_int,

@@ -1,0 +1,552 @@
+// sampling.cu -- the next token of a language model from its logits and one given random
+// number per row:
+//
+//   w_i = exp((x_i - max x) / temperature)
+//   in the order of falling x (the lower index first of equals), keep the tokens that
+//   are among the first top_k, have less than top_p of those' weight before them, and
+//   weigh at least min_p (the best token always)
+//   token = the first kept one, by index, where the running sum passes uniform * total
+//
+// A token is a whole number: a sum that is rounded one way here and another way there
+// gives another token, so the weights are computed in 64 bits and summed as integers,
+// w * 2^44 rounded: sums that no order changes, exact but for half a unit per token (a
+// token below 2^-45 of the best is never taken).
+//
+// A row is a cluster of 1 to 8 blocks that exchange through shared memory.  Its logits
+// are read once from DRAM and then from the L2.  Without top_k and top_p: maximum, sum,
+// then the part of the row where the sum is passed.  With them, the tokens are counted
+// into bins of equal width below the maximum, those of the best bins that make at most
+// CANDIDATES gathered into one block, sorted, and cut off there.  Where that does not
+// reach (flat rows under top_p, top_k above CANDIDATES), the threshold is found bit by
+// bit over all tokens.
+#include <algorithm>
+
+#include "decode.cuh"
+
+namespace tp {
+
+namespace {
+
+constexpr int THREADS = 1024, WARPS = THREADS / 32, BINS = 2048, CANDIDATES = 1024, MAX_CLUSTER = 8;
+constexpr double UNIT = 17592186044416.0;       // 2^44
+constexpr float REACH = 31.5f;                  // w < 2^-45 beyond this many units of temperature
+
+typedef unsigned long long u64;
+
+struct Shared {
+  u64 exchange[2][2][MAX_CLUSTER];
+  u64 reduce[2][WARPS];
+  u64 candidate[CANDIDATES];
+  u64 weight[CANDIDATES];
+  u64 warp_sum[WARPS];
+  int hist[BINS];
+  int warp_ties[WARPS];
+  int count, last_bin, gathered, universe;
+};
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t remote(const void* p, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(tp_smem_addr(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void remote_store(uint32_t at, u64 v) {
+  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(at), "l"(v) : "memory");
+}
+__device__ __forceinline__ void remote_store(uint32_t at, int v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
+}
+__device__ __forceinline__ int remote_load(uint32_t at) {
+  int v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ int remote_add(uint32_t at, int v) {
+  int old;
+  asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(old) : "r"(at), "r"(v) : "memory");
+  return old;
+}
+
+// floats in order as unsigned numbers; NaN counts as -inf
+__device__ __forceinline__ uint32_t key_of(float x) {
+  if (x != x) x = -__int_as_float(0x7f800000);
+  const uint32_t u = __float_as_uint(x + 0.0f);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float value_of(uint32_t key) {
+  return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+}
+
+struct Add {
+  __device__ __forceinline__ u64 operator()(u64 a, u64 b) const { return a + b; }
+};
+struct Max {
+  __device__ __forceinline__ u64 operator()(u64 a, u64 b) const { return a > b ? a : b; }
+};
+
+__device__ __forceinline__ u64 warp_inclusive(u64 v, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o *= 2) {
+    const u64 y = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += y;
+  }
+  return v;
+}
+
+template <typename T>
+struct Row {
+  static constexpr int PER = 16 / sizeof(T);      // tokens of a lane's step, next to one another
+  const T* x;
+  int begin, end;                                 // this warp's part of the row
+  bool vec;
+
+  // f(first index, values, how many) of each step's PER tokens of this lane; the whole warp runs
+  // every step
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+    const int lane = threadIdx.x & 31;
+    for (int i0 = begin; i0 < end; i0 += 32 * PER) {
+      const int i = i0 + lane * PER;
+      const int some = max(0, min(PER, end - i));
+      float v[PER];
+      load(i, some, v);
+      f(i, v, some);
+    }
+  }
+  __device__ __forceinline__ void load(int i, int some, float (&v)[PER]) const {
+    if (vec && some == PER) {
+      const uint4 u = __ldg((const uint4*)(x + i));
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+      if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = __uint_as_float(w[k]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          v[2 * k] = __uint_as_float(w[k] << 16);
+          v[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < PER; ++k) v[k] = k < some ? tp_load_as_f32<T>(x + i + k) : 0.0f;
+    }
+  }
+};
+
+struct Weights {
+  float top;
+  double top64, per;              // the maximum, 1 / temperature
+  __device__ __forceinline__ double real(float x) const {
+    if (x == top) return 1.0;
+    if (!(x > -__int_as_float(0x7f800000))) return 0.0;
+    return exp(((double)x - top64) * per);
+  }
+  __device__ __forceinline__ u64 whole(double w) const { return (u64)__double2ll_rn(w * UNIT); }
+};
+
+template <typename T>
+__global__ void __launch_bounds__(THREADS) sample_kernel(const SampleArgs a, int cluster) {
+  __shared__ Shared s;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t rank = cluster_rank();
+  const int64_t b = blockIdx.x / cluster;
+  const int V = (int)a.V;
+
+  Row<T> row;
+  row.x = (const T*)a.logits + b * a.ld;
+  row.vec = (((uintptr_t)row.x) & 15) == 0;
+  {
+    constexpr int P = Row<T>::PER;
+    const int parts = cluster * WARPS;
+    const int per = ((V + parts - 1) / parts + P - 1) / P * P;
+    const int64_t begin = (int64_t)((int)rank * WARPS + warp) * per;
+    row.begin = (int)min((int64_t)V, begin);
+    row.end = (int)min((int64_t)V, begin + per);
+  }
+
+  // Sum (or maximum) of v over the cluster's threads.  Two calls' slots never meet: a block is
+  // past a call's barrier only when all have read the one before.
+  int calls = 0;
+  auto all = [&](u64 v, int which, auto op) {
+#pragma unroll
+    for (int o = 16; o > 0; o /= 2) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
+    if (lane == 0) s.reduce[which][warp] = v;
+  };
+  auto finish = [&](int which, auto op) {         // after a __syncthreads: one warp, to every block
+    u64 v = s.reduce[which][lane];
+#pragma unroll
+    for (int o = 16; o > 0; o /= 2) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
+    if (lane < cluster) remote_store(remote(&s.exchange[calls & 1][which][rank], lane), v);
+  };
+  auto joined = [&](int which, auto op) {
+    u64 v = 0;
+    for (int r = 0; r < cluster; ++r) v = op(v, s.exchange[calls & 1][which][r]);
+    return v;
+  };
+  auto reduce = [&](u64 v, auto op) {
+    all(v, 0, op);
+    __syncthreads();
+    if (warp == 0) finish(0, op);
+    cluster_sync();
+    const u64 r = joined(0, op);
+    ++calls;
+    return r;
+  };
+
+  // ---- the best token
+  if (tid == 0) s.count = 0;
+  for (int i = tid; i < BINS; i += THREADS) s.hist[i] = 0;
+  u64 best = 0;
+  row.each([&](int i, const float* v, int some) {
+    for (int k = 0; k < some; ++k) {
+      const u64 c = (u64)key_of(v[k]) << 32 | (0xffffffffu - (uint32_t)(i + k));
+      best = c > best ? c : best;
+    }
+  });
+  best = reduce(best, Max());
+  Weights wt;
+  wt.top = value_of((uint32_t)(best >> 32));
+  const int first = (int)(0xffffffffu - (uint32_t)best);
+  const double temperature = a.temperature.of_row ? (double)a.temperature.of_row[b] : a.temperature.all;
+  const double top_p = a.top_p.of_row ? (double)a.top_p.of_row[b] : a.top_p.all;
+  const double min_p = a.min_p.of_row ? (double)a.min_p.of_row[b] : a.min_p.all;
+  const int64_t asked = a.top_k_of_row ? (int64_t)a.top_k_of_row[b] : a.top_k;
+  const bool by_k = asked > 0 && asked < V, by_p = top_p < 1.0;
+  const int top_k = by_k ? (int)asked : V;
+  const bool leader = rank == 0 && tid == 0;
+  if (wt.top == -__int_as_float(0x7f800000)) {                   // nothing to take
+    if (leader) {
+      a.token[b] = -1;
+      if (a.logprob) a.logprob[b] = __int_as_float(0x7fc00000);
+    }
+    return;
+  }
+  if (!(temperature > 0.0) || top_k == 1 || top_p <= 0.0 || min_p > 1.0) {
+    if (leader) {
+      a.token[b] = first;
+      if (a.logprob) a.logprob[b] = 0.0f;
+    }
+    return;
+  }
+  wt.top64 = (double)wt.top;
+  wt.per = 1.0 / temperature;
+  const double u = a.uniform64 ? ((const double*)a.uniform)[b] : (double)((const float*)a.uniform)[b];
+  // the place in the running sum: the first token whose sum is above it
+  auto place = [&](u64 total) {
+    const double t = u * (double)total;
+    return t >= 0.0 && t < (double)total ? min((u64)t, total - 1) : (t < 0.0 ? 0ull : total - 1);
+  };
+  auto write = [&](int token, float x, u64 total) {
+    a.token[b] = token;
+    if (a.logprob)
+      a.logprob[b] = (float)((x == wt.top ? 0.0 : ((double)x - wt.top64) * wt.per) - log((double)total / UNIT));
+  };
+
+  uint32_t cut = 0;                     // kept: keys above it, and the first `ties` equal to it
+  int64_t ties = INT64_MAX;
+  if (by_k || by_p) {
+    // ---- bins below the maximum
+    const float reach = (float)(REACH * temperature), bins_per = (float)(BINS / (REACH * temperature));
+    auto bin_of = [&](float x) {        // BINS: weighs nothing
+      if (x == wt.top) return 0;
+      const float d = wt.top - x;
+      return d < reach ? min(BINS - 1, (int)(d * bins_per)) : BINS;
+    };
+    row.each([&](int i, const float* v, int some) {
+      for (int k = 0; k < some; ++k) {
+        const int bin = bin_of(v[k]);
+        if (bin < BINS) atomicAdd(&s.hist[bin], 1);
+      }
+    });
+    cluster_sync();
+    if (rank == 0) {                    // the bins that are gathered
+      int mine[2] = {0, 0};
+      for (int r = 0; r < cluster; ++r)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) mine[k] += remote_load(remote(&s.hist[2 * tid + k], r));
+      const int sum = mine[0] + mine[1];
+      int at = (int)warp_inclusive(sum, lane);
+      if (lane == 31) s.warp_ties[warp] = at;
+      if (tid == 0) {
+        s.last_bin = -1;
+        s.gathered = 0;
+      }
+      __syncthreads();
+      int before = 0, everything = 0;
+      for (int w = 0; w < WARPS; ++w) {
+        before += w < warp ? s.warp_ties[w] : 0;
+        everything += s.warp_ties[w];
+      }
+      at += before;                     // tokens up to this thread's second bin
+      // the fewest that hold the first top_k; under top_p alone as many as there is room for
+      const int want = by_k ? min(top_k, everything) : CANDIDATES + 1;
+      int to = -1;
+      if (at - mine[1] <= CANDIDATES && at - sum < want) to = 2 * tid;
+      if (at <= CANDIDATES && at - mine[1] < want) to = 2 * tid + 1;
+      if (to >= 0) atomicMax(&s.last_bin, to);
+      __syncthreads();
+      if (to >= 0 && to == s.last_bin) s.gathered = (to & 1) ? at : at - mine[1];
+      __syncthreads();
+      if (tid > 0 && tid < cluster) {
+        remote_store(remote(&s.last_bin, tid), s.last_bin);
+        remote_store(remote(&s.gathered, tid), s.gathered);
+      }
+      if (tid < cluster) remote_store(remote(&s.universe, tid), everything);
+    }
+    cluster_sync();
+    const int last_bin = s.last_bin, universe = s.universe;
+    // ---- gather them; under top_p alone the weight of all is wanted too
+    u64 sum_all = 0, sum_some = 0;
+    row.each([&](int i, const float* v, int some) {
+      for (int k = 0; k < Row<T>::PER; ++k) {
+        const int bin = k < some ? bin_of(v[k]) : BINS;
+        const bool take = bin <= last_bin;
+        const uint32_t takers = __ballot_sync(0xffffffffu, take);
+        if (takers) {
+          int at = 0;
+          if (lane == __ffs(takers) - 1) at = remote_add(remote(&s.count, 0), __popc(takers));
+          at = __shfl_sync(0xffffffffu, at, __ffs(takers) - 1) + __popc(takers & ((1u << lane) - 1));
+          if (take)
+            remote_store(remote(&s.candidate[at], 0),
+                         (u64)key_of(v[k]) << 32 | (0xffffffffu - (uint32_t)(i + k)));
+        }
+        if (!by_k && bin < BINS) {
+          const u64 w = wt.whole(wt.real(v[k]));
+          sum_all += w;
+          sum_some += take ? w : 0;
+        }
+      }
+    });
+    all(sum_all, 0, Add());
+    all(sum_some, 1, Add());
+    __syncthreads();
+    if (warp == 0) {
+      finish(0, Add());
+      finish(1, Add());
+    }
+    cluster_sync();
+    sum_all = joined(0, Add());
+    sum_some = joined(1, Add());
+    ++calls;
+    const int count = s.gathered;
+    const bool enough = by_k ? count >= min(top_k, universe)
+                             : count == universe || (double)sum_some >= top_p * (double)sum_all;
+    if (enough) {
+      if (rank != 0) return;
+      // ---- sort, cut off, sort by index, find the place
+      auto sort = [&](u64 v, int n) {   // falling; threads from n on hold zeros
+        for (int k = 2; k <= n; k *= 2)
+          for (int j = k / 2; j > 0; j /= 2) {
+            u64 other;
+            if (j >= 32) {
+              s.candidate[tid] = v;
+              __syncthreads();
+              other = s.candidate[tid ^ j];
+              __syncthreads();
+            } else {
+              other = __shfl_xor_sync(0xffffffffu, v, j);
+            }
+            const bool larger = ((tid & j) == 0) == ((tid & k) == 0);
+            v = (v > other) == larger ? v : other;
+          }
+        return v;
+      };
+      auto scan = [&](u64 w) {          // inclusive over the block
+        u64 at = warp_inclusive(w, lane);
+        if (lane == 31) s.warp_sum[warp] = at;
+        __syncthreads();
+        for (int k = 0; k < warp; ++k) at += s.warp_sum[k];
+        __syncthreads();
+        return at;
+      };
+      int size = 32;
+      while (size < count) size *= 2;
+      u64 v = tid < count ? s.candidate[tid] : 0;
+      __syncthreads();
+      v = sort(v, size);
+      const bool there = tid < count;
+      const float x = value_of((uint32_t)(v >> 32));
+      const double w = there && tid < top_k ? wt.real(x) : 0.0;
+      const u64 whole = wt.whole(w);
+      const u64 sum = scan(whole);
+      if (tid == THREADS - 1) s.weight[0] = sum;
+      __syncthreads();
+      const u64 share = by_k ? s.weight[0] : sum_all;
+      bool keep = there && tid < top_k && w >= min_p;
+      if (by_p) keep = keep && (double)(sum - whole) < top_p * (double)share;
+      keep = keep || tid == 0;
+      __syncthreads();
+      s.weight[tid] = whole;
+      const uint32_t index = 0xffffffffu - (uint32_t)v;
+      // falling again: the lowest index first; what is not kept last
+      u64 o = keep ? (u64)(0xffffffffu - index) << 32 | (uint32_t)(tid + 1) : 0;
+      o = sort(o, size);
+      __syncthreads();
+      const int from = (int)(uint32_t)o - 1;
+      const u64 ow = from >= 0 ? s.weight[from] : 0;
+      const u64 run = scan(ow);
+      s.candidate[tid] = v;             // (by rank)
+      if (tid == THREADS - 1) s.reduce[0][0] = run;
+      __syncthreads();
+      const u64 total = s.reduce[0][0], t = place(total);
+      if (ow > 0 && run > t && run - ow <= t)
+        write((int)(0xffffffffu - (uint32_t)(o >> 32)), value_of((uint32_t)(s.candidate[from] >> 32)), total);
+      return;
+    }
+    // ---- bit by bit over all tokens
+    auto weigh_from = [&](uint32_t key) {
+      u64 sum = 0;
+      row.each([&](int i, const float* v, int some) {
+        for (int k = 0; k < some; ++k)
+          if (key_of(v[k]) >= key) sum += wt.whole(wt.real(v[k]));
+      });
+      return reduce(sum, Add());
+    };
+    auto count_from = [&](uint32_t key) {
+      u64 sum = 0;
+      row.each([&](int i, const float* v, int some) {
+        for (int k = 0; k < some; ++k) sum += key_of(v[k]) >= key;
+      });
+      return reduce(sum, Add());
+    };
+    // (no key of a token is 2^32 - 1, so that cut + 1 is one)
+    u64 share = sum_all;
+    if (by_k) {
+      for (uint32_t bit = 1u << 31; bit; bit >>= 1)
+        if (count_from(cut | bit) >= (u64)top_k) cut |= bit;
+      ties = top_k - (int64_t)count_from(cut + 1);
+      if (by_p) share = weigh_from(cut + 1) + (u64)ties * wt.whole(wt.real(value_of(cut)));
+    }
+    if (by_p) {
+      const double least = top_p * (double)share;
+      uint32_t p = 0;
+      for (uint32_t bit = 1u << 31; bit; bit >>= 1)
+        if ((double)weigh_from(p | bit) >= least) p |= bit;
+      if (p >= cut) {
+        const u64 above = weigh_from(p + 1), one = wt.whole(wt.real(value_of(p)));
+        // the first of the ties whose sum before it reaches the share is left out
+        int64_t r = one > 0 ? (int64_t)ceil((least - (double)above) / (double)one) : INT64_MAX;
+        r = max(r, (int64_t)1);
+        ties = p > cut ? r : min(ties, r);
+        cut = p;
+      }
+    }
+  }
+
+  // ---- the place among the kept tokens, by index
+  int64_t tie_base = 0;
+  if (ties != INT64_MAX) {
+    u64 mine = 0;
+    row.each([&](int i, const float* v, int some) {
+      for (int k = 0; k < some; ++k) mine += key_of(v[k]) == cut;
+    });
+#pragma unroll
+    for (int o = 16; o > 0; o /= 2) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    __syncthreads();
+    if (lane == 0) s.warp_ties[warp] = (int)mine;
+    (void)reduce(lane == 0 ? mine : 0, Add());
+    for (int w = 0; w < warp; ++w) tie_base += s.warp_ties[w];
+    for (uint32_t r = 0; r < rank; ++r) tie_base += (int64_t)s.exchange[(calls - 1) & 1][0][r];
+  }
+  // weights of a step's tokens; `base`: ties before the step
+  auto kept = [&](int i, const float* v, int some, int64_t& base, u64 (&w)[Row<T>::PER]) {
+    int mine = 0;
+#pragma unroll
+    for (int k = 0; k < Row<T>::PER; ++k) mine += k < some && key_of(v[k]) == cut;
+    int64_t at = base;
+    if (ties != INT64_MAX) {
+      const int upto = (int)warp_inclusive(mine, lane);
+      at += upto - mine;
+      base += __shfl_sync(0xffffffffu, upto, 31);
+    }
+#pragma unroll
+    for (int k = 0; k < Row<T>::PER; ++k) {
+      w[k] = 0;
+      if (k >= some) continue;
+      const uint32_t key = key_of(v[k]);
+      const bool tie = key == cut;
+      if (key > cut || (tie && at < ties)) {
+        const double real = wt.real(v[k]);
+        if (real >= min_p || i + k == first) w[k] = wt.whole(real);
+      }
+      at += tie;
+    }
+  };
+  u64 sum = 0;
+  {
+    int64_t base = tie_base;
+    row.each([&](int i, const float* v, int some) {
+      u64 w[Row<T>::PER];
+      kept(i, v, some, base, w);
+#pragma unroll
+      for (int k = 0; k < Row<T>::PER; ++k) sum += w[k];
+    });
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  __syncthreads();
+  if (lane == 0) s.warp_sum[warp] = sum;
+  const u64 total = reduce(lane == 0 ? sum : 0, Add());
+  u64 before = 0;
+  for (uint32_t r = 0; r < rank; ++r) before += s.exchange[(calls - 1) & 1][0][r];
+  for (int w = 0; w < warp; ++w) before += s.warp_sum[w];
+  const u64 t = place(total);
+  if (!(before <= t && t < before + sum)) return;                // another warp's
+  int64_t base = tie_base;
+  u64 run = before;
+  row.each([&](int i, const float* v, int some) {
+    u64 w[Row<T>::PER], mine = 0;
+    kept(i, v, some, base, w);
+#pragma unroll
+    for (int k = 0; k < Row<T>::PER; ++k) mine += w[k];
+    const u64 upto = run + warp_inclusive(mine, lane);
+    u64 at = upto - mine;
+    if (at <= t && t < upto) {
+#pragma unroll
+      for (int k = 0; k < Row<T>::PER; ++k) {
+        if (at <= t && t < at + w[k]) write(i + k, v[k], total);
+        at += w[k];
+      }
+    }
+    run = __shfl_sync(0xffffffffu, upto, 31);
+  });
+}
+
+template <typename T>
+int sample(const SampleArgs& a, cudaStream_t stream) {
+  // as many blocks for a row as leave its warps a few steps, while two waves of blocks hold all
+  // rows
+  int cluster = 1;
+  while (cluster < MAX_CLUSTER && a.V > (int64_t)cluster * WARPS * 64 * (16 / (int)sizeof(T)) &&
+         a.B * cluster * 2 <= 4 * num_sms())
+    cluster *= 2;
+  TP_RETURN_IF(a.B * cluster > INT32_MAX, TP_ERR_TOO_LARGE);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(a.B * cluster));
+  cfg.blockDim = dim3(THREADS);
+  cfg.stream = stream;
+  cudaLaunchAttribute together;
+  together.id = cudaLaunchAttributeClusterDimension;
+  together.val.clusterDim.x = cluster;
+  together.val.clusterDim.y = 1;
+  together.val.clusterDim.z = 1;
+  cfg.attrs = &together;
+  cfg.numAttrs = 1;
+  return cuda_status(cudaLaunchKernelEx(&cfg, sample_kernel<T>, a, cluster));
+}
+
+}  // namespace
+
+int launch_sample_tokens(const SampleArgs& a, cudaStream_t stream) {
+  return a.dtype == TP_DTYPE_BF16 ? sample<uint16_t>(a, stream) : sample<float>(a, stream);
+}
+
+}  // namespace tp

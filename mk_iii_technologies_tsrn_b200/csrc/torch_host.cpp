@@ -1,5 +1,6 @@
-// torch_host.cpp -- the host side of ops.embedding, ops.gated_scan(_step) and
-// ops.residual_norm: outputs and workspaces, the call of the C entry point on the
+// torch_host.cpp -- the host side of ops.embedding, ops.gated_scan(_step),
+// ops.residual_norm and the decoding operators (ops.paged_attention, paged_append,
+// cache_evict, sample_tokens): outputs and workspaces, the call of the C entry point on the
 // tensors' device and its current stream, and the autograd nodes.
 //
 // These operators are also called on single tokens and small batches, where the
@@ -19,6 +20,8 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
+#include <algorithm>
+#include <cmath>
 #include <optional>
 #include <stdexcept>
 #include <string>
@@ -561,6 +564,182 @@ Tensor embedding_fwd(Tensor ids, Tensor weight, Maybe pos_weight, Maybe position
   return embed_run(ids, weight, or_none(pos_weight), or_none(positions), scale);
 }
 
+// ---------------------------------------------------------------- decoding
+// no two elements of the first dimensions at one address: rows of `row` contiguous elements
+bool rows_apart(const Tensor& t, int64_t row) {
+  for (int64_t i = 0; i + 1 < t.dim(); ++i)
+    if (t.size(i) > 1 && t.stride(i) < row) return false;
+  return true;
+}
+bool is_i32(const Tensor& t, const Tensor& on) {
+  return t.device() == on.device() && t.scalar_type() == at::kInt;
+}
+// [pages, page size, heads, channels] caches of one type, and their table of B rows
+bool paged_ok(const Tensor& k, const Tensor& v, const Tensor& table, int64_t B) {
+  if (!k.is_cuda() || !is_float(k) || k.dim() != 4 || !alike(v, k)) return false;
+  for (const Tensor* t : {&k, &v})
+    if ((t->size(3) > 1 && t->stride(3) != 1) || !rows_apart(*t, t->size(3))) return false;
+  return is_i32(table, k) && table.dim() == 2 && table.size(0) == B &&
+         (table.size(1) <= 1 || table.stride(1) == 1) && k.size(1) > 0;
+}
+tp_paged_cache paged_of(const Tensor& k, const Tensor& v, const Tensor& table) {
+  return {at_(k), at_(v), k.size(0), k.size(1), k.size(2), k.size(3), k.stride(0), k.stride(1),
+          k.stride(2), v.stride(0), v.stride(1), v.stride(2), (const int32_t*)at_(table),
+          table.stride(0), table.size(1)};
+}
+bool lengths_ok(const Tensor& t, const Tensor& on, int64_t B) {
+  return is_i32(t, on) && t.dim() == 1 && t.size(0) == B && t.is_contiguous();
+}
+// [B, heads, slots] float32, slots contiguous
+bool mass_ok(const Tensor& t, const Tensor& k, int64_t B) {
+  return t.device() == k.device() && t.scalar_type() == at::kFloat && t.dim() == 3 &&
+         t.size(0) == B && t.size(1) == k.size(2) && (t.size(2) <= 1 || t.stride(2) == 1) &&
+         rows_apart(t, t.size(2));
+}
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+Maybe paged_attention(Tensor q_, Tensor k, Tensor v, Tensor table, Tensor lengths, Maybe key_,
+                      Maybe value_, std::optional<double> scale, Maybe gate_, Maybe tau_,
+                      Maybe mass_) {
+  Tensor key = or_none(key_), value = or_none(value_), gate = or_none(gate_), tau = or_none(tau_);
+  const Tensor mass = or_none(mass_);
+  no_transforms({&q_, &k, &v, &table, &lengths, &key, &value, &gate, &tau, &mass},
+                "paged_attention");
+  if (q_.dim() != 3 || !paged_ok(k, v, table, q_.size(0))) return std::nullopt;
+  const int64_t B = q_.size(0), H = q_.size(1), D = q_.size(2), heads = k.size(2);
+  if (q_.device() != k.device() || q_.scalar_type() != k.scalar_type() || D != k.size(3) ||
+      D < 1 || D > 256 || heads < 1 || H % heads != 0 || !lengths_ok(lengths, k, B))
+    return std::nullopt;
+  if (key.defined() != value.defined()) return std::nullopt;
+  for (const Tensor* t : {&key, &value})
+    if (t->defined() && (t->device() != k.device() || t->scalar_type() != k.scalar_type() ||
+                         t->sizes() != at::IntArrayRef({B, heads, D})))
+      return std::nullopt;
+  if (gate.defined() && (gate.device() != k.device() || gate.scalar_type() != at::kFloat ||
+                         gate.sizes() != at::IntArrayRef({B, H})))
+    return std::nullopt;
+  if (tau.defined() && (tau.device() != k.device() || tau.scalar_type() != at::kFloat ||
+                        tau.sizes() != at::IntArrayRef({H})))
+    return std::nullopt;
+  if (mass.defined() && !mass_ok(mass, k, B)) return std::nullopt;
+  if (any_needs_grad({&q_, &k, &v, &key, &value, &gate, &tau, &mass})) return std::nullopt;
+  at::NoGradGuard off;
+  const On device(k);
+  const Tensor q = channels(q_);
+  if (key.defined()) {
+    key = channels(key);
+    value = channels(value);
+  }
+  gate = contiguous(gate);
+  tau = contiguous(tau);
+  Tensor out = empty_as(q_);
+  const tp_paged_cache cache = paged_of(k, v, table);
+  int64_t slots = cache.table_cols * cache.page_size;
+  if (mass.defined() && mass.size(2) < slots) slots = mass.size(2);
+  const int64_t need = tp_paged_attention_workspace_bytes(code_of(k), B, H, heads, D, slots,
+                                                          mass.defined());
+  const Tensor ws = need > 0 ? bytes_on(k, need) : Tensor();
+  check(tp_paged_attention(code_of(k), B, H, &cache, (const int32_t*)at_(lengths), at_(q),
+                           q.stride(0), q.stride(1), at_(key), key.defined() ? key.stride(0) : 0,
+                           key.defined() ? key.stride(1) : 0, at_(value),
+                           value.defined() ? value.stride(0) : 0,
+                           value.defined() ? value.stride(1) : 0, floats(gate), floats(tau),
+                           (float)(scale.has_value() ? *scale : 1.0 / std::sqrt((double)D)),
+                           floats(mass), mass.defined() ? mass.stride(0) : 0,
+                           mass.defined() ? mass.stride(1) : 0, mass.defined() ? mass.size(2) : 0,
+                           at_(out), at_(ws), need, stream_of(k)),
+        "tp_paged_attention");
+  if (key.defined()) {
+    written(k);
+    written(v);
+  }
+  if (mass.defined()) written(mass);
+  return out;
+}
+
+bool paged_append(Tensor key_, Tensor value_, Tensor k, Tensor v, Tensor table, Tensor starts,
+                  Maybe counts_) {
+  const Tensor counts = or_none(counts_);
+  no_transforms({&key_, &value_, &k, &v, &table, &starts, &counts}, "paged_append");
+  if (key_.dim() != 4 || !paged_ok(k, v, table, key_.size(0)) || key_.device() != k.device() ||
+      key_.scalar_type() != k.scalar_type() || !alike(value_, key_) ||
+      key_.size(2) != k.size(2) || key_.size(3) != k.size(3))
+    return false;
+  const int64_t B = key_.size(0);
+  if (!lengths_ok(starts, k, B) || (counts.defined() && !lengths_ok(counts, k, B))) return false;
+  if (any_needs_grad({&key_, &value_, &k, &v})) return false;
+  at::NoGradGuard off;
+  const On device(k);
+  const Tensor key = channels(key_), value = channels(value_);
+  const tp_paged_cache cache = paged_of(k, v, table);
+  check(tp_paged_append(code_of(k), B, key.size(1), &cache, (const int32_t*)at_(starts),
+                        (const int32_t*)at_(counts), at_(key), key.stride(0), key.stride(1),
+                        key.stride(2), at_(value), value.stride(0), value.stride(1),
+                        value.stride(2), stream_of(k)),
+        "tp_paged_append");
+  written(k);
+  written(v);
+  return true;
+}
+
+Maybe cache_evict(Tensor k, Tensor v, Tensor table, Tensor lengths, Tensor mass, int64_t keep,
+                  int64_t recent, Maybe out_) {
+  const Tensor out = out_.has_value() ? *out_ : mass;
+  no_transforms({&k, &v, &table, &lengths, &mass, &out}, "cache_evict");
+  const int64_t B = mass.dim() == 3 ? mass.size(0) : -1;
+  if (!paged_ok(k, v, table, B) || !lengths_ok(lengths, k, B) || !mass_ok(mass, k, B) ||
+      !mass_ok(out, k, B) || out.size(2) < std::min(keep, mass.size(2)) || keep < 1 ||
+      recent < 0 || recent > keep)
+    return std::nullopt;
+  if (any_needs_grad({&k, &v, &mass, &out})) return std::nullopt;
+  at::NoGradGuard off;
+  const On device(k);
+  Tensor kept = at::empty({B, k.size(2), keep}, lengths.options());
+  const tp_paged_cache cache = paged_of(k, v, table);
+  check(tp_cache_evict(code_of(k), B, &cache, (const int32_t*)at_(lengths), floats(mass),
+                       mass.stride(0), mass.stride(1), mass.size(2), floats(out), out.stride(0),
+                       out.stride(1), keep, recent, (int32_t*)at_(kept), stream_of(k)),
+        "tp_cache_evict");
+  written(k);
+  written(v);
+  written(out);
+  return kept;
+}
+
+std::optional<std::tuple<Tensor, Tensor>> sample_tokens(Tensor logits_, Tensor uniform_, double T,
+                                                        Maybe Ts_, int64_t top_k, Maybe top_ks_,
+                                                        double top_p, Maybe top_ps_, double min_p,
+                                                        Maybe min_ps_, bool logprob) {
+  const Tensor Ts = or_none(Ts_), ks = or_none(top_ks_), ps = or_none(top_ps_),
+               ms = or_none(min_ps_);
+  no_transforms({&logits_, &uniform_, &Ts, &ks, &ps, &ms}, "sample_tokens");
+  if (!logits_.is_cuda() || !is_float(logits_) || logits_.dim() != 2 || logits_.size(1) < 1)
+    return std::nullopt;
+  const int64_t B = logits_.size(0);
+  auto of_rows = [&](const Tensor& t, at::ScalarType type) {
+    return t.device() == logits_.device() && t.scalar_type() == type && t.dim() == 1 &&
+           t.size(0) == B && t.is_contiguous();
+  };
+  if (!of_rows(uniform_, at::kFloat) && !of_rows(uniform_, at::kDouble)) return std::nullopt;
+  for (const Tensor* t : {&Ts, &ps, &ms})
+    if (t->defined() && !of_rows(*t, at::kFloat)) return std::nullopt;
+  if (ks.defined() && !of_rows(ks, at::kInt)) return std::nullopt;
+  if (any_needs_grad({&logits_, &uniform_, &Ts, &ps, &ms})) return std::nullopt;
+  at::NoGradGuard off;
+  const On device(logits_);
+  const Tensor logits = channels(logits_);
+  Tensor token = at::empty({B}, logits.options().dtype(at::kLong)), lp;
+  if (logprob) lp = at::empty({B}, logits.options().dtype(at::kFloat));
+  check(tp_sample_tokens(code_of(logits), B, logits.size(1), at_(logits), logits.stride(0),
+                         uniform_.scalar_type() == at::kFloat ? 32 : 64, at_(uniform_), T,
+                         floats(Ts), top_k, (const int32_t*)at_(ks), top_p, floats(ps), min_p,
+                         floats(ms), (int64_t*)at_(token), floats(lp), stream_of(logits)),
+        "tp_sample_tokens");
+  return std::make_tuple(token, lp);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -581,6 +760,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gated_scan_bwd", &gated_scan_bwd);
   m.def("gated_scan_step", &gated_scan_step);
   m.def("embedding", &embedding);
+  m.def("paged_attention", &paged_attention);
+  m.def("paged_append", &paged_append);
+  m.def("cache_evict", &cache_evict);
+  m.def("sample_tokens", &sample_tokens);
   m.def("embedding_fwd", &embedding_fwd);
   m.def("embedding_bwd", [](Tensor ids, Tensor dout, int64_t rows, double scale, int64_t padding) {
     at::NoGradGuard off;

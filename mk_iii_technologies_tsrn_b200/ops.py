@@ -25,6 +25,14 @@ Operators around them in a language model, with their gradients:
   block's norm in one pass (``research/tsrn_dml.py:975-980,1096-1106``).
 * :func:`gated_scan`, :func:`gated_scan_step` -- the gated linear recurrence, the (plus, times)
   counterpart of :func:`tropical_scan`, over sequences and for one token.
+
+Operators of its decoding:
+
+* :func:`paged_attention` -- one new token against a paged key-value cache, with the blended
+  tropical and classical score of ``tropformer_dropin.py:236-260`` or the classical one.
+* :func:`paged_append`, :func:`cache_evict` -- prompts into the pages, and slots out of them by
+  their accumulated attention weight.
+* :func:`sample_tokens` -- temperature, top-k, top-p and min-p from given random numbers.
 """
 from __future__ import annotations
 
@@ -76,12 +84,15 @@ class DeviceWaitTimeout(RuntimeError):
 
 
 class DeviceIndexError(IndexError):
-    """A token id or position given to :func:`embedding` was outside its table;
-    the token's row of the output is NaN and it added to no gradient."""
+    """A token id or position given to :func:`embedding` was outside its table (the token's row
+    of the output is NaN and it added to no gradient), or a length, start or page given to
+    :func:`paged_attention`, :func:`paged_append` or :func:`cache_evict` outside its cache (NaN
+    in that sequence's output, or nothing written)."""
 
     def __init__(self, device):
         super().__init__(f"an id or position given to ops.embedding on {device} is outside its "
-                         "table; its rows of the output are NaN")
+                         "table, or a length or page of a paged cache outside that; rows of the "
+                         "output are NaN")
         self.code = _lib.TP_DEVERR_INDEX
 
 
@@ -1585,6 +1596,230 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, *,
         positions = _embedding_inputs(ids, weight, pos_weight, positions)
         out = call(ids, weight, pos_weight, positions, scale, padding)
     return out if out is not None else _refused()
+
+
+# --------------------------------------------------------------------------- decoding
+def _paged_inputs(k_cache, v_cache, block_table, B, what):
+    """Checks of a cache and its table of B rows."""
+    _floating(k_cache, "paged caches")
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype:
+        raise ValueError("k_cache and v_cache must be [pages, page size, heads, channels] of one "
+                         f"shape and dtype, got {tuple(k_cache.shape)} {k_cache.dtype} and "
+                         f"{tuple(v_cache.shape)} {v_cache.dtype}")
+    for t in (k_cache, v_cache):
+        if t.shape[3] > 1 and t.stride(3) != 1 or any(
+                t.shape[i] > 1 and t.stride(i) < t.shape[3] for i in range(3)):
+            raise ValueError("a cache's channels must be contiguous and its rows apart, got "
+                             f"strides {t.stride()}")
+    if k_cache.shape[1] < 1:
+        raise ValueError("pages must have at least one slot")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B or (
+            block_table.shape[1] > 1 and block_table.stride(1) != 1):
+        raise ValueError(f"block_table must be [{B}, pages of a sequence] of int32 with contiguous "
+                         f"rows ({what}), got {tuple(block_table.shape)} {block_table.dtype}")
+
+
+def _slot_counts(t: torch.Tensor, B: int, what: str) -> torch.Tensor:
+    """Lengths, starts or counts [B] as contiguous int32."""
+    if t.shape != (B,) or t.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{what} must be [{B}] of int32 or int64, got {tuple(t.shape)} {t.dtype}")
+    if t.dtype == torch.int64:
+        t = t.clamp(-2 ** 31, 2 ** 31 - 1).to(torch.int32)      # (what is outside stays so)
+    return t.contiguous()
+
+
+def _mass_inputs(mass, B, heads, what):
+    if _f32(mass).dim() != 3 or mass.shape[:2] != (B, heads) or (
+            mass.shape[2] > 1 and mass.stride(2) != 1) or any(
+            mass.shape[i] > 1 and mass.stride(i) < mass.shape[2] for i in range(2)):
+        raise ValueError(f"{what} must be [{B}, {heads}, slots] with contiguous, separate rows, "
+                         f"got {tuple(mass.shape)} at strides {mass.stride()}")
+
+
+def _no_gradient(what, *tensors):
+    if torch.is_grad_enabled() and any(
+            isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what} is not differentiable; call it under torch.no_grad()")
+
+
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                    block_table: torch.Tensor, lengths: torch.Tensor, *,
+                    key: Optional[torch.Tensor] = None, value: Optional[torch.Tensor] = None,
+                    scale: Optional[float] = None, gate: Optional[torch.Tensor] = None,
+                    tau: Optional[torch.Tensor] = None,
+                    mass: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of one new token per sequence over its paged key-value cache::
+
+        s_j = scale / tau_h * ((1 - gate) q.k_j + gate * max_f(q_f + k_jf)),  j < lengths[b]
+        out = sum_j softmax(s)_j v_j
+
+    the blended score of ``TropicalMultiHeadAttention`` (tropformer_dropin.py:236-260) for one
+    token; without ``gate`` the classical score alone.
+
+    ``q``: [B, H, D], float32 or bfloat16, D up to 256.  ``k_cache``, ``v_cache``: [pages, page
+    size, Hkv, D] of q's dtype, channels contiguous, other strides free (transposed views of
+    [pages, Hkv, page size, D] too); H a multiple of Hkv, query head h reads key head
+    h // (H // Hkv).  ``block_table`` [B, n] int32: slot j of sequence b is slot j % page size of
+    page block_table[b, j // page size]; only pages of slots in use are read.  ``lengths`` [B]:
+    the slots in use, the new token's among them; 0 gives zeros.
+
+    ``key``, ``value``: [B, Hkv, D], the new token's: they count as slot lengths[b] - 1 and are
+    stored there.  ``scale``: None for D ** -0.5.  ``gate``: [B, H] and ``tau``: [H], float32.
+    ``mass``: [B, Hkv, slots] float32 (slots contiguous): the softmax weights, summed over the
+    query heads of a key head, are added to it in place, for :func:`cache_evict`; with ``key`` the
+    new slot is set to its weight.  Scores, statistics and sums are float32.  Returns
+    [B, H, D] in q's dtype.  Not differentiable.
+
+    A length beyond the table (or beyond ``mass``), or a page outside the cache, makes the
+    sequence's rows NaN, and :func:`check_device_error` raises :class:`DeviceIndexError`.
+    Sequences may share pages they read; pages that are written belong to one sequence."""
+    call = _lib.host().paged_attention
+    out = call(q, k_cache, v_cache, block_table, lengths, key, value, scale, gate, tau, mass)
+    if out is not None:
+        return out
+    _require_cuda(q, k_cache, v_cache, block_table, lengths, key, value, gate, tau, mass)
+    _floating(q, "paged_attention inputs")
+    if q.dim() != 3 or q.dtype != k_cache.dtype or not 1 <= q.shape[2] <= 256:
+        raise ValueError("q must be [B, H, D] of the caches' dtype with D from 1 to 256, got "
+                         f"{tuple(q.shape)} {q.dtype}")
+    B, H, D = q.shape
+    _paged_inputs(k_cache, v_cache, block_table, B, "one row of each q")
+    heads = k_cache.shape[2]
+    if k_cache.shape[3] != D or heads < 1 or H % heads:
+        raise ValueError(f"q {tuple(q.shape)} does not go with caches {tuple(k_cache.shape)}: as "
+                         "many channels, and a multiple of their heads")
+    if (key is None) != (value is None):
+        raise ValueError("key and value come together")
+    for t, what in ((key, "key"), (value, "value")):
+        if t is not None and (t.shape != (B, heads, D) or t.dtype != q.dtype):
+            raise ValueError(f"{what} must be [{B}, {heads}, {D}] {q.dtype}, got "
+                             f"{tuple(t.shape)} {t.dtype}")
+    if gate is not None and _f32(gate).shape != (B, H):
+        raise ValueError(f"gate must be [{B}, {H}], got {tuple(gate.shape)}")
+    if tau is not None and _f32(tau).shape != (H,):
+        raise ValueError(f"tau must be [{H}], got {tuple(tau.shape)}")
+    if mass is not None:
+        _mass_inputs(mass, B, heads, "mass")
+    _no_gradient("paged_attention", q, k_cache, v_cache, key, value, gate, tau, mass)
+    lengths = _slot_counts(lengths, B, "lengths")
+    out = call(q, k_cache, v_cache, block_table, lengths, key, value, scale, gate, tau, mass)
+    return out if out is not None else _refused()
+
+
+def paged_append(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor,
+                 v_cache: torch.Tensor, block_table: torch.Tensor, starts: torch.Tensor,
+                 counts: Optional[torch.Tensor] = None) -> None:
+    """Stores the keys and values [B, T, Hkv, D] of T tokens of each sequence in its pages (see
+    :func:`paged_attention`): token t of sequence b at slot starts[b] + t, for t < counts[b] (None:
+    T; the others are not looked at).  ``TropicalKVCache.update`` (tropformer_dropin.py:143-164)
+    without copying what is there.  A slot outside the table or a page outside the cache is not
+    written, and :func:`check_device_error` raises :class:`DeviceIndexError`."""
+    call = _lib.host().paged_append
+    if call(key, value, k_cache, v_cache, block_table, starts, counts):
+        return
+    _require_cuda(key, value, k_cache, v_cache, block_table, starts, counts)
+    if key.dim() != 4 or value.shape != key.shape or key.dtype != k_cache.dtype or \
+            value.dtype != key.dtype:
+        raise ValueError("key and value must be [B, T, heads, channels] of one shape and the "
+                         f"caches' dtype, got {tuple(key.shape)} {key.dtype} and "
+                         f"{tuple(value.shape)} {value.dtype}")
+    B = key.shape[0]
+    _paged_inputs(k_cache, v_cache, block_table, B, "one row of each sequence")
+    if key.shape[2:] != k_cache.shape[2:]:
+        raise ValueError(f"key {tuple(key.shape)} does not go with caches {tuple(k_cache.shape)}")
+    _no_gradient("paged_append", key, value, k_cache, v_cache)
+    starts = _slot_counts(starts, B, "starts")
+    counts = None if counts is None else _slot_counts(counts, B, "counts")
+    if not call(key, value, k_cache, v_cache, block_table, starts, counts):
+        _refused()
+
+
+def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                lengths: torch.Tensor, mass: torch.Tensor, keep: int, recent: int = 0, *,
+                out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Shortens the caches of sequences with more than ``keep`` slots, each key head by itself:
+    the last ``recent`` slots stay, and of the others those with the most accumulated attention
+    weight ``mass`` [B, Hkv, slots] (of equals the lower slot; NaN counts as the most), ``keep`` in
+    all.  Their rows move to the front of the sequence's pages, in their order; ``mass`` (or
+    ``out``) gets theirs likewise.  What lies behind is left as it was.
+
+    Returns kept [B, Hkv, keep] int32, the slots that stayed (-1 behind a shorter sequence's).
+    ``lengths`` is not changed, as layers share it: ``lengths.clamp_(max=keep)`` after the last
+    layer.  Caches, table and lengths are those of :func:`paged_attention`.  A length outside the
+    table leaves its sequence as it is (kept: -1), a page outside the cache the rows that are or
+    would be in it, and :func:`check_device_error` raises :class:`DeviceIndexError`."""
+    call = _lib.host().cache_evict
+    kept = call(k_cache, v_cache, block_table, lengths, mass, keep, recent, out)
+    if kept is not None:
+        return kept
+    _require_cuda(k_cache, v_cache, block_table, lengths, mass, out)
+    if not 1 <= keep or not 0 <= recent <= keep:
+        raise ValueError(f"keep must be at least 1 and recent from 0 to keep, got {keep} and "
+                         f"{recent}")
+    B = block_table.shape[0] if block_table.dim() else 0
+    _paged_inputs(k_cache, v_cache, block_table, B, "one row of each sequence")
+    _mass_inputs(mass, B, k_cache.shape[2], "mass")
+    if out is not None:
+        _mass_inputs(out, B, k_cache.shape[2], "out")
+        if out.shape[2] < min(keep, mass.shape[2]):
+            raise ValueError(f"out must have {min(keep, mass.shape[2])} slots, got {out.shape[2]}")
+    _no_gradient("cache_evict", k_cache, v_cache, mass, out)
+    lengths = _slot_counts(lengths, B, "lengths")
+    kept = call(k_cache, v_cache, block_table, lengths, mass, keep, recent, out)
+    return kept if kept is not None else _refused()
+
+
+def _choice(x, what, off, ok, dtype=torch.float32):
+    """(number, tensor of the rows or None) of a sampling choice."""
+    if isinstance(x, torch.Tensor):
+        return off, x if x.dtype == dtype and x.is_contiguous() else x.to(dtype).contiguous()
+    if not ok(x):
+        raise ValueError(f"{what}, got {x}")
+    return x, None
+
+
+def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature=1.0, top_k=0,
+                  top_p=1.0, min_p=0.0, return_logprob: bool = False):
+    """The next token of each row of ``logits`` [B, V] (float32 or bfloat16, V below 2^19) from
+    the given random numbers ``uniform`` [B] (float32 or float64, in [0, 1))::
+
+        w_i = exp((x_i - max x) / temperature)
+
+    In the order of falling logits (the lower index first of equals) the tokens are kept that are
+    among the first ``top_k`` (0: all), of those the ones with less than ``top_p`` of their weight
+    before them, and of those the ones with w >= ``min_p``; the best token always.  The result is
+    the first kept token, by index, where the running sum of w passes ``uniform`` times the sum.
+    Weights are computed in 64 bits and summed as integers (w * 2^44, so a token below 2^-45 of the
+    best is never taken): the same token on every call.
+
+    Each choice is a number or a tensor [B], one of each request.  A temperature of 0 (in a
+    tensor: not above 0) takes the best token.  NaN counts as -inf, +inf as the whole weight; a
+    row of nothing but -inf gives -1.  In tensors top_k <= 0 and top_p >= 1 are off.  Returns the
+    tokens [B] int64, with ``return_logprob`` also the float32 log of each one's share of the kept
+    weight (NaN for a token of -1)."""
+    T, Ts = _choice(temperature, "temperature must be 0 or more", 1.0, lambda t: t >= 0.0)
+    k, ks = _choice(top_k, "top_k must be 0 or more", 0, lambda n: n >= 0, torch.int32)
+    p, ps = _choice(top_p, "top_p must be above 0 and at most 1", 1.0, lambda t: 0.0 < t <= 1.0)
+    m, ms = _choice(min_p, "min_p must be from 0 to 1", 0.0, lambda t: 0.0 <= t <= 1.0)
+    out = _lib.host().sample_tokens(logits, uniform, T, Ts, k, ks, p, ps, m, ms, return_logprob)
+    if out is not None:
+        return out if return_logprob else out[0]
+    _require_cuda(logits, uniform, Ts, ks, ps, ms)
+    _floating(logits, "logits")
+    if logits.dim() != 2 or logits.shape[1] < 1:
+        raise ValueError(f"logits must be [B, V], got {tuple(logits.shape)}")
+    B = logits.shape[0]
+    if uniform.shape != (B,) or uniform.dtype not in (torch.float32, torch.float64):
+        raise ValueError(f"uniform must be [{B}] of float32 or float64, got "
+                         f"{tuple(uniform.shape)} {uniform.dtype}")
+    for t, what in ((Ts, "temperature"), (ks, "top_k"), (ps, "top_p"), (ms, "min_p")):
+        if t is not None and t.shape != (B,):
+            raise ValueError(f"{what} must be a number or [{B}], got {tuple(t.shape)}")
+    _no_gradient("sample_tokens", logits, uniform, temperature, top_p, min_p)
+    if not uniform.is_contiguous():
+        return sample_tokens(logits, uniform.contiguous(), temperature=temperature, top_k=top_k,
+                             top_p=top_p, min_p=min_p, return_logprob=return_logprob)
+    _refused()
 
 
 def tsrn_attention_host(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor,
