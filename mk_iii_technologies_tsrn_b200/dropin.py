@@ -18,7 +18,13 @@ with the tropical parts on this library's kernels:
   (:616-720): one kernel, its gradient by sorted tokens (``ops.embedding``; the
   values are those of the PyTorch expression bit for bit).  An id outside the
   table makes its rows NaN, and a later call of the model raises
-  ``ops.DeviceIndexError``, where PyTorch's embedding ends the CUDA context.
+  ``ops.DeviceIndexError``, where PyTorch's embedding ends the CUDA context;
+* decoding: ``TropicalDecoderModel.generate`` keeps keys and values in pages
+  (``TropicalPagedKVCache``), each token's attention is one kernel over them
+  (``ops.paged_attention``), the next token one more (``ops.sample_tokens``),
+  and a budget of slots evicts by accumulated attention weight
+  (``ops.cache_evict``).  The reference has no decoding loop; its concatenated
+  ``TropicalKVCache`` stays as it is.
 
 Everything else (projections, gate, masks, Maslov softmax, layer norms,
 residuals) is the reference's PyTorch expression.  The encoder /
@@ -45,7 +51,7 @@ from .tropical import MaslovTemperature, TropicalLinear
 
 __all__ = [
     "TropicalLinear", "MaslovTemperature", "LFDualActivation", "TropicalKVCache",
-    "TropicalMultiHeadAttention", "TropicalHybridFFN", "TropicalEncoderLayer",
+    "TropicalPagedKVCache", "TropicalMultiHeadAttention", "TropicalHybridFFN", "TropicalEncoderLayer",
     "TropicalDecoderLayer", "TropicalEncoder", "TropicalDecoder", "TropicalTransformer",
     "TropicalEncoderModel", "TropicalDecoderModel", "TropicalViT",
     "TropicalViTForClassification", "make_causal_mask", "maslov_summary", "lf_blend_summary",
@@ -78,6 +84,85 @@ class TropicalKVCache:
 
     def reset(self):
         self.k = self.v = None
+
+
+class TropicalPagedKVCache:
+    """Keys and values of a model's layers in pages, for decoding (no reference counterpart; the
+    single-layer :class:`TropicalKVCache` copies all of a cache for every token).
+
+    ``num_layers`` pairs of [pages, page_size, num_heads, head_dim] tensors with room for
+    ``max_slots`` slots of each of ``batch`` sequences, one ``block_table`` and one ``lengths`` for
+    all layers.  A model's attention modules get ``cache.layer(i)`` as their ``cache``: between
+    :meth:`begin` and the first :meth:`step` they attend over the prompt as without a cache and
+    store it, after a :meth:`step` over the slots.  ``collect_mass`` sums the attention weights
+    that :meth:`evict` goes by.  Inference only."""
+
+    def __init__(self, num_layers: int, batch: int, num_heads: int, head_dim: int, max_slots: int,
+                 *, page_size: int = 16, collect_mass: bool = False,
+                 dtype: torch.dtype = torch.float32, device=None):
+        per = -(-max_slots // page_size)
+        shape = (batch * per, page_size, num_heads, head_dim)
+        self.max_slots, self.most, self.prompting = max_slots, 0, False
+        self.k = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(num_layers)]
+        self.v = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(num_layers)]
+        self.block_table = torch.arange(batch * per, dtype=torch.int32,
+                                        device=device).view(batch, per)
+        self.lengths = torch.zeros(batch, dtype=torch.int32, device=device)
+        self.mass = [torch.zeros(batch, num_heads, per * page_size, device=device)
+                     for _ in range(num_layers)] if collect_mass else [None] * num_layers
+
+    def layer(self, i: int) -> "_PagedLayer":
+        return _PagedLayer(self, i)
+
+    def _room(self, slots: int) -> None:
+        if slots > self.max_slots:
+            raise ValueError(f"{slots} slots do not fit a cache of {self.max_slots}")
+        self.most = slots
+
+    def begin(self, counts: torch.Tensor, width: int) -> None:
+        """A prompt of ``counts`` [batch] tokens (of ``width`` at most) follows."""
+        self._room(width)
+        self.prompting = True
+        self.lengths.copy_(counts)
+
+    def step(self) -> None:
+        """One more token of every sequence follows."""
+        self._room(self.most + 1)
+        self.prompting = False
+        self.lengths.add_(1)
+
+    def evict(self, keep: int, recent: int = 0) -> None:
+        """Leaves ``keep`` slots of each sequence (``ops.cache_evict``, every layer and head by its
+        own weights)."""
+        if self.mass[0] is None:
+            raise ValueError("eviction needs collect_mass=True")
+        for k, v, mass in zip(self.k, self.v, self.mass):
+            ops.cache_evict(k, v, self.block_table, self.lengths, mass, keep, recent)
+        self.lengths.clamp_(max=keep)
+        self.most = min(self.most, keep)
+
+
+@dataclass
+class _PagedLayer:
+    cache: TropicalPagedKVCache
+    index: int
+
+    def store(self, K: torch.Tensor, V: torch.Tensor, attn: torch.Tensor) -> None:
+        # a prompt's keys and values [B, H, L, d_k] and softmax weights [B, H, L, L]
+        c, i = self.cache, self.index
+        ops.paged_append(K.transpose(1, 2), V.transpose(1, 2), c.k[i], c.v[i], c.block_table,
+                         torch.zeros_like(c.lengths), c.lengths)
+        if c.mass[i] is not None:
+            L = attn.shape[-1]
+            there = torch.arange(L, device=attn.device) < c.lengths[:, None]
+            c.mass[i][:, :, :L] = (attn * there[:, None, :, None]).sum(2)
+
+    def attend(self, Q, K, V, scale, gate, tau):
+        # Q, K, V [B, H, 1, d_k] of the new token
+        c, i = self.cache, self.index
+        return ops.paged_attention(Q[:, :, 0], c.k[i], c.v[i], c.block_table, c.lengths,
+                                   key=K[:, :, 0], value=V[:, :, 0], scale=scale, gate=gate,
+                                   tau=tau, mass=c.mass[i])
 
 
 def _grad_needed(*tensors) -> bool:
@@ -126,7 +211,19 @@ class TropicalMultiHeadAttention(nn.Module):
         Q = self._split_heads(self.q_proj(query))
         K = self._split_heads(self.k_proj(key))
         V = self._split_heads(self.v_proj(value))
-        if cache is not None:
+        paged = cache if isinstance(cache, _PagedLayer) else None
+        if paged is not None:
+            if self.is_cross_attention or (self.training and self.attn_dropout.p > 0):
+                raise RuntimeError("a paged cache serves self-attention without dropout")
+            if not paged.cache.prompting:
+                if L_q != 1 or need_weights or attn_mask is not None or \
+                        key_padding_mask is not None:
+                    raise ValueError("after a prompt a paged cache takes one token at a time, "
+                                     "without masks or weights")
+                gate = torch.sigmoid(self.score_gate(query))[:, 0]                # (B, H)
+                out = paged.attend(Q, K, V, self._scale, gate, self.maslov.temperatures)
+                return self.out_proj(out.reshape(B, 1, D)), None
+        elif cache is not None:
             K, V = cache.update(K, V)
         class_scores = torch.matmul(Q, K.transpose(-2, -1)) * self._scale
         trop_scores = self._tropical_scores(Q, K)
@@ -146,6 +243,8 @@ class TropicalMultiHeadAttention(nn.Module):
         if key_padding_mask is not None:
             scores = scores.masked_fill(key_padding_mask[:, None, None, :], -1e9)
         attn = self.attn_dropout(self.maslov(scores))
+        if paged is not None:
+            paged.store(K, V, attn)
         out = torch.matmul(attn, V).transpose(1, 2).contiguous().view(B, L_q, D)
         return self.out_proj(out), (attn if need_weights else None)
 
@@ -196,9 +295,10 @@ class TropicalEncoderLayer(nn.Module):
         self.dropout2 = nn.Dropout(dropout)
 
     def forward(self, src: torch.Tensor, src_mask: Optional[torch.Tensor] = None,
-                src_key_padding_mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+                src_key_padding_mask: Optional[torch.Tensor] = None,
+                cache: Optional[TropicalKVCache] = None) -> torch.Tensor:
         x = src if self.batch_first else src.transpose(0, 1)
-        masks = dict(attn_mask=src_mask, key_padding_mask=src_key_padding_mask)
+        masks = dict(attn_mask=src_mask, key_padding_mask=src_key_padding_mask, cache=cache)
         if self.norm_first:
             h = self.norm1(x)
             x = x + self.dropout1(self.self_attn(h, h, h, **masks)[0])
@@ -368,7 +468,8 @@ class _TokenModel(nn.Module):
                                      lf_mode, init_temp)
         return TropicalEncoder(layer, num_layers, norm=nn.LayerNorm(d_model))
 
-    def _embed(self, input_ids: torch.Tensor) -> torch.Tensor:
+    def _embed(self, input_ids: torch.Tensor,
+               positions: Optional[torch.Tensor] = None) -> torch.Tensor:
         tok, pos = self.embed, self.pos_embed
         if (input_ids.is_cuda and input_ids.dtype in (torch.int32, torch.int64)
                 and _plain_table(tok) and _plain_table(pos) and pos.padding_idx is None
@@ -377,9 +478,10 @@ class _TokenModel(nn.Module):
                 and not any(map(_transformed, (input_ids, tok.weight, pos.weight)))):
             ops.raise_seen_index_error(input_ids.device)      # of an earlier call
             return self.embed_drop(ops.embedding(input_ids, tok.weight, self.embed_scale,
-                                                 pos_weight=pos.weight,
+                                                 pos_weight=pos.weight, positions=positions,
                                                  padding_idx=tok.padding_idx))
-        positions = torch.arange(input_ids.shape[1], device=input_ids.device)[None]
+        if positions is None:
+            positions = torch.arange(input_ids.shape[1], device=input_ids.device)[None]
         return self.embed_drop(self.embed(input_ids) * self.embed_scale +
                                self.pos_embed(positions))
 
@@ -418,6 +520,67 @@ class TropicalDecoderModel(_TokenModel):
         pad = (attention_mask == 0) if attention_mask is not None else None
         x = self.layers(self._embed(input_ids), mask=mask, src_key_padding_mask=pad)
         return self.lm_head(x)
+
+    def _cached(self, x, cache: TropicalPagedKVCache, mask=None, pad=None) -> torch.Tensor:
+        # the stack over a cache's layers
+        for i, layer in enumerate(self.layers.layers):
+            x = layer(x, src_mask=mask, src_key_padding_mask=pad, cache=cache.layer(i))
+        return self.layers.norm(x) if self.layers.norm is not None else x
+
+    @torch.no_grad()
+    def generate(self, input_ids: torch.Tensor, max_new_tokens: int, *,
+                 attention_mask: Optional[torch.Tensor] = None, temperature=1.0, top_k=0,
+                 top_p=1.0, min_p=0.0, uniform: Optional[torch.Tensor] = None,
+                 generator: Optional[torch.Generator] = None, page_size: int = 16,
+                 keep: Optional[int] = None, recent: Optional[int] = None) -> torch.Tensor:
+        """``max_new_tokens`` tokens [B, max_new_tokens] behind the prompts ``input_ids`` [B, L]
+        (no reference counterpart), sampled as :func:`ops.sample_tokens` does (``temperature=0``:
+        the best one).  ``attention_mask``: 1 = keep, 0 = padding, at the right of each row.
+        ``uniform`` [max_new_tokens, B]: the random numbers, drawn from ``generator`` where None.
+
+        ``keep``: a budget of cache slots for each sequence; a sequence over it by a page goes
+        back to it, the last ``recent`` (None: a quarter) and those with the most accumulated
+        attention weight staying.  Needs a CUDA device and a model in eval mode (or without
+        dropout)."""
+        B, L = input_ids.shape
+        if max_new_tokens < 1 or L + max_new_tokens - 1 > self.pos_embed.num_embeddings:
+            raise ValueError(f"{L} tokens and {max_new_tokens} new ones: needs at least one new "
+                             f"one, within {self.pos_embed.num_embeddings} positions")
+        if keep is not None and (keep < 1 or not 0 <= (recent or 0) <= keep):
+            raise ValueError("keep must be at least 1 and recent from 0 to keep, got "
+                             f"{keep} and {recent}")
+        pad, counts = None, torch.full((B,), L, dtype=torch.int32, device=input_ids.device)
+        if attention_mask is not None:
+            live = attention_mask != 0
+            if not bool(live[:, 0].all()) or bool((live[:, 1:] > live[:, :-1]).any()):
+                raise ValueError("prompts must have a token and be padded at the right")
+            pad, counts = ~live, live.sum(1, dtype=torch.int32)
+        if uniform is None:
+            uniform = torch.rand(max_new_tokens, B, device=input_ids.device, generator=generator)
+        elif uniform.shape != (max_new_tokens, B):
+            raise ValueError(f"uniform must be [{max_new_tokens}, {B}], got {tuple(uniform.shape)}")
+        slots = L + max_new_tokens - 1 if keep is None else max(L, keep + page_size)
+        attn = self.layers.layers[0].self_attn
+        cache = TropicalPagedKVCache(len(self.layers.layers), B, attn.num_heads, attn.d_k, slots,
+                                     page_size=page_size, collect_mass=keep is not None,
+                                     dtype=attn.k_proj.weight.dtype, device=input_ids.device)
+        choices = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+        cache.begin(counts, L)
+        x = self._cached(self._embed(input_ids), cache, make_causal_mask(L, input_ids.device), pad)
+        x = x[torch.arange(B, device=x.device), counts.long() - 1]
+        out = torch.empty(max_new_tokens, B, dtype=torch.int64, device=x.device)
+        positions = counts.to(input_ids.dtype)[:, None]
+        for t in range(max_new_tokens):
+            out[t] = ops.sample_tokens(self.lm_head(x), uniform[t], **choices)
+            if t + 1 == max_new_tokens:
+                break
+            if keep is not None and cache.most >= min(slots, keep + page_size):
+                cache.evict(keep, keep // 4 if recent is None else recent)
+            cache.step()
+            ids = out[t].to(input_ids.dtype)[:, None]
+            x = self._cached(self._embed(ids, positions), cache)[:, 0]
+            positions = positions + 1
+        return out.t().contiguous()
 
 
 class TropicalViT(nn.Module):
