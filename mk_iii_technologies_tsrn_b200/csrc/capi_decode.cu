@@ -35,6 +35,9 @@ int paged_cache(PagedCache& c, int dtype, const tp_paged_cache* p, bool rows) {
   c.v = (char*)p->v;
   c.pages = p->pages;
   c.page_size = (int)p->page_size;
+  c.page_shift = -1;
+  for (int i = 0; i < 31; ++i)
+    if (c.page_size == 1 << i) c.page_shift = i;
   c.heads = (int)p->heads;
   c.channels = (int)p->channels;
   c.esize = (int)e;
@@ -64,7 +67,7 @@ int64_t tp_paged_attention_workspace_bytes(int dtype, int64_t B, int64_t H, int6
       slots > INT32_MAX)
     return -1;
   if (B == 0 || H == 0) return 0;
-  return paged_attention_cut(dtype, B, H, heads, channels, slots, mass != 0).bytes();
+  return paged_attention_cut(B, H, heads, channels, slots, mass != 0).bytes();
 }
 
 int tp_paged_attention(int dtype, int64_t B, int64_t H, const tp_paged_cache* cache,
@@ -87,21 +90,19 @@ int tp_paged_attention(int dtype, int64_t B, int64_t H, const tp_paged_cache* ca
   if (B == 0 || H == 0) return TP_OK;
   int64_t capacity = cache->table_cols * cache->page_size;
   if (mass != nullptr && mass_slots < capacity) capacity = mass_slots;
-  const PagedAttentionCut cut = paged_attention_cut(dtype, B, H, cache->heads, cache->channels,
+  const PagedAttentionCut cut = paged_attention_cut(B, H, cache->heads, cache->channels,
                                                     capacity, mass != nullptr);
-  TP_RETURN_IF(B > INT32_MAX || H > INT32_MAX || B * H > INT32_MAX / cut.splits ||
-                   B * cache->heads > INT32_MAX / (capacity / MASS_SLOTS + 1) - B * H,
+  TP_RETURN_IF(B > INT32_MAX || H > INT32_MAX || B * H > INT32_MAX / 16 ||
+                   B * cache->heads > (INT32_MAX - B * H) / (capacity / MASS_SLOTS + 1),
                TP_ERR_TOO_LARGE);
   TP_CHECK_PTR(lengths);
   TP_CHECK_PTR(q);
   TP_CHECK_PTR(out);
   for (const void* p : {key, value, (const void*)gate, (const void*)tau, (const void*)mass})
     TP_CHECK_OPT_PTR(p);
-  if (cut.bytes() > 0) {
-    TP_RETURN_IF(workspace == nullptr || workspace_bytes < cut.bytes(), TP_ERR_WORKSPACE);
-    TP_CHECK_PTR(workspace);
-    TP_RETURN_IF(!aligned16(workspace), TP_ERR_MISALIGNED);
-  }
+  TP_RETURN_IF(workspace == nullptr || workspace_bytes < cut.bytes(), TP_ERR_WORKSPACE);
+  TP_CHECK_PTR(workspace);
+  TP_RETURN_IF(!aligned16(workspace), TP_ERR_MISALIGNED);
   a.dtype = dtype;
   a.B = (int)B;
   a.H = (int)H;
@@ -124,12 +125,12 @@ int tp_paged_attention(int dtype, int64_t B, int64_t H, const tp_paged_cache* ca
   a.mass_sb = mass_sb;
   a.mass_sh = mass_sh;
   a.out = out;
-  a.splits = cut.splits;
-  a.unit = cut.unit;
   float* ws = (float*)workspace;
-  a.ml = cut.ml > 0 ? (float2*)ws : nullptr;
-  a.part = cut.part > 0 ? ws + cut.ml : nullptr;
-  a.scores = cut.scores > 0 ? ws + cut.ml + cut.part : nullptr;
+  a.scores = mass != nullptr ? ws : nullptr;
+  a.score_row = cut.score_row;
+  a.runs_of = (int2*)(ws + cut.scores);
+  a.ml = (float2*)(ws + cut.scores + cut.runs);
+  a.part = ws + cut.scores + cut.runs + cut.ml;
   a.bad = index_error_words();
   return launch_paged_attention(a, as_stream(stream));
 }

@@ -12,11 +12,16 @@ struct PagedCache {
   char* k;
   char* v;
   int64_t pages;
-  int page_size, heads, channels, esize;
+  int page_size, page_shift, heads, channels, esize;      // page_shift: -1 if no power of two
   int64_t k_page, k_slot, k_head, v_page, v_slot, v_head;
   const int* table;
   int64_t table_row;       // elements from one sequence's row to the next
   int table_cols;
+  // the column of a slot's page in its sequence's row, and its place in the page
+  __device__ __forceinline__ int column(int slot) const {
+    return page_shift >= 0 ? slot >> page_shift : slot / page_size;
+  }
+  __device__ __forceinline__ int within(int slot, int column) const { return slot - column * page_size; }
 };
 
 struct PagedAttentionArgs {
@@ -36,30 +41,29 @@ struct PagedAttentionArgs {
   float* mass;             // [B, heads, slots], or NULL
   int64_t mass_sb, mass_sh;
   void* out;               // [B, H, channels]
-  int head_blocks;         // blocks of query heads over a key head
-  int splits, unit;        // the split over the cache's length (paged_attention_cut)
-  float* part;             // [B * H][splits][channels] sums of a split
-  float2* ml;              // [B * H][splits] (maximum, sum) of a split, base 2
-  float* scores;           // [B * H][capacity] scores, base 2, where mass is wanted
+  // the split of the work (paged_attention.cuh), chosen with the kernel
+  int block_heads;         // query heads that a warp takes at a time
+  int head_blocks;         // blocks of them over a key head
+  int runs, tile;          // runs of the list of tiles, slots of a tile
+  int2* runs_of;           // [B] the first run with a segment of the sequence, and how many have
+  float2* ml;              // [segments][block_heads] (maximum, sum) of a segment, base 2
+  float* part;             // [segments][block_heads][channels] sums of a segment
+  float* scores;           // [B * H][score_row] scores, base 2, where mass is wanted
+  int64_t score_row;       // a multiple of four
   IndexErrorWords bad;
 };
 
-constexpr int MASS_SLOTS = 512;      // slots that a block adds weights to
+constexpr int MASS_SLOTS = 1024;     // slots that a block adds weights to
 
-// Splits of a row of n slots among at most `splits` blocks, no less than `unit` slots each.
-__host__ __device__ __forceinline__ int paged_splits(int n, int splits, int unit) {
-  const int e = (n + unit - 1) / unit;
-  return e < 1 ? 1 : (e < splits ? e : splits);
-}
+constexpr int ATT_WARPS = 4;         // of a block
+constexpr int ATT_MOST_BLOCKS = 4;   // on an SM
 
 struct PagedAttentionCut {
-  int splits, unit;
-  int64_t part, ml, scores;      // floats
-  int64_t bytes() const { return 4 * (part + ml + scores); }
+  int64_t scores, runs, ml, part, score_row;      // floats, in this order in the workspace
+  int64_t bytes() const { return 4 * (scores + runs + ml + part); }
 };
-PagedAttentionCut paged_attention_cut(int dtype, int64_t B, int64_t H, int64_t heads, int64_t D,
+PagedAttentionCut paged_attention_cut(int64_t B, int64_t H, int64_t heads, int64_t D,
                                       int64_t capacity, bool mass);
-// (both: part, ml and scores set, the split and head blocks chosen here)
 int launch_paged_attention(PagedAttentionArgs a, cudaStream_t stream);
 // vec: rows of the cache, the key and the value begin and end on 16 bytes
 int launch_paged_attention_f32(PagedAttentionArgs a, bool vec, cudaStream_t stream);

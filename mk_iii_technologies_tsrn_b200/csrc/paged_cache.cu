@@ -6,20 +6,18 @@
 
 namespace tp {
 
-PagedAttentionCut paged_attention_cut(int dtype, int64_t B, int64_t H, int64_t heads, int64_t D,
+PagedAttentionCut paged_attention_cut(int64_t B, int64_t H, int64_t heads, int64_t D,
                                       int64_t capacity, bool mass) {
-  // A block's share is at least a tile for each of its warps (paged_attention.cuh); rows are
-  // cut further until there are two waves of blocks.
-  const int64_t row = D * (dtype == TP_DTYPE_BF16 ? 2 : 4);
-  const int tile = row <= 128 ? 32 : row <= 256 ? 16 : 8;
+  // one for each sequence and each run, for every query head, their number rounded up to blocks
+  // of at most eight of a key head
+  const int64_t heads8 = heads * (H / heads + 7);
+  const int64_t segments = B * heads8 + std::max(heads8, 8 * (int64_t)num_sms() * ATT_WARPS * ATT_MOST_BLOCKS);
   PagedAttentionCut cut{};
-  cut.unit = 4 * tile;
-  const int64_t rows = std::max<int64_t>(1, B * heads * ceil_div(H / heads, 4));
-  cut.splits = (int)std::max<int64_t>(
-      1, std::min(ceil_div(4 * num_sms(), rows), ceil_div(capacity, (int64_t)cut.unit)));
-  if (cut.splits > 1) cut.part = B * H * cut.splits * D;
-  if (cut.splits > 1 || mass) cut.ml = B * H * cut.splits * 2;
-  if (mass) cut.scores = B * H * capacity;
+  cut.score_row = ceil_div(capacity, 4) * 4;
+  if (mass) cut.scores = B * H * cut.score_row;
+  cut.runs = ceil_div(B, 2) * 4;
+  cut.ml = ceil_div(segments, 2) * 4;
+  cut.part = segments * D;
   return cut;
 }
 

@@ -33,7 +33,6 @@ def test_paged_attention_entry_refuses(lib):
     size = lib.tp_paged_attention_workspace_bytes
     need = size(0, 2, 4, 2, 64, 48, 1)
     assert need >= 4 * 2 * 4 * 48 and need % 4 == 0        # the scores at least
-    assert size(0, 64, 32, 8, 64, 64, 0) == 0              # many short rows: one block each
     assert size(0, 1, 1, 1, 64, 65536, 0) > 0
     assert size(2, 1, 1, 1, 64, 48, 0) == -1 and size(0, -1, 1, 1, 64, 48, 0) == -1
     assert size(0, 1, 3, 2, 64, 48, 0) == -1 and size(0, 1, 1, 0, 64, 48, 0) == -1
