@@ -12,13 +12,17 @@
 // w * 2^44 rounded: sums that no order changes, exact but for half a unit per token (a
 // token below 2^-45 of the best is never taken).
 //
-// A row is a cluster of 1 to 8 blocks that exchange through shared memory.  Its logits
-// are read once from DRAM and then from the L2.  Without top_k and top_p: maximum, sum,
-// then the part of the row where the sum is passed.  With them, the tokens are counted
-// into bins of equal width below the maximum, those of the best bins that make at most
-// CANDIDATES gathered into one block, sorted, and cut off there.  Where that does not
-// reach (flat rows under top_p, top_k above CANDIDATES), the threshold is found bit by
-// bit over all tokens.
+// A row is a cluster of 1 to 8 blocks that exchange through shared memory.  Its logits are read
+// once from DRAM and then from the L2.
+//   - Without top_k and top_p: the maximum, the sum, and the part of the row where it is passed.
+//   - With top_k: tokens are counted into bins of equal width below the maximum (of the threads'
+//     best tokens alone, where top_k is far below the threads: a bin that holds top_k of those holds
+//     as many tokens).  With top_p alone: the weights are added into the bins, exactly.
+//   - The tokens of the bins up to the border go to one block, which sorts them, cuts them off
+//     and finds the token.  Where they are more than CANDIDATES, those of the border's bin alone:
+//     then the row has a threshold, and is read twice more as without filters.
+//   - Where even that bin holds too many (flat rows, ties), and for a share of a top_k above
+//     CANDIDATES, the threshold is found bit by bit over all tokens.
 #include <algorithm>
 
 #include "decode.cuh"
@@ -36,12 +40,15 @@ typedef unsigned long long u64;
 struct Shared {
   u64 exchange[2][2][MAX_CLUSTER];
   u64 reduce[2][WARPS];
-  u64 candidate[CANDIDATES];
+  u64 candidate[2][CANDIDATES];        // of the bins before the border's, and of that
   u64 weight[CANDIDATES];
   u64 warp_sum[WARPS];
-  int hist[BINS];
+  u64 before_border, sum_all;
+  uint32_t low[BINS], high[BINS];      // counts, or weights in two halves
   int warp_ties[WARPS];
-  int count, last_bin, gathered, universe;
+  int count[2], border;
+  uint32_t cut;
+  int ties;
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -63,8 +70,8 @@ __device__ __forceinline__ void remote_store(uint32_t at, u64 v) {
 __device__ __forceinline__ void remote_store(uint32_t at, int v) {
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
 }
-__device__ __forceinline__ int remote_load(uint32_t at) {
-  int v;
+__device__ __forceinline__ uint32_t remote_load(uint32_t at) {
+  uint32_t v;
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
   return v;
 }
@@ -83,6 +90,8 @@ __device__ __forceinline__ uint32_t key_of(float x) {
 __device__ __forceinline__ float value_of(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
+
+constexpr uint32_t LOWEST = 0x007fffffu;          // key_of(-inf)
 
 struct Add {
   __device__ __forceinline__ u64 operator()(u64 a, u64 b) const { return a + b; }
@@ -201,17 +210,33 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const SampleArgs a, int
     return r;
   };
 
-  // ---- the best token
-  if (tid == 0) s.count = 0;
-  for (int i = tid; i < BINS; i += THREADS) s.hist[i] = 0;
+  // ---- the best token, of this thread and of all; the lowest number
+  if (tid < 2) s.count[tid] = 0;
+  for (int i = tid; i < BINS; i += THREADS) s.low[i] = s.high[i] = 0;
   u64 best = 0;
+  uint32_t least = 0;                   // the largest of the inverted keys above -inf's
   row.each([&](int i, const float* v, int some) {
-    for (int k = 0; k < some; ++k) {
-      const u64 c = (u64)key_of(v[k]) << 32 | (0xffffffffu - (uint32_t)(i + k));
+#pragma unroll
+    for (int k = 0; k < Row<T>::PER; ++k) {
+      if (k >= some) continue;
+      const uint32_t key = key_of(v[k]);
+      const u64 c = (u64)key << 32 | (0xffffffffu - (uint32_t)(i + k));
       best = c > best ? c : best;
+      if (key > LOWEST) least = max(least, ~key);
     }
   });
-  best = reduce(best, Max());
+  const float mine_best = best ? value_of((uint32_t)(best >> 32)) : -__int_as_float(0x7f800000);
+  all(best, 0, Max());
+  all(least, 1, Max());
+  __syncthreads();
+  if (warp == 0) {
+    finish(0, Max());
+    finish(1, Max());
+  }
+  cluster_sync();
+  best = joined(0, Max());
+  least = (uint32_t)joined(1, Max());
+  ++calls;
   Weights wt;
   wt.top = value_of((uint32_t)(best >> 32));
   const int first = (int)(0xffffffffu - (uint32_t)best);
@@ -253,103 +278,114 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const SampleArgs a, int
   uint32_t cut = 0;                     // kept: keys above it, and the first `ties` equal to it
   int64_t ties = INT64_MAX;
   if (by_k || by_p) {
-    // ---- bins below the maximum
-    const float reach = (float)(REACH * temperature), bins_per = (float)(BINS / (REACH * temperature));
+    // ---- bins below the maximum, down to the lowest number or to where a token weighs nothing
+    const float span = wt.top - value_of(~least);
+    const float reach = fminf((float)(REACH * temperature), span), bins_per = BINS / reach;
     auto bin_of = [&](float x) {        // BINS: weighs nothing
       if (x == wt.top) return 0;
       const float d = wt.top - x;
-      return d < reach ? min(BINS - 1, (int)(d * bins_per)) : BINS;
+      return d <= reach ? min(BINS - 1, (int)(d * bins_per)) : BINS;
     };
-    row.each([&](int i, const float* v, int some) {
-      for (int k = 0; k < some; ++k) {
-        const int bin = bin_of(v[k]);
-        if (bin < BINS) atomicAdd(&s.hist[bin], 1);
-      }
-    });
+    const bool of_threads = by_k && top_k <= cluster * THREADS / 8 && V >= cluster * THREADS;
+    if (of_threads) {
+      const int bin = bin_of(mine_best);
+      if (bin < BINS) atomicAdd(&s.low[bin], 1u);
+    } else {
+      row.each([&](int i, const float* v, int some) {
+        for (int k = 0; k < some; ++k) {
+          const int bin = bin_of(v[k]);
+          if (bin >= BINS) continue;
+          if (by_k) {
+            atomicAdd(&s.low[bin], 1u);
+          } else {
+            const u64 w = wt.whole(wt.real(v[k]));
+            const uint32_t lo = (uint32_t)w, old = atomicAdd(&s.low[bin], lo);
+            const uint32_t hi = (uint32_t)(w >> 32) + (old + lo < old);
+            if (hi) atomicAdd(&s.high[bin], hi);
+          }
+        }
+      });
+    }
     cluster_sync();
-    if (rank == 0) {                    // the bins that are gathered
-      int mine[2] = {0, 0};
+    if (rank == 0) {                    // the border's bin: the first where the sum reaches it
+      u64 mine[2] = {0, 0};
       for (int r = 0; r < cluster; ++r)
 #pragma unroll
-        for (int k = 0; k < 2; ++k) mine[k] += remote_load(remote(&s.hist[2 * tid + k], r));
-      const int sum = mine[0] + mine[1];
-      int at = (int)warp_inclusive(sum, lane);
-      if (lane == 31) s.warp_ties[warp] = at;
-      if (tid == 0) {
-        s.last_bin = -1;
-        s.gathered = 0;
-      }
+        for (int k = 0; k < 2; ++k) {
+          mine[k] += remote_load(remote(&s.low[2 * tid + k], r));
+          if (!by_k) mine[k] += (u64)remote_load(remote(&s.high[2 * tid + k], r)) << 32;
+        }
+      u64 at = warp_inclusive(mine[0] + mine[1], lane);
+      if (lane == 31) s.warp_sum[warp] = at;
+      if (tid == 0) s.border = BINS;
       __syncthreads();
-      int before = 0, everything = 0;
+      u64 everything = 0;
       for (int w = 0; w < WARPS; ++w) {
-        before += w < warp ? s.warp_ties[w] : 0;
-        everything += s.warp_ties[w];
+        at += w < warp ? s.warp_sum[w] : 0;
+        everything += s.warp_sum[w];
       }
-      at += before;                     // tokens up to this thread's second bin
-      // the fewest that hold the first top_k; under top_p alone as many as there is room for
-      const int want = by_k ? min(top_k, everything) : CANDIDATES + 1;
-      int to = -1;
-      if (at - mine[1] <= CANDIDATES && at - sum < want) to = 2 * tid;
-      if (at <= CANDIDATES && at - mine[1] < want) to = 2 * tid + 1;
-      if (to >= 0) atomicMax(&s.last_bin, to);
-      __syncthreads();
-      if (to >= 0 && to == s.last_bin) s.gathered = (to & 1) ? at : at - mine[1];
+      // (with top_k above the universe's tokens: the last bin that has any)
+      const u64 first = at - mine[1], none = first - mine[0];
+      auto reaches = [&](u64 sum) {
+        return by_k ? sum >= min((u64)top_k, everything) : (double)sum >= top_p * (double)everything;
+      };
+      if (reaches(at) && !reaches(none) && !(of_threads && everything < (u64)top_k)) {
+        const int border = reaches(first) ? 2 * tid : 2 * tid + 1;
+        s.border = border;
+        s.before_border = border & 1 ? first : none;
+        s.sum_all = everything;
+      }
+      // (fewer threads with a token than top_k: all tokens that weigh something)
+      if (of_threads && everything < (u64)top_k && tid == 0) s.border = BINS - 1;
       __syncthreads();
       if (tid > 0 && tid < cluster) {
-        remote_store(remote(&s.last_bin, tid), s.last_bin);
-        remote_store(remote(&s.gathered, tid), s.gathered);
+        remote_store(remote(&s.border, tid), s.border);
+        remote_store(remote(&s.sum_all, tid), s.sum_all);
       }
-      if (tid < cluster) remote_store(remote(&s.universe, tid), everything);
     }
     cluster_sync();
-    const int last_bin = s.last_bin, universe = s.universe;
-    // ---- gather them; under top_p alone the weight of all is wanted too
-    u64 sum_all = 0, sum_some = 0;
+    const int border = s.border;
+    // ---- gather
     row.each([&](int i, const float* v, int some) {
+#pragma unroll
       for (int k = 0; k < Row<T>::PER; ++k) {
         const int bin = k < some ? bin_of(v[k]) : BINS;
-        const bool take = bin <= last_bin;
-        const uint32_t takers = __ballot_sync(0xffffffffu, take);
-        if (takers) {
+        if (!__any_sync(0xffffffffu, bin <= border && bin < BINS)) continue;
+#pragma unroll
+        for (int list = 0; list < 2; ++list) {
+          const bool take = list ? bin == border && bin < BINS : bin < border;
+          const uint32_t takers = __ballot_sync(0xffffffffu, take);
+          if (!takers) continue;
           int at = 0;
-          if (lane == __ffs(takers) - 1) at = remote_add(remote(&s.count, 0), __popc(takers));
+          if (lane == __ffs(takers) - 1) at = remote_add(remote(&s.count[list], 0), __popc(takers));
           at = __shfl_sync(0xffffffffu, at, __ffs(takers) - 1) + __popc(takers & ((1u << lane) - 1));
-          if (take)
-            remote_store(remote(&s.candidate[at], 0),
+          if (take && at < CANDIDATES)
+            remote_store(remote(&s.candidate[list][at], 0),
                          (u64)key_of(v[k]) << 32 | (0xffffffffu - (uint32_t)(i + k)));
-        }
-        if (!by_k && bin < BINS) {
-          const u64 w = wt.whole(wt.real(v[k]));
-          sum_all += w;
-          sum_some += take ? w : 0;
         }
       }
     });
-    all(sum_all, 0, Add());
-    all(sum_some, 1, Add());
-    __syncthreads();
-    if (warp == 0) {
-      finish(0, Add());
-      finish(1, Add());
+    cluster_sync();
+    if (rank == 0 && tid > 0 && tid < cluster) {
+      remote_store(remote(&s.count[0], tid), s.count[0]);
+      remote_store(remote(&s.count[1], tid), s.count[1]);
     }
     cluster_sync();
-    sum_all = joined(0, Add());
-    sum_some = joined(1, Add());
-    ++calls;
-    const int count = s.gathered;
-    const bool enough = by_k ? count >= min(top_k, universe)
-                             : count == universe || (double)sum_some >= top_p * (double)sum_all;
-    if (enough) {
-      if (rank != 0) return;
-      // ---- sort, cut off, sort by index, find the place
+    const int above = s.count[0], in_border = s.count[1], count = above + in_border;
+    const u64 sum_all = s.sum_all;      // (under top_p alone: the weight of all)
+    const bool few = count <= CANDIDATES;
+    const bool one_bin = !few && in_border <= CANDIDATES && !(of_threads && above >= top_k);
+    if (few && rank != 0) return;
+    if (few || one_bin) {
+      // ---- sort, cut off, sort by index, find the place (or, of one bin, the threshold)
       auto sort = [&](u64 v, int n) {   // falling; threads from n on hold zeros
         for (int k = 2; k <= n; k *= 2)
           for (int j = k / 2; j > 0; j /= 2) {
             u64 other;
             if (j >= 32) {
-              s.candidate[tid] = v;
+              s.candidate[0][tid] = v;
               __syncthreads();
-              other = s.candidate[tid ^ j];
+              other = s.candidate[0][tid ^ j];
               __syncthreads();
             } else {
               other = __shfl_xor_sync(0xffffffffu, v, j);
@@ -367,39 +403,59 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const SampleArgs a, int
         __syncthreads();
         return at;
       };
-      int size = 32;
-      while (size < count) size *= 2;
-      u64 v = tid < count ? s.candidate[tid] : 0;
-      __syncthreads();
-      v = sort(v, size);
-      const bool there = tid < count;
-      const float x = value_of((uint32_t)(v >> 32));
-      const double w = there && tid < top_k ? wt.real(x) : 0.0;
-      const u64 whole = wt.whole(w);
-      const u64 sum = scan(whole);
-      if (tid == THREADS - 1) s.weight[0] = sum;
-      __syncthreads();
-      const u64 share = by_k ? s.weight[0] : sum_all;
-      bool keep = there && tid < top_k && w >= min_p;
-      if (by_p) keep = keep && (double)(sum - whole) < top_p * (double)share;
-      keep = keep || tid == 0;
-      __syncthreads();
-      s.weight[tid] = whole;
-      const uint32_t index = 0xffffffffu - (uint32_t)v;
-      // falling again: the lowest index first; what is not kept last
-      u64 o = keep ? (u64)(0xffffffffu - index) << 32 | (uint32_t)(tid + 1) : 0;
-      o = sort(o, size);
-      __syncthreads();
-      const int from = (int)(uint32_t)o - 1;
-      const u64 ow = from >= 0 ? s.weight[from] : 0;
-      const u64 run = scan(ow);
-      s.candidate[tid] = v;             // (by rank)
-      if (tid == THREADS - 1) s.reduce[0][0] = run;
-      __syncthreads();
-      const u64 total = s.reduce[0][0], t = place(total);
-      if (ow > 0 && run > t && run - ow <= t)
-        write((int)(0xffffffffu - (uint32_t)(o >> 32)), value_of((uint32_t)(s.candidate[from] >> 32)), total);
-      return;
+      if (rank == 0) {
+        const int listed = few ? count : in_border, skipped = few ? 0 : above;
+        int size = 32;
+        while (size < listed) size *= 2;
+        u64 v = 0;
+        if (tid < listed) v = few && tid < above ? s.candidate[0][tid] : s.candidate[1][few ? tid - above : tid];
+        __syncthreads();
+        v = sort(v, size);
+        const bool there = tid < listed && skipped + tid < top_k;
+        const float x = value_of((uint32_t)(v >> 32));
+        const double w = there ? wt.real(x) : 0.0;
+        const u64 whole = wt.whole(w);
+        const u64 sum = scan(whole) + (one_bin && !by_k ? s.before_border : 0);
+        if (tid == THREADS - 1) s.weight[0] = sum;
+        __syncthreads();
+        const u64 share = by_k ? s.weight[0] : sum_all;
+        bool keep = there;
+        if (by_p && !(one_bin && by_k)) keep = keep && (double)(sum - whole) < top_p * (double)share;
+        if (one_bin) {                  // the last one kept, and how many equal to it are
+          const int n = __syncthreads_count(keep);
+          s.candidate[0][tid] = v;
+          __syncthreads();
+          const uint32_t last = (uint32_t)(s.candidate[0][max(n - 1, 0)] >> 32);
+          const int equal = __syncthreads_count(keep && (uint32_t)(v >> 32) == last);
+          if (tid < cluster) {
+            remote_store(remote(&s.cut, tid), (int)last);
+            remote_store(remote(&s.ties, tid), equal);
+          }
+        } else {
+          keep = (keep && w >= min_p) || tid == 0;
+          __syncthreads();
+          s.weight[tid] = whole;
+          const uint32_t index = 0xffffffffu - (uint32_t)v;
+          // falling again: the lowest index first; what is not kept last
+          u64 o = keep ? (u64)(0xffffffffu - index) << 32 | (uint32_t)(tid + 1) : 0;
+          o = sort(o, size);
+          __syncthreads();
+          const int from = (int)(uint32_t)o - 1;
+          const u64 ow = from >= 0 ? s.weight[from] : 0;
+          const u64 run = scan(ow);
+          s.candidate[0][tid] = v;      // (by rank)
+          if (tid == THREADS - 1) s.reduce[0][0] = run;
+          __syncthreads();
+          const u64 total = s.reduce[0][0], t = place(total);
+          if (ow > 0 && run > t && run - ow <= t)
+            write((int)(0xffffffffu - (uint32_t)(o >> 32)),
+                  value_of((uint32_t)(s.candidate[0][from] >> 32)), total);
+          return;
+        }
+      }
+      cluster_sync();
+      cut = s.cut;
+      ties = s.ties;
     }
     // ---- bit by bit over all tokens
     auto weigh_from = [&](uint32_t key) {
@@ -420,20 +476,22 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const SampleArgs a, int
     // (no key of a token is 2^32 - 1, so that cut + 1 is one)
     u64 share = sum_all;
     if (by_k) {
-      for (uint32_t bit = 1u << 31; bit; bit >>= 1)
-        if (count_from(cut | bit) >= (u64)top_k) cut |= bit;
-      ties = top_k - (int64_t)count_from(cut + 1);
+      if (!one_bin) {
+        for (uint32_t bit = 1u << 31; bit; bit >>= 1)
+          if (count_from(cut | bit) >= (u64)top_k) cut |= bit;
+        ties = top_k - (int64_t)count_from(cut + 1);
+      }
       if (by_p) share = weigh_from(cut + 1) + (u64)ties * wt.whole(wt.real(value_of(cut)));
     }
-    if (by_p) {
-      const double least = top_p * (double)share;
+    if (by_p && !(one_bin && !by_k)) {
+      const double wanted = top_p * (double)share;
       uint32_t p = 0;
       for (uint32_t bit = 1u << 31; bit; bit >>= 1)
-        if ((double)weigh_from(p | bit) >= least) p |= bit;
+        if ((double)weigh_from(p | bit) >= wanted) p |= bit;
       if (p >= cut) {
-        const u64 above = weigh_from(p + 1), one = wt.whole(wt.real(value_of(p)));
+        const u64 above_p = weigh_from(p + 1), one = wt.whole(wt.real(value_of(p)));
         // the first of the ties whose sum before it reaches the share is left out
-        int64_t r = one > 0 ? (int64_t)ceil((least - (double)above) / (double)one) : INT64_MAX;
+        int64_t r = one > 0 ? (int64_t)ceil((wanted - (double)above_p) / (double)one) : INT64_MAX;
         r = max(r, (int64_t)1);
         ties = p > cut ? r : min(ties, r);
         cut = p;
@@ -522,11 +580,10 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const SampleArgs a, int
 
 template <typename T>
 int sample(const SampleArgs& a, cudaStream_t stream) {
-  // as many blocks for a row as leave its warps a few steps, while two waves of blocks hold all
-  // rows
+  // as many blocks for a row as leave its warps a few steps, while the SMs hold all rows' at once
   int cluster = 1;
   while (cluster < MAX_CLUSTER && a.V > (int64_t)cluster * WARPS * 64 * (16 / (int)sizeof(T)) &&
-         a.B * cluster * 2 <= 4 * num_sms())
+         a.B * cluster * 2 <= num_sms())
     cluster *= 2;
   TP_RETURN_IF(a.B * cluster > INT32_MAX, TP_ERR_TOO_LARGE);
   cudaLaunchConfig_t cfg = {};

@@ -173,3 +173,25 @@ def test_counts_follow_the_weights(cuda):
     u = (torch.arange(n, device=cuda, dtype=torch.float64) + 0.5) / n
     t = ops.sample_tokens(w.log().expand(n, -1).contiguous(), u)
     assert ((torch.bincount(t, minlength=5) - w * n).abs() <= 1).all()
+
+
+def test_best_tokens_next_to_one_another(cuda):
+    # the best tokens lie in a few threads' parts of the row, or in one part of it
+    for V, n in ((131072, 700), (50000, 300), (8192, 2000)):
+        for dtype in (torch.float32, torch.bfloat16):
+            x, u = _logits(cuda, 3, V, dtype, seed=V)
+            x[0, 1000:1000 + n] += 30.0
+            x[1, ::2] = float("-inf")
+            x[1, 40:] = float("-inf")                     # twenty tokens
+            x[2, :n] = 9.0                                # and equal ones
+            for c in (dict(k=100), dict(k=30, p=0.8), dict(k=900), dict(p=0.9), dict(p=0.5, T=3.0), dict(k=250, m=0.1)):
+                _check(x, u, **c)
+
+
+def test_flat_rows(cuda):
+    # logits of an untrained model: every token in the nucleus, the border between close values
+    for dtype in (torch.float32, torch.bfloat16):
+        for spread in (1e-3, 0.05, 0.5):
+            x, u = _logits(cuda, 3, 40000, dtype, spread=spread)
+            for c in (dict(p=0.9), dict(p=0.3, m=0.999), dict(k=5000), dict(k=5000, p=0.5), dict(k=40)):
+                _check(x, u, **c)
