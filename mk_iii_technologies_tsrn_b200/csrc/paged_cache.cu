@@ -2,6 +2,7 @@
 // prompts into the pages, and eviction from them by accumulated attention weight.
 #include <algorithm>
 
+#include "cluster.cuh"
 #include "decode.cuh"
 
 namespace tp {
@@ -82,77 +83,99 @@ __device__ __forceinline__ uint32_t ordered_bits(float f) {
   return f != f ? 0xffffffffu : (u & 0x80000000u ? ~u : u | 0x80000000u);
 }
 
-// One block per sequence and key head: the kept slots, in order, and their mass.  The mass is read
-// once where it fits shared memory (STAGED slots).  The place of the last kept slot among the old
-// ones is found by digits of 11, 11 and 10 bits from the top (integer counts: any order of the
-// atomics gives the same; of 8 bits, nearly all slots would meet in a few counters); then each
-// warp counts what it keeps of its part, and writes it.
-constexpr int STAGED = 49152, DIGITS = 2048;
+// A cluster of blocks per sequence and key head: the kept slots, in order, and their mass.  Blocks
+// take parts of the slots next to one another, EVICT_PER for a thread, in registers (and chunks of
+// that, where the slots are more).  The place of the last kept slot among the old ones is found by
+// digits of 8 bits from the top: each block counts its own, and adds up all blocks' counts (integers:
+// any order of the atomics gives the same).  Then every warp's kept slots are counted by ballots, the
+// counts summed in the order of the slots, and written.  What bounds it is instructions, so few rows
+// go over many SMs (16 rows of 32768 slots in a block each: 31 us).
+constexpr int EVICT_THREADS = 256, EVICT_PER = 16;
 
-template <int THREADS>
-__global__ void __launch_bounds__(THREADS) evict_select_kernel(const CacheEvictArgs a, int staged) {
-  constexpr int WARPS = THREADS / 32, EACH = DIGITS / THREADS;
-  extern __shared__ float stage[];
-  __shared__ int hist[DIGITS];
-  __shared__ int sums[2][WARPS];
+__global__ void __launch_bounds__(EVICT_THREADS) evict_select_kernel(const CacheEvictArgs a, int cluster) {
+  constexpr int THREADS = EVICT_THREADS, WARPS = THREADS / 32, PART = THREADS * EVICT_PER;
+  __shared__ int hist[2][256], merged[256];
+  __shared__ u64 counts[EVICT_PER * WARPS], sums[WARPS];
+  __shared__ u64 of_block[2][MAX_CLUSTER];
   __shared__ uint32_t s_digit;
   __shared__ int s_left;
-  const int kvh = blockIdx.x % a.c.heads, b = blockIdx.x / a.c.heads, tid = threadIdx.x, lane = tid & 31,
-            warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = (int)cluster_rank();
+  const int row_index = blockIdx.x / cluster, kvh = row_index % a.c.heads, b = row_index / a.c.heads;
   const int given = __ldg(a.lengths + b);
   const bool bad = given < 0 || given > a.capacity;
   if (bad && tid == 0) tp_record_index_error(a.bad.error, a.bad.seen);
   const int n = bad ? 0 : given;
   const float* row = a.mass + (int64_t)b * a.mass_sb + (int64_t)kvh * a.mass_sh;
   float* out = a.out + (int64_t)b * a.out_sb + (int64_t)kvh * a.out_sh;
-  int* kept = a.kept + (int64_t)blockIdx.x * a.keep;
-  if (n <= a.keep) {
-    for (int i = tid; i < a.keep; i += THREADS) {
+  int* kept = a.kept + (int64_t)row_index * a.keep;
+  if (n <= a.keep) {               // (all blocks of the cluster alike)
+    for (int i = rank * THREADS + tid; i < a.keep; i += cluster * THREADS) {
       kept[i] = i < n ? i : -1;
       if (i < n && out != row) out[i] = row[i];
     }
     return;
   }
-  const bool in_smem = n <= staged;
-  if (in_smem)
-    for (int i = tid; i < n; i += THREADS) stage[i] = row[i];
-  const float* mass = in_smem ? stage : row;
   // slots before `old` compete for `need` places
-  const int old = n - min(a.recent, n), need = a.keep - (n - old);
+  const int old = n - min(a.recent, n), need = a.keep - (n - old), chunk = cluster * PART;
+  float v[EVICT_PER];              // slots base + rank * PART + k * THREADS + tid
+  auto load = [&](int base) {
+#pragma unroll
+    for (int k = 0; k < EVICT_PER; ++k) {
+      const int64_t i = (int64_t)base + rank * PART + k * THREADS + tid;
+      v[k] = i < n ? row[i] : 0.0f;
+    }
+  };
+  // this block's slots of a chunk, in steps of THREADS
+  auto steps = [&](int base, int end) {
+    const int64_t some = (int64_t)end - base - (int64_t)rank * PART;
+    return some <= 0 ? 0 : (int)min((int64_t)EVICT_PER, (some + THREADS - 1) / THREADS);
+  };
   uint32_t prefix = 0;
   int left = need;                 // places among the slots whose high bits are `prefix`
+  load(0);
   if (need > 0) {
-    for (int round = 0; round < 3; ++round) {
-      const int shift = round == 0 ? 21 : round == 1 ? 10 : 0, bits = round == 2 ? 10 : 11;
-      for (int i = tid; i < DIGITS; i += THREADS) hist[i] = 0;
-      __syncthreads();
-      for (int i = tid; i < old; i += THREADS) {
-        const uint32_t u = ordered_bits(mass[i]);
-        if (round == 0 || (u >> (shift + bits)) == (prefix >> (shift + bits)))
-          atomicAdd(&hist[(u >> shift) & ((1u << bits) - 1)], 1);
-      }
-      __syncthreads();
-      // the digit where the sum from above passes `left`
-      int mine[EACH], all = 0;
+    hist[0][tid] = 0;
+    __syncthreads();
+    for (int round = 0; round < 4; ++round) {
+      const int shift = 24 - 8 * round;
+      int* const mine = hist[round & 1];
+      for (int64_t base = 0; base < old; base += chunk) {
+        if (old > chunk) load((int)base);
+        const int in_use = steps((int)base, old);
 #pragma unroll
-      for (int k = 0; k < EACH; ++k) all += mine[k] = hist[DIGITS - 1 - (tid * EACH + k)];
-      int above = all;
-#pragma unroll
-      for (int o = 1; o < 32; o *= 2) {
-        const int y = __shfl_up_sync(0xffffffffu, above, o);
-        if (lane >= o) above += y;
-      }
-      if (lane == 31) sums[0][warp] = above;
-      __syncthreads();
-      above -= all;
-      for (int w = 0; w < warp; ++w) above += sums[0][w];
-#pragma unroll
-      for (int k = 0; k < EACH; ++k) {
-        if (above < left && above + mine[k] >= left) {
-          s_digit = (uint32_t)(DIGITS - 1 - (tid * EACH + k));
-          s_left = left - above;
+        for (int k = 0; k < EVICT_PER; ++k) {
+          if (k >= in_use) continue;
+          const uint32_t u = ordered_bits(v[k]);
+          if (base + rank * PART + k * THREADS + tid < old &&
+              (round == 0 || (u >> (shift + 8)) == (prefix >> (shift + 8))))
+            atomicAdd(&mine[(u >> shift) & 255], 1);
         }
-        above += mine[k];
+      }
+      cluster_sync();              // every block has counted, and read the counts before these
+      hist[(round + 1) & 1][tid] = 0;
+      int sum = 0;
+      for (int r = 0; r < cluster; ++r) sum += (int)remote_load(remote(&mine[tid], r));
+      merged[tid] = sum;
+      __syncthreads();
+      if (tid < 32) {              // the digit where the sum from above passes `left`
+        int some[8], all = 0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) all += some[k] = merged[255 - (tid * 8 + k)];
+        int above = all;
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+          const int y = __shfl_up_sync(0xffffffffu, above, o);
+          if (tid >= o) above += y;
+        }
+        above -= all;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          if (above < left && above + some[k] >= left) {
+            s_digit = (uint32_t)(255 - (tid * 8 + k));
+            s_left = left - above;
+          }
+          above += some[k];
+        }
       }
       __syncthreads();
       prefix |= s_digit << shift;
@@ -160,51 +183,69 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const CacheEvictA
     }
   }
   // in order of the slots: those above `prefix`, the first `left` of those equal to it, and
-  // the recent ones
-  __syncthreads();                 // (mass of all slots is read before `out` is written)
-  const int part = ((n + WARPS - 1) / WARPS + 31) / 32 * 32, from = min(n, warp * part), to = min(n, from + part);
-  auto more = [&](uint32_t u, int i) { return i >= old || (need > 0 && u > prefix); };
-  auto equal = [&](uint32_t u, int i) { return i < old && need > 0 && u == prefix; };
-  int sure = 0, ties = 0;
-  for (int base = from; base < to; base += 32) {
-    const int i = base + lane;
-    const uint32_t u = i < to ? ordered_bits(mass[i]) : 0;
-    sure += __popc(__ballot_sync(0xffffffffu, i < to && more(u, i)));
-    ties += __popc(__ballot_sync(0xffffffffu, i < to && equal(u, i)));
-  }
-  if (lane == 0) {
-    sums[0][warp] = sure;
-    sums[1][warp] = ties;
-  }
-  __syncthreads();
-  int at = 0, tie = 0;
-  for (int w = 0; w < warp; ++w) {
-    at += sums[0][w];
-    tie += sums[1][w];
-  }
-  at += min(tie, left);
-  // A warp's part may be written while another's is still to be read: only where mass is staged,
-  // or `out` is another tensor, may all go on at once.
-  const bool apart = in_smem || out != row;
-  for (int turn = 0; turn < (apart ? 1 : WARPS); ++turn) {
-    if (!apart) __syncthreads();
-    if (apart || turn == warp)
-      for (int base = from; base < to; base += 32) {
-        const int i = base + lane;
-        const float m = i < to ? mass[i] : 0.0f;
-        const uint32_t u = ordered_bits(m);
-        const unsigned is_tie = __ballot_sync(0xffffffffu, i < to && equal(u, i));
-        const bool mine = i < to && equal(u, i) && tie + __popc(is_tie & ((1u << lane) - 1)) < left;
-        const bool take = i < to && (more(u, i) || mine);
-        const unsigned takers = __ballot_sync(0xffffffffu, take);
-        const int place = at + __popc(takers & ((1u << lane) - 1));
-        if (take) {
-          kept[place] = i;
-          out[place] = m;
-        }
-        at += __popc(takers);
-        tie += __popc(is_tie);
+  // the recent ones.  (A chunk is in all blocks' registers before any of it is written, and what it
+  // writes is not behind it: `out` may be the mass itself.)
+  int taken = 0, tied = 0, turn = 0;       // of the chunks before
+  for (int64_t base = 0; base < n; base += chunk, turn ^= 1) {
+    if (n > chunk) load((int)base);
+    const int in_use = steps((int)base, n);
+    uint32_t sure = 0, tie = 0;            // of this thread's slots, a bit each
+#pragma unroll
+    for (int k = 0; k < EVICT_PER; ++k) {
+      u64 both = 0;
+      if (k < in_use) {
+        const int64_t i = base + rank * PART + k * THREADS + tid;
+        const uint32_t u = ordered_bits(v[k]);
+        const bool s = i < n && (i >= old || (need > 0 && u > prefix));
+        const bool t = i < old && need > 0 && u == prefix;
+        sure |= (uint32_t)s << k;
+        tie |= (uint32_t)t << k;
+        both = (u64)__popc(__ballot_sync(0xffffffffu, s)) << 32 | __popc(__ballot_sync(0xffffffffu, t));
       }
+      if (lane == 0) counts[k * WARPS + warp] = both;
+    }
+    __syncthreads();
+    // the warps' counts of all steps, summed over those before
+    u64 upto = tid < EVICT_PER * WARPS ? counts[tid] : 0;
+    const u64 one = upto;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const u64 y = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += y;
+    }
+    if (lane == 31) sums[warp] = upto;
+    __syncthreads();
+    u64 before = 0, mine = 0;
+    for (int w = 0; w < WARPS; ++w) {
+      before += w < warp ? sums[w] : 0;
+      mine += sums[w];
+    }
+    if (tid < cluster) remote_store(remote(&of_block[turn][rank], tid), mine);
+    cluster_sync();                        // (a chunk on, the other half is written: read by then)
+    u64 earlier = 0, whole = 0;
+    for (int r = 0; r < cluster; ++r) {
+      earlier += r < rank ? of_block[turn][r] : 0;
+      whole += of_block[turn][r];
+    }
+    if (tid < EVICT_PER * WARPS) counts[tid] = earlier + before + upto - one;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < EVICT_PER; ++k) {
+      if (k >= in_use) continue;
+      const u64 first = counts[k * WARPS + warp];
+      const bool t = tie >> k & 1;
+      const unsigned ties = __ballot_sync(0xffffffffu, t), low = (1u << lane) - 1;
+      const int tie_rank = tied + (int)(uint32_t)first + __popc(ties & low);
+      const unsigned sures = __ballot_sync(0xffffffffu, sure >> k & 1);
+      const int place = taken + (int)(first >> 32) + __popc(sures & low) + min(tie_rank, left);
+      if ((sure >> k & 1) || (t && tie_rank < left)) {
+        kept[place] = (int)base + rank * PART + k * THREADS + tid;
+        out[place] = v[k];
+      }
+    }
+    taken += (int)(whole >> 32);
+    tied += (int)(uint32_t)whole;
+    __syncthreads();
   }
 }
 
@@ -337,16 +378,6 @@ int move(const CacheEvictArgs& a, cudaStream_t stream) {
   return cuda_status(cudaLaunchKernelEx(&cfg, kernel, a, words, width, slices));
 }
 
-template <int THREADS>
-int select(const CacheEvictArgs& a, cudaStream_t stream) {
-  const int staged = std::min(a.capacity, STAGED);
-  auto* kernel = evict_select_kernel<THREADS>;
-  const int st = allow_smem((const void*)kernel, (size_t)staged * 4);
-  if (st != TP_OK) return st;
-  kernel<<<(unsigned)(a.B * a.c.heads), THREADS, (size_t)staged * 4, stream>>>(a, staged);
-  return launch_status();
-}
-
 // the widest word (16, 8, 4 or 2 bytes) that divides all of them
 int word_bytes(std::initializer_list<int64_t> of) {
   int64_t all = 0;
@@ -371,7 +402,12 @@ int launch_paged_append(const PagedAppendArgs& a, cudaStream_t stream) {
 
 int launch_cache_evict(const CacheEvictArgs& a, cudaStream_t stream) {
   const PagedCache& c = a.c;
-  const int st = a.capacity <= 4096 ? select<256>(a, stream) : select<1024>(a, stream);
+  int cluster = 1;
+  while (cluster < MAX_CLUSTER && a.capacity > cluster * EVICT_THREADS * EVICT_PER &&
+         a.B * c.heads * cluster * 2 <= 8 * num_sms())
+    cluster *= 2;
+  const int st = launch_clusters(evict_select_kernel, a.B * c.heads * cluster, EVICT_THREADS, cluster,
+                                 stream, a, cluster);
   if (st != TP_OK) return st;
   switch (word_bytes({(int64_t)c.channels * c.esize, address(c.k), c.k_page, c.k_slot, c.k_head,
                       address(c.v), c.v_page, c.v_slot, c.v_head})) {

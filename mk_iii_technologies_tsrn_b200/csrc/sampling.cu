@@ -25,17 +25,16 @@
 //     CANDIDATES, the threshold is found bit by bit over all tokens.
 #include <algorithm>
 
+#include "cluster.cuh"
 #include "decode.cuh"
 
 namespace tp {
 
 namespace {
 
-constexpr int THREADS = 1024, WARPS = THREADS / 32, BINS = 2048, CANDIDATES = 1024, MAX_CLUSTER = 8;
+constexpr int THREADS = 1024, WARPS = THREADS / 32, BINS = 2048, CANDIDATES = 1024;
 constexpr double UNIT = 17592186044416.0;       // 2^44
 constexpr float REACH = 31.5f;                  // w < 2^-45 beyond this many units of temperature
-
-typedef unsigned long long u64;
 
 struct Shared {
   u64 exchange[2][2][MAX_CLUSTER];
@@ -50,36 +49,6 @@ struct Shared {
   uint32_t cut;
   int ties;
 };
-
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
-}
-__device__ __forceinline__ uint32_t remote(const void* p, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(tp_smem_addr(p)), "r"(rank));
-  return r;
-}
-__device__ __forceinline__ void remote_store(uint32_t at, u64 v) {
-  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(at), "l"(v) : "memory");
-}
-__device__ __forceinline__ void remote_store(uint32_t at, int v) {
-  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
-}
-__device__ __forceinline__ uint32_t remote_load(uint32_t at) {
-  uint32_t v;
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
-  return v;
-}
-__device__ __forceinline__ int remote_add(uint32_t at, int v) {
-  int old;
-  asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(old) : "r"(at), "r"(v) : "memory");
-  return old;
-}
 
 // floats in order as unsigned numbers; NaN counts as -inf
 __device__ __forceinline__ uint32_t key_of(float x) {
@@ -586,18 +555,7 @@ int sample(const SampleArgs& a, cudaStream_t stream) {
          a.B * cluster * 2 <= num_sms())
     cluster *= 2;
   TP_RETURN_IF(a.B * cluster > INT32_MAX, TP_ERR_TOO_LARGE);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(a.B * cluster));
-  cfg.blockDim = dim3(THREADS);
-  cfg.stream = stream;
-  cudaLaunchAttribute together;
-  together.id = cudaLaunchAttributeClusterDimension;
-  together.val.clusterDim.x = cluster;
-  together.val.clusterDim.y = 1;
-  together.val.clusterDim.z = 1;
-  cfg.attrs = &together;
-  cfg.numAttrs = 1;
-  return cuda_status(cudaLaunchKernelEx(&cfg, sample_kernel<T>, a, cluster));
+  return launch_clusters(sample_kernel<T>, a.B * cluster, THREADS, cluster, stream, a, cluster);
 }
 
 }  // namespace

@@ -61,6 +61,8 @@ CASES = [
     (4, 1, 16, 50, 16, 60, 20, "slots"),             # room for all
     (1, 2, 256, 1025, 16, 512, 100, "slots"),
     (1, 1, 4, 9000, 16, 100, 3, "slots"),
+    (1, 2, 4, 70000, 64, 40000, 1000, "slots"),      # more than stays in a block's registers
+    (1, 1, 1, 33000, 100, 32900, 0, "slots"),
 ]
 
 
