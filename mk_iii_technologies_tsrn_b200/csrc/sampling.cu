@@ -32,17 +32,20 @@ namespace tp {
 
 namespace {
 
-constexpr int THREADS = 1024, WARPS = THREADS / 32, BINS = 2048, CANDIDATES = 1024;
+constexpr int BINS = 2048;
 constexpr double UNIT = 17592186044416.0;       // 2^44
 constexpr float REACH = 31.5f;                  // w < 2^-45 beyond this many units of temperature
 
+template <int THREADS>
 struct Shared {
+  static constexpr int WARPS = THREADS / 32, CANDIDATES = THREADS;      // a candidate for each thread
   u64 exchange[2][2][MAX_CLUSTER];
   u64 reduce[2][WARPS];
   u64 candidate[2][CANDIDATES];        // of the bins before the border's, and of that
   u64 weight[CANDIDATES];
   u64 warp_sum[WARPS];
   u64 before_border, sum_all;
+  double table[32];
   uint32_t low[BINS], high[BINS];      // counts, or weights in two halves
   int warp_ties[WARPS];
   int count[2], border;
@@ -60,8 +63,6 @@ __device__ __forceinline__ float value_of(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
-constexpr uint32_t LOWEST = 0x007fffffu;          // key_of(-inf)
-
 struct Add {
   __device__ __forceinline__ u64 operator()(u64 a, u64 b) const { return a + b; }
 };
@@ -78,77 +79,98 @@ __device__ __forceinline__ u64 warp_inclusive(u64 v, int lane) {
   return v;
 }
 
+// A warp's part of a row, in steps of 16 bytes a lane.  They lie on 16-byte boundaries wherever the
+// row begins; where a step reaches over an end of the row it takes single numbers, and -inf for those
+// that are not there.
 template <typename T>
 struct Row {
   static constexpr int PER = 16 / sizeof(T);      // tokens of a lane's step, next to one another
   const T* x;
-  int begin, end;                                 // this warp's part of the row
-  bool vec;
+  int off, begin, end;                            // tokens before x to a boundary; part, counted from there
 
-  // f(first index, values, how many) of each step's PER tokens of this lane; the whole warp runs
-  // every step
+  __device__ __forceinline__ Row(const T* row, int V, int part, int parts) : x(row) {
+    off = (int)(((uintptr_t)row & 15) / sizeof(T));
+    const int per = ((V + off + parts - 1) / parts + PER - 1) / PER * PER;
+    const int64_t first = (int64_t)part * per;
+    begin = (int)min((int64_t)V + off, first);
+    end = (int)min((int64_t)V + off, first + per);
+  }
+  // f(index of the first, values) of each step of this lane; the whole warp runs every step
   template <typename F>
   __device__ __forceinline__ void each(F f) const {
-    const int lane = threadIdx.x & 31;
-    for (int i0 = begin; i0 < end; i0 += 32 * PER) {
-      const int i = i0 + lane * PER;
-      const int some = max(0, min(PER, end - i));
+    for (int p0 = begin; p0 < end; p0 += 32 * PER) {
+      const int p = p0 + ((int)threadIdx.x & 31) * PER;
       float v[PER];
-      load(i, some, v);
-      f(i, v, some);
-    }
-  }
-  __device__ __forceinline__ void load(int i, int some, float (&v)[PER]) const {
-    if (vec && some == PER) {
-      const uint4 u = __ldg((const uint4*)(x + i));
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-      if constexpr (sizeof(T) == 4) {
+      if (p >= off && p + PER <= end) {
+        const uint4 u = __ldg((const uint4*)(x + (p - off)));
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+        if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = __uint_as_float(w[k]);
+          for (int k = 0; k < 4; ++k) v[k] = __uint_as_float(w[k]);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            v[2 * k] = __uint_as_float(w[k] << 16);
+            v[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+          }
+        }
       } else {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          v[2 * k] = __uint_as_float(w[k] << 16);
-          v[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
-        }
+        for (int k = 0; k < PER; ++k)
+          v[k] = p + k >= off && p + k < end ? tp_load_as_f32<T>(x + (p + k - off))
+                                             : -__int_as_float(0x7f800000);
       }
-    } else {
-#pragma unroll
-      for (int k = 0; k < PER; ++k) v[k] = k < some ? tp_load_as_f32<T>(x + i + k) : 0.0f;
+      f(p - off, v);
     }
   }
 };
 
+// w = exp((x - top) / temperature) = 2^t as 2^n 2^(j / 32) 2^f with |f| <= 1 / 64: the middle factor
+// from a table, the last by its Taylor series to f^5 (the rest is below (ln 2 / 64)^6 / 720 <
+// 2^-48).  An exponential of full precision and its conversion to an integer took 100 instructions
+// of a token, this takes 25.
 struct Weights {
   float top;
-  double top64, per;              // the maximum, 1 / temperature
+  double top64, per, per2;        // the maximum, 1 / temperature, and that for base 2
+  const double* table;            // 2^(j / 32)
   __device__ __forceinline__ double real(float x) const {
     if (x == top) return 1.0;
-    if (!(x > -__int_as_float(0x7f800000))) return 0.0;
-    return exp(((double)x - top64) * per);
+    const double t = ((double)x - top64) * per2;
+    if (!(t > -60.0)) return 0.0;                        // (and NaN)
+    const double shift = 0x1.8p47;                       // t to a 32nd, in its low bits
+    const double s = t + shift, f = t - (s - shift);
+    const int at = __double2loint(s), j = at & 31, n = at >> 5;
+    const double z = f * 0.693147180559945309417;
+    double p = fma(z, 1.0 / 120, 1.0 / 24);
+    p = fma(z, p, 1.0 / 6);
+    p = fma(z, p, 0.5);
+    p = fma(z, p, 1.0);
+    p = fma(z, p, 1.0) * table[j];
+    return __hiloint2double(__double2hiint(p) + (n << 20), __double2loint(p));
   }
-  __device__ __forceinline__ u64 whole(double w) const { return (u64)__double2ll_rn(w * UNIT); }
+  // w * 2^44 to the nearest, read from the low bits of a sum
+  __device__ __forceinline__ u64 whole(double w) const {
+    return (u64)__double_as_longlong(fma(w, UNIT, 0x1p52)) & 0xfffffffffffffull;
+  }
 };
 
-template <typename T>
+template <typename T, int THREADS>
 __global__ void __launch_bounds__(THREADS) sample_kernel(const SampleArgs a, int cluster) {
-  __shared__ Shared s;
+  constexpr int WARPS = THREADS / 32, CANDIDATES = THREADS;
+  __shared__ Shared<THREADS> s;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t rank = cluster_rank();
   const int64_t b = blockIdx.x / cluster;
   const int V = (int)a.V;
 
-  Row<T> row;
-  row.x = (const T*)a.logits + b * a.ld;
-  row.vec = (((uintptr_t)row.x) & 15) == 0;
-  {
-    constexpr int P = Row<T>::PER;
-    const int parts = cluster * WARPS;
-    const int per = ((V + parts - 1) / parts + P - 1) / P * P;
-    const int64_t begin = (int64_t)((int)rank * WARPS + warp) * per;
-    row.begin = (int)min((int64_t)V, begin);
-    row.end = (int)min((int64_t)V, begin + per);
-  }
+  const Row<T> row((const T*)a.logits + b * a.ld, V, (int)rank * WARPS + warp, cluster * WARPS);
+
+  // (asked for before the logits: their loads are under way together)
+  const double temperature = a.temperature.of_row ? (double)a.temperature.of_row[b] : a.temperature.all;
+  const double top_p = a.top_p.of_row ? (double)a.top_p.of_row[b] : a.top_p.all;
+  const double min_p = a.min_p.of_row ? (double)a.min_p.of_row[b] : a.min_p.all;
+  const int64_t asked = a.top_k_of_row ? (int64_t)a.top_k_of_row[b] : a.top_k;
+  const double u = a.uniform64 ? ((const double*)a.uniform)[b] : (double)((const float*)a.uniform)[b];
 
   // Sum (or maximum) of v over the cluster's threads.  Two calls' slots never meet: a block is
   // past a call's barrier only when all have read the one before.
@@ -159,7 +181,7 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const SampleArgs a, int
     if (lane == 0) s.reduce[which][warp] = v;
   };
   auto finish = [&](int which, auto op) {         // after a __syncthreads: one warp, to every block
-    u64 v = s.reduce[which][lane];
+    u64 v = lane < WARPS ? s.reduce[which][lane] : 0;
 #pragma unroll
     for (int o = 16; o > 0; o /= 2) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
     if (lane < cluster) remote_store(remote(&s.exchange[calls & 1][which][rank], lane), v);
@@ -181,20 +203,24 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const SampleArgs a, int
 
   // ---- the best token, of this thread and of all; the lowest number
   if (tid < 2) s.count[tid] = 0;
+  if (tid < 32) s.table[tid] = exp2(tid / 32.0);
   for (int i = tid; i < BINS; i += THREADS) s.low[i] = s.high[i] = 0;
-  u64 best = 0;
-  uint32_t least = 0;                   // the largest of the inverted keys above -inf's
-  row.each([&](int i, const float* v, int some) {
+  const float inf = __int_as_float(0x7f800000);
+  float mine_best = -inf, lowest = inf;
+  int mine_at = 0;                      // (a row without a token above -inf is none to take from)
+  row.each([&](int i, const float* v) {
 #pragma unroll
     for (int k = 0; k < Row<T>::PER; ++k) {
-      if (k >= some) continue;
-      const uint32_t key = key_of(v[k]);
-      const u64 c = (u64)key << 32 | (0xffffffffu - (uint32_t)(i + k));
-      best = c > best ? c : best;
-      if (key > LOWEST) least = max(least, ~key);
+      const float x = v[k];
+      if (x > mine_best) {              // (the first of equals; NaN is not)
+        mine_best = x;
+        mine_at = i + k;
+      }
+      if (x > -inf) lowest = fminf(lowest, x);
     }
   });
-  const float mine_best = best ? value_of((uint32_t)(best >> 32)) : -__int_as_float(0x7f800000);
+  u64 best = (u64)key_of(mine_best) << 32 | (0xffffffffu - (uint32_t)mine_at);
+  uint32_t least = ~key_of(lowest);     // (the largest of the inverted keys)
   all(best, 0, Max());
   all(least, 1, Max());
   __syncthreads();
@@ -209,14 +235,10 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const SampleArgs a, int
   Weights wt;
   wt.top = value_of((uint32_t)(best >> 32));
   const int first = (int)(0xffffffffu - (uint32_t)best);
-  const double temperature = a.temperature.of_row ? (double)a.temperature.of_row[b] : a.temperature.all;
-  const double top_p = a.top_p.of_row ? (double)a.top_p.of_row[b] : a.top_p.all;
-  const double min_p = a.min_p.of_row ? (double)a.min_p.of_row[b] : a.min_p.all;
-  const int64_t asked = a.top_k_of_row ? (int64_t)a.top_k_of_row[b] : a.top_k;
   const bool by_k = asked > 0 && asked < V, by_p = top_p < 1.0;
   const int top_k = by_k ? (int)asked : V;
   const bool leader = rank == 0 && tid == 0;
-  if (wt.top == -__int_as_float(0x7f800000)) {                   // nothing to take
+  if (wt.top == -inf) {                   // nothing to take
     if (leader) {
       a.token[b] = -1;
       if (a.logprob) a.logprob[b] = __int_as_float(0x7fc00000);
@@ -232,7 +254,8 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const SampleArgs a, int
   }
   wt.top64 = (double)wt.top;
   wt.per = 1.0 / temperature;
-  const double u = a.uniform64 ? ((const double*)a.uniform)[b] : (double)((const float*)a.uniform)[b];
+  wt.per2 = wt.per * 1.44269504088896340736;
+  wt.table = s.table;
   // the place in the running sum: the first token whose sum is above it
   auto place = [&](u64 total) {
     const double t = u * (double)total;
@@ -249,7 +272,7 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const SampleArgs a, int
   if (by_k || by_p) {
     // ---- bins below the maximum, down to the lowest number or to where a token weighs nothing
     const float span = wt.top - value_of(~least);
-    const float reach = fminf((float)(REACH * temperature), span), bins_per = BINS / reach;
+    const float reach = fminf(fminf((float)(REACH * temperature), span), 3e38f), bins_per = BINS / reach;
     auto bin_of = [&](float x) {        // BINS: weighs nothing
       if (x == wt.top) return 0;
       const float d = wt.top - x;
@@ -260,8 +283,9 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const SampleArgs a, int
       const int bin = bin_of(mine_best);
       if (bin < BINS) atomicAdd(&s.low[bin], 1u);
     } else {
-      row.each([&](int i, const float* v, int some) {
-        for (int k = 0; k < some; ++k) {
+      row.each([&](int i, const float* v) {
+#pragma unroll
+        for (int k = 0; k < Row<T>::PER; ++k) {
           const int bin = bin_of(v[k]);
           if (bin >= BINS) continue;
           if (by_k) {
@@ -277,32 +301,44 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const SampleArgs a, int
     }
     cluster_sync();
     if (rank == 0) {                    // the border's bin: the first where the sum reaches it
-      u64 mine[2] = {0, 0};
-      for (int r = 0; r < cluster; ++r)
+      constexpr int EACH = BINS / THREADS;
+      u64 mine[EACH], at = 0;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          mine[k] += remote_load(remote(&s.low[2 * tid + k], r));
-          if (!by_k) mine[k] += (u64)remote_load(remote(&s.high[2 * tid + k], r)) << 32;
+      for (int k = 0; k < EACH; ++k) {
+        mine[k] = 0;
+        for (int r = 0; r < cluster; ++r) {
+          mine[k] += remote_load(remote(&s.low[EACH * tid + k], r));
+          if (!by_k) mine[k] += (u64)remote_load(remote(&s.high[EACH * tid + k], r)) << 32;
         }
-      u64 at = warp_inclusive(mine[0] + mine[1], lane);
+        at += mine[k];
+      }
+      const u64 own = at;
+      at = warp_inclusive(at, lane);
       if (lane == 31) s.warp_sum[warp] = at;
       if (tid == 0) s.border = BINS;
       __syncthreads();
+      at -= own;
       u64 everything = 0;
       for (int w = 0; w < WARPS; ++w) {
         at += w < warp ? s.warp_sum[w] : 0;
         everything += s.warp_sum[w];
       }
       // (with top_k above the universe's tokens: the last bin that has any)
-      const u64 first = at - mine[1], none = first - mine[0];
       auto reaches = [&](u64 sum) {
         return by_k ? sum >= min((u64)top_k, everything) : (double)sum >= top_p * (double)everything;
       };
-      if (reaches(at) && !reaches(none) && !(of_threads && everything < (u64)top_k)) {
-        const int border = reaches(first) ? 2 * tid : 2 * tid + 1;
-        s.border = border;
-        s.before_border = border & 1 ? first : none;
-        s.sum_all = everything;
+      if (!reaches(at) && reaches(at + own) && !(of_threads && everything < (u64)top_k)) {
+        bool found = false;
+#pragma unroll
+        for (int k = 0; k < EACH; ++k) {
+          if (!found && reaches(at + mine[k])) {
+            found = true;
+            s.border = EACH * tid + k;
+            s.before_border = at;
+            s.sum_all = everything;
+          }
+          at += mine[k];
+        }
       }
       // (fewer threads with a token than top_k: all tokens that weigh something)
       if (of_threads && everything < (u64)top_k && tid == 0) s.border = BINS - 1;
@@ -314,26 +350,47 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const SampleArgs a, int
     }
     cluster_sync();
     const int border = s.border;
-    // ---- gather
-    row.each([&](int i, const float* v, int some) {
+    // ---- gather: the border's bin and, at once under top_k, where they are needed as a rule, the
+    // bins before it; under top_p these are counted first
+    const float past = border < BINS - 1 ? (float)(border + 1) : inf;
+    auto gather = [&](bool before, bool at_border) {
+      int counted = 0;
+      row.each([&](int i, const float* v) {
+        bool any = false;
 #pragma unroll
-      for (int k = 0; k < Row<T>::PER; ++k) {
-        const int bin = k < some ? bin_of(v[k]) : BINS;
-        if (!__any_sync(0xffffffffu, bin <= border && bin < BINS)) continue;
-#pragma unroll
-        for (int list = 0; list < 2; ++list) {
-          const bool take = list ? bin == border && bin < BINS : bin < border;
-          const uint32_t takers = __ballot_sync(0xffffffffu, take);
-          if (!takers) continue;
-          int at = 0;
-          if (lane == __ffs(takers) - 1) at = remote_add(remote(&s.count[list], 0), __popc(takers));
-          at = __shfl_sync(0xffffffffu, at, __ffs(takers) - 1) + __popc(takers & ((1u << lane) - 1));
-          if (take && at < CANDIDATES)
-            remote_store(remote(&s.candidate[list][at], 0),
-                         (u64)key_of(v[k]) << 32 | (0xffffffffu - (uint32_t)(i + k)));
+        for (int k = 0; k < Row<T>::PER; ++k) {        // (bin_of(x) <= border)
+          const float d = wt.top - v[k];
+          any |= (d <= reach && d * bins_per < past) || v[k] == wt.top;
         }
-      }
-    });
+        if (!__any_sync(0xffffffffu, any)) return;
+#pragma unroll
+        for (int k = 0; k < Row<T>::PER; ++k) {
+          const int bin = bin_of(v[k]);
+          counted += bin < border;
+#pragma unroll
+          for (int list = 0; list < 2; ++list) {
+            const bool take = list ? at_border && bin == border && bin < BINS : before && bin < border;
+            const uint32_t takers = __ballot_sync(0xffffffffu, take);
+            if (!takers) continue;
+            int at = 0;
+            if (lane == __ffs(takers) - 1) at = remote_add(remote(&s.count[list], 0), __popc(takers));
+            at = __shfl_sync(0xffffffffu, at, __ffs(takers) - 1) + __popc(takers & ((1u << lane) - 1));
+            if (take && at < CANDIDATES)
+              remote_store(remote(&s.candidate[list][at], 0),
+                           (u64)key_of(v[k]) << 32 | (0xffffffffu - (uint32_t)(i + k)));
+          }
+        }
+      });
+      return counted;
+    };
+    if (by_k) {
+      gather(true, true);
+    } else {
+      const u64 counted = reduce((u64)gather(false, true), Add());
+      // (the border's tokens are in rank 0's count, which only it may look at before a barrier)
+      if (counted <= CANDIDATES) gather(true, false);
+      else if (rank == 0 && tid == 0) s.count[0] = (int)counted;
+    }
     cluster_sync();
     if (rank == 0 && tid > 0 && tid < cluster) {
       remote_store(remote(&s.count[0], tid), s.count[0]);
@@ -429,16 +486,18 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const SampleArgs a, int
     // ---- bit by bit over all tokens
     auto weigh_from = [&](uint32_t key) {
       u64 sum = 0;
-      row.each([&](int i, const float* v, int some) {
-        for (int k = 0; k < some; ++k)
+      row.each([&](int i, const float* v) {
+#pragma unroll
+        for (int k = 0; k < Row<T>::PER; ++k)
           if (key_of(v[k]) >= key) sum += wt.whole(wt.real(v[k]));
       });
       return reduce(sum, Add());
     };
     auto count_from = [&](uint32_t key) {
       u64 sum = 0;
-      row.each([&](int i, const float* v, int some) {
-        for (int k = 0; k < some; ++k) sum += key_of(v[k]) >= key;
+      row.each([&](int i, const float* v) {
+#pragma unroll
+        for (int k = 0; k < Row<T>::PER; ++k) sum += key_of(v[k]) >= key;
       });
       return reduce(sum, Add());
     };
@@ -472,8 +531,9 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const SampleArgs a, int
   int64_t tie_base = 0;
   if (ties != INT64_MAX) {
     u64 mine = 0;
-    row.each([&](int i, const float* v, int some) {
-      for (int k = 0; k < some; ++k) mine += key_of(v[k]) == cut;
+    row.each([&](int i, const float* v) {
+#pragma unroll
+      for (int k = 0; k < Row<T>::PER; ++k) mine += key_of(v[k]) == cut;
     });
 #pragma unroll
     for (int o = 16; o > 0; o /= 2) mine += __shfl_xor_sync(0xffffffffu, mine, o);
@@ -484,10 +544,10 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const SampleArgs a, int
     for (uint32_t r = 0; r < rank; ++r) tie_base += (int64_t)s.exchange[(calls - 1) & 1][0][r];
   }
   // weights of a step's tokens; `base`: ties before the step
-  auto kept = [&](int i, const float* v, int some, int64_t& base, u64 (&w)[Row<T>::PER]) {
+  auto kept = [&](int i, const float* v, int64_t& base, u64 (&w)[Row<T>::PER]) {
     int mine = 0;
 #pragma unroll
-    for (int k = 0; k < Row<T>::PER; ++k) mine += k < some && key_of(v[k]) == cut;
+    for (int k = 0; k < Row<T>::PER; ++k) mine += key_of(v[k]) == cut;
     int64_t at = base;
     if (ties != INT64_MAX) {
       const int upto = (int)warp_inclusive(mine, lane);
@@ -497,7 +557,6 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const SampleArgs a, int
 #pragma unroll
     for (int k = 0; k < Row<T>::PER; ++k) {
       w[k] = 0;
-      if (k >= some) continue;
       const uint32_t key = key_of(v[k]);
       const bool tie = key == cut;
       if (key > cut || (tie && at < ties)) {
@@ -510,9 +569,9 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const SampleArgs a, int
   u64 sum = 0;
   {
     int64_t base = tie_base;
-    row.each([&](int i, const float* v, int some) {
+    row.each([&](int i, const float* v) {
       u64 w[Row<T>::PER];
-      kept(i, v, some, base, w);
+      kept(i, v, base, w);
 #pragma unroll
       for (int k = 0; k < Row<T>::PER; ++k) sum += w[k];
     });
@@ -529,9 +588,9 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const SampleArgs a, int
   if (!(before <= t && t < before + sum)) return;                // another warp's
   int64_t base = tie_base;
   u64 run = before;
-  row.each([&](int i, const float* v, int some) {
+  row.each([&](int i, const float* v) {
     u64 w[Row<T>::PER], mine = 0;
-    kept(i, v, some, base, w);
+    kept(i, v, base, w);
 #pragma unroll
     for (int k = 0; k < Row<T>::PER; ++k) mine += w[k];
     const u64 upto = run + warp_inclusive(mine, lane);
@@ -547,21 +606,27 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const SampleArgs a, int
   });
 }
 
-template <typename T>
+template <typename T, int THREADS>
 int sample(const SampleArgs& a, cudaStream_t stream) {
+  constexpr int WARPS = THREADS / 32;
   // as many blocks for a row as leave its warps a few steps, while the SMs hold all rows' at once
   int cluster = 1;
   while (cluster < MAX_CLUSTER && a.V > (int64_t)cluster * WARPS * 64 * (16 / (int)sizeof(T)) &&
          a.B * cluster * 2 <= num_sms())
     cluster *= 2;
   TP_RETURN_IF(a.B * cluster > INT32_MAX, TP_ERR_TOO_LARGE);
-  return launch_clusters(sample_kernel<T>, a.B * cluster, THREADS, cluster, stream, a, cluster);
+  return launch_clusters(sample_kernel<T, THREADS>, a.B * cluster, THREADS, cluster, stream, a, cluster);
 }
 
 }  // namespace
 
 int launch_sample_tokens(const SampleArgs& a, cudaStream_t stream) {
-  return a.dtype == TP_DTYPE_BF16 ? sample<uint16_t>(a, stream) : sample<float>(a, stream);
+  // (a small vocabulary in small blocks, whose barriers are shorter: 16 rows of 256 logits
+  // 10.5 us in blocks of 1024, 7.5 in these, the launch among them)
+  const bool small = a.V <= 4096;
+  if (a.dtype == TP_DTYPE_BF16)
+    return small ? sample<uint16_t, 256>(a, stream) : sample<uint16_t, 1024>(a, stream);
+  return small ? sample<float, 256>(a, stream) : sample<float, 1024>(a, stream);
 }
 
 }  // namespace tp
