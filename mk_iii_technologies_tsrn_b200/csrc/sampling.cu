@@ -82,6 +82,14 @@ __device__ __forceinline__ u64 warp_inclusive(u64 v, int lane) {
 // A warp's part of a row, in steps of 16 bytes a lane.  They lie on 16-byte boundaries wherever the
 // row begins; where a step reaches over an end of the row it takes single numbers, and -inf for those
 // that are not there.
+// Sum of sums[0 .. warp) over a block's warps, and of all of them.
+template <int WARPS>
+__device__ __forceinline__ u64 before_warp(const u64* sums, int warp, int lane, u64& all) {
+  const u64 mine = lane < WARPS ? sums[lane] : 0, upto = warp_inclusive(mine, lane);
+  all = __shfl_sync(0xffffffffu, upto, WARPS - 1);
+  return __shfl_sync(0xffffffffu, upto - mine, warp);
+}
+
 template <typename T>
 struct Row {
   static constexpr int PER = 16 / sizeof(T);      // tokens of a lane's step, next to one another
@@ -171,10 +179,16 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const SampleArgs a, int
   const double min_p = a.min_p.of_row ? (double)a.min_p.of_row[b] : a.min_p.all;
   const int64_t asked = a.top_k_of_row ? (int64_t)a.top_k_of_row[b] : a.top_k;
   const double u = a.uniform64 ? ((const double*)a.uniform)[b] : (double)((const float*)a.uniform)[b];
+  const bool by_k = asked > 0 && asked < V, by_p = top_p < 1.0;
+  const int top_k = by_k ? (int)asked : V;
 
   // Sum (or maximum) of v over the cluster's threads.  Two calls' slots never meet: a block is
   // past a call's barrier only when all have read the one before.
   int calls = 0;
+  auto meet = [&] {
+    if (cluster > 1) cluster_sync();
+    else __syncthreads();
+  };
   auto all = [&](u64 v, int which, auto op) {
 #pragma unroll
     for (int o = 16; o > 0; o /= 2) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
@@ -195,7 +209,7 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const SampleArgs a, int
     all(v, 0, op);
     __syncthreads();
     if (warp == 0) finish(0, op);
-    cluster_sync();
+    meet();
     const u64 r = joined(0, op);
     ++calls;
     return r;
@@ -208,15 +222,19 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const SampleArgs a, int
   const float inf = __int_as_float(0x7f800000);
   float mine_best = -inf, lowest = inf;
   int mine_at = 0;                      // (a row without a token above -inf is none to take from)
+  const bool of_threads = by_k && top_k <= cluster * THREADS / 8 && V >= cluster * THREADS;
   row.each([&](int i, const float* v) {
+    float top = v[0];
 #pragma unroll
-    for (int k = 0; k < Row<T>::PER; ++k) {
-      const float x = v[k];
-      if (x > mine_best) {              // (the first of equals; NaN is not)
-        mine_best = x;
-        mine_at = i + k;
-      }
-      if (x > -inf) lowest = fminf(lowest, x);
+    for (int k = 1; k < Row<T>::PER; ++k) top = fmaxf(top, v[k]);      // (NaN is not)
+    if (top > mine_best) {              // the first of equals
+      mine_best = top;
+#pragma unroll
+      for (int k = Row<T>::PER - 1; k >= 0; --k) mine_at = v[k] == top ? i + k : mine_at;
+    }
+    if ((by_k || by_p) && !of_threads) {
+#pragma unroll
+      for (int k = 0; k < Row<T>::PER; ++k) lowest = fminf(lowest, v[k] > -inf ? v[k] : inf);
     }
   });
   u64 best = (u64)key_of(mine_best) << 32 | (0xffffffffu - (uint32_t)mine_at);
@@ -228,15 +246,13 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const SampleArgs a, int
     finish(0, Max());
     finish(1, Max());
   }
-  cluster_sync();
+  meet();
   best = joined(0, Max());
   least = (uint32_t)joined(1, Max());
   ++calls;
   Weights wt;
   wt.top = value_of((uint32_t)(best >> 32));
   const int first = (int)(0xffffffffu - (uint32_t)best);
-  const bool by_k = asked > 0 && asked < V, by_p = top_p < 1.0;
-  const int top_k = by_k ? (int)asked : V;
   const bool leader = rank == 0 && tid == 0;
   if (wt.top == -inf) {                   // nothing to take
     if (leader) {
@@ -271,14 +287,13 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const SampleArgs a, int
   int64_t ties = INT64_MAX;
   if (by_k || by_p) {
     // ---- bins below the maximum, down to the lowest number or to where a token weighs nothing
-    const float span = wt.top - value_of(~least);
+    const float span = of_threads ? inf : wt.top - value_of(~least);
     const float reach = fminf(fminf((float)(REACH * temperature), span), 3e38f), bins_per = BINS / reach;
     auto bin_of = [&](float x) {        // BINS: weighs nothing
       if (x == wt.top) return 0;
       const float d = wt.top - x;
       return d <= reach ? min(BINS - 1, (int)(d * bins_per)) : BINS;
     };
-    const bool of_threads = by_k && top_k <= cluster * THREADS / 8 && V >= cluster * THREADS;
     if (of_threads) {
       const int bin = bin_of(mine_best);
       if (bin < BINS) atomicAdd(&s.low[bin], 1u);
@@ -299,30 +314,32 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const SampleArgs a, int
         }
       });
     }
-    cluster_sync();
+    meet();
     if (rank == 0) {                    // the border's bin: the first where the sum reaches it
       constexpr int EACH = BINS / THREADS;
       u64 mine[EACH], at = 0;
 #pragma unroll
-      for (int k = 0; k < EACH; ++k) {
-        mine[k] = 0;
-        for (int r = 0; r < cluster; ++r) {
-          mine[k] += remote_load(remote(&s.low[EACH * tid + k], r));
-          if (!by_k) mine[k] += (u64)remote_load(remote(&s.high[EACH * tid + k], r)) << 32;
-        }
-        at += mine[k];
+      for (int k = 0; k < EACH; ++k) mine[k] = 0;
+#pragma unroll
+      for (int r = 0; r < MAX_CLUSTER; ++r) {          // (without a turn's loads waiting for the last's)
+        if (r >= cluster) continue;
+        uint32_t low[EACH], high[EACH];
+#pragma unroll
+        for (int k = 0; k < EACH; ++k) low[k] = remote_load(remote(&s.low[EACH * tid + k], r));
+#pragma unroll
+        for (int k = 0; k < EACH; ++k) high[k] = by_k ? 0 : remote_load(remote(&s.high[EACH * tid + k], r));
+#pragma unroll
+        for (int k = 0; k < EACH; ++k) mine[k] += (u64)high[k] << 32 | low[k];
       }
+#pragma unroll
+      for (int k = 0; k < EACH; ++k) at += mine[k];
       const u64 own = at;
       at = warp_inclusive(at, lane);
       if (lane == 31) s.warp_sum[warp] = at;
       if (tid == 0) s.border = BINS;
       __syncthreads();
-      at -= own;
-      u64 everything = 0;
-      for (int w = 0; w < WARPS; ++w) {
-        at += w < warp ? s.warp_sum[w] : 0;
-        everything += s.warp_sum[w];
-      }
+      u64 everything;
+      at += before_warp<WARPS>(s.warp_sum, warp, lane, everything) - own;
       // (with top_k above the universe's tokens: the last bin that has any)
       auto reaches = [&](u64 sum) {
         return by_k ? sum >= min((u64)top_k, everything) : (double)sum >= top_p * (double)everything;
@@ -348,20 +365,18 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const SampleArgs a, int
         remote_store(remote(&s.sum_all, tid), s.sum_all);
       }
     }
-    cluster_sync();
+    meet();
     const int border = s.border;
     // ---- gather: the border's bin and, at once under top_k, where they are needed as a rule, the
     // bins before it; under top_p these are counted first
-    const float past = border < BINS - 1 ? (float)(border + 1) : inf;
+    // (no token below `floor` is in them: the border's far end with more than its rounding to spare)
+    const float floor = border < BINS - 1 ? wt.top - (border + 2) / bins_per : -inf;
     auto gather = [&](bool before, bool at_border) {
       int counted = 0;
       row.each([&](int i, const float* v) {
         bool any = false;
 #pragma unroll
-        for (int k = 0; k < Row<T>::PER; ++k) {        // (bin_of(x) <= border)
-          const float d = wt.top - v[k];
-          any |= (d <= reach && d * bins_per < past) || v[k] == wt.top;
-        }
+        for (int k = 0; k < Row<T>::PER; ++k) any |= v[k] >= floor;
         if (!__any_sync(0xffffffffu, any)) return;
 #pragma unroll
         for (int k = 0; k < Row<T>::PER; ++k) {
@@ -391,12 +406,12 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const SampleArgs a, int
       if (counted <= CANDIDATES) gather(true, false);
       else if (rank == 0 && tid == 0) s.count[0] = (int)counted;
     }
-    cluster_sync();
+    meet();
     if (rank == 0 && tid > 0 && tid < cluster) {
       remote_store(remote(&s.count[0], tid), s.count[0]);
       remote_store(remote(&s.count[1], tid), s.count[1]);
     }
-    cluster_sync();
+    meet();
     const int above = s.count[0], in_border = s.count[1], count = above + in_border;
     const u64 sum_all = s.sum_all;      // (under top_p alone: the weight of all)
     const bool few = count <= CANDIDATES;
@@ -425,7 +440,8 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const SampleArgs a, int
         u64 at = warp_inclusive(w, lane);
         if (lane == 31) s.warp_sum[warp] = at;
         __syncthreads();
-        for (int k = 0; k < warp; ++k) at += s.warp_sum[k];
+        u64 sum;
+        at += before_warp<WARPS>(s.warp_sum, warp, lane, sum);
         __syncthreads();
         return at;
       };
@@ -479,7 +495,7 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const SampleArgs a, int
           return;
         }
       }
-      cluster_sync();
+      meet();
       cut = s.cut;
       ties = s.ties;
     }
@@ -581,9 +597,9 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const SampleArgs a, int
   __syncthreads();
   if (lane == 0) s.warp_sum[warp] = sum;
   const u64 total = reduce(lane == 0 ? sum : 0, Add());
-  u64 before = 0;
+  u64 own_block;
+  u64 before = before_warp<WARPS>(s.warp_sum, warp, lane, own_block);
   for (uint32_t r = 0; r < rank; ++r) before += s.exchange[(calls - 1) & 1][0][r];
-  for (int w = 0; w < warp; ++w) before += s.warp_sum[w];
   const u64 t = place(total);
   if (!(before <= t && t < before + sum)) return;                // another warp's
   int64_t base = tie_base;
