@@ -181,25 +181,26 @@ struct TileRows {
   const int kvh;
   int page, slot, whole;               // whole: tiles without the new token or a slot too many
   const unsigned pages;
-  const bool one_page, same;           // a tile is in one page; K and V are strided alike
+  const bool halves, same;             // half a tile is in one page; K and V are strided alike
   __device__ __forceinline__ TileRows(const PagedAttentionArgs& args, int key_head)
       : a(args), kvh(key_head), page(0), slot(0), whole(0),
-        pages((unsigned)min(args.c.pages, (int64_t)INT32_MAX)), one_page(args.c.page_size % TK == 0),
+        pages((unsigned)min(args.c.pages, (int64_t)INT32_MAX)), halves(args.c.page_size % (TK / 2) == 0),
         same(args.c.k_page == args.c.v_page && args.c.k_slot == args.c.v_slot) {}
   __device__ __forceinline__ void ask(const Place& p) {
     whole = (p.n - (a.key != nullptr)) / TK;
     slot = min(p.tile * TK + ((int)threadIdx.x & (TK - 1)), p.n - 1);
     page = __ldg(a.c.table + (int64_t)p.b * a.c.table_row + a.c.column(slot));
   }
-  // Whether all slots of the tile are in one page, and none of them is the new token or behind
-  // the last one; then where the first of them lies behind a slot 0 of page 0.
-  __device__ __forceinline__ bool in_one_page(const Place& p) const {
-    return __all_sync(0xffffffffu, one_page && p.tile < whole && (unsigned)page < pages);
+  // Whether each half of the tile is in one page, and no slot of it the new token's or behind the
+  // last one; then where the half's first slot lies behind slot 0 of page 0.
+  __device__ __forceinline__ bool in_halves(const Place& p) const {
+    return __all_sync(0xffffffffu, halves && p.tile < whole && (unsigned)page < pages);
   }
-  __device__ __forceinline__ void first_of(const Place& p, int64_t& k_at, int64_t& v_at) const {
-    const int first = p.tile * TK, in = a.c.within(first, a.c.column(first));
-    k_at = page * a.c.k_page + in * a.c.k_slot;
-    v_at = same ? k_at : page * a.c.v_page + in * a.c.v_slot;
+  __device__ __forceinline__ void half_at(const Place& p, int half, int64_t& k_at, int64_t& v_at) const {
+    const int first = p.tile * TK + half * (TK / 2), in = a.c.within(first, a.c.column(first));
+    const int64_t its = __shfl_sync(0xffffffffu, page, half * (TK / 2));
+    k_at = its * a.c.k_page + in * a.c.k_slot;
+    v_at = same ? k_at : its * a.c.v_page + in * a.c.v_slot;
   }
   __device__ __forceinline__ void get(const Place& p, const char*& kp, const char*& vp) {
     const int in = a.c.within(slot, a.c.column(slot));
@@ -298,15 +299,18 @@ __global__ void __launch_bounds__(ATT_WARPS * 32) paged_attend_kernel(const Page
       uint4* const dst = ring + (size_t)(i % STAGES) * STAGE;
       const uint32_t to = tp_smem_addr(dst);
       const char* from[2 * ATT_STEPS];                        // K, then V
-      if (rows.in_one_page(ahead)) {
-        int64_t k_at, v_at;
-        rows.first_of(ahead, k_at, v_at);
-        kp = kmine + k_at;
-        vp = vmine + v_at;
+      if (rows.in_halves(ahead)) {
 #pragma unroll
-        for (int step = 0; step < ATT_STEPS; ++step, kp += k_step, vp += v_step) {
-          from[step] = kp;
-          from[ATT_STEPS + step] = vp;
+        for (int half = 0; half < 2; ++half) {
+          int64_t k_at, v_at;
+          rows.half_at(ahead, half, k_at, v_at);
+          kp = kmine + k_at;
+          vp = vmine + v_at;
+#pragma unroll
+          for (int step = half * ATT_STEPS / 2; step < (half + 1) * ATT_STEPS / 2; ++step, kp += k_step, vp += v_step) {
+            from[step] = kp;
+            from[ATT_STEPS + step] = vp;
+          }
         }
       } else {
         rows.get(ahead, kp, vp);
@@ -501,20 +505,34 @@ __global__ void __launch_bounds__(ATT_WARPS * 32) paged_attend_kernel(const Page
 }
 
 // ---------------------------------------------------------------- the rows joined
-// (maximum, sum) over the segments of a head, the same in every lane
+// (maximum, sum) over the segments of a head, the same in every lane; the loads of 256 segments
+// under way together
 __device__ __forceinline__ float2 whole_row(const float2* ml, int64_t stride, int parts) {
   const int lane = threadIdx.x & 31;
   float top = neg_inf(), all = 0.0f;
-  for (int s = lane; s < parts; s += 32) top = fmaxf(top, ml[s * stride].x);
+  for (int s0 = 0; s0 < parts; s0 += 256) {
+    float2 x[8];
 #pragma unroll
-  for (int o = 16; o > 0; o /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  for (int s = lane; s < parts; s += 32) {
-    const float2 x = ml[s * stride];
-    all += x.y * (x.x == neg_inf() ? 0.0f : tp_ex2(x.x - top));
+    for (int k = 0; k < 8; ++k) {
+      const int s = s0 + 32 * k + lane;
+      x[k] = s < parts ? ml[s * stride] : make_float2(neg_inf(), 0.0f);
+    }
+    float most = top;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) most = fmaxf(most, x[k].x);
+    // (a segment without a maximum counts by its sum, 0 or NaN)
+    all = top == neg_inf() ? all : all * tp_ex2(top - most);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) all += x[k].y * (x[k].x == neg_inf() ? 0.0f : tp_ex2(x[k].x - most));
+    top = most;
   }
+  float most = top;
+#pragma unroll
+  for (int o = 16; o > 0; o /= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+  if (top != neg_inf()) all *= tp_ex2(top - most);
 #pragma unroll
   for (int o = 16; o > 0; o /= 2) all += __shfl_xor_sync(0xffffffffu, all, o);
-  return make_float2(top, all);
+  return make_float2(most, all);
 }
 
 // Blocks [0, joins): the segments of JOIN_WARPS / TEAM query heads joined, each by TEAM warps with
@@ -522,13 +540,14 @@ __device__ __forceinline__ float2 whole_row(const float2* ml, int64_t stride, in
 // of a key head, which add the weights to `mass`.
 constexpr int JOIN_WARPS = 8;
 
-template <typename T, int TEAM>
+// KD: channels of a lane.
+template <typename T, int TEAM, int KD>
 __global__ void __launch_bounds__(JOIN_WARPS * 32) paged_join_kernel(const PagedAttentionArgs a, int joins) {
   constexpr int THREADS = JOIN_WARPS * 32;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t G = a.block_heads, stride = (int64_t)a.c.heads * a.head_blocks * G;
   if ((int)blockIdx.x < joins) {
-    __shared__ float sums[TEAM > 1 ? JOIN_WARPS : 1][256];
+    __shared__ float sums[TEAM > 1 ? JOIN_WARPS : 1][32 * KD];
     const int row = blockIdx.x * (JOIN_WARPS / TEAM) + warp / TEAM, member = warp % TEAM;
     const bool there = row < a.B * a.H;
     const int b = there ? row / a.H : 0, h = there ? row - b * a.H : 0;
@@ -536,7 +555,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) paged_join_kernel(const Paged
     const int given = __ldg(a.lengths + b), n = there ? slots_of(a, b) : 0;
     T* const out = (T*)a.out + (int64_t)row * D;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    float sum[8] = {};
+    float sum[KD] = {};
     float all = 1.0f;
     if (n > 0) {
       const int hblk = in_group / (int)G, g = in_group - hblk * (int)G;
@@ -545,33 +564,33 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) paged_join_kernel(const Paged
       const float2* ml = a.ml + first;
       const float2 whole = whole_row(ml, stride, runs.y);
       all = whole.y;
-      constexpr int AT_ONCE = 4;        // segments whose loads are under way together
+      constexpr int AT_ONCE = 32 / KD;  // segments whose loads are under way together
       for (int s0 = member; s0 < runs.y; s0 += AT_ONCE * TEAM) {
-        float f[AT_ONCE], x[AT_ONCE][8];
+        float f[AT_ONCE], x[AT_ONCE][KD];
 #pragma unroll
         for (int u = 0; u < AT_ONCE; ++u) {
           const int s = min(s0 + u * TEAM, runs.y - 1);
           f[u] = ml[s * stride].x;
           const float* p = a.part + (first + s * stride) * D;
 #pragma unroll
-          for (int k = 0; k < 8; ++k) x[u][k] = lane + 32 * k < D ? p[lane + 32 * k] : 0.0f;
+          for (int k = 0; k < KD; ++k) x[u][k] = lane + 32 * k < D ? p[lane + 32 * k] : 0.0f;
         }
 #pragma unroll
         for (int u = 0; u < AT_ONCE; ++u) {
           const bool counts = s0 + u * TEAM < runs.y && f[u] != neg_inf();
           f[u] = counts ? tp_ex2(f[u] - whole.x) : 0.0f;
 #pragma unroll
-          for (int k = 0; k < 8; ++k) sum[k] += x[u][k] * f[u];
+          for (int k = 0; k < KD; ++k) sum[k] += x[u][k] * f[u];
         }
       }
     }
     if constexpr (TEAM > 1) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) sums[warp][lane + 32 * k] = sum[k];
+      for (int k = 0; k < KD; ++k) sums[warp][lane + 32 * k] = sum[k];
       __syncthreads();
       if (member > 0) return;
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
+      for (int k = 0; k < KD; ++k)
 #pragma unroll
         for (int w = 1; w < TEAM; ++w) sum[k] += sums[warp + w][lane + 32 * k];
     }
@@ -581,7 +600,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) paged_join_kernel(const Paged
       all = quiet_nan();
     }
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
+    for (int k = 0; k < KD; ++k)
       if (lane + 32 * k < D) store_as(out + lane + 32 * k, sum[k] / all);
     if (a.key != nullptr && in_group == 0 && n > 0) {     // the new token's row to slot n - 1
       const int column = a.c.column(n - 1), in = a.c.within(n - 1, column);
@@ -660,13 +679,10 @@ int attend_and_join(PagedAttentionArgs& a, K* kernel, size_t smem, int tile, int
   a.block_heads = heads;
   a.head_blocks = (a.group + heads - 1) / heads;
   a.tile = tile;
-#ifndef MIN_TILES
-#define MIN_TILES 2
-#endif
-  // as many runs as the SMs hold warps for, with at least MIN_TILES tiles each
+  // as many runs as the SMs hold warps for, with at least two tiles each
   const int64_t per_sm = std::min<size_t>(ATT_MOST_BLOCKS, (227 * 1024) / (smem + 1024 + 1100));
   const int64_t subs = (int64_t)a.c.heads * a.head_blocks, tiles = a.B * ceil_div(a.capacity, tile);
-  a.runs = (int)std::max<int64_t>(1, std::min(num_sms() * per_sm * ATT_WARPS / subs, ceil_div(tiles, MIN_TILES)));
+  a.runs = (int)std::max<int64_t>(1, std::min(num_sms() * per_sm * ATT_WARPS / subs, ceil_div(tiles, 2)));
   const int64_t blocks = ceil_div(a.runs * subs, ATT_WARPS);
   kernel<<<(unsigned)blocks, ATT_WARPS * 32, smem, stream>>>(a);
   st = launch_status();
@@ -686,16 +702,16 @@ int attend_and_join(PagedAttentionArgs& a, K* kernel, size_t smem, int tile, int
   early.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &early;
   cfg.numAttrs = 1;
-  return cuda_status(team > 1 ? cudaLaunchKernelEx(&cfg, paged_join_kernel<T, JOIN_WARPS>, a, (int)joins)
-                              : cudaLaunchKernelEx(&cfg, paged_join_kernel<T, 1>, a, (int)joins));
+  auto run = [&](auto* one, auto* many) { return cuda_status(cudaLaunchKernelEx(&cfg, team > 1 ? many : one, a, (int)joins)); };
+  return a.c.channels <= 64    ? run(paged_join_kernel<T, 1, 2>, paged_join_kernel<T, JOIN_WARPS, 2>)
+         : a.c.channels <= 128 ? run(paged_join_kernel<T, 1, 4>, paged_join_kernel<T, JOIN_WARPS, 4>)
+                               : run(paged_join_kernel<T, 1, 8>, paged_join_kernel<T, JOIN_WARPS, 8>);
 }
 
-#ifndef CORE_STAGES
-#define CORE_STAGES 3
-#endif
 template <typename T, int LPK, int NCH, int G, bool GATED, bool VEC>
 int attend(PagedAttentionArgs& a, cudaStream_t stream) {
-  constexpr int STAGES = NCH > 1 ? 2 : CORE_STAGES;
+  // (two stages and twelve warps on an SM; three and eight: 32 x 2048 gated slots 31.5 us for 29.0)
+  constexpr int STAGES = 2;
   return attend_and_join<T>(a, paged_attend_kernel<T, LPK, NCH, G, GATED, VEC, STAGES>,
                             (size_t)ATT_WARPS * STAGES * 2 * ATT_STEPS * NCH * 512,
                             ATT_STEPS * 32 / LPK, G, stream);

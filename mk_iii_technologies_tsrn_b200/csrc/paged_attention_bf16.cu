@@ -105,15 +105,18 @@ __global__ void __launch_bounds__(ATT_WARPS * 32) paged_attend_mma_kernel(const 
     if (i < count) {
       const uint32_t to = tp_smem_addr(ring + (size_t)(i % STAGES) * P::STAGE) + mine_at;
       const char *kp, *vp, *kfrom[P::STEPS], *vfrom[P::STEPS];
-      if (rows.in_one_page(ahead)) {
-        int64_t k_at, v_at;
-        rows.first_of(ahead, k_at, v_at);
-        kp = kmine + k_at;
-        vp = vmine + v_at;
+      if (rows.in_halves(ahead)) {
 #pragma unroll
-        for (int s = 0; s < P::STEPS; ++s, kp += k_step, vp += v_step) {
-          kfrom[s] = kp;
-          vfrom[s] = vp;
+        for (int half = 0; half < 2; ++half) {
+          int64_t k_at, v_at;
+          rows.half_at(ahead, half, k_at, v_at);
+          kp = kmine + k_at;
+          vp = vmine + v_at;
+#pragma unroll
+          for (int s = half * P::STEPS / 2; s < (half + 1) * P::STEPS / 2; ++s, kp += k_step, vp += v_step) {
+            kfrom[s] = kp;
+            vfrom[s] = vp;
+          }
         }
       } else {
         rows.get(ahead, kp, vp);
@@ -265,12 +268,9 @@ __global__ void __launch_bounds__(ATT_WARPS * 32) paged_attend_mma_kernel(const 
   tp_cp_async_wait<0>();
 }
 
-#ifndef MMA_STAGES
-#define MMA_STAGES 3
-#endif
 template <int KB>
 int attend_mma(PagedAttentionArgs& a, cudaStream_t stream) {
-  constexpr int STAGES = KB > 4 ? 2 : MMA_STAGES;
+  constexpr int STAGES = KB > 4 ? 2 : 3;
   using P = MmaTile<KB>;
   return attend_and_join<uint16_t>(a, paged_attend_mma_kernel<KB, STAGES>,
                                    (size_t)ATT_WARPS * STAGES * P::STAGE * 16, P::TK, HEADS, stream);
