@@ -20,7 +20,8 @@ int paged_cache(PagedCache& c, int dtype, const tp_paged_cache* p, bool rows) {
     TP_RETURN_IF(s < 0, TP_ERR_INVALID_ARG);
   // (slots are counted in 32 bits; tiles look a few past the end)
   TP_RETURN_IF(p->page_size > INT32_MAX || p->table_cols > INT32_MAX || p->heads > INT32_MAX ||
-                   p->channels > INT32_MAX / 8 ||
+                   p->channels > INT32_MAX / 16 ||
+                   (p->channels > 0 && p->heads > INT32_MAX / 16 / p->channels) ||
                    (p->table_cols > 0 && p->page_size > ((int64_t)INT32_MAX - 65536) / p->table_cols),
                TP_ERR_TOO_LARGE);
   if (rows && p->table_cols > 0) {

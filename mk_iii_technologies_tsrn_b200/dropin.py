@@ -543,9 +543,10 @@ class TropicalDecoderModel(_TokenModel):
         attention weight staying.  Needs a CUDA device and a model in eval mode (or without
         dropout)."""
         B, L = input_ids.shape
-        if max_new_tokens < 1 or L + max_new_tokens - 1 > self.pos_embed.num_embeddings:
-            raise ValueError(f"{L} tokens and {max_new_tokens} new ones: needs at least one new "
-                             f"one, within {self.pos_embed.num_embeddings} positions")
+        if L < 1 or max_new_tokens < 1 or \
+                L + max_new_tokens - 1 > self.pos_embed.num_embeddings:
+            raise ValueError(f"{L} tokens and {max_new_tokens} new ones: needs at least one of "
+                             f"each, within {self.pos_embed.num_embeddings} positions")
         if keep is not None and (keep < 1 or not 0 <= (recent or 0) <= keep):
             raise ValueError("keep must be at least 1 and recent from 0 to keep, got "
                              f"{keep} and {recent}")

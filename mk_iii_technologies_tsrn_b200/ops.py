@@ -1668,7 +1668,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     ``mass``: [B, Hkv, slots] float32 (slots contiguous): the softmax weights, summed over the
     query heads of a key head, are added to it in place, for :func:`cache_evict`; with ``key`` the
     new slot is set to its weight.  Scores, statistics and sums are float32.  Returns
-    [B, H, D] in q's dtype.  Not differentiable.
+    [B, H, D] in q's dtype.  Not differentiable.  The same inputs give the same bits; with other
+    sequences around it a sequence's sums may be cut, and so rounded, elsewhere.
 
     A length beyond the table (or beyond ``mass``), or a page outside the cache, makes the
     sequence's rows NaN, and :func:`check_device_error` raises :class:`DeviceIndexError`.
@@ -1741,7 +1742,7 @@ def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch
     the last ``recent`` slots stay, and of the others those with the most accumulated attention
     weight ``mass`` [B, Hkv, slots] (of equals the lower slot; NaN counts as the most), ``keep`` in
     all.  Their rows move to the front of the sequence's pages, in their order; ``mass`` (or
-    ``out``) gets theirs likewise.  What lies behind is left as it was.
+    ``out``, memory of its own) gets theirs likewise.  What lies behind is left as it was.
 
     Returns kept [B, Hkv, keep] int32, the slots that stayed (-1 behind a shorter sequence's).
     ``lengths`` is not changed, as layers share it: ``lengths.clamp_(max=keep)`` after the last
@@ -1769,13 +1770,9 @@ def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch
     return kept if kept is not None else _refused()
 
 
-def _choice(x, what, off, ok, dtype=torch.float32):
-    """(number, tensor of the rows or None) of a sampling choice."""
-    if isinstance(x, torch.Tensor):
-        return off, x if x.dtype == dtype and x.is_contiguous() else x.to(dtype).contiguous()
-    if not ok(x):
-        raise ValueError(f"{what}, got {x}")
-    return x, None
+def _choice(x, dtype=torch.float32):
+    """A sampling choice of each row as the kernel reads it."""
+    return x if x.dtype == dtype and x.is_contiguous() else x.to(dtype).contiguous()
 
 
 def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature=1.0, top_k=0,
@@ -1797,10 +1794,23 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature=1.
     row of nothing but -inf gives -1.  In tensors top_k <= 0 and top_p >= 1 are off.  Returns the
     tokens [B] int64, with ``return_logprob`` also the float32 log of each one's share of the kept
     weight (NaN for a token of -1)."""
-    T, Ts = _choice(temperature, "temperature must be 0 or more", 1.0, lambda t: t >= 0.0)
-    k, ks = _choice(top_k, "top_k must be 0 or more", 0, lambda n: n >= 0, torch.int32)
-    p, ps = _choice(top_p, "top_p must be above 0 and at most 1", 1.0, lambda t: 0.0 < t <= 1.0)
-    m, ms = _choice(min_p, "min_p must be from 0 to 1", 0.0, lambda t: 0.0 <= t <= 1.0)
+    T, k, p, m, Ts, ks, ps, ms = temperature, top_k, top_p, min_p, None, None, None, None
+    if isinstance(T, torch.Tensor):
+        T, Ts = 1.0, _choice(T)
+    elif not T >= 0.0:
+        raise ValueError(f"temperature must be 0 or more, got {T}")
+    if isinstance(k, torch.Tensor):
+        k, ks = 0, _choice(k, torch.int32)
+    elif not k >= 0:
+        raise ValueError(f"top_k must be 0 or more, got {k}")
+    if isinstance(p, torch.Tensor):
+        p, ps = 1.0, _choice(p)
+    elif not 0.0 < p <= 1.0:
+        raise ValueError(f"top_p must be above 0 and at most 1, got {p}")
+    if isinstance(m, torch.Tensor):
+        m, ms = 0.0, _choice(m)
+    elif not 0.0 <= m <= 1.0:
+        raise ValueError(f"min_p must be from 0 to 1, got {m}")
     out = _lib.host().sample_tokens(logits, uniform, T, Ts, k, ks, p, ps, m, ms, return_logprob)
     if out is not None:
         return out if return_logprob else out[0]

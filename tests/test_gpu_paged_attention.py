@@ -278,6 +278,61 @@ def test_offsets_beyond_32_bits(cuda):
     assert torch.equal(k[pages - 2, 63], key[0, 0]) and torch.equal(v[pages - 3, 1], key[1, 0])
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("case", [
+    # B, H, Hkv, D, L, page, gated
+    (3000, 2, 1, 64, 20, 4, False),          # many short sequences, some without a slot
+    (3000, 2, 2, 64, 20, 16, True),
+    (2, 300, 1, 64, 70, 16, False),          # many query heads of one key head
+    (2, 70, 1, 32, 70, 8, True),
+    (1, 2, 2, 128, 9000, 1, False),          # pages of one slot
+    (3, 4, 4, 64, 4100, 8, True),
+    (2, 4, 2, 96, 2000, 128, False),
+    (2, 4, 4, 192, 500, 12, False),
+], ids=str)
+def test_shapes_of_the_cut(cuda, case, dtype):
+    from mk_iii_technologies_tsrn_b200 import ops
+    B, H, Hkv, D, L, page, gated = case
+    k, v, table, g = _cache(cuda, B, L, Hkv, D, page, dtype)
+    lengths = torch.randint(0, L + 1, (B,), device=cuda, generator=g, dtype=torch.int32)
+    if B > 100:                              # runs of sequences without a slot, at both ends too
+        lengths[:40] = 0
+        lengths[500:900] = 0
+        lengths[-300:] = 0
+    q = torch.randn(B, H, D, device=cuda, generator=g).to(dtype)
+    key, value = (torch.randn(B, Hkv, D, device=cuda, generator=g).to(dtype) for _ in range(2))
+    gate = torch.rand(B, H, device=cuda, generator=g) if gated else None
+    mass = torch.rand(B, Hkv, table.shape[1] * page, device=cuda, generator=g)
+    some = lengths > 0
+    last = (lengths.long() - 1).clamp(min=0)
+    at = table.long().gather(1, (last // page)[:, None])[:, 0]
+    before, k2, v2, mass2 = mass.clone(), k.clone(), v.clone(), mass.clone()
+    o = ops.paged_attention(q, k, v, table, lengths, key=key, value=value, gate=gate, mass=mass)
+    assert torch.equal(o, ops.paged_attention(q, k2, v2, table, lengths, key=key, value=value, gate=gate, mass=mass2))
+    assert torch.equal(mass, mass2)
+    assert torch.equal(k[at, last % page][some], key[some]) and torch.equal(v[at, last % page][some], value[some])
+    pick = torch.randperm(B, device=cuda, generator=g)[:40]
+    want, weights, off = _reference(q[pick], k, v, table[pick], lengths[pick], D ** -0.5,
+                                    gate[pick] if gated else None)
+    _check(o[pick], want, off, v, dtype)
+    _check_mass(mass[pick], before[pick], weights, lengths[pick], off, H, Hkv, True)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_lengths_around_the_tiles(cuda, dtype):
+    from mk_iii_technologies_tsrn_b200 import ops
+    for page in (16, 24, 64):
+        for gated in (False, True):
+            n = torch.tensor([1, 7, 8, 9, 15, 16, 17, 31, 32, 33, 47, 48, 49, 63, 64, 65, 96, 97], device=cuda).int()
+            k, v, table, g = _cache(cuda, len(n), 97, 2, 64, page, dtype)
+            q = torch.randn(len(n), 4, 64, device=cuda, generator=g).to(dtype)
+            key = torch.randn(len(n), 2, 64, device=cuda, generator=g).to(dtype)
+            gate = torch.rand(len(n), 4, device=cuda, generator=g) if gated else None
+            o = ops.paged_attention(q, k, v, table, n, key=key, value=key, gate=gate)
+            want, _, off = _reference(q, k, v, table, n, 0.125, gate)      # (the token is stored by now)
+            _check(o, want, off, v, dtype)
+
+
 # ----------------------------------------------------------------------------- append
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("case", [(3, 5, 2, 64, 16, "slots"), (2, 40, 3, 33, 7, "heads"), (4, 1, 8, 80, 16, "slots"),
