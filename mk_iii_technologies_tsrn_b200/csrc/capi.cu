@@ -129,9 +129,9 @@ int allow_smem(const void* kernel, size_t bytes) {
   if (e != cudaSuccess) return cuda_status(e);
   std::lock_guard<std::mutex> lock(mu);
   size_t& known = most[{kernel, dev}];
-  const size_t want = bytes > known ? bytes : known;
-  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)want);
-  if (e == cudaSuccess) known = want;
+  if (bytes <= known) return TP_OK;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e == cudaSuccess) known = bytes;
   return cuda_status(e);
 }
 

@@ -41,7 +41,7 @@ __device__ __forceinline__ int remote_add(uint32_t at, int v) {
   return old;
 }
 
-// Launches `kernel` with `cluster` blocks to a cluster.
+// Launches `kernel` with `cluster` blocks to a cluster (a block by itself is one).
 template <typename... P, typename... A>
 int launch_clusters(void (*kernel)(P...), int64_t blocks, int threads, int cluster, cudaStream_t stream,
                     A... args) {
@@ -55,7 +55,7 @@ int launch_clusters(void (*kernel)(P...), int64_t blocks, int threads, int clust
   together.val.clusterDim.y = 1;
   together.val.clusterDim.z = 1;
   cfg.attrs = &together;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = cluster > 1 ? 1 : 0;
   return cuda_status(cudaLaunchKernelEx(&cfg, kernel, args...));
 }
 

@@ -16,7 +16,7 @@
 // sequence is a segment: softmax statistics (maximum and sum, base 2) and sums over V in fp32,
 // written out; a second kernel joins the segments of each sequence and head, stores the new token
 // and adds the weights to `mass`.  (A block per row and split of its length instead: 4 us of every
-// block went into its beginning and end, 237 us where this takes 203.)
+// block went into its beginning and end, 237 us where this takes 198.)
 //
 // Rows come through asynchronous copies into shared memory, STAGES - 1 tiles ahead and
 // across the ends of sequences.  The ring begins on 128 bytes: pieces whose place in shared memory
@@ -24,7 +24,7 @@
 // alone instead of 7.1).
 //
 // Measured: 48 sequences of 4096 to 8192 slots of 8 key heads of 128 bf16 channels, 4 query heads
-// each, 203 us for 1.22 GB (6.0 TB/s, 92 % of the card's copy rate).
+// each, 198 us for 1.22 GB (6.2 TB/s, 94 % of the card's copy rate).
 #pragma once
 
 #include <algorithm>
