@@ -103,14 +103,23 @@ struct Row {
     begin = (int)min((int64_t)V + off, first);
     end = (int)min((int64_t)V + off, first + per);
   }
-  // f(index of the first, values) of each step of this lane; the whole warp runs every step
-  template <typename F>
+  // f(index of the first, values) of each step of this lane; the whole warp runs every step.  AHEAD:
+  // the next step's numbers are asked for before this one's are looked at (where that leaves
+  // registers for it).
+  template <bool AHEAD = false, typename F>
   __device__ __forceinline__ void each(F f) const {
+    const int lane_at = ((int)threadIdx.x & 31) * PER;
+    auto whole = [&](int p) { return p >= off && p + PER <= end; };
+    auto get = [&](int p) { return __ldg((const uint4*)(x + (p - off))); };
+    uint4 next = make_uint4(0, 0, 0, 0);
+    if (AHEAD && whole(begin + lane_at)) next = get(begin + lane_at);
     for (int p0 = begin; p0 < end; p0 += 32 * PER) {
-      const int p = p0 + ((int)threadIdx.x & 31) * PER;
+      const int p = p0 + lane_at;
+      uint4 u = next;
+      if (AHEAD && whole(p + 32 * PER)) next = get(p + 32 * PER);
       float v[PER];
-      if (p >= off && p + PER <= end) {
-        const uint4 u = __ldg((const uint4*)(x + (p - off)));
+      if (whole(p)) {
+        if (!AHEAD) u = get(p);
         const uint32_t w[4] = {u.x, u.y, u.z, u.w};
         if constexpr (sizeof(T) == 4) {
 #pragma unroll
@@ -142,9 +151,7 @@ struct Weights {
   double top64, per, per2;        // the maximum, 1 / temperature, and that for base 2
   const double* table;            // 2^(j / 32)
   __device__ __forceinline__ double real(float x) const {
-    if (x == top) return 1.0;
     const double t = ((double)x - top64) * per2;
-    if (!(t > -60.0)) return 0.0;                        // (and NaN)
     const double shift = 0x1.8p47;                       // t to a 32nd, in its low bits
     const double s = t + shift, f = t - (s - shift);
     const int at = __double2loint(s), j = at & 31, n = at >> 5;
@@ -154,7 +161,8 @@ struct Weights {
     p = fma(z, p, 0.5);
     p = fma(z, p, 1.0);
     p = fma(z, p, 1.0) * table[j];
-    return __hiloint2double(__double2hiint(p) + (n << 20), __double2loint(p));
+    const double w = __hiloint2double(__double2hiint(p) + (n << 20), __double2loint(p));
+    return x == top ? 1.0 : t > -60.0 ? w : 0.0;         // (of NaN nothing)
   }
   // w * 2^44 to the nearest, read from the low bits of a sum
   __device__ __forceinline__ u64 whole(double w) const {
@@ -223,7 +231,7 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const SampleArgs a, int
   float mine_best = -inf, lowest = inf;
   int mine_at = 0;                      // (a row without a token above -inf is none to take from)
   const bool of_threads = by_k && top_k <= cluster * THREADS / 8 && V >= cluster * THREADS;
-  row.each([&](int i, const float* v) {
+  row.template each<true>([&](int i, const float* v) {
     float top = v[0];
 #pragma unroll
     for (int k = 1; k < Row<T>::PER; ++k) top = fmaxf(top, v[k]);      // (NaN is not)
@@ -373,7 +381,7 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const SampleArgs a, int
     const float floor = border < BINS - 1 ? wt.top - (border + 2) / bins_per : -inf;
     auto gather = [&](bool before, bool at_border) {
       int counted = 0;
-      row.each([&](int i, const float* v) {
+      row.template each<true>([&](int i, const float* v) {
         bool any = false;
 #pragma unroll
         for (int k = 0; k < Row<T>::PER; ++k) any |= v[k] >= floor;
@@ -428,8 +436,10 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const SampleArgs a, int
               __syncthreads();
               other = s.candidate[0][tid ^ j];
               __syncthreads();
-            } else {
+            } else if (tid < n) {       // (whole warps)
               other = __shfl_xor_sync(0xffffffffu, v, j);
+            } else {
+              continue;
             }
             const bool larger = ((tid & j) == 0) == ((tid & k) == 0);
             v = (v > other) == larger ? v : other;
@@ -468,10 +478,11 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const SampleArgs a, int
           s.candidate[0][tid] = v;
           __syncthreads();
           const uint32_t last = (uint32_t)(s.candidate[0][max(n - 1, 0)] >> 32);
-          const int equal = __syncthreads_count(keep && (uint32_t)(v >> 32) == last);
+          const bool same = tid < listed && (uint32_t)(v >> 32) == last;
+          const int equal = __syncthreads_count(keep && same), all_equal = __syncthreads_count(same);
           if (tid < cluster) {
             remote_store(remote(&s.cut, tid), (int)last);
-            remote_store(remote(&s.ties, tid), equal);
+            remote_store(remote(&s.ties, tid), equal == all_equal ? -1 : equal);      // -1: all
           }
         } else {
           keep = (keep && w >= min_p) || tid == 0;
@@ -497,7 +508,7 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const SampleArgs a, int
       }
       meet();
       cut = s.cut;
-      ties = s.ties;
+      ties = s.ties < 0 ? INT64_MAX : s.ties;
     }
     // ---- bit by bit over all tokens
     auto weigh_from = [&](uint32_t key) {
@@ -525,7 +536,9 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const SampleArgs a, int
           if (count_from(cut | bit) >= (u64)top_k) cut |= bit;
         ties = top_k - (int64_t)count_from(cut + 1);
       }
-      if (by_p) share = weigh_from(cut + 1) + (u64)ties * wt.whole(wt.real(value_of(cut)));
+      if (by_p)
+        share = ties == INT64_MAX ? weigh_from(cut)
+                                  : weigh_from(cut + 1) + (u64)ties * wt.whole(wt.real(value_of(cut)));
     }
     if (by_p && !(one_bin && !by_k)) {
       const double wanted = top_p * (double)share;
@@ -570,16 +583,21 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const SampleArgs a, int
       at += upto - mine;
       base += __shfl_sync(0xffffffffu, upto, 31);
     }
+    bool in[Row<T>::PER], any = false;
 #pragma unroll
     for (int k = 0; k < Row<T>::PER; ++k) {
-      w[k] = 0;
       const uint32_t key = key_of(v[k]);
       const bool tie = key == cut;
-      if (key > cut || (tie && at < ties)) {
-        const double real = wt.real(v[k]);
-        if (real >= min_p || i + k == first) w[k] = wt.whole(real);
-      }
+      in[k] = key > cut || (tie && at < ties);
+      any |= in[k];
       at += tie;
+      w[k] = 0;
+    }
+    if (!__any_sync(0xffffffffu, any)) return;
+#pragma unroll
+    for (int k = 0; k < Row<T>::PER; ++k) {            // (all of them, rather than one after another)
+      const double real = wt.real(v[k]);
+      if (in[k] && (real >= min_p || i + k == first)) w[k] = wt.whole(real);
     }
   };
   u64 sum = 0;
