@@ -259,7 +259,8 @@ constexpr int MOVE_THREADS = 512, MOVE_DEPTH = 8;
 struct RowMove {
   int64_t from, to;                // in bytes from the head's first row; -1: stays
 };
-template <typename W>
+// LOOK: rows of a batch that a thread looks up.
+template <typename W, int LOOK>
 __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const CacheEvictArgs a, int words,
                                                                   int width, int slices) {
   extern __shared__ __align__(16) RowMove ring[];      // three batches
@@ -279,42 +280,44 @@ __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const CacheEvi
   const int64_t page_bytes = value ? a.c.v_page : a.c.k_page, slot_bytes = value ? a.c.v_slot : a.c.k_slot;
   const int per = MOVE_THREADS / width, mine = threadIdx.x / width;
   const bool active = mine < per && w < words;
-  const int batch = per * MOVE_DEPTH;          // rows; at most MOVE_DEPTH for a thread to look up
+  const int batch = per * MOVE_DEPTH;          // rows; at most LOOK * MOVE_THREADS
   const int batches = (a.keep + batch - 1) / batch;
 
-  int slot[MOVE_DEPTH], from_page[MOVE_DEPTH], to_page[MOVE_DEPTH];
-  auto ask_slots = [&](int t) {
+  int slot[LOOK], after[LOOK], from_page[LOOK], to_page[LOOK];
+  auto ask_slots = [&](int t, int (&into)[LOOK]) {
 #pragma unroll
-    for (int k = 0; k < MOVE_DEPTH; ++k) {
+    for (int k = 0; k < LOOK; ++k) {
       const int in = threadIdx.x + k * MOVE_THREADS, i = t * batch + in;
-      slot[k] = in < batch && i < a.keep && t < batches ? kept[i] : -1;
+      into[k] = in < batch && t < batches && i < a.keep ? kept[i] : -1;
     }
   };
-  auto ask_pages = [&](int t) {
+  auto ask_pages = [&](int t) {                // of batch t, whose slots are in `slot`
 #pragma unroll
-    for (int k = 0; k < MOVE_DEPTH; ++k) {
+    for (int k = 0; k < LOOK; ++k) {
       const int i = t * batch + threadIdx.x + k * MOVE_THREADS;
       if (slot[k] < 0 || slot[k] == i) continue;
       from_page[k] = __ldg(row + a.c.column(slot[k]));
       to_page[k] = __ldg(row + a.c.column(i));
     }
   };
-  auto note = [&](int t) {                     // batch t's rows into the ring
+  auto note = [&](int t) {                     // batch t's rows into the ring; on to the next slots
     RowMove* const to = ring + t % 3 * batch;
 #pragma unroll
-    for (int k = 0; k < MOVE_DEPTH; ++k) {
+    for (int k = 0; k < LOOK; ++k) {
       const int in = threadIdx.x + k * MOVE_THREADS, i = t * batch + in;
-      if (in >= batch) continue;
-      RowMove m{-1, -1};
-      if (slot[k] >= 0 && slot[k] != i) {
-        if (from_page[k] < 0 || from_page[k] >= a.c.pages || to_page[k] < 0 || to_page[k] >= a.c.pages) {
-          tp_record_index_error(a.bad.error, a.bad.seen);
-        } else {
-          m.from = from_page[k] * page_bytes + a.c.within(slot[k], a.c.column(slot[k])) * slot_bytes;
-          m.to = to_page[k] * page_bytes + a.c.within(i, a.c.column(i)) * slot_bytes;
+      if (in < batch) {
+        RowMove m{-1, -1};
+        if (slot[k] >= 0 && slot[k] != i) {
+          if (from_page[k] < 0 || from_page[k] >= a.c.pages || to_page[k] < 0 || to_page[k] >= a.c.pages) {
+            tp_record_index_error(a.bad.error, a.bad.seen);
+          } else {
+            m.from = from_page[k] * page_bytes + a.c.within(slot[k], a.c.column(slot[k])) * slot_bytes;
+            m.to = to_page[k] * page_bytes + a.c.within(i, a.c.column(i)) * slot_bytes;
+          }
         }
+        to[in] = m;
       }
-      to[in] = m;
+      slot[k] = after[k];
     }
   };
   W x[MOVE_DEPTH], y[MOVE_DEPTH];
@@ -326,15 +329,16 @@ __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const CacheEvi
       if (from >= 0) into[k] = *(const W*)(base + from);
     }
   };
+  ask_slots(0, slot);
   for (int t = 0; t < 2; ++t) {
-    ask_slots(t);
+    ask_slots(t + 1, after);
     ask_pages(t);
     note(t);
   }
-  ask_slots(2);
   __syncthreads();
   read(0, x);
   for (int t = 0; t < batches; ++t) {
+    ask_slots(t + 3, after);
     ask_pages(t + 2);
     read(t + 1, y);
     __syncthreads();                           // batch t has been read by all
@@ -346,7 +350,6 @@ __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const CacheEvi
         x[k] = y[k];
       }
     note(t + 2);
-    ask_slots(t + 3);
     __syncthreads();
   }
 }
@@ -362,7 +365,8 @@ int move(const CacheEvictArgs& a, cudaStream_t stream) {
   const int64_t blocks = a.B * a.c.heads * 2 * slices;
   TP_RETURN_IF(blocks > INT32_MAX, TP_ERR_TOO_LARGE);
   const size_t smem = (size_t)3 * (MOVE_THREADS / width) * MOVE_DEPTH * sizeof(RowMove);
-  auto* kernel = evict_move_kernel<W>;
+  constexpr int FEW = 2;                 // (8 rows a thread looked up leave the others no registers)
+  auto* kernel = width * FEW >= MOVE_DEPTH ? evict_move_kernel<W, FEW> : evict_move_kernel<W, MOVE_DEPTH>;
   const int st = allow_smem((const void*)kernel, smem);
   if (st != TP_OK) return st;
   cudaLaunchConfig_t cfg = {};
