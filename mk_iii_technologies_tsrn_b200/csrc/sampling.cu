@@ -23,6 +23,11 @@
 //     then the row has a threshold, and is read twice more as without filters.
 //   - Where even that bin holds too many (flat rows, ties), and for a share of a top_k above
 //     CANDIDATES, the threshold is found bit by bit over all tokens.
+//
+// Measured (in a CUDA graph): 16 x 256 fp32 without filters 5.5 us, 64 x 131072 bf16 with top_k
+// around 50 and top_p 26 (2.6 us of bytes), 32 x 49999 fp32 with top_p 0.95 and 2300 tokens kept
+// 38.  What bounds it is latency: passes of a few steps with an exchange of the cluster between
+// them; in the last case half of it are instructions (weights in 64 bits).
 #include <algorithm>
 
 #include "cluster.cuh"
@@ -644,6 +649,8 @@ template <typename T, int THREADS>
 int sample(const SampleArgs& a, cudaStream_t stream) {
   constexpr int WARPS = THREADS / 32;
   // as many blocks for a row as leave its warps a few steps, while the SMs hold all rows' at once
+  // (32 x 49999: 69 us with one block, 38 with four, 81 with eight, which take turns; 64 x 131072:
+  // 30, 26 with two, 72 with eight)
   int cluster = 1;
   while (cluster < MAX_CLUSTER && a.V > (int64_t)cluster * WARPS * 64 * (16 / (int)sizeof(T)) &&
          a.B * cluster * 2 <= num_sms())
@@ -656,7 +663,7 @@ int sample(const SampleArgs& a, cudaStream_t stream) {
 
 int launch_sample_tokens(const SampleArgs& a, cudaStream_t stream) {
   // (a small vocabulary in small blocks, whose barriers are shorter: 16 rows of 256 logits
-  // 10.5 us in blocks of 1024, 7.5 in these, the launch among them)
+  // 10.5 us in blocks of 1024, 7.5 in these at that stage, 5.5 now, the launch among them)
   const bool small = a.V <= 4096;
   if (a.dtype == TP_DTYPE_BF16)
     return small ? sample<uint16_t, 256>(a, stream) : sample<uint16_t, 1024>(a, stream);
