@@ -298,7 +298,9 @@ class TropicalEncoderLayer(nn.Module):
                 src_key_padding_mask: Optional[torch.Tensor] = None,
                 cache: Optional[TropicalKVCache] = None) -> torch.Tensor:
         x = src if self.batch_first else src.transpose(0, 1)
-        masks = dict(attn_mask=src_mask, key_padding_mask=src_key_padding_mask, cache=cache)
+        masks = dict(attn_mask=src_mask, key_padding_mask=src_key_padding_mask)
+        if cache is not None:           # (an attention of another make need not know of it)
+            masks["cache"] = cache
         if self.norm_first:
             h = self.norm1(x)
             x = x + self.dropout1(self.self_attn(h, h, h, **masks)[0])

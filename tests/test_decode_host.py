@@ -105,3 +105,17 @@ def test_cpu_tensors_and_choices_are_refused():
         for x in bad:
             with pytest.raises(ValueError, match=name):
                 ops.sample_tokens(q[0], u, **{name: x})
+
+
+def test_encoder_layers_without_a_cache_call_their_attention_as_before():
+    from mk_iii_technologies_tsrn_b200 import dropin
+
+    class Plain(torch.nn.Module):                 # an attention that knows of no cache
+        def forward(self, q, k, v, attn_mask=None, key_padding_mask=None):
+            return q, None
+
+    layer = dropin.TropicalEncoderLayer(8, 2, 16, dropout=0.0)
+    layer.self_attn, layer.ffn = Plain(), torch.nn.Identity()
+    assert layer(torch.randn(1, 3, 8)).shape == (1, 3, 8)
+    with pytest.raises(TypeError, match="cache"):
+        layer(torch.randn(1, 3, 8), cache=dropin.TropicalKVCache())
