@@ -12,8 +12,13 @@
 //     four slots whose weights it holds; pairs of slots are interleaved in registers.
 // Every second row is moved on by 32 bytes, and column g of the eight slots of an instruction is
 // slot `slot_of(g)`, so that neither read meets a bank twice.
-// P is rounded to two bf16 parts, the second in the rows that the heads leave free, so that a
-// weight is off by at most 2^-16 of itself.  Everything else is fp32.
+// A weight is a sum of bf16 parts (products of two bf16 numbers are exact in fp32).  Blocks of up to
+// four query heads have each head in rows g and g + 4 of S, so that P's rows g, g + 8 and g + 4 take
+// its three parts: all 24 bits (48 x 8192 of 4 query heads each 198.7 us for 197.7 with two parts, of one
+// head of 64 channels 106 for 107.5).  Blocks of five to eight have rows g and g + 8 alone: two parts,
+// which lose at most 2^-16 of a weight, where the output is rounded by 2^-8 (a second product for the
+// other bits: 24 x 8192 of 16 query heads each 95 -> 105 us, 48 x 8192 of 8 heads of 64 115 -> 122).
+// Everything else is fp32.
 #include "paged_attention.cuh"
 
 namespace tp {
@@ -33,8 +38,6 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
   return *(const uint32_t*)&p;
 }
-
-constexpr int HEADS = 8;
 
 // KB blocks of 32 channels
 template <int KB>
@@ -70,9 +73,11 @@ __device__ __forceinline__ void copy_rows(uint32_t to, const char* const (&kfrom
   if constexpr (S + 1 < P::STEPS) copy_rows<P, S + 1>(to, kfrom, vfrom);
 }
 
-template <int KB, int STAGES>
+// FEW: blocks of up to four query heads
+template <int KB, int STAGES, bool FEW>
 __global__ void __launch_bounds__(ATT_WARPS * 32) paged_attend_mma_kernel(const PagedAttentionArgs a) {
   using P = MmaTile<KB>;
+  constexpr int HEADS = FEW ? 4 : 8;
   constexpr int VB = P::VB, GROUPS = P::GROUPS, TK = P::TK;
   extern __shared__ __align__(128) char smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -137,13 +142,15 @@ __global__ void __launch_bounds__(ATT_WARPS * 32) paged_attend_mma_kernel(const 
 
   const int kslot = slot_of(g), slot0 = slot_of(2 * t);      // of each eight; slot0 ^ 4: column 2t + 1
   uint4 q[KB];
-  float factor = 0.0f, m = neg_inf(), l = 0.0f;      // of head g; l: the sum of this lane's slots
+  const int head = FEW ? g & 3 : g;        // of the block: this lane's
+  float factor = 0.0f, m = neg_inf(), l = 0.0f;      // of that head; l: the sum of this lane's slots
   int h = 0;
-  bool head_there = false;
+  bool head_there = false, writes = false;
   float acc[VB][8][4];
   auto begin_row = [&]() {
-    const int in_group = hblk * HEADS + g;
+    const int in_group = hblk * HEADS + head;
     head_there = in_group < a.group;
+    writes = head_there && head == g;
     h = kvh * a.group + (head_there ? in_group : 0);
     const uint16_t* src = (const uint16_t*)a.q + (int64_t)at.b * a.q_sb + (int64_t)h * a.q_sh;
 #pragma unroll
@@ -167,21 +174,26 @@ __global__ void __launch_bounds__(ATT_WARPS * 32) paged_attend_mma_kernel(const 
     const int64_t seg = segment(a, at.b, run, hsub);
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
-    if (!head_there) return;
-    float* const to = a.part + (seg * HEADS + g) * D + 16 * t;
+    float* const to = a.part + (seg * HEADS + head) * D + 16 * t;
 #pragma unroll
     for (int vb = 0; vb < VB; ++vb)
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
-        if (vb * 64 + 16 * t + 8 * e < D) {
-          float4* const at4 = (float4*)(to + vb * 64 + 8 * e);
+      for (int e = 0; e < 2; ++e) {
+        float x[8];
 #pragma unroll
-          for (int j = 0; j < 8; j += 4)
-            at4[j / 4] = make_float4(acc[vb][j][e] + acc[vb][j][2 + e], acc[vb][j + 1][e] + acc[vb][j + 1][2 + e],
-                                     acc[vb][j + 2][e] + acc[vb][j + 2][2 + e],
-                                     acc[vb][j + 3][e] + acc[vb][j + 3][2 + e]);
+        for (int j = 0; j < 8; ++j) {
+          const float most = acc[vb][j][e];
+          float rest = acc[vb][j][2 + e];
+          if constexpr (FEW) rest += __shfl_xor_sync(0xffffffffu, most, 16);      // (of row g + 4)
+          x[j] = most + rest;
         }
-    if (t == 0) a.ml[seg * HEADS + g] = make_float2(m, l);
+        if (writes && vb * 64 + 16 * t + 8 * e < D) {
+          float4* const at4 = (float4*)(to + vb * 64 + 8 * e);
+          at4[0] = make_float4(x[0], x[1], x[2], x[3]);
+          at4[1] = make_float4(x[4], x[5], x[6], x[7]);
+        }
+      }
+    if (writes && t == 0) a.ml[seg * HEADS + head] = make_float2(m, l);
   };
 
 #pragma unroll
@@ -215,7 +227,7 @@ __global__ void __launch_bounds__(ATT_WARPS * 32) paged_attend_mma_kernel(const 
       s[j][0] = at0 < n ? c[0] * factor : neg_inf();
       s[j][1] = at1 < n ? c[1] * factor : neg_inf();
       top = fmaxf(top, fmaxf(s[j][0], s[j][1]));
-      if (a.scores != nullptr && head_there) {
+      if (a.scores != nullptr && writes) {
         float* sc = a.scores + ((int64_t)at.b * a.H + h) * a.score_row;
         if (at0 < n) sc[at0] = s[j][0];
         if (at1 < n) sc[at1] = s[j][1];
@@ -237,14 +249,26 @@ __global__ void __launch_bounds__(ATT_WARPS * 32) paged_attend_mma_kernel(const 
     }
 #pragma unroll
     for (int u = 0; u < GROUPS; ++u) {
-      uint32_t p[4];                       // both parts of slots 2t, 2t + 1 of two eights
+      uint32_t p[4];                       // parts of slots 2t, 2t + 1 of two eights, rows g and g + 8
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const float p0 = tp_ex2(s[2 * u + e][0] - from), p1 = tp_ex2(s[2 * u + e][1] - from);
+        float p0 = tp_ex2(s[2 * u + e][0] - from), p1 = tp_ex2(s[2 * u + e][1] - from);
         l += p0 + p1;
-        const uint32_t hi = pack_bf16(p0, p1);
-        p[2 * e] = hi;
-        p[2 * e + 1] = pack_bf16(p0 - __uint_as_float(hi << 16), p1 - __uint_as_float(hi & 0xffff0000u));
+        if constexpr (FEW) {
+          auto part = [&]() {              // the first 8 bits, cut off; what is left is exact
+            const uint32_t x0 = __float_as_uint(p0), x1 = __float_as_uint(p1);
+            p0 -= __uint_as_float(x0 & 0xffff0000u);
+            p1 -= __uint_as_float(x1 & 0xffff0000u);
+            return __byte_perm(x0, x1, 0x7632);
+          };
+          const uint32_t first = part(), second = part(), third = part();
+          p[2 * e] = head == g ? first : third;
+          p[2 * e + 1] = head == g ? second : 0u;
+        } else {
+          const uint32_t hi = pack_bf16(p0, p1);
+          p[2 * e] = hi;
+          p[2 * e + 1] = pack_bf16(p0 - __uint_as_float(hi << 16), p1 - __uint_as_float(hi & 0xffff0000u));
+        }
       }
 #pragma unroll
       for (int vb = 0; vb < VB; ++vb) {
@@ -272,8 +296,9 @@ template <int KB>
 int attend_mma(PagedAttentionArgs& a, cudaStream_t stream) {
   constexpr int STAGES = KB > 4 ? 2 : 3;
   using P = MmaTile<KB>;
-  return attend_and_join<uint16_t>(a, paged_attend_mma_kernel<KB, STAGES>,
-                                   (size_t)ATT_WARPS * STAGES * P::STAGE * 16, P::TK, HEADS, stream);
+  const size_t smem = (size_t)ATT_WARPS * STAGES * P::STAGE * 16;
+  return a.group <= 4 ? attend_and_join<uint16_t>(a, paged_attend_mma_kernel<KB, STAGES, true>, smem, P::TK, 4, stream)
+                      : attend_and_join<uint16_t>(a, paged_attend_mma_kernel<KB, STAGES, false>, smem, P::TK, 8, stream);
 }
 
 int on_tensor_cores(PagedAttentionArgs& a, cudaStream_t stream) {

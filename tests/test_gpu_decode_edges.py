@@ -1,0 +1,38 @@
+"""Edges of the decoding operators: precision of the weights."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+
+
+@pytest.mark.parametrize("group", [1, 2, 3, 4])
+def test_bf16_weights_keep_their_bits(cuda, group):
+    """A slot of weight w and value -1 against two of weight 1 whose values make up for it, in 64 bits
+    to 2^-16 or so: what is left is what the weights lost.
+
+    Scores are single products of bf16 numbers, exact; their base-2 form is off by 2 U of a score below
+    1, the exponential by 2^-22, so a weight by at most 2^-22 + 3 U of itself.  A sum of n products in
+    fp32 is off by at most n 2^-23 of the sum of their sizes (steps may be cut off rather than rounded),
+    in the output and in the sum of the weights.  The output is rounded by 2^-8 of its value at most."""
+    from mk_iii_technologies_tsrn_b200 import ops
+    B, Hkv, D, n = 64, 2, 64, 3
+    g = torch.Generator(device=cuda).manual_seed(group)
+    x = (0.1 + 0.8 * torch.rand(B, Hkv, device=cuda, generator=g)).bfloat16()
+    k = torch.zeros(B, 16, Hkv, D, device=cuda, dtype=torch.bfloat16)
+    v = torch.full_like(k, -1.0)
+    k[:, 0, :, 0] = -x
+    w = torch.exp(-x.double())
+    v[:, 1] = w.bfloat16()[..., None]
+    v[:, 2] = (w - w.bfloat16().double()).bfloat16()[..., None]
+    q = torch.zeros(B, Hkv * group, D, device=cuda, dtype=torch.bfloat16)
+    q[..., 0] = 1.0
+    table = torch.arange(B, device=cuda, dtype=torch.int32)[:, None]
+    o = ops.paged_attention(q, k, v, table, torch.full((B,), n, device=cuda), scale=1.0)
+    want = (v[:, 1:3, :, 0].double().sum(1) - w) / (2 + w)
+    assert float(want.abs().max()) < 2.0 ** -16
+    sizes = 2 * w / (2 + w)
+    tol = sizes * (2.0 ** -22 + 3 * U + 2 * n * 2.0 ** -23) + want.abs() * 2.0 ** -8
+    off = (o.double().view(B, Hkv, group, D) - want[:, :, None, None]).abs()
+    assert (off <= tol[:, :, None, None]).all()
