@@ -117,6 +117,7 @@ __global__ void __launch_bounds__(EVICT_THREADS) evict_select_kernel(const Cache
     }
     return;
   }
+  cluster_arrive();
   // slots before `old` compete for `need` places
   const int old = n - min(a.recent, n), need = a.keep - (n - old), chunk = cluster * PART;
   float v[EVICT_PER];              // slots base + rank * PART + k * THREADS + tid
@@ -135,6 +136,7 @@ __global__ void __launch_bounds__(EVICT_THREADS) evict_select_kernel(const Cache
   uint32_t prefix = 0;
   int left = need;                 // places among the slots whose high bits are `prefix`
   load(0);
+  cluster_wait();                  // every block of the cluster runs
   if (need > 0) {
     hist[0][tid] = 0;
     __syncthreads();

@@ -183,6 +183,7 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const SampleArgs a, int
   const uint32_t rank = cluster_rank();
   const int64_t b = blockIdx.x / cluster;
   const int V = (int)a.V;
+  if (cluster > 1) cluster_arrive();
 
   const Row<T> row((const T*)a.logits + b * a.ld, V, (int)rank * WARPS + warp, cluster * WARPS);
 
@@ -255,6 +256,7 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const SampleArgs a, int
   all(best, 0, Max());
   all(least, 1, Max());
   __syncthreads();
+  if (cluster > 1) cluster_wait();      // every block of the row runs
   if (warp == 0) {
     finish(0, Max());
     finish(1, Max());

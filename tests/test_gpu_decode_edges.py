@@ -1,4 +1,4 @@
-"""Edges of the decoding operators: precision of the weights."""
+"""Edges of the decoding operators: precision of the weights, clusters of blocks."""
 import pytest
 import torch
 
@@ -36,3 +36,25 @@ def test_bf16_weights_keep_their_bits(cuda, group):
     tol = sizes * (2.0 ** -22 + 3 * U + 2 * n * 2.0 ** -23) + want.abs() * 2.0 ** -8
     off = (o.double().view(B, Hkv, group, D) - want[:, :, None, None]).abs()
     assert (off <= tol[:, :, None, None]).all()
+
+
+@pytest.mark.parametrize("L", [4097, 9000, 33000, 40000])
+def test_eviction_of_all_but_the_recent_slots_by_clusters(cuda, L):
+    # nothing to choose: the blocks of a cluster meet for the counts alone
+    from mk_iii_technologies_tsrn_b200 import ops
+    import test_gpu_cache_evict as evict
+    for B, Hkv, keep in ((1, 1, 1), (3, 2, 777), (9, 8, 4096)):
+        k, v, table, mass, n = evict._case(cuda, B, Hkv, 8, L, 64, torch.bfloat16, "slots")
+        kept, k2, v2, out = evict._want(k, v, table, mass, n, keep, keep)
+        got = ops.cache_evict(k, v, table, n, mass, keep, keep)
+        assert torch.equal(got, kept) and torch.equal(k, k2) and torch.equal(v, v2) and torch.equal(mass, out)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_sampling_around_the_sizes_of_clusters(cuda, dtype):
+    # rows of one block and of two, small blocks and large ones, few rows and many
+    import test_gpu_sampling as sampling
+    for V in (2048, 2049, 4096, 4097, 8192, 8193, 16385):
+        for B in (1, 40, 160):
+            for c in (dict(T=0.8), dict(k=20, p=0.9)):
+                sampling._check(*sampling._logits(cuda, B, V, dtype, seed=V), **c)
