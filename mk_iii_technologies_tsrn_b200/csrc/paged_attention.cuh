@@ -171,10 +171,13 @@ __device__ __forceinline__ int64_t segment(const PagedAttentionArgs& a, int b, i
 #define TP_NANS_8 0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu
 #define TP_NANS_64 TP_NANS_8, TP_NANS_8, TP_NANS_8, TP_NANS_8, TP_NANS_8, TP_NANS_8, TP_NANS_8, TP_NANS_8
 __device__ __align__(16) const uint32_t nan_row[256] = {TP_NANS_64, TP_NANS_64, TP_NANS_64, TP_NANS_64};
+// What is multiplied with the weight 0 of a slot behind the last one.
+__device__ __align__(16) const uint32_t zero_row[256] = {};
 
 // The rows of K and V that a warp copies: each lane knows one slot of a tile.  Slots behind the
-// last one are taken for it: their weight is 0, and what they are multiplied with is in use
-// anyway.  The page is asked for one tile before it is needed.
+// last one have its keys, for scores that are not used, and zeros for values (an infinity of the
+// last slot's, times their weight of 0, would be NaN).  The page is asked for one tile before it is
+// needed.
 template <typename T, int TK>
 struct TileRows {
   const PagedAttentionArgs& a;
@@ -215,6 +218,7 @@ struct TileRows {
       kp = (const char*)((const T*)a.key + (int64_t)p.b * a.key_sb + (int64_t)kvh * a.key_sh);
       vp = (const char*)((const T*)a.value + (int64_t)p.b * a.value_sb + (int64_t)kvh * a.value_sh);
     }
+    if (p.tile * TK + ((int)threadIdx.x & (TK - 1)) >= p.n) vp = (const char*)zero_row;
   }
 };
 
@@ -569,11 +573,12 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) paged_join_kernel(const Paged
         float f[AT_ONCE], x[AT_ONCE][KD];
 #pragma unroll
         for (int u = 0; u < AT_ONCE; ++u) {
-          const int s = min(s0 + u * TEAM, runs.y - 1);
+          const bool in = s0 + u * TEAM < runs.y;
+          const int s = in ? s0 + u * TEAM : runs.y - 1;
           f[u] = ml[s * stride].x;
           const float* p = a.part + (first + s * stride) * D;
 #pragma unroll
-          for (int k = 0; k < KD; ++k) x[u][k] = lane + 32 * k < D ? p[lane + 32 * k] : 0.0f;
+          for (int k = 0; k < KD; ++k) x[u][k] = in && lane + 32 * k < D ? p[lane + 32 * k] : 0.0f;
         }
 #pragma unroll
         for (int u = 0; u < AT_ONCE; ++u) {

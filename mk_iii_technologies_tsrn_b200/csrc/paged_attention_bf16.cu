@@ -185,7 +185,8 @@ __global__ void __launch_bounds__(ATT_WARPS * 32) paged_attend_mma_kernel(const 
           const float most = acc[vb][j][e];
           float rest = acc[vb][j][2 + e];
           if constexpr (FEW) rest += __shfl_xor_sync(0xffffffffu, most, 16);      // (of row g + 4)
-          x[j] = most + rest;
+          // (an infinite value makes NaN of the lesser parts, which may be 0 or of the other sign)
+          x[j] = fabsf(most) < -neg_inf() ? most + rest : most;
         }
         if (writes && vb * 64 + 16 * t + 8 * e < D) {
           float4* const at4 = (float4*)(to + vb * 64 + 8 * e);

@@ -1,4 +1,5 @@
-"""Edges of the decoding operators: precision of the weights, clusters of blocks."""
+"""Edges of the decoding operators: precision of the weights, clusters of blocks,
+infinite values."""
 import pytest
 import torch
 
@@ -58,3 +59,50 @@ def test_sampling_around_the_sizes_of_clusters(cuda, dtype):
         for B in (1, 40, 160):
             for c in (dict(T=0.8), dict(k=20, p=0.9)):
                 sampling._check(*sampling._logits(cuda, B, V, dtype, seed=V), **c)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("case", [(1, 64), (2, 64), (4, 128), (3, 33), (8, 80), (12, 256)], ids=str)
+def test_infinite_values(cuda, case, gated, dtype):
+    """An infinity in a value in use makes its channel that infinity, two of both signs or a NaN make it
+    NaN, and the other channels are what they are; wherever the slot lies, the last one too.  Finite
+    channels within the tolerance of test_gpu_paged_attention.py."""
+    from mk_iii_technologies_tsrn_b200 import ops
+    import test_gpu_paged_attention as base
+    group, D = case
+    inf, nan = float("inf"), float("nan")
+    lengths = torch.tensor([1, 2, 7, 8, 16, 17, 250, 601, 5003], device=cuda, dtype=torch.int32)
+    for store in (False, True):
+        for B in (len(lengths), 1):                          # (one sequence: its segments are joined by teams)
+            n = lengths[-B:].contiguous()
+            k, v, table, g = base._cache(cuda, B, 5003, 2, D, 16, dtype)
+            q = (0.2 * torch.randn(B, 2 * group, D, device=cuda, generator=g)).to(dtype)
+            key, value = (torch.randn(B, 2, D, device=cuda, generator=g).to(dtype) for _ in range(2))
+            gate = torch.rand(B, 2 * group, device=cuda, generator=g) if gated else None
+            for b, m in enumerate(n.tolist()):
+                for slot, channel, x in ((m - 1, 0, inf), (0, 1, -inf), (m // 2, 2, inf), (0, 3, inf), (m - 1, 3, -inf),
+                                         (m // 3, 4, nan), (m - 1, D - 1, -inf), (m * 2 // 3, 9, inf)):
+                    if x == -inf and channel == 3 and m == 1:
+                        continue
+                    v[table[b, slot // 16].long(), slot % 16, 1, channel] = x
+                    if slot == m - 1:
+                        value[b, 1, channel] = x
+                last = m - 1
+                at = table[b, last // 16].long()
+                if not store:
+                    key[b], value[b] = k[at, last % 16], v[at, last % 16]
+            kw, vw = k.clone(), v.clone()
+            for b, m in enumerate(n.tolist()):
+                at = table[b, (m - 1) // 16].long()
+                kw[at, (m - 1) % 16], vw[at, (m - 1) % 16] = key[b], value[b]
+            new = dict(key=key, value=value) if store else {}
+            o = ops.paged_attention(q, k, v, table, n, gate=gate, **new)
+            want, _, off = base._reference(q, kw, vw, table, n, D ** -0.5, gate)
+            o = o.double()
+            assert torch.equal(o.isnan(), want.isnan()) and torch.equal(o.isinf(), want.isinf())
+            assert torch.equal(o[o.isinf()], want[want.isinf()])
+            fine = want.isfinite()
+            top = v[v.isfinite()].double().abs().max()
+            tol = 2 * off[..., None] * top + (want.abs() * 2.0 ** -8 + top * 2.0 ** -16 if dtype == torch.bfloat16 else 0)
+            assert bool(((o - want).abs() <= tol)[fine].all())
