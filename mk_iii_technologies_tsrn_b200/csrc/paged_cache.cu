@@ -417,7 +417,7 @@ int launch_cache_evict(const CacheEvictArgs& a, cudaStream_t stream) {
     cluster *= 2;
   const int st = launch_clusters(evict_select_kernel, a.B * c.heads * cluster, EVICT_THREADS, cluster,
                                  stream, a, cluster);
-  if (st != TP_OK) return st;
+  if (st != TP_OK || c.channels == 0) return st;       // (rows without a channel: none to move)
   switch (word_bytes({(int64_t)c.channels * c.esize, address(c.k), c.k_page, c.k_slot, c.k_head,
                       address(c.v), c.v_page, c.v_slot, c.v_head})) {
     case 16: return move<uint4>(a, stream);

@@ -1,5 +1,5 @@
 """Edges of the decoding operators: precision of the weights, clusters of blocks,
-infinite values."""
+infinite values, rows without a channel."""
 import pytest
 import torch
 
@@ -106,3 +106,18 @@ def test_infinite_values(cuda, case, gated, dtype):
             top = v[v.isfinite()].double().abs().max()
             tol = 2 * off[..., None] * top + (want.abs() * 2.0 ** -8 + top * 2.0 ** -16 if dtype == torch.bfloat16 else 0)
             assert bool(((o - want).abs() <= tol)[fine].all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_eviction_without_channels(cuda, dtype):
+    # no rows to move; the choice of slots and their weights are due
+    from mk_iii_technologies_tsrn_b200 import ops
+    import test_gpu_cache_evict as evict
+    for L, keep in ((40, 16), (5000, 700), (9, 20)):
+        _, _, table, mass, n = evict._case(cuda, 2, 3, 8, L, 16, dtype, "slots")
+        k = torch.empty(table.numel() + 1, 16, 3, 0, device=cuda, dtype=dtype)
+        kept, _, _, out = evict._want(k, k, table, mass, n, keep, 4)
+        got = ops.cache_evict(k, k.clone(), table, n, mass, keep, 4)
+        assert torch.equal(got, kept) and torch.equal(mass, out)
+    key = torch.empty(2, 5, 3, 0, device=cuda, dtype=dtype)
+    ops.paged_append(key, key, k, k.clone(), table, torch.zeros_like(n))
