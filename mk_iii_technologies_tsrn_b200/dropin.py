@@ -562,7 +562,9 @@ class TropicalDecoderModel(_TokenModel):
             uniform = torch.rand(max_new_tokens, B, device=input_ids.device, generator=generator)
         elif uniform.shape != (max_new_tokens, B):
             raise ValueError(f"uniform must be [{max_new_tokens}, {B}], got {tuple(uniform.shape)}")
-        slots = L + max_new_tokens - 1 if keep is None else max(L, keep + page_size)
+        slots = L + max_new_tokens - 1
+        if keep is not None:
+            slots = min(slots, max(L, keep + page_size))
         attn = self.layers.layers[0].self_attn
         cache = TropicalPagedKVCache(len(self.layers.layers), B, attn.num_heads, attn.d_k, slots,
                                      page_size=page_size, collect_mass=keep is not None,
@@ -577,7 +579,7 @@ class TropicalDecoderModel(_TokenModel):
             out[t] = ops.sample_tokens(self.lm_head(x), uniform[t], **choices)
             if t + 1 == max_new_tokens:
                 break
-            if keep is not None and cache.most >= min(slots, keep + page_size):
+            if keep is not None and cache.most >= keep + page_size:
                 cache.evict(keep, keep // 4 if recent is None else recent)
             cache.step()
             ids = out[t].to(input_ids.dtype)[:, None]

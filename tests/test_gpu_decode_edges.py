@@ -121,3 +121,11 @@ def test_eviction_without_channels(cuda, dtype):
         assert torch.equal(got, kept) and torch.equal(mass, out)
     key = torch.empty(2, 5, 3, 0, device=cuda, dtype=dtype)
     ops.paged_append(key, key, k, k.clone(), table, torch.zeros_like(n))
+
+
+def test_generate_under_a_budget_beyond_all_tokens(cuda):
+    import test_gpu_decode_run as decode
+    m = decode._model(cuda)
+    ids = torch.randint(0, 97, (2, 9), device=cuda, generator=torch.Generator(device=cuda).manual_seed(2))
+    u = torch.rand(20, 2, device=cuda, generator=torch.Generator(device=cuda).manual_seed(3))
+    assert torch.equal(m.generate(ids, 20, uniform=u), m.generate(ids, 20, uniform=u, keep=2 ** 40))
