@@ -1770,9 +1770,18 @@ def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch
     return kept if kept is not None else _refused()
 
 
-def _choice(x, dtype=torch.float32):
+def _choice(x):
     """A sampling choice of each row as the kernel reads it."""
-    return x if x.dtype == dtype and x.is_contiguous() else x.to(dtype).contiguous()
+    return x if x.dtype == torch.float32 and x.is_contiguous() else x.float().contiguous()
+
+
+def _counts_of_rows(k):
+    """top_k of each row as the kernel reads it."""
+    if k.dtype not in (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8):
+        raise ValueError(f"top_k must be whole numbers, got {k.dtype}")
+    if k.dtype == torch.int64:
+        k = k.clamp(-2 ** 31, 2 ** 31 - 1)                     # (beyond 32 bits: all tokens)
+    return k.to(torch.int32).contiguous()
 
 
 def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature=1.0, top_k=0,
@@ -1800,7 +1809,7 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature=1.
     elif not T >= 0.0:
         raise ValueError(f"temperature must be 0 or more, got {T}")
     if isinstance(k, torch.Tensor):
-        k, ks = 0, _choice(k, torch.int32)
+        k, ks = 0, _counts_of_rows(k)
     elif not k >= 0:
         raise ValueError(f"top_k must be 0 or more, got {k}")
     if isinstance(p, torch.Tensor):

@@ -1,8 +1,8 @@
-"""Host side of the decoding path, without a GPU: sizes of caches."""
+"""Host side of the decoding path, without a GPU: sizes of caches, counts of 64 bits."""
 import pytest
 import torch
 
-from mk_iii_technologies_tsrn_b200 import dropin
+from mk_iii_technologies_tsrn_b200 import dropin, ops
 
 
 class _Asked(Exception):
@@ -34,3 +34,13 @@ def test_a_budget_takes_no_more_room_than_the_tokens(asked):
     assert asked(10, 100, keep=20, page_size=16) == 36            # the budget and a page
     assert asked(60, 100, keep=20, page_size=16) == 60            # the prompt
     assert asked(10, 100, keep=20, page_size=10 ** 6) == 109      # (a page is beyond all tokens)
+
+
+def test_counts_of_requests_keep_their_meaning():
+    k = torch.tensor([2 ** 32 + 1, 2 ** 31, -2 ** 40, 0, 50, 2 ** 63 - 1])
+    assert ops._counts_of_rows(k).tolist() == [2 ** 31 - 1, 2 ** 31 - 1, -2 ** 31, 0, 50, 2 ** 31 - 1]
+    for dtype in (torch.int32, torch.int16, torch.uint8):
+        assert ops._counts_of_rows(torch.tensor([3, 0], dtype=dtype)).tolist() == [3, 0]
+    for bad in (torch.tensor([0.9, 5.0]), torch.tensor([True, False])):
+        with pytest.raises(ValueError, match="top_k"):
+            ops.sample_tokens(torch.randn(2, 9), torch.rand(2), top_k=bad)

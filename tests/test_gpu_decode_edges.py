@@ -129,3 +129,12 @@ def test_generate_under_a_budget_beyond_all_tokens(cuda):
     ids = torch.randint(0, 97, (2, 9), device=cuda, generator=torch.Generator(device=cuda).manual_seed(2))
     u = torch.rand(20, 2, device=cuda, generator=torch.Generator(device=cuda).manual_seed(3))
     assert torch.equal(m.generate(ids, 20, uniform=u), m.generate(ids, 20, uniform=u, keep=2 ** 40))
+
+
+def test_counts_beyond_32_bits_keep_all_tokens(cuda):
+    from mk_iii_technologies_tsrn_b200 import ops
+    x = torch.randn(4, 900, device=cuda, generator=torch.Generator(device=cuda).manual_seed(0))
+    u = torch.tensor([0.1, 0.5, 0.9, 0.99], device=cuda)
+    k = torch.tensor([2 ** 32 + 1, 2 ** 32 + 5, 2 ** 31, -2 ** 32 + 1], device=cuda)
+    assert torch.equal(ops.sample_tokens(x, u, top_k=k), ops.sample_tokens(x, u))
+    assert torch.equal(ops.sample_tokens(x, u, top_k=2 ** 40), ops.sample_tokens(x, u))
