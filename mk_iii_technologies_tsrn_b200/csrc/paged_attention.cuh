@@ -573,19 +573,18 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) paged_join_kernel(const Paged
         float f[AT_ONCE], x[AT_ONCE][KD];
 #pragma unroll
         for (int u = 0; u < AT_ONCE; ++u) {
-          const bool in = s0 + u * TEAM < runs.y;
-          const int s = in ? s0 + u * TEAM : runs.y - 1;
+          const int s = min(s0 + u * TEAM, runs.y - 1);
           f[u] = ml[s * stride].x;
           const float* p = a.part + (first + s * stride) * D;
 #pragma unroll
-          for (int k = 0; k < KD; ++k) x[u][k] = in && lane + 32 * k < D ? p[lane + 32 * k] : 0.0f;
+          for (int k = 0; k < KD; ++k) x[u][k] = lane + 32 * k < D ? p[lane + 32 * k] : 0.0f;
         }
 #pragma unroll
         for (int u = 0; u < AT_ONCE; ++u) {
-          const bool counts = s0 + u * TEAM < runs.y && f[u] != neg_inf();
-          f[u] = counts ? tp_ex2(f[u] - whole.x) : 0.0f;
+          const bool in = s0 + u * TEAM < runs.y;        // (an infinity twice, once times 0, would be NaN)
+          f[u] = f[u] != neg_inf() ? tp_ex2(f[u] - whole.x) : 0.0f;
 #pragma unroll
-          for (int k = 0; k < KD; ++k) sum[k] += x[u][k] * f[u];
+          for (int k = 0; k < KD; ++k) sum[k] += in ? x[u][k] * f[u] : 0.0f;
         }
       }
     }
