@@ -565,10 +565,28 @@ Tensor embedding_fwd(Tensor ids, Tensor weight, Maybe pos_weight, Maybe position
 }
 
 // ---------------------------------------------------------------- decoding
-// no two elements of the first dimensions at one address: rows of `row` contiguous elements
-bool rows_apart(const Tensor& t, int64_t row) {
-  for (int64_t i = 0; i + 1 < t.dim(); ++i)
-    if (t.size(i) > 1 && t.stride(i) < row) return false;
+// no two elements of t, whose last dimension is contiguous, at one address: every dimension steps
+// over all that the ones of smaller steps reach
+bool rows_apart(const Tensor& t) {
+  const at::IntArrayRef sizes = t.sizes(), strides = t.strides();
+  const int64_t dims = (int64_t)sizes.size() - 1;
+  int64_t reach = sizes[dims], step[3], last[3], n = 0;      // (callers look at the dimensions first)
+  for (int64_t i = 0; i < dims; ++i) {
+    if (sizes[i] == 0) return true;
+    if (sizes[i] == 1) continue;
+    int64_t at = n++;                  // by falling step
+    for (; at > 0 && step[at - 1] < strides[i]; --at) {
+      step[at] = step[at - 1];
+      last[at] = last[at - 1];
+    }
+    step[at] = strides[i];
+    last[at] = sizes[i] - 1;
+  }
+  if (reach == 0) return true;
+  while (n-- > 0) {
+    if (step[n] < reach) return false;
+    reach += step[n] * last[n];
+  }
   return true;
 }
 bool is_i32(const Tensor& t, const Tensor& on) {
@@ -578,7 +596,7 @@ bool is_i32(const Tensor& t, const Tensor& on) {
 bool paged_ok(const Tensor& k, const Tensor& v, const Tensor& table, int64_t B) {
   if (!k.is_cuda() || !is_float(k) || k.dim() != 4 || !alike(v, k)) return false;
   for (const Tensor* t : {&k, &v})
-    if ((t->size(3) > 1 && t->stride(3) != 1) || !rows_apart(*t, t->size(3))) return false;
+    if ((t->size(3) > 1 && t->stride(3) != 1) || !rows_apart(*t)) return false;
   return is_i32(table, k) && table.dim() == 2 && table.size(0) == B &&
          (table.size(1) <= 1 || table.stride(1) == 1) && k.size(1) > 0;
 }
@@ -594,7 +612,7 @@ bool lengths_ok(const Tensor& t, const Tensor& on, int64_t B) {
 bool mass_ok(const Tensor& t, const Tensor& k, int64_t B) {
   return t.device() == k.device() && t.scalar_type() == at::kFloat && t.dim() == 3 &&
          t.size(0) == B && t.size(1) == k.size(2) && (t.size(2) <= 1 || t.stride(2) == 1) &&
-         rows_apart(t, t.size(2));
+         rows_apart(t);
 }
 void written(const Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();

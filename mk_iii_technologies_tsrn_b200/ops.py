@@ -1599,6 +1599,17 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, *,
 
 
 # --------------------------------------------------------------------------- decoding
+def _rows_apart(t):
+    """Whether no two elements of t, whose last dimension is contiguous, share an address: every
+    dimension steps over all that the ones of smaller steps reach."""
+    reach = t.shape[-1]
+    for step, n in sorted((t.stride(i), t.shape[i]) for i in range(t.dim() - 1) if t.shape[i] > 1):
+        if step < reach:
+            return t.numel() == 0
+        reach += step * (n - 1)
+    return True
+
+
 def _paged_inputs(k_cache, v_cache, block_table, B, what):
     """Checks of a cache and its table of B rows."""
     _floating(k_cache, "paged caches")
@@ -1607,8 +1618,7 @@ def _paged_inputs(k_cache, v_cache, block_table, B, what):
                          f"shape and dtype, got {tuple(k_cache.shape)} {k_cache.dtype} and "
                          f"{tuple(v_cache.shape)} {v_cache.dtype}")
     for t in (k_cache, v_cache):
-        if t.shape[3] > 1 and t.stride(3) != 1 or any(
-                t.shape[i] > 1 and t.stride(i) < t.shape[3] for i in range(3)):
+        if t.shape[3] > 1 and t.stride(3) != 1 or not _rows_apart(t):
             raise ValueError("a cache's channels must be contiguous and its rows apart, got "
                              f"strides {t.stride()}")
     if k_cache.shape[1] < 1:
@@ -1630,8 +1640,7 @@ def _slot_counts(t: torch.Tensor, B: int, what: str) -> torch.Tensor:
 
 def _mass_inputs(mass, B, heads, what):
     if _f32(mass).dim() != 3 or mass.shape[:2] != (B, heads) or (
-            mass.shape[2] > 1 and mass.stride(2) != 1) or any(
-            mass.shape[i] > 1 and mass.stride(i) < mass.shape[2] for i in range(2)):
+            mass.shape[2] > 1 and mass.stride(2) != 1) or not _rows_apart(mass):
         raise ValueError(f"{what} must be [{B}, {heads}, slots] with contiguous, separate rows, "
                          f"got {tuple(mass.shape)} at strides {mass.stride()}")
 

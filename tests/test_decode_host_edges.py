@@ -1,4 +1,5 @@
-"""Host side of the decoding path, without a GPU: sizes of caches, counts of 64 bits."""
+"""Host side of the decoding path, without a GPU: sizes of caches, counts of 64 bits, rows
+that share memory."""
 import pytest
 import torch
 
@@ -44,3 +45,45 @@ def test_counts_of_requests_keep_their_meaning():
     for bad in (torch.tensor([0.9, 5.0]), torch.tensor([True, False])):
         with pytest.raises(ValueError, match="top_k"):
             ops.sample_tokens(torch.randn(2, 9), torch.rand(2), top_k=bad)
+
+
+def _layouts(dtype=torch.float32, device="cpu"):
+    """(cache [pages, slots, heads, 8], whether its rows lie apart)."""
+    flat = torch.zeros(4096, dtype=dtype, device=device)
+
+    def view(shape, *strides):
+        return flat.as_strided((*shape, 8), (*strides, 1))
+
+    return [
+        (view((4, 4, 2), 64, 16, 8), True),
+        (view((4, 4, 2), 64, 8, 32), True),                   # heads before slots
+        (view((4, 4, 2), 16, 64, 8), True),                   # slots before pages
+        (view((4, 4, 2), 8, 64, 32), True),
+        (view((3, 5, 1), 80, 16, 0), True),                   # room behind every row; a single head
+        (view((1, 1, 7), 0, 0, 9), True),
+        (view((0, 4, 2), 0, 0, 0), True),
+        (flat.view(4, 2, 8, 64).transpose(1, 2)[..., :8], True),
+        (view((4, 4, 2), 64, 8, 8), False),                   # a slot's second head is the next one's first
+        (view((4, 4, 2), 16, 8, 64), False),
+        (view((4, 4, 2), 56, 16, 8), False),                  # a page begins in the one before
+        (view((4, 4, 2), 64, 12, 8), False),
+        (view((4, 4, 2), 64, 16, 4), False),
+        (view((4, 4, 2), 0, 16, 8), False),
+        (view((2, 2, 2), 8, 8, 8), False),
+    ]
+
+
+def test_caches_whose_rows_overlap_are_refused():
+    table = torch.zeros(1, 2, dtype=torch.int32)
+    for k, apart in _layouts():
+        if apart:
+            ops._paged_inputs(k, k, table, 1, "")
+        else:
+            with pytest.raises(ValueError, match="apart"):
+                ops._paged_inputs(k, k, table, 1, "")
+    flat = torch.zeros(400)
+    ops._mass_inputs(flat.as_strided((3, 2, 10), (10, 30, 1)), 3, 2, "mass")
+    ops._mass_inputs(flat.as_strided((1, 2, 10), (0, 12, 1)), 1, 2, "mass")
+    for strides in ((10, 20, 1), (20, 9, 1), (10, 10, 1), (15, 10, 1)):
+        with pytest.raises(ValueError, match="separate"):
+            ops._mass_inputs(flat.as_strided((3, 2, 10), strides), 3, 2, "mass")

@@ -138,3 +138,41 @@ def test_counts_beyond_32_bits_keep_all_tokens(cuda):
     k = torch.tensor([2 ** 32 + 1, 2 ** 32 + 5, 2 ** 31, -2 ** 32 + 1], device=cuda)
     assert torch.equal(ops.sample_tokens(x, u, top_k=k), ops.sample_tokens(x, u))
     assert torch.equal(ops.sample_tokens(x, u, top_k=2 ** 40), ops.sample_tokens(x, u))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_caches_whose_rows_overlap_are_refused(cuda, dtype):
+    from mk_iii_technologies_tsrn_b200 import ops
+    from test_decode_host_edges import _layouts
+    n = torch.tensor([1], device=cuda, dtype=torch.int32)
+    for k, apart in _layouts(dtype, cuda):
+        v, heads, slots = k.clone(), k.shape[2], k.shape[1]
+        table = torch.arange(max(1, k.shape[0]), device=cuda, dtype=torch.int32)[None]
+        key = torch.randn(1, slots * k.shape[0], heads, 8, device=cuda).to(dtype)
+        mass = torch.rand(1, heads, table.shape[1] * slots, device=cuda)
+        calls = (lambda: ops.paged_append(key, key, k, v, table, n - 1),
+                 lambda: ops.paged_append(key, key, v, k, table, n - 1),
+                 lambda: ops.paged_attention(key[:, 0] if key.shape[1] else mass[..., :8].to(dtype), k, v, table, n * 0),
+                 lambda: ops.cache_evict(k, v, table, n, mass, 1))
+        if not apart:
+            for call in calls:
+                with pytest.raises(ValueError, match="apart"):
+                    call()
+            continue
+        for call in calls[:2] + calls[3:]:
+            call()
+        if k.numel():
+            assert torch.equal(k.flatten(0, 1), key[0]) and torch.equal(v.flatten(0, 1), key[0])
+    k, v = torch.zeros(2, 20, 16, 2, 8, device=cuda, dtype=dtype)
+    table = torch.arange(6, device=cuda, dtype=torch.int32).view(3, 2)
+    flat = torch.rand(400, device=cuda)
+    lengths = torch.tensor([10, 7, 0], device=cuda, dtype=torch.int32)
+    for strides, apart in (((32, 96, 1), True), ((15, 10, 1), False), ((64, 32, 1), True), ((32, 32, 1), False)):
+        mass = flat.as_strided((3, 2, 32), strides)
+        if apart:
+            ops.cache_evict(k, v, table, lengths, mass, 4)
+        else:
+            with pytest.raises(ValueError, match="separate"):
+                ops.cache_evict(k, v, table, lengths, mass, 4)
+            with pytest.raises(ValueError, match="separate"):
+                ops.paged_attention(k[:3, 0], k, v, table, lengths, mass=mass)
