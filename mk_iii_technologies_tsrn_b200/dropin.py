@@ -359,7 +359,8 @@ class TropicalDecoderLayer(nn.Module):
 
 class TropicalEncoder(nn.Module):
     """Stack of copies of an encoder layer, optional final norm
-    (tropformer_dropin.py:495-515)."""
+    (tropformer_dropin.py:495-515).  ``cache``: a :class:`TropicalPagedKVCache`, whose layers go to
+    the stack's in turn."""
 
     def __init__(self, encoder_layer: TropicalEncoderLayer, num_layers: int,
                  norm: Optional[nn.Module] = None):
@@ -368,10 +369,12 @@ class TropicalEncoder(nn.Module):
         self.norm = norm
 
     def forward(self, src: torch.Tensor, mask: Optional[torch.Tensor] = None,
-                src_key_padding_mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+                src_key_padding_mask: Optional[torch.Tensor] = None,
+                cache: Optional[TropicalPagedKVCache] = None) -> torch.Tensor:
         out = src
-        for layer in self.layers:
-            out = layer(out, src_mask=mask, src_key_padding_mask=src_key_padding_mask)
+        for i, layer in enumerate(self.layers):
+            cached = {} if cache is None else {"cache": cache.layer(i)}
+            out = layer(out, src_mask=mask, src_key_padding_mask=src_key_padding_mask, **cached)
         return self.norm(out) if self.norm is not None else out
 
 
@@ -523,12 +526,6 @@ class TropicalDecoderModel(_TokenModel):
         x = self.layers(self._embed(input_ids), mask=mask, src_key_padding_mask=pad)
         return self.lm_head(x)
 
-    def _cached(self, x, cache: TropicalPagedKVCache, mask=None, pad=None) -> torch.Tensor:
-        # the stack over a cache's layers
-        for i, layer in enumerate(self.layers.layers):
-            x = layer(x, src_mask=mask, src_key_padding_mask=pad, cache=cache.layer(i))
-        return self.layers.norm(x) if self.layers.norm is not None else x
-
     @torch.no_grad()
     def generate(self, input_ids: torch.Tensor, max_new_tokens: int, *,
                  attention_mask: Optional[torch.Tensor] = None, temperature=1.0, top_k=0,
@@ -571,7 +568,8 @@ class TropicalDecoderModel(_TokenModel):
                                      dtype=attn.k_proj.weight.dtype, device=input_ids.device)
         choices = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
         cache.begin(counts, L)
-        x = self._cached(self._embed(input_ids), cache, make_causal_mask(L, input_ids.device), pad)
+        x = self.layers(self._embed(input_ids), mask=make_causal_mask(L, input_ids.device),
+                        src_key_padding_mask=pad, cache=cache)
         x = x[torch.arange(B, device=x.device), counts.long() - 1]
         out = torch.empty(max_new_tokens, B, dtype=torch.int64, device=x.device)
         positions = counts.to(input_ids.dtype)[:, None]
@@ -583,7 +581,7 @@ class TropicalDecoderModel(_TokenModel):
                 cache.evict(keep, keep // 4 if recent is None else recent)
             cache.step()
             ids = out[t].to(input_ids.dtype)[:, None]
-            x = self._cached(self._embed(ids, positions), cache)[:, 0]
+            x = self.layers(self._embed(ids, positions), cache=cache)[:, 0]
             positions = positions + 1
         return out.t().contiguous()
 

@@ -176,3 +176,26 @@ def test_caches_whose_rows_overlap_are_refused(cuda, dtype):
                 ops.cache_evict(k, v, table, lengths, mass, 4)
             with pytest.raises(ValueError, match="separate"):
                 ops.paged_attention(k[:3, 0], k, v, table, lengths, mass=mass)
+
+
+def test_generate_runs_the_models_stack(cuda):
+    # hooks on the stack of layers, and a forward of its own, count in generate as in forward
+    import test_gpu_decode_run as decode
+    from mk_iii_technologies_tsrn_b200 import dropin
+    m = decode._model(cuda)
+    ids = torch.randint(0, 97, (3, 9), device=cuda, generator=torch.Generator(device=cuda).manual_seed(2))
+    plain = m.generate(ids, 4, temperature=0.0)
+    calls = []
+    hook = m.layers.register_forward_hook(lambda mod, a, out: calls.append(out.shape) or -out)
+    got = m.generate(ids, 4, temperature=0.0)
+    assert calls == [(3, 9, 64)] + [(3, 1, 64)] * 3 and not torch.equal(got, plain)
+    with torch.no_grad():
+        assert torch.equal(got[:, 0], m(ids)[:, -1].argmax(-1))
+    hook.remove()
+
+    class Turned(dropin.TropicalEncoder):
+        def forward(self, *args, **kw):
+            return -super().forward(*args, **kw)
+
+    m.layers.__class__ = Turned
+    assert torch.equal(m.generate(ids, 4, temperature=0.0), got)
