@@ -155,14 +155,14 @@ class _PagedLayer:
         if c.mass[i] is not None:
             L = attn.shape[-1]
             there = torch.arange(L, device=attn.device) < c.lengths[:, None]
-            c.mass[i][:, :, :L] = (attn * there[:, None, :, None]).sum(2)
+            c.mass[i][:, :, :L] = (attn.float() * there[:, None, :, None]).sum(2)
 
     def attend(self, Q, K, V, scale, gate, tau):
-        # Q, K, V [B, H, 1, d_k] of the new token
+        # Q, K, V [B, H, 1, d_k] of the new token (under autocast the gate is of their type)
         c, i = self.cache, self.index
         return ops.paged_attention(Q[:, :, 0], c.k[i], c.v[i], c.block_table, c.lengths,
-                                   key=K[:, :, 0], value=V[:, :, 0], scale=scale, gate=gate,
-                                   tau=tau, mass=c.mass[i])
+                                   key=K[:, :, 0], value=V[:, :, 0], scale=scale,
+                                   gate=gate.float(), tau=tau.float(), mass=c.mass[i])
 
 
 def _grad_needed(*tensors) -> bool:
@@ -540,7 +540,7 @@ class TropicalDecoderModel(_TokenModel):
         ``keep``: a budget of cache slots for each sequence; a sequence over it by a page goes
         back to it, the last ``recent`` (None: a quarter) and those with the most accumulated
         attention weight staying.  Needs a CUDA device and a model in eval mode (or without
-        dropout)."""
+        dropout).  Under ``torch.autocast`` in bfloat16 the cache is of that type."""
         B, L = input_ids.shape
         if L < 1 or max_new_tokens < 1 or \
                 L + max_new_tokens - 1 > self.pos_embed.num_embeddings:
@@ -563,9 +563,12 @@ class TropicalDecoderModel(_TokenModel):
         if keep is not None:
             slots = min(slots, max(L, keep + page_size))
         attn = self.layers.layers[0].self_attn
+        # keys and values come in the type of their projections
+        dtype = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else \
+            attn.k_proj.weight.dtype
         cache = TropicalPagedKVCache(len(self.layers.layers), B, attn.num_heads, attn.d_k, slots,
                                      page_size=page_size, collect_mass=keep is not None,
-                                     dtype=attn.k_proj.weight.dtype, device=input_ids.device)
+                                     dtype=dtype, device=input_ids.device)
         choices = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
         cache.begin(counts, L)
         x = self.layers(self._embed(input_ids), mask=make_causal_mask(L, input_ids.device),

@@ -199,3 +199,42 @@ def test_generate_runs_the_models_stack(cuda):
 
     m.layers.__class__ = Turned
     assert torch.equal(m.generate(ids, 4, temperature=0.0), got)
+
+
+def test_generate_under_autocast(cuda, monkeypatch):
+    # as forward runs there; every token's attention within the tolerance of test_gpu_paged_attention.py
+    import test_gpu_decode_run as decode
+    import test_gpu_paged_attention as base
+    import test_gpu_paged_attention_finite as finite
+    from mk_iii_technologies_tsrn_b200 import dropin
+    m = decode._model(cuda)
+    g = torch.Generator(device=cuda).manual_seed(2)
+    ids = torch.randint(0, 97, (3, 9), device=cuda, generator=g)
+    mask = (torch.arange(9, device=cuda) < torch.tensor([[9], [1], [5]], device=cuda)).long()
+    u = torch.rand(12, 3, device=cuda, generator=g)
+    own, steps = dropin._PagedLayer.attend, []
+
+    def attend(self, Q, K, V, scale, gate, tau):
+        c, i = self.cache, self.index
+        assert Q.dtype == c.k[i].dtype == torch.bfloat16
+        o = own(self, Q, K, V, scale, gate, tau)
+        want, _, off = base._reference(Q[:, :, 0], c.k[i], c.v[i], c.block_table, c.lengths, scale, gate.float(), tau)
+        finite._check(o, want, off, c.v[i], torch.bfloat16)
+        last = c.lengths.long() - 1
+        at = c.block_table[torch.arange(3), last // 16].long()
+        assert torch.equal(c.k[i][at, last % 16], K[:, :, 0]) and torch.equal(c.v[i][at, last % 16], V[:, :, 0])
+        steps.append(i)
+        return o
+
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        plain = m.generate(ids, 12, attention_mask=mask, uniform=u, top_k=20)
+        short = m.generate(ids, 12, attention_mask=mask, uniform=u, keep=4, recent=1, page_size=2)
+        best = m.generate(ids, 1, attention_mask=mask, temperature=0.0)[:, 0]
+        with torch.no_grad():
+            logits = m(ids, mask)[torch.arange(3), mask.sum(1) - 1]
+        monkeypatch.setattr(dropin._PagedLayer, "attend", attend)
+        assert torch.equal(m.generate(ids, 12, attention_mask=mask, uniform=u, top_k=20), plain)
+    assert steps == [0, 1] * 11 and logits.dtype == torch.bfloat16
+    assert torch.equal(logits.gather(1, best[:, None])[:, 0], logits.amax(1))
+    for t in (plain, short):
+        assert t.shape == (3, 12) and int(t.min()) >= 0 and int(t.max()) < 97
