@@ -18,7 +18,8 @@
 // head of 64 channels 106 for 107.5).  Blocks of five to eight have rows g and g + 8 alone: two parts,
 // which lose at most 2^-16 of a weight, where the output is rounded by 2^-8 (a second product for the
 // other bits: 24 x 8192 of 16 query heads each 95 -> 105 us, 48 x 8192 of 8 heads of 64 115 -> 122).
-// Everything else is fp32.
+// So do all above 192 channels, whose registers are full (48 x 4096 of 4 heads of 256 channels 256 us,
+// 286 with three parts).  Everything else is fp32.
 #include "paged_attention.cuh"
 
 namespace tp {
@@ -298,8 +299,10 @@ int attend_mma(PagedAttentionArgs& a, cudaStream_t stream) {
   constexpr int STAGES = KB > 4 ? 2 : 3;
   using P = MmaTile<KB>;
   const size_t smem = (size_t)ATT_WARPS * STAGES * P::STAGE * 16;
-  return a.group <= 4 ? attend_and_join<uint16_t>(a, paged_attend_mma_kernel<KB, STAGES, true>, smem, P::TK, 4, stream)
-                      : attend_and_join<uint16_t>(a, paged_attend_mma_kernel<KB, STAGES, false>, smem, P::TK, 8, stream);
+  if constexpr (KB <= 6)
+    if (a.group <= 4)
+      return attend_and_join<uint16_t>(a, paged_attend_mma_kernel<KB, STAGES, true>, smem, P::TK, 4, stream);
+  return attend_and_join<uint16_t>(a, paged_attend_mma_kernel<KB, STAGES, false>, smem, P::TK, 8, stream);
 }
 
 int on_tensor_cores(PagedAttentionArgs& a, cudaStream_t stream) {
