@@ -9,6 +9,7 @@
 #include <initializer_list>
 #include <map>
 #include <mutex>
+#include <tuple>
 #include <utility>
 
 #include "maxplus_internal.cuh"
@@ -133,6 +134,26 @@ int allow_smem(const void* kernel, size_t bytes) {
   e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
   if (e == cudaSuccess) known = bytes;
   return cuda_status(e);
+}
+
+int resident_blocks(const void* kernel, int threads, size_t bytes, int& blocks) {
+  static std::mutex mu;
+  static std::map<std::tuple<const void*, int, int, size_t>, int> known;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_status(e);
+  std::lock_guard<std::mutex> lock(mu);
+  int& most = known[{kernel, dev, threads, bytes}];
+  if (most == 0) {
+    const int st = allow_smem(kernel, bytes);
+    if (st != TP_OK) return st;
+    int n = 0;
+    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, bytes);
+    if (e != cudaSuccess) return cuda_status(e);
+    most = n > 0 ? n : 1;
+  }
+  blocks = most;
+  return TP_OK;
 }
 
 int check_scan_bwd_pointers(int64_t T, const float* gh, const float* bb, const float* xx,

@@ -279,6 +279,8 @@ int num_sms();
 // ever rises: another thread's smaller call between this and the launch would otherwise
 // have the launch refused.
 int allow_smem(const void* kernel, size_t bytes);
+// The same, and how many blocks of `threads` threads an SM then holds, by all of its resources.
+int resident_blocks(const void* kernel, int threads, size_t bytes, int& blocks);
 
 // Device address of the library's error word on the current device (resolved
 // once per device with cudaGetSymbolAddress); nullptr if unavailable.

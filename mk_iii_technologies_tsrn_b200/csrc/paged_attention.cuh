@@ -678,16 +678,18 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) paged_join_kernel(const Paged
 template <typename T, typename K>
 int attend_and_join(PagedAttentionArgs& a, K* kernel, size_t smem, int tile, int heads,
                     cudaStream_t stream) {
-  int st = allow_smem((const void*)kernel, smem);
+  int per_sm = 1;
+  int st = resident_blocks((const void*)kernel, ATT_WARPS * 32, smem, per_sm);
   if (st != TP_OK) return st;
   a.block_heads = heads;
   a.head_blocks = (a.group + heads - 1) / heads;
   a.tile = tile;
-  // as many runs as the SMs hold warps for, with at least two tiles each (four: 4 x 512 slots of 8
-  // heads of 64 fp32 12.1 us for 10.0)
-  const int64_t per_sm = std::min<size_t>(ATT_MOST_BLOCKS, (227 * 1024) / (smem + 1024 + 1100));
+  // as many runs as the SMs hold warps for by registers and shared memory (by the latter alone, 32 x 2048
+  // gated slots of 4 query heads a key head ran as a wave and a half: 65 us for 54), with at least two
+  // tiles each (four: 4 x 512 slots of 8 heads of 64 fp32 12.1 us for 10.0)
+  per_sm = std::min(per_sm, ATT_MOST_BLOCKS);
   const int64_t subs = (int64_t)a.c.heads * a.head_blocks, tiles = a.B * ceil_div(a.capacity, tile);
-  a.runs = (int)std::max<int64_t>(1, std::min(num_sms() * per_sm * ATT_WARPS / subs, ceil_div(tiles, 2)));
+  a.runs = (int)std::max<int64_t>(1, std::min((int64_t)num_sms() * per_sm * ATT_WARPS / subs, ceil_div(tiles, 2)));
   const int64_t blocks = ceil_div(a.runs * subs, ATT_WARPS);
   kernel<<<(unsigned)blocks, ATT_WARPS * 32, smem, stream>>>(a);
   st = launch_status();
