@@ -819,8 +819,9 @@ TP_API int tp_convert_bf16_to_f32(int64_t n, const void* src, float* dst, void* 
  *  table[b][j / page_size].  Pages may be read by several sequences; what is
  *  written (a new token's slot, prompts, evicted rows) must be in pages of one
  *  sequence.  A length, start or page outside its range is never followed:
- *  TP_DEVERR_INDEX is noted, that row of an output is NaN (attention), nothing is
- *  written (append), and the sequence, or a row whose page it is, stays (evict).
+ *  TP_DEVERR_INDEX is noted, that row of an output is NaN (attention; for a page
+ *  its weights in mass too), nothing is written (append), and the sequence, or a row
+ *  whose page it is, stays (evict).  No two rows may share memory.
  *
  *  tp_paged_attention: for b in [0, B), query head h over key head
  *  h / (H / heads) and the slots j < lengths[b]:

@@ -24,10 +24,14 @@
 //   - Where even that bin holds too many (flat rows, ties), and for a share of a top_k above
 //     CANDIDATES, the threshold is found bit by bit over all tokens.
 //
-// Measured (in a CUDA graph): 16 x 256 fp32 without filters 5.5 us, 64 x 131072 bf16 with top_k
+// Measured (in a CUDA graph): 16 x 256 fp32 without filters 5.4 us, 64 x 131072 bf16 with top_k
 // around 50 and top_p 26 (2.6 us of bytes), 32 x 49999 fp32 with top_p 0.95 and 2300 tokens kept
-// 38.  What bounds it is latency: passes of a few steps with an exchange of the cluster between
-// them; in the last case half of it are instructions (weights in 64 bits).
+// 37 to 39.  What bounds it is latency: passes of a few steps with an exchange of the cluster between
+// them; in the last case half of it are instructions (weights in 64 bits).  Without filters 17 us at
+// 32 x 49999 and 46 at 64 x 131072 bf16 (a weight for every token, twice), the best token alone 6 and 7.
+// The search bit by bit takes up to 33 passes: 32 x 49999 equal logits 123 us with top_k, 147 with
+// top_p, top_k of 5000 with top_p 184.
+// 64 registers for 1024 threads: the bf16 form spills (188 bytes of stores, 248 of loads).
 #include <algorithm>
 
 #include "cluster.cuh"
@@ -84,9 +88,6 @@ __device__ __forceinline__ u64 warp_inclusive(u64 v, int lane) {
   return v;
 }
 
-// A warp's part of a row, in steps of 16 bytes a lane.  They lie on 16-byte boundaries wherever the
-// row begins; where a step reaches over an end of the row it takes single numbers, and -inf for those
-// that are not there.
 // Sum of sums[0 .. warp) over a block's warps, and of all of them.
 template <int WARPS>
 __device__ __forceinline__ u64 before_warp(const u64* sums, int warp, int lane, u64& all) {
@@ -95,6 +96,9 @@ __device__ __forceinline__ u64 before_warp(const u64* sums, int warp, int lane, 
   return __shfl_sync(0xffffffffu, upto - mine, warp);
 }
 
+// A warp's part of a row, in steps of 16 bytes a lane.  They lie on 16-byte boundaries wherever the
+// row begins; where a step reaches over an end of the row it takes single numbers, and -inf for those
+// that are not there.
 template <typename T>
 struct Row {
   static constexpr int PER = 16 / sizeof(T);      // tokens of a lane's step, next to one another

@@ -1676,13 +1676,17 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     stored there.  ``scale``: None for D ** -0.5.  ``gate``: [B, H] and ``tau``: [H], float32.
     ``mass``: [B, Hkv, slots] float32 (slots contiguous): the softmax weights, summed over the
     query heads of a key head, are added to it in place, for :func:`cache_evict`; with ``key`` the
-    new slot is set to its weight.  Scores, statistics and sums are float32.  Returns
-    [B, H, D] in q's dtype.  Not differentiable.  The same inputs give the same bits; with other
-    sequences around it a sequence's sums may be cut, and so rounded, elsewhere.
+    new slot is set to its weight.  With it the call's workspace holds 4 bytes for every query head
+    and slot that the table (or ``mass``) has room for, whatever the lengths: B * H * slots.  Scores,
+    statistics and sums are float32; bfloat16 weights lose at most 2^-16 of themselves, and nothing
+    where a key head has up to four query heads of up to 192 channels.  Returns [B, H, D] in q's
+    dtype.  Not differentiable.  The same inputs give the same bits; with other sequences around it
+    a sequence's sums may be cut, and so rounded, elsewhere.
 
     A length beyond the table (or beyond ``mass``), or a page outside the cache, makes the
-    sequence's rows NaN, and :func:`check_device_error` raises :class:`DeviceIndexError`.
-    Sequences may share pages they read; pages that are written belong to one sequence."""
+    sequence's rows NaN (a page also its weights in ``mass``), and :func:`check_device_error` raises
+    :class:`DeviceIndexError`.  Sequences may share pages they read; pages that are written belong to
+    one sequence.  Caches and ``mass`` whose rows share memory are refused."""
     call = _lib.host().paged_attention
     out = call(q, k_cache, v_cache, block_table, lengths, key, value, scale, gate, tau, mass)
     if out is not None:

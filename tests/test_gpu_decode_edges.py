@@ -238,3 +238,21 @@ def test_generate_under_autocast(cuda, monkeypatch):
     assert torch.equal(logits.gather(1, best[:, None])[:, 0], logits.amax(1))
     for t in (plain, short):
         assert t.shape == (3, 12) and int(t.min()) >= 0 and int(t.max()) < 97
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_bad_page_shows_in_the_weights_of_its_sequence_alone(cuda, dtype):
+    from mk_iii_technologies_tsrn_b200 import ops
+    import test_gpu_paged_attention as base
+    k, v, table, g = base._cache(cuda, 3, 200, 2, 64, 16, dtype)
+    n = torch.tensor([150, 200, 203], device=cuda, dtype=torch.int32)
+    q = torch.randn(3, 4, 64, device=cuda, generator=g).to(dtype)
+    table[1, 4] = k.shape[0]
+    n[2] = 210                                                # beyond the table: its weights stay
+    mass = torch.rand(3, 2, 208, device=cuda, generator=g)
+    before = mass.clone()
+    ops.paged_attention(q, k, v, table, n, mass=mass)
+    with pytest.raises(ops.DeviceIndexError):
+        ops.check_device_error(cuda)
+    assert bool(mass[1, :, :200].isnan().all()) and torch.equal(mass[1, :, 200:], before[1, :, 200:])
+    assert torch.equal(mass[2], before[2]) and not bool(mass[0].isnan().any())
