@@ -18,7 +18,7 @@
 // head of 64 channels 106 for 107.5).  Blocks of five to eight have rows g and g + 8 alone: two parts,
 // which lose at most 2^-16 of a weight, where the output is rounded by 2^-8 (a second product for the
 // other bits: 24 x 8192 of 16 query heads each 95 -> 105 us, 48 x 8192 of 8 heads of 64 115 -> 122).
-// So do all above 192 channels, whose registers are full (48 x 4096 of 4 heads of 256 channels 256 us,
+// So do all above 192 channels, whose registers are full (48 x 4096 of 4 heads of 256 channels 249 us,
 // 286 with three parts).  Everything else is fp32.
 #include "paged_attention.cuh"
 
